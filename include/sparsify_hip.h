@@ -515,6 +515,61 @@ int sphip_add(const float* a, const void* b, int b_dtype, float* out, int64_t n,
 int sphip_muon_apply(float* p, const void* o_bf16, int64_t n, float decay, float step, void* bf16_shadow,
                      void* stream);
 
+/* ---------------------------------------------------------------- dense product with its epilogue, and its gradients
+ *
+ * The skip connection of a transcoder (sparse_coder.py:219-222: sae_out += x @ W_skip.mT) and the dense layers a
+ * transcoder stands in for. All tensors row-major with unit inner stride and a row stride ld* in elements (>= the
+ * row); any sizes, strides and element-aligned addresses (16-byte aligned rows take wider accesses). dtype codes
+ * SPHIP_F32 / SPHIP_BF16; sums are fp32, each output is rounded once when stored. Workspaces: the *_workspace_bytes
+ * query of the same call, 16-byte aligned (0 bytes: may be NULL). */
+enum { SPHIP_ACT_NONE = 0, SPHIP_ACT_RELU = 1, SPHIP_ACT_GELU = 2 /* z Phi(z) */, SPHIP_ACT_SILU = 3 /* z / (1 + e^-z) */ };
+
+/* what an operand of the gradients may be besides SPHIP_F32 / SPHIP_BF16: an 8-bit checkpoint (below) */
+enum { SPHIP_INT8 = 16, SPHIP_E4M3 = 17 };
+
+/* out = act(x W^T + bias) + residual. x (N,D) and W (M,D) of `dtype`; bias (M), residual (N,M) or NULL; out (N,M).
+ * z, or NULL: receives x W^T + bias (before the activation) for the gradient. out may be residual (same stride and
+ * type); it may not overlap x or W. */
+size_t sphip_linear_workspace_bytes(int64_t N, int64_t D, int64_t M);
+int sphip_linear(const void* x, int64_t ldx, const void* W, int64_t ldw, int dtype, const void* bias, int bias_dtype,
+                 int act, const void* residual, int res_dtype, int64_t ldr, void* out, int out_dtype, int64_t ldo,
+                 void* z, int z_dtype, int64_t ldz, int64_t N, int64_t D, int64_t M, void* ws, size_t ws_bytes,
+                 void* stream);
+
+/* dz = g act'(z) (N,M) and db = its column sums (M); either may be NULL. z: values (z_kind a dtype) or codes with
+ * scales (z_kind SPHIP_INT8 / SPHIP_E4M3, ldz their row stride); ignored for SPHIP_ACT_NONE. lddz % 4 == 0, dz 16-byte aligned;
+ * columns [M, lddz) of dz are written as zeros. db sums the unrounded products, in a fixed order. */
+size_t sphip_linear_grad_preact_workspace_bytes(int64_t N, int64_t M);
+int sphip_linear_grad_preact(const void* g, int g_dtype, int64_t ldg, const void* z, int z_kind, const uint8_t* z_scales,
+                             int64_t ldz, int act, void* dz, int dz_dtype, int64_t lddz, void* db, int db_dtype, int64_t N,
+                             int64_t M, void* ws, size_t ws_bytes, void* stream);
+
+/* dx = dz W: dz (N,M) and W (M,D) of `dtype`, dx (N,D). */
+size_t sphip_linear_grad_input_workspace_bytes(int64_t N, int64_t D, int64_t M);
+int sphip_linear_grad_input(const void* dz, int64_t lddz, const void* W, int64_t ldw, int dtype, void* dx, int dx_dtype,
+                            int64_t lddx, int64_t N, int64_t D, int64_t M, void* ws, size_t ws_bytes, void* stream);
+
+/* dW = dz^T x: dz (N,M) of `dtype`; x (N,D) of `dtype` (x_kind = dtype) or an 8-bit checkpoint of it (x_kind
+ * SPHIP_INT8 / SPHIP_E4M3, ldx = ldq, x_scales); dW (M,D). */
+size_t sphip_linear_grad_weight_workspace_bytes(int64_t N, int64_t D, int64_t M);
+int sphip_linear_grad_weight(const void* dz, int64_t lddz, int dtype, const void* x, const uint8_t* x_scales, int x_kind,
+                             int64_t ldx, void* dW, int dw_dtype, int64_t lddw, int64_t N, int64_t D, int64_t M, void* ws,
+                             size_t ws_bytes, void* stream);
+
+/* ---------------------------------------------------------------- 8-bit checkpoint of an activation
+ *
+ * x (N,D) as codes (32 ceil(N/32), ldq) and scales (ceil(N/32), ldq), ldq % 16 == 0, 16-byte aligned. 32 consecutive
+ * tokens of one feature share the scale 2^(byte - 127), the smallest that keeps them within 127 (SPHIP_INT8: signed
+ * integers) or 448 (SPHIP_E4M3: 8-bit floats, 4 exponent and 3 mantissa bits), at least
+ * 2^-126 or 2^-117 (the smallest code is a normal number); values are rounded to the nearest code,
+ * ties to even. keep_sign: a non-zero value never becomes zero (smallest code of its sign). A group holding an infinity
+ * or a NaN restores as NaN. Padding rows and columns are written as zero codes.
+ * restore: the values, exact in either dtype. */
+int sphip_checkpoint8_save(const void* x, int dtype, int64_t ldx, int fmt, int keep_sign, uint8_t* codes, uint8_t* scales,
+                           int64_t ldq, int64_t N, int64_t D, void* stream);
+int sphip_checkpoint8_restore(const uint8_t* codes, const uint8_t* scales, int64_t ldq, int fmt, void* out, int dtype,
+                              int64_t ldo, int64_t N, int64_t D, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -15,6 +15,8 @@ LIB_PATH = Path(__file__).resolve().parent / LIB_NAME
 ABI_VERSION = 3
 
 F32, BF16 = 0, 1
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}      # SPHIP_ACT_*
+CODES = {"int8": 16, "e4m3": 17}                                 # SPHIP_INT8 / SPHIP_E4M3
 
 
 SPHIP_EUNSUPPORTED = 2        # include/sparsify_hip.h
@@ -98,6 +100,16 @@ SIGNATURES: dict[str, tuple] = {
     "sphip_transpose": (_I, [_P, _P, _L, _L, _L, _I, _P]),
     "sphip_add": (_I, [_P, _P, _I, _P, _L, _P]),
     "sphip_muon_apply": (_I, [_P, _P, _L, _F, _F, _P, _P]),
+    "sphip_linear_workspace_bytes": (_Z, [_L, _L, _L]),
+    "sphip_linear": (_I, [_P, _L, _P, _L, _I, _P, _I, _I, _P, _I, _L, _P, _I, _L, _P, _I, _L, _L, _L, _L, _P, _Z, _P]),
+    "sphip_linear_grad_preact_workspace_bytes": (_Z, [_L, _L]),
+    "sphip_linear_grad_preact": (_I, [_P, _I, _L, _P, _I, _P, _L, _I, _P, _I, _L, _P, _I, _L, _L, _P, _Z, _P]),
+    "sphip_linear_grad_input_workspace_bytes": (_Z, [_L, _L, _L]),
+    "sphip_linear_grad_input": (_I, [_P, _L, _P, _L, _I, _P, _I, _L, _L, _L, _L, _P, _Z, _P]),
+    "sphip_linear_grad_weight_workspace_bytes": (_Z, [_L, _L, _L]),
+    "sphip_linear_grad_weight": (_I, [_P, _L, _I, _P, _P, _I, _L, _P, _I, _L, _L, _L, _L, _P, _Z, _P]),
+    "sphip_checkpoint8_save": (_I, [_P, _I, _L, _I, _I, _P, _P, _L, _L, _L, _P]),
+    "sphip_checkpoint8_restore": (_I, [_P, _P, _L, _I, _P, _I, _L, _L, _L, _P]),
 }
 
 _lib = None

@@ -1,0 +1,114 @@
+// The dense product's epilogue (linear.hip, linear256.hip, linear_few.hip): y = act(z + b) + r, and the derivative of act
+// for its gradient. Everything in fp32; the store rounds once.
+#pragma once
+#include "common.hpp"
+
+namespace sphip {
+
+// Phi(x) = (1 + erf(x / sqrt 2)) / 2 from the complementary error function of Abramowitz & Stegun 7.1.26:
+// erfc(u) = (a1 t + .. + a5 t^5) exp(-u^2), t = 1 / (1 + p u), u = |x| / sqrt 2, absolute error below 1.5e-7.
+// One exponential, one reciprocal and 6 FMAs: the library's erff is three times as long, and this runs once
+// per output behind a matrix product (67 M outputs of a 16384 x 4096 product: 30 us of VALU work against 80).
+__device__ __forceinline__ float phi_tail(float x, float& e) {
+    const float u = fabsf(x) * 0.70710678118654752f;
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, u, 1.f));
+    e = __expf(-u * u);
+    float p = fmaf(1.061405429f, t, -1.453152027f);
+    p = fmaf(p, t, 1.421413741f);
+    p = fmaf(p, t, -0.284496736f);
+    p = fmaf(p, t, 0.254829592f);
+    return 0.5f * p * t * e;                       // Phi(-|x|)
+}
+
+__device__ __forceinline__ float act_value(float z, int act) {
+    if (act == SPHIP_ACT_RELU) return z > 0.f ? z : (z != z ? z : 0.f);
+    if (act == SPHIP_ACT_SILU) return z * __builtin_amdgcn_rcpf(1.f + __expf(-z));
+    if (act == SPHIP_ACT_GELU) {
+        float e;
+        const float q = phi_tail(z, e);
+        return z * (z > 0.f ? 1.f - q : q);
+    }
+    return z;
+}
+
+__device__ __forceinline__ float act_slope(float z, int act) {
+    if (act == SPHIP_ACT_RELU) return z > 0.f ? 1.f : (z != z ? z : 0.f);
+    if (act == SPHIP_ACT_SILU) {
+        const float s = __builtin_amdgcn_rcpf(1.f + __expf(-z));
+        return s * fmaf(z, 1.f - s, 1.f);
+    }
+    if (act == SPHIP_ACT_GELU) {
+        float e;
+        const float q = phi_tail(z, e);
+        return fmaf(z * e, 0.39894228040143268f, z > 0.f ? 1.f - q : q);
+    }
+    return 1.f;
+}
+
+__device__ __forceinline__ float load_as_f32(const void* p, int dt, int64_t i) {
+    return dt == SPHIP_BF16 ? bf16_to_f32(((const bf16_t*)p)[i]) : ((const float*)p)[i];
+}
+
+struct Epilogue {
+    const void* bias = nullptr;       // (M) or null
+    const void* res = nullptr;        // (N, M), row stride ldr, or null
+    void* out = nullptr;              // (N, M), row stride ldo
+    void* z = nullptr;                // (N, M), row stride ldz, or null: z + b before the activation
+    int64_t ldr = 0, ldo = 0, ldz = 0;
+    int bias_dt = 0, res_dt = 0, out_dt = 0, z_dt = 0;
+    int act = 0;
+    int vec = 0;                      // every row of res / out / z / bias takes 4-element vector accesses
+};
+
+__device__ __forceinline__ void load4_as_f32(const void* p, int dt, int64_t i, float (&v)[4]) {
+    const float4 t = dt == SPHIP_BF16 ? load4((const bf16_t*)p + i) : load4((const float*)p + i);
+    v[0] = t.x, v[1] = t.y, v[2] = t.z, v[3] = t.w;
+}
+__device__ __forceinline__ void store4_from_f32(void* p, int dt, int64_t i, const float (&v)[4]) {
+    if (dt == SPHIP_BF16)
+        *reinterpret_cast<uint2*>((bf16_t*)p + i) =
+            make_uint2((unsigned)f32_to_bf16(v[0]) | ((unsigned)f32_to_bf16(v[1]) << 16),
+                       (unsigned)f32_to_bf16(v[2]) | ((unsigned)f32_to_bf16(v[3]) << 16));
+    else *reinterpret_cast<float4*>((float*)p + i) = make_float4(v[0], v[1], v[2], v[3]);
+}
+__device__ __forceinline__ void store_from_f32(void* p, int dt, int64_t i, float v) {
+    if (dt == SPHIP_BF16) ((bf16_t*)p)[i] = f32_to_bf16(v);
+    else ((float*)p)[i] = v;
+}
+
+// outputs (n, m .. m + 3) of the accumulated product v; columns past M are left alone
+__device__ __forceinline__ void epilogue4(const Epilogue& e, int64_t n, int m, int M, float (&v)[4]) {
+    if (e.vec && m + 3 < M) {
+        if (e.bias != nullptr) {
+            float b[4];
+            load4_as_f32(e.bias, e.bias_dt, m, b);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] += b[j];
+        }
+        if (e.z != nullptr) store4_from_f32(e.z, e.z_dt, n * e.ldz + m, v);
+        if (e.act != SPHIP_ACT_NONE) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = act_value(v[j], e.act);
+        }
+        if (e.res != nullptr) {
+            float r[4];
+            load4_as_f32(e.res, e.res_dt, n * e.ldr + m, r);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] += r[j];
+        }
+        store4_from_f32(e.out, e.out_dt, n * e.ldo + m, v);
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if (m + j >= M) continue;
+        float t = v[j];
+        if (e.bias != nullptr) t += load_as_f32(e.bias, e.bias_dt, m + j);
+        if (e.z != nullptr) store_from_f32(e.z, e.z_dt, n * e.ldz + m + j, t);
+        t = act_value(t, e.act);
+        if (e.res != nullptr) t += load_as_f32(e.res, e.res_dt, n * e.ldr + m + j);
+        store_from_f32(e.out, e.out_dt, n * e.ldo + m + j, t);
+    }
+}
+
+}  // namespace sphip

@@ -1,0 +1,605 @@
+// A dense product with bias, activation and residual in its epilogue, and its gradients:
+//     y = act(x W^T + b) + r           (sphip_linear)
+//     dz = g act'(z), db = sum_n dz    (sphip_linear_grad_preact)
+//     dx = dz W                        (sphip_linear_grad_input)
+//     dW = dz^T x                      (sphip_linear_grad_weight; x as it is or an 8-bit checkpoint of it)
+// The skip connection of a transcoder (sparsify/sparse_coder.py:219-222) is the first user.
+//
+// All three products are C[n, m] = sum_k A(n, k) B(m, k); what differs is which index of an operand is contiguous in
+// memory. The tile kernel here takes any of them, any size, stride and alignment: a 128 x 128 tile of C per workgroup of
+// four waves (2 x 2 of 64 x 64, 32x32 MFMA tiles), 128 bytes of K per step, staged through registers into a double-buffered
+// LDS image [row][8 chunks of 16 bytes of K], chunk index XOR (row >> 1) & 7 (16 lanes of a ds_read_b128 then touch 16
+// bank groups). An operand whose rows are contiguous in K goes in as 16-byte pieces; one whose K stride is the long one is
+// transposed on the way: a thread loads 4 rows x 8 (bf16) or 4 (fp32) consecutive K and interleaves them in registers
+// (v_perm: half an instruction per element), so one LDS image and one inner loop serve every combination.
+// Loads are unaligned-tolerant vectors; only the last chunk of a row or the last rows of a matrix take element loads.
+// Few tiles: the K range is split over workgroups, fp32 partial tiles are joined in a fixed order by a second kernel.
+#include "codes8.hpp"
+#include "epilogue.hpp"
+
+namespace sphip {
+
+typedef __bf16 lbf16x8 __attribute__((ext_vector_type(8)));
+typedef float lf32x2 __attribute__((ext_vector_type(2)));
+typedef float lf32x4 __attribute__((ext_vector_type(4)));
+typedef float lf32x16 __attribute__((ext_vector_type(16)));
+
+// how element (row, k) of an operand is found
+enum { OP_ROWS = 0,      // p[row * ld + k]
+       OP_COLS = 1,      // p[k * ld + row]
+       OP_COLS_I8 = 2,   // 8-bit codes at p[k * ld + row], scale byte at scales[(k / 32) * ld + row] (checkpoint8.hip)
+       OP_COLS_E4M3 = 3 };
+
+struct Operand {
+    const void* p;
+    const uint8_t* scales;
+    int64_t ld;
+    int rows;
+};
+
+constexpr int LT = 128;                 // tile rows of either operand
+constexpr int LCH = 8;                  // 16-byte chunks of K per row and step
+
+__device__ __forceinline__ unsigned pack2(bf16_t lo, bf16_t hi) { return (unsigned)lo | ((unsigned)hi << 16); }
+
+template <typename T> struct Chunk;
+template <> struct Chunk<bf16_t> {
+    static constexpr int E = 8;
+    // n valid elements from p, zeros after
+    static __device__ __forceinline__ uint4 load(const bf16_t* p, int n) {
+        uint4 r = make_uint4(0, 0, 0, 0);
+        if (n >= 8) {
+            __builtin_memcpy(&r, p, 16);
+        } else if (n > 0) {
+            unsigned w[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int j = 0; j < 7; ++j)
+                if (j < n) w[j >> 1] |= (unsigned)p[j] << ((j & 1) * 16);
+            r = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        return r;
+    }
+};
+template <> struct Chunk<float> {
+    static constexpr int E = 4;
+    static __device__ __forceinline__ uint4 load(const float* p, int n) {
+        uint4 r = make_uint4(0, 0, 0, 0);
+        if (n >= 4) {
+            __builtin_memcpy(&r, p, 16);
+        } else if (n > 0) {
+            r.x = __float_as_uint(p[0]);
+            if (n > 1) r.y = __float_as_uint(p[1]);
+            if (n > 2) r.z = __float_as_uint(p[2]);
+        }
+        return r;
+    }
+};
+
+__device__ __forceinline__ int chunk_slot(int row, int ch) { return row * LCH + (ch ^ ((row >> 1) & 7)); }
+
+// One operand's 128 x 128-byte step, 4 chunks per thread (256 threads): fetch() into registers, put() into LDS.
+template <typename T, int MODE> struct Stage;
+
+template <typename T> struct Stage<T, OP_ROWS> {
+    static constexpr int E = Chunk<T>::E;
+    uint4 v[4];
+    __device__ __forceinline__ void fetch(const Operand& a, int row0, int64_t k0, int64_t K, int tid) {
+        const int ch = tid & 7, r = tid >> 3;
+        const int64_t k = k0 + ch * E;
+        const int n = (int)min((int64_t)E, K - k);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int row = row0 + r + 32 * i;
+            v[i] = Chunk<T>::load((const T*)a.p + (int64_t)row * a.ld + k, row < a.rows ? n : 0);
+        }
+    }
+    __device__ __forceinline__ void put(uint4* lds, int tid) const {
+        const int ch = tid & 7, r = tid >> 3;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) lds[chunk_slot(r + 32 * i, ch)] = v[i];
+    }
+};
+
+// thread: rows 4 rg .. 4 rg + 3, K chunk kc
+template <> struct Stage<bf16_t, OP_COLS> {
+    uint2 v[8];
+    __device__ __forceinline__ void fetch(const Operand& a, int row0, int64_t k0, int64_t K, int tid) {
+        const int row = row0 + 4 * (tid & 31), n = a.rows - row;
+        const int64_t k = k0 + (tid >> 5) * 8;
+        const bf16_t* p = (const bf16_t*)a.p + k * a.ld + row;
+#pragma unroll
+        for (int i = 0; i < 8; ++i, p += a.ld) {
+            v[i] = make_uint2(0, 0);
+            if (k + i >= K || n <= 0) continue;
+            if (n >= 4) __builtin_memcpy(&v[i], p, 8);
+            else v[i] = make_uint2((unsigned)p[0] | (n > 1 ? (unsigned)p[1] << 16 : 0u), n > 2 ? (unsigned)p[2] : 0u);
+        }
+    }
+    __device__ __forceinline__ void put(uint4* lds, int tid) const {
+        const int r = 4 * (tid & 31), kc = tid >> 5;
+        // dword of row j holding K (2 i, 2 i + 1): the low (j even) or high halves of two K rows' dwords
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            unsigned w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const unsigned lo = j < 2 ? v[2 * i].x : v[2 * i].y, hi = j < 2 ? v[2 * i + 1].x : v[2 * i + 1].y;
+                w[i] = __builtin_amdgcn_perm(hi, lo, (j & 1) ? 0x07060302u : 0x05040100u);
+            }
+            lds[chunk_slot(r + j, kc)] = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    }
+};
+template <> struct Stage<float, OP_COLS> {
+    uint4 v[4];
+    __device__ __forceinline__ void fetch(const Operand& a, int row0, int64_t k0, int64_t K, int tid) {
+        const int row = row0 + 4 * (tid & 31);
+        const int64_t k = k0 + (tid >> 5) * 4;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            v[i] = Chunk<float>::load((const float*)a.p + (k + i) * a.ld + row, k + i < K ? a.rows - row : 0);
+    }
+    __device__ __forceinline__ void put(uint4* lds, int tid) const {
+        const int r = 4 * (tid & 31), kc = tid >> 5;
+        lds[chunk_slot(r + 0, kc)] = make_uint4(v[0].x, v[1].x, v[2].x, v[3].x);
+        lds[chunk_slot(r + 1, kc)] = make_uint4(v[0].y, v[1].y, v[2].y, v[3].y);
+        lds[chunk_slot(r + 2, kc)] = make_uint4(v[0].z, v[1].z, v[2].z, v[3].z);
+        lds[chunk_slot(r + 3, kc)] = make_uint4(v[0].w, v[1].w, v[2].w, v[3].w);
+    }
+};
+
+template <typename T, int FMT> struct StageCodes {
+    static constexpr int E = Chunk<T>::E;
+    unsigned v[E], s;
+    // ld is a multiple of 16, the code rows are padded to whole 32-token groups (zeros): whole dwords, no partial pieces
+    __device__ __forceinline__ void fetch(const Operand& a, int row0, int64_t k0, int64_t K, int tid) {
+        const int row = row0 + 4 * (tid & 31);
+        const int64_t k = k0 + (tid >> 5) * E;
+        const bool in = row < a.ld && k < K;
+        const uint8_t* p = (const uint8_t*)a.p + k * a.ld + row;
+        s = in ? *reinterpret_cast<const unsigned*>(a.scales + (k >> 5) * a.ld + row) : 0u;
+#pragma unroll
+        for (int i = 0; i < E; ++i, p += a.ld) v[i] = in ? *reinterpret_cast<const unsigned*>(p) : 0u;
+    }
+    __device__ __forceinline__ void put(uint4* lds, int tid) const {
+        const int r = 4 * (tid & 31), kc = tid >> 5;
+        // bytes transposed 4 x 4: w[h][j] holds K 4 h .. 4 h + 3 of row j
+        unsigned w[E / 4][4];
+#pragma unroll
+        for (int h = 0; h < E / 4; ++h) {
+            const unsigned a0 = __builtin_amdgcn_perm(v[4 * h + 1], v[4 * h], 0x05010400u);
+            const unsigned a1 = __builtin_amdgcn_perm(v[4 * h + 1], v[4 * h], 0x07030602u);
+            const unsigned b0 = __builtin_amdgcn_perm(v[4 * h + 3], v[4 * h + 2], 0x05010400u);
+            const unsigned b1 = __builtin_amdgcn_perm(v[4 * h + 3], v[4 * h + 2], 0x07030602u);
+            w[h][0] = __builtin_amdgcn_perm(b0, a0, 0x05040100u), w[h][1] = __builtin_amdgcn_perm(b0, a0, 0x07060302u);
+            w[h][2] = __builtin_amdgcn_perm(b1, a1, 0x05040100u), w[h][3] = __builtin_amdgcn_perm(b1, a1, 0x07060302u);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float sj = scale_value((s >> (8 * j)) & 0xffu);
+            uint4 c;
+            float o[4];
+            code_values<FMT>(w[0][j], sj, o);
+            if constexpr (E == 8) {
+                float q[4];
+                code_values<FMT>(w[1][j], sj, q);
+                // (8-bit codes times a power of two are bf16 values: nothing is rounded)
+                c = make_uint4(pack2(f32_to_bf16(o[0]), f32_to_bf16(o[1])), pack2(f32_to_bf16(o[2]), f32_to_bf16(o[3])),
+                               pack2(f32_to_bf16(q[0]), f32_to_bf16(q[1])), pack2(f32_to_bf16(q[2]), f32_to_bf16(q[3])));
+            } else {
+                c = make_uint4(__float_as_uint(o[0]), __float_as_uint(o[1]), __float_as_uint(o[2]), __float_as_uint(o[3]));
+            }
+            lds[chunk_slot(r + j, kc)] = c;
+        }
+    }
+};
+template <typename T> struct Stage<T, OP_COLS_I8> : StageCodes<T, SPHIP_INT8> {};
+template <typename T> struct Stage<T, OP_COLS_E4M3> : StageCodes<T, SPHIP_E4M3> {};
+
+__device__ __forceinline__ void mma_step(const uint4& a, const uint4& b, lf32x16& c, bf16_t) {
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(lbf16x8, a), __builtin_bit_cast(lbf16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ void mma_step(const uint4& a, const uint4& b, lf32x16& c, float) {
+    // lane half h holds K 4 h + i of an 8-wide K group for MFMA i; both operands agree, the four together sum all 8
+    const lf32x4 fa = __builtin_bit_cast(lf32x4, a), fb = __builtin_bit_cast(lf32x4, b);
+    c = __builtin_amdgcn_mfma_f32_32x32x2f32(fa[0], fb[0], c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x2f32(fa[1], fb[1], c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x2f32(fa[2], fb[2], c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x2f32(fa[3], fb[3], c, 0, 0, 0);
+}
+
+struct TileGrid {
+    int tilesM, tilesN, splits, steps_per;      // steps_per: K steps of one split
+    float* part;                                // [splits][N][Mp] fp32 partial sums, Mp = M rounded up to 4; splits > 1
+};
+
+// B (rows m) is the MFMA's first operand: a lane then holds 4 consecutive m of one n per accumulator quad, i.e. vector
+// stores along a row of C.
+template <typename T, int MODE_A, int MODE_B>
+__global__ __launch_bounds__(256, 2) void linear_tile_kernel(Operand A, Operand B, Epilogue epi, int64_t K, TileGrid g) {
+    constexpr int E = Chunk<T>::E, STEP = LCH * E;
+    __shared__ uint4 lds[2][2][LT * LCH];       // [buffer][B | A]
+
+    // workgroup -> (split, tile): each XCD (workgroup id mod 8) walks a contiguous range, 8-tall bands of tiles
+    const unsigned nb = gridDim.x, xcd = blockIdx.x & 7, slot = blockIdx.x >> 3;
+    const unsigned q8 = nb >> 3, r8 = nb & 7;
+    const unsigned L = (xcd < r8 ? xcd * (q8 + 1) : r8 * (q8 + 1) + (xcd - r8) * q8) + slot;
+    const unsigned tiles = (unsigned)g.tilesM * (unsigned)g.tilesN;
+    const unsigned split = L / tiles, Lt = L % tiles;
+    const unsigned band = 8u * (unsigned)g.tilesN, gi = Lt / band, within = Lt % band;
+    const unsigned gsize = min((unsigned)g.tilesM - gi * 8, 8u);
+    const int m0 = (int)(gi * 8 + within % gsize) * LT, n0 = (int)(within / gsize) * LT;
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int wm = wave >> 1, wn = wave & 1, r = lane & 31, h = lane >> 5;
+    const int step0 = (int)split * g.steps_per;
+    const int steps = min(g.steps_per, (int)((K + STEP - 1) / STEP) - step0);
+
+    Stage<T, MODE_A> sa;
+    Stage<T, MODE_B> sb;
+    lf32x16 acc[2][2];
+#pragma unroll
+    for (int mi = 0; mi < 2; ++mi)
+#pragma unroll
+        for (int ni = 0; ni < 2; ++ni)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) acc[mi][ni][j] = 0.f;
+
+    sb.fetch(B, m0, (int64_t)step0 * STEP, K, tid);
+    sa.fetch(A, n0, (int64_t)step0 * STEP, K, tid);
+    sb.put(lds[0][0], tid);
+    sa.put(lds[0][1], tid);
+    __syncthreads();
+    for (int s = 0; s < steps; ++s) {
+        const int buf = s & 1;
+        if (s + 1 < steps) {
+            sb.fetch(B, m0, (int64_t)(step0 + s + 1) * STEP, K, tid);
+            sa.fetch(A, n0, (int64_t)(step0 + s + 1) * STEP, K, tid);
+        }
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) {
+            uint4 fb[2], fa[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                fb[i] = lds[buf][0][chunk_slot(wm * 64 + i * 32 + r, 2 * ks + h)];
+                fa[i] = lds[buf][1][chunk_slot(wn * 64 + i * 32 + r, 2 * ks + h)];
+            }
+#pragma unroll
+            for (int mi = 0; mi < 2; ++mi)
+#pragma unroll
+                for (int ni = 0; ni < 2; ++ni) mma_step(fb[mi], fa[ni], acc[mi][ni], T{});
+        }
+        if (s + 1 < steps) {
+            sb.put(lds[buf ^ 1][0], tid);
+            sa.put(lds[buf ^ 1][1], tid);
+        }
+        __syncthreads();
+    }
+
+    const int N = A.rows, M = B.rows;
+    const int Mp = (M + 3) & ~3;
+#pragma unroll
+    for (int mi = 0; mi < 2; ++mi)
+#pragma unroll
+        for (int qd = 0; qd < 4; ++qd) {
+            const int m = m0 + wm * 64 + mi * 32 + 8 * qd + 4 * h;
+            if (m >= M) continue;
+#pragma unroll
+            for (int ni = 0; ni < 2; ++ni) {
+                const int n = n0 + wn * 64 + ni * 32 + r;
+                if (n >= N) continue;
+                float v[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] = acc[mi][ni][4 * qd + j];
+                if (g.splits > 1)
+                    *reinterpret_cast<float4*>(g.part + ((int64_t)split * N + n) * Mp + m) = make_float4(v[0], v[1], v[2], v[3]);
+                else epilogue4(epi, n, m, M, v);
+            }
+        }
+}
+
+// Sum of the splits' partial tiles in split order, then the epilogue. One thread per 4 outputs.
+__global__ __launch_bounds__(256) void linear_join_kernel(const float* __restrict__ part, Epilogue epi, int64_t N, int M,
+                                                          int splits) {
+    const int quads = (M + 3) >> 2;
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= N * quads) return;
+    const int64_t n = i / quads, stride = N * quads * 4;
+    const int m = (int)(i % quads) * 4;
+    const float* p = part + i * 4;
+    float4 t = load4(p);
+    float v[4] = {t.x, t.y, t.z, t.w};
+    for (int s = 1; s < splits; ++s) {
+        t = load4(p + s * stride);
+        v[0] += t.x, v[1] += t.y, v[2] += t.z, v[3] += t.w;
+    }
+    epilogue4(epi, n, m, M, v);
+}
+
+// How many ways the K range of an (N, M) product of `steps` K steps is split: none when the tiles fill the 256 compute
+// units once, else towards two workgroups per unit, at least 4 steps each.
+static int split_count(int64_t N, int64_t M, int64_t steps) {
+    const int64_t tiles = cdiv(N, LT) * cdiv(M, LT);
+    if (tiles >= 256) return 1;
+    int64_t s = cdiv(512, tiles);
+    if (s > steps / 4) s = steps / 4;
+    return s < 1 ? 1 : (int)s;
+}
+static size_t split_bytes(int64_t N, int64_t M, int64_t K) {
+    // (a K step is 64 bf16 or 32 fp32 elements: the latter has more steps and so at least as many splits)
+    const int s = split_count(N, M, cdiv(K, 32));
+    return s > 1 ? (size_t)s * N * ((M + 3) / 4 * 4) * 4 : 0;
+}
+
+template <typename T, int MODE_A, int MODE_B>
+static int launch_tiles(const char* what, const Operand& A, const Operand& B, const Epilogue& epi, int64_t K, void* ws,
+                        size_t ws_bytes, hipStream_t s) {
+    constexpr int STEP = LCH * Chunk<T>::E;
+    const int64_t N = A.rows, M = B.rows, steps = cdiv(K, STEP);
+    TileGrid g;
+    g.tilesM = (int)cdiv(M, LT), g.tilesN = (int)cdiv(N, LT);
+    const int want = split_count(N, M, steps);
+    g.steps_per = (int)cdiv(steps, want);
+    g.splits = (int)cdiv(steps, g.steps_per);
+    g.part = (float*)ws;
+    if (g.splits > 1) {
+        const size_t need = (size_t)g.splits * N * ((M + 3) / 4 * 4) * 4;
+        SPHIP_REQUIRE(ws != nullptr && ws_bytes >= need && ((uintptr_t)ws & 15) == 0, SPHIP_EWORKSPACE,
+                      "%s: workspace of %zu bytes, needs %zu, 16-byte aligned", what, ws_bytes, need);
+    }
+    const int64_t nblocks = (int64_t)g.tilesM * g.tilesN * g.splits;
+    SPHIP_REQUIRE(nblocks < (1ll << 31), SPHIP_EUNSUPPORTED, "%s: grid too large", what);
+    hipLaunchKernelGGL((linear_tile_kernel<T, MODE_A, MODE_B>), dim3((unsigned)nblocks), dim3(256), 0, s, A, B, epi, K, g);
+    SPHIP_CHECK_LAUNCH(what);
+    if (g.splits > 1) {
+        const int64_t threads = N * ((M + 3) / 4);
+        SPHIP_REQUIRE(cdiv(threads, 256) < (1ll << 31), SPHIP_EUNSUPPORTED, "%s: grid too large", what);
+        hipLaunchKernelGGL(linear_join_kernel, dim3((unsigned)cdiv(threads, 256)), dim3(256), 0, s, g.part, epi, N, (int)M,
+                           g.splits);
+        SPHIP_CHECK_LAUNCH(what);
+    }
+    return SPHIP_OK;
+}
+
+static inline bool aligned4(const void* p, int dt, int64_t ld) {
+    return ((uintptr_t)p % (4 * dtype_size(dt))) == 0 && ld % 4 == 0;
+}
+static void set_vec(Epilogue& e) {
+    e.vec = aligned4(e.out, e.out_dt, e.ldo) && (e.bias == nullptr || aligned4(e.bias, e.bias_dt, 0)) &&
+            (e.res == nullptr || aligned4(e.res, e.res_dt, e.ldr)) && (e.z == nullptr || aligned4(e.z, e.z_dt, e.ldz));
+}
+
+// ---- dz = g act'(z) and its column sums. A thread owns 4 columns of one 32-row group (the group one scale of an 8-bit
+// z covers); its 32 rows' sum goes to part[group][M], added up in group order by the second kernel.
+struct PreactArgs {
+    const void* g;
+    const void* z;                 // values (z_kind = a dtype) or codes (SPHIP_INT8 / SPHIP_E4M3), row stride ldz
+    const uint8_t* scales;
+    void* dz;                      // row stride lddz (zeros in [M, lddz)), or null
+    float* part;                   // [ceil(N / 32)][M], or null
+    int64_t ldg, ldz, lddz;
+    int g_dt, z_kind, dz_dt, act, vec;
+};
+
+__global__ __launch_bounds__(256) void linear_preact_kernel(PreactArgs a, int64_t N, int M) {
+    const int quads = (int)(a.dz != nullptr ? a.lddz : (M + 3)) >> 2;
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t grp = i / quads;
+    const int m = (int)(i % quads) * 4;
+    if (grp * 32 >= N) return;
+    const int n_rows = (int)min((int64_t)32, N - grp * 32);
+    const int cols = min(4, M - m);                        // <= 0: padding columns of dz
+    float sc[4] = {0.f, 0.f, 0.f, 0.f}, sum[4] = {0.f, 0.f, 0.f, 0.f};
+    const bool codes = a.z_kind >= SPHIP_INT8 && a.act != SPHIP_ACT_NONE;
+    if (codes && cols > 0) {
+        const unsigned s4 = *reinterpret_cast<const unsigned*>(a.scales + grp * a.ldz + m);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sc[j] = scale_value((s4 >> (8 * j)) & 0xffu);
+    }
+#pragma unroll 4
+    for (int t = 0; t < n_rows; ++t) {
+        const int64_t n = grp * 32 + t;
+        float v[4] = {0.f, 0.f, 0.f, 0.f}, z[4] = {0.f, 0.f, 0.f, 0.f};
+        if (cols == 4 && a.vec) {
+            load4_as_f32(a.g, a.g_dt, n * a.ldg + m, v);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (j < cols) v[j] = load_as_f32(a.g, a.g_dt, n * a.ldg + m + j);
+        }
+        if (a.act != SPHIP_ACT_NONE) {
+            if (codes) {
+                if (cols > 0) {
+                    const unsigned w = *reinterpret_cast<const unsigned*>((const uint8_t*)a.z + n * a.ldz + m);
+                    if (a.z_kind == SPHIP_INT8) code_values<SPHIP_INT8>(w, sc, z);
+                    else code_values<SPHIP_E4M3>(w, sc, z);
+                }
+            } else if (cols == 4 && a.vec) {
+                load4_as_f32(a.z, a.z_kind, n * a.ldz + m, z);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (j < cols) z[j] = load_as_f32(a.z, a.z_kind, n * a.ldz + m + j);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (j < cols) v[j] *= act_slope(z[j], a.act);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sum[j] += v[j];
+        if (a.dz != nullptr) store4_from_f32(a.dz, a.dz_dt, n * a.lddz + m, v);
+    }
+    if (a.part != nullptr)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (j < cols) a.part[grp * M + m + j] = sum[j];
+}
+
+// column sums of part (P, M) in row order by 16 interleaved chains: 64 columns per workgroup of 1024 threads
+__global__ __launch_bounds__(1024) void linear_bias_grad_kernel(const float* __restrict__ part, int64_t P, int M, void* db, int dt) {
+    __shared__ float red[16][64];
+    const int c = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int m = blockIdx.x * 64 + c;
+    float s = 0.f;
+    if (m < M)
+        for (int64_t p = w; p < P; p += 16) s += part[p * M + m];
+    red[w][c] = s;
+    __syncthreads();
+    if (w == 0 && m < M) {
+        float t = 0.f;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) t += red[j][c];
+        store_from_f32(db, dt, m, t);
+    }
+}
+
+static bool valid_act(int act) { return act >= SPHIP_ACT_NONE && act <= SPHIP_ACT_SILU; }
+static bool aligned_elem(const void* p, int dt) { return ((uintptr_t)p & (dtype_size(dt) - 1)) == 0; }
+
+}  // namespace sphip
+
+#define SPHIP_LINEAR_SIZES(what)                                                                                        \
+    SPHIP_REQUIRE(N > 0 && D > 0 && M > 0, SPHIP_EINVAL, what ": empty shape N=%lld D=%lld M=%lld", (long long)N,        \
+                  (long long)D, (long long)M);                                                                          \
+    SPHIP_REQUIRE(N < (1ll << 31) - 256 && D < (1ll << 31) - 256 && M < (1ll << 31) - 256, SPHIP_EUNSUPPORTED,           \
+                  what ": dimension exceeds int32")
+
+extern "C" size_t sphip_linear_workspace_bytes(int64_t N, int64_t D, int64_t M) {
+    if (N <= 0 || D <= 0 || M <= 0) return 0;
+    return sphip::split_bytes(N, M, D);
+}
+
+extern "C" int sphip_linear(const void* x, int64_t ldx, const void* W, int64_t ldw, int dtype, const void* bias,
+                            int bias_dtype, int act, const void* residual, int res_dtype, int64_t ldr, void* out,
+                            int out_dtype, int64_t ldo, void* z, int z_dtype, int64_t ldz, int64_t N, int64_t D, int64_t M,
+                            void* ws, size_t ws_bytes, void* stream) {
+    using namespace sphip;
+    SPHIP_REQUIRE(valid_dtype(dtype) && valid_dtype(out_dtype) && (!bias || valid_dtype(bias_dtype)) &&
+                      (!residual || valid_dtype(res_dtype)) && (!z || valid_dtype(z_dtype)),
+                  SPHIP_EINVAL, "linear: bad dtype");
+    SPHIP_REQUIRE(valid_act(act), SPHIP_EINVAL, "linear: bad activation %d", act);
+    SPHIP_REQUIRE(x && W && out, SPHIP_EINVAL, "linear: null pointer");
+    SPHIP_LINEAR_SIZES("linear");
+    SPHIP_REQUIRE(ldx >= D && ldw >= D && ldo >= M && (!residual || ldr >= M) && (!z || ldz >= M), SPHIP_EINVAL,
+                  "linear: a row stride is shorter than its row");
+    SPHIP_REQUIRE(aligned_elem(x, dtype) && aligned_elem(W, dtype) && aligned_elem(out, out_dtype) &&
+                      (!bias || aligned_elem(bias, bias_dtype)) && (!residual || aligned_elem(residual, res_dtype)) &&
+                      (!z || aligned_elem(z, z_dtype)),
+                  SPHIP_EINVAL, "linear: a pointer is not aligned to its element");
+    Epilogue e;
+    e.bias = bias, e.bias_dt = bias_dtype, e.res = residual, e.res_dt = res_dtype, e.ldr = ldr;
+    e.out = out, e.out_dt = out_dtype, e.ldo = ldo, e.z = z, e.z_dt = z_dtype, e.ldz = ldz, e.act = act;
+    set_vec(e);
+    const Operand A = {x, nullptr, ldx, (int)N}, B = {W, nullptr, ldw, (int)M};
+    if (dtype == SPHIP_BF16)
+        return launch_tiles<bf16_t, OP_ROWS, OP_ROWS>("linear", A, B, e, D, ws, ws_bytes, (hipStream_t)stream);
+    return launch_tiles<float, OP_ROWS, OP_ROWS>("linear", A, B, e, D, ws, ws_bytes, (hipStream_t)stream);
+}
+
+extern "C" size_t sphip_linear_grad_preact_workspace_bytes(int64_t N, int64_t M) {
+    return N > 0 && M > 0 ? (size_t)sphip::cdiv(N, 32) * M * 4 : 0;
+}
+
+extern "C" int sphip_linear_grad_preact(const void* g, int g_dtype, int64_t ldg, const void* z, int z_kind,
+                                        const uint8_t* z_scales, int64_t ldz, int act, void* dz, int dz_dtype,
+                                        int64_t lddz, void* db, int db_dtype, int64_t N, int64_t M, void* ws,
+                                        size_t ws_bytes, void* stream) {
+    using namespace sphip;
+    SPHIP_REQUIRE(valid_dtype(g_dtype) && (!dz || valid_dtype(dz_dtype)) && (!db || valid_dtype(db_dtype)), SPHIP_EINVAL,
+                  "linear_grad_preact: bad dtype");
+    SPHIP_REQUIRE(valid_act(act), SPHIP_EINVAL, "linear_grad_preact: bad activation %d", act);
+    SPHIP_REQUIRE(g && (dz || db), SPHIP_EINVAL, "linear_grad_preact: null pointer");
+    SPHIP_REQUIRE(N > 0 && M > 0 && N < (1ll << 31) - 256 && M < (1ll << 31) - 256, SPHIP_EINVAL,
+                  "linear_grad_preact: bad shape N=%lld M=%lld", (long long)N, (long long)M);
+    const bool codes = z_kind == SPHIP_INT8 || z_kind == SPHIP_E4M3;
+    if (act != SPHIP_ACT_NONE) {
+        SPHIP_REQUIRE(z && (codes ? z_scales != nullptr : valid_dtype(z_kind)), SPHIP_EINVAL,
+                      "linear_grad_preact: an activation needs z (values, or codes with scales)");
+        SPHIP_REQUIRE(ldz >= M && (!codes || (ldz % 16 == 0 && ((uintptr_t)z & 3) == 0 && ((uintptr_t)z_scales & 3) == 0)),
+                      SPHIP_EINVAL, "linear_grad_preact: bad row stride or alignment of z");
+    }
+    SPHIP_REQUIRE(ldg >= M && (!dz || (lddz >= M && lddz % 4 == 0)), SPHIP_EINVAL, "linear_grad_preact: bad row stride");
+    SPHIP_REQUIRE(aligned_elem(g, g_dtype) && (!dz || ((uintptr_t)dz & 15) == 0) && (!db || aligned_elem(db, db_dtype)) &&
+                      (act == SPHIP_ACT_NONE || codes || aligned_elem(z, z_kind)),
+                  SPHIP_EINVAL, "linear_grad_preact: misaligned pointer");
+    const int64_t P = cdiv(N, 32);
+    if (db) {
+        const size_t need = (size_t)P * M * 4;
+        SPHIP_REQUIRE(ws && ws_bytes >= need && ((uintptr_t)ws & 15) == 0, SPHIP_EWORKSPACE,
+                      "linear_grad_preact: workspace of %zu bytes, needs %zu, 16-byte aligned", ws_bytes, need);
+    }
+    PreactArgs a;
+    a.g = g, a.z = z, a.scales = z_scales, a.dz = dz, a.part = db ? (float*)ws : nullptr;
+    a.ldg = ldg, a.ldz = ldz, a.lddz = lddz, a.g_dt = g_dtype, a.z_kind = z_kind, a.dz_dt = dz_dtype, a.act = act;
+    a.vec = aligned4(g, g_dtype, ldg) && (act == SPHIP_ACT_NONE || codes || aligned4(z, z_kind, ldz));
+    const int64_t quads = (dz ? lddz : M + 3) / 4, blocks = cdiv(P * quads, 256);
+    SPHIP_REQUIRE(blocks < (1ll << 31), SPHIP_EUNSUPPORTED, "linear_grad_preact: grid too large");
+    hipStream_t s = (hipStream_t)stream;
+    hipLaunchKernelGGL(linear_preact_kernel, dim3((unsigned)blocks), dim3(256), 0, s, a, N, (int)M);
+    SPHIP_CHECK_LAUNCH("linear_grad_preact");
+    if (db) {
+        hipLaunchKernelGGL(linear_bias_grad_kernel, dim3((unsigned)cdiv(M, 64)), dim3(1024), 0, s, (const float*)ws, P, (int)M,
+                           db, db_dtype);
+        SPHIP_CHECK_LAUNCH("linear_grad_preact(db)");
+    }
+    return SPHIP_OK;
+}
+
+extern "C" size_t sphip_linear_grad_input_workspace_bytes(int64_t N, int64_t D, int64_t M) {
+    if (N <= 0 || D <= 0 || M <= 0) return 0;
+    return sphip::split_bytes(N, D, M);
+}
+
+extern "C" int sphip_linear_grad_input(const void* dz, int64_t lddz, const void* W, int64_t ldw, int dtype, void* dx,
+                                       int dx_dtype, int64_t lddx, int64_t N, int64_t D, int64_t M, void* ws,
+                                       size_t ws_bytes, void* stream) {
+    using namespace sphip;
+    SPHIP_REQUIRE(valid_dtype(dtype) && valid_dtype(dx_dtype), SPHIP_EINVAL, "linear_grad_input: bad dtype");
+    SPHIP_REQUIRE(dz && W && dx, SPHIP_EINVAL, "linear_grad_input: null pointer");
+    SPHIP_LINEAR_SIZES("linear_grad_input");
+    SPHIP_REQUIRE(lddz >= M && ldw >= D && lddx >= D, SPHIP_EINVAL, "linear_grad_input: a row stride is shorter than its row");
+    SPHIP_REQUIRE(aligned_elem(dz, dtype) && aligned_elem(W, dtype) && aligned_elem(dx, dx_dtype), SPHIP_EINVAL,
+                  "linear_grad_input: a pointer is not aligned to its element");
+    Epilogue e;
+    e.out = dx, e.out_dt = dx_dtype, e.ldo = lddx;
+    set_vec(e);
+    const Operand A = {dz, nullptr, lddz, (int)N}, B = {W, nullptr, ldw, (int)D};
+    if (dtype == SPHIP_BF16)
+        return launch_tiles<bf16_t, OP_ROWS, OP_COLS>("linear_grad_input", A, B, e, M, ws, ws_bytes, (hipStream_t)stream);
+    return launch_tiles<float, OP_ROWS, OP_COLS>("linear_grad_input", A, B, e, M, ws, ws_bytes, (hipStream_t)stream);
+}
+
+extern "C" size_t sphip_linear_grad_weight_workspace_bytes(int64_t N, int64_t D, int64_t M) {
+    if (N <= 0 || D <= 0 || M <= 0) return 0;
+    return sphip::split_bytes(M, D, N);
+}
+
+extern "C" int sphip_linear_grad_weight(const void* dz, int64_t lddz, int dtype, const void* x, const uint8_t* x_scales,
+                                        int x_kind, int64_t ldx, void* dW, int dw_dtype, int64_t lddw, int64_t N, int64_t D,
+                                        int64_t M, void* ws, size_t ws_bytes, void* stream) {
+    using namespace sphip;
+    SPHIP_REQUIRE(valid_dtype(dtype) && valid_dtype(dw_dtype), SPHIP_EINVAL, "linear_grad_weight: bad dtype");
+    const bool codes = x_kind == SPHIP_INT8 || x_kind == SPHIP_E4M3;
+    SPHIP_REQUIRE(codes || x_kind == dtype, SPHIP_EINVAL, "linear_grad_weight: x must be of dz's type or 8-bit codes");
+    SPHIP_REQUIRE(dz && x && dW && (!codes || x_scales), SPHIP_EINVAL, "linear_grad_weight: null pointer");
+    SPHIP_LINEAR_SIZES("linear_grad_weight");
+    SPHIP_REQUIRE(lddz >= M && ldx >= D && lddw >= D, SPHIP_EINVAL, "linear_grad_weight: a row stride is shorter than its row");
+    SPHIP_REQUIRE(!codes || (ldx % 16 == 0 && ((uintptr_t)x & 15) == 0 && ((uintptr_t)x_scales & 15) == 0), SPHIP_EINVAL,
+                  "linear_grad_weight: codes need 16-byte aligned rows");
+    SPHIP_REQUIRE(aligned_elem(dz, dtype) && (codes || aligned_elem(x, dtype)) && aligned_elem(dW, dw_dtype), SPHIP_EINVAL,
+                  "linear_grad_weight: a pointer is not aligned to its element");
+    Epilogue e;
+    e.out = dW, e.out_dt = dw_dtype, e.ldo = lddw;
+    set_vec(e);
+    const Operand A = {dz, nullptr, lddz, (int)M}, B = {x, x_scales, ldx, (int)D};
+    hipStream_t s = (hipStream_t)stream;
+    const char* what = "linear_grad_weight";
+    if (dtype == SPHIP_BF16) {
+        if (x_kind == SPHIP_INT8) return launch_tiles<bf16_t, OP_COLS, OP_COLS_I8>(what, A, B, e, N, ws, ws_bytes, s);
+        if (x_kind == SPHIP_E4M3) return launch_tiles<bf16_t, OP_COLS, OP_COLS_E4M3>(what, A, B, e, N, ws, ws_bytes, s);
+        return launch_tiles<bf16_t, OP_COLS, OP_COLS>(what, A, B, e, N, ws, ws_bytes, s);
+    }
+    if (x_kind == SPHIP_INT8) return launch_tiles<float, OP_COLS, OP_COLS_I8>(what, A, B, e, N, ws, ws_bytes, s);
+    if (x_kind == SPHIP_E4M3) return launch_tiles<float, OP_COLS, OP_COLS_E4M3>(what, A, B, e, N, ws, ws_bytes, s);
+    return launch_tiles<float, OP_COLS, OP_COLS>(what, A, B, e, N, ws, ws_bytes, s);
+}
