@@ -528,33 +528,27 @@ enum { SPHIP_ACT_NONE = 0, SPHIP_ACT_RELU = 1, SPHIP_ACT_GELU = 2 /* z Phi(z) */
 enum { SPHIP_INT8 = 16, SPHIP_E4M3 = 17 };
 
 /* out = act(x W^T + bias) + residual. x (N,D) and W (M,D) of `dtype`; bias (M), residual (N,M) or NULL; out (N,M).
- * z, or NULL: receives x W^T + bias (before the activation) for the gradient. out may be residual (same stride and
- * type); it may not overlap x or W. */
-size_t sphip_linear_workspace_bytes(int64_t N, int64_t D, int64_t M);
+ * What a gradient will need, or NULL: z = x W^T + bias (before the activation) as values (z_kind a dtype) or, rounded once
+ * from the fp32 sums, as an 8-bit checkpoint with scales (z_kind SPHIP_INT8 / SPHIP_E4M3, keep_sign for a ReLU);
+ * x_codes / x_scales: the 8-bit checkpoint of x (format x_fmt, row stride ldq).
+ * out may be residual (same stride and type); no other output may overlap an input. */
+size_t sphip_linear_workspace_bytes(int dtype, int z_kind, int64_t N, int64_t D, int64_t M);
 int sphip_linear(const void* x, int64_t ldx, const void* W, int64_t ldw, int dtype, const void* bias, int bias_dtype,
                  int act, const void* residual, int res_dtype, int64_t ldr, void* out, int out_dtype, int64_t ldo,
-                 void* z, int z_dtype, int64_t ldz, int64_t N, int64_t D, int64_t M, void* ws, size_t ws_bytes,
-                 void* stream);
+                 void* z, int z_kind, uint8_t* z_scales, int64_t ldz, uint8_t* x_codes, uint8_t* x_scales, int x_fmt,
+                 int64_t ldq, int64_t N, int64_t D, int64_t M, void* ws, size_t ws_bytes, void* stream);
 
-/* dz = g act'(z) (N,M) and db = its column sums (M); either may be NULL. z: values (z_kind a dtype) or codes with
- * scales (z_kind SPHIP_INT8 / SPHIP_E4M3, ldz their row stride); ignored for SPHIP_ACT_NONE. lddz % 4 == 0, dz 16-byte aligned;
- * columns [M, lddz) of dz are written as zeros. db sums the unrounded products, in a fixed order. */
-size_t sphip_linear_grad_preact_workspace_bytes(int64_t N, int64_t M);
-int sphip_linear_grad_preact(const void* g, int g_dtype, int64_t ldg, const void* z, int z_kind, const uint8_t* z_scales,
-                             int64_t ldz, int act, void* dz, int dz_dtype, int64_t lddz, void* db, int db_dtype, int64_t N,
-                             int64_t M, void* ws, size_t ws_bytes, void* stream);
-
-/* dx = dz W: dz (N,M) and W (M,D) of `dtype`, dx (N,D). */
-size_t sphip_linear_grad_input_workspace_bytes(int64_t N, int64_t D, int64_t M);
-int sphip_linear_grad_input(const void* dz, int64_t lddz, const void* W, int64_t ldw, int dtype, void* dx, int dx_dtype,
-                            int64_t lddx, int64_t N, int64_t D, int64_t M, void* ws, size_t ws_bytes, void* stream);
-
-/* dW = dz^T x: dz (N,M) of `dtype`; x (N,D) of `dtype` (x_kind = dtype) or an 8-bit checkpoint of it (x_kind
- * SPHIP_INT8 / SPHIP_E4M3, ldx = ldq, x_scales); dW (M,D). */
-size_t sphip_linear_grad_weight_workspace_bytes(int64_t N, int64_t D, int64_t M);
-int sphip_linear_grad_weight(const void* dz, int64_t lddz, int dtype, const void* x, const uint8_t* x_scales, int x_kind,
-                             int64_t ldx, void* dW, int dw_dtype, int64_t lddw, int64_t N, int64_t D, int64_t M, void* ws,
-                             size_t ws_bytes, void* stream);
+/* Its gradients from g = dL/dout (N,M): dz = g act'(z), dx = dz W (N,D), dW = dz^T x (M,D), db = column sums of the
+ * unrounded dz (M); any of dx, dW, db may be NULL, and W (for dx), x (for dW), z (SPHIP_ACT_NONE) then are not read.
+ * dz is rounded once to `dtype`, the products' type (that of W). z and x: values (z_kind a dtype, x_kind = dtype) or
+ * 8-bit checkpoints with scales. The residual's gradient is g. Sums have a fixed order. */
+size_t sphip_linear_backward_workspace_bytes(int dtype, int x_kind, int want_dx, int want_dw, int want_db, int64_t N,
+                                             int64_t D, int64_t M);
+int sphip_linear_backward(const void* g, int g_dtype, int64_t ldg, const void* W, int64_t ldw, int dtype, int act,
+                          const void* z, int z_kind, const uint8_t* z_scales, int64_t ldz, const void* x, int x_kind,
+                          const uint8_t* x_scales, int64_t ldx, void* dx, int dx_dtype, int64_t lddx, void* dW, int dw_dtype,
+                          int64_t lddw, void* db, int db_dtype, int64_t N, int64_t D, int64_t M, void* ws, size_t ws_bytes,
+                          void* stream);
 
 /* ---------------------------------------------------------------- 8-bit checkpoint of an activation
  *

@@ -1,7 +1,7 @@
 """8-bit checkpoints: what a backward pass keeps of an activation, in half (bf16) or a quarter (fp32) of its bytes.
 
 32 consecutive tokens of one feature share a power-of-two scale: the large values of a residual stream sit in a few
-features at nearly all tokens, so a group holds values of one size. ``"int8"`` rounds to 255 even steps (at most 1/128 of
+features at nearly all tokens, so a group holds values of one size. ``"int8"`` rounds to 255 even steps (at most 1/127 of
 the group's largest value off), ``"e4m3"`` to 8-bit floats with 4 exponent bits (at most 2^-4 of each value off). Values
 times scales are exact in bf16 and fp32. A group that holds an infinity or a NaN restores as NaN."""
 from __future__ import annotations
@@ -14,12 +14,14 @@ from . import ops
 
 class Checkpoint8:
     """An activation held in 8 bits: ``checkpoint8(x, fmt)``, read back by ``restore()`` or, without being restored, by
-    the gradients of ``fused_linear(..., checkpoint=...)`` and of the encoder (``SparseCoder.checkpoint``)."""
+    the gradients of ``fused_linear(..., checkpoint=...)``.
 
-    __slots__ = ("codes", "scales", "fmt", "shape", "dtype")
+    data: the buffer ops.checkpoint8_save writes; fmt: "int8" / "e4m3"; shape, dtype: of what was saved."""
 
-    def __init__(self, codes: Tensor, scales: Tensor, fmt: str, shape: torch.Size, dtype: torch.dtype):
-        self.codes, self.scales, self.fmt, self.shape, self.dtype = codes, scales, fmt, torch.Size(shape), dtype
+    __slots__ = ("data", "fmt", "shape", "dtype")
+
+    def __init__(self, data: Tensor, fmt: str, shape: torch.Size, dtype: torch.dtype):
+        self.data, self.fmt, self.shape, self.dtype = data, fmt, torch.Size(shape), dtype
 
     @property
     def columns(self) -> int:
@@ -31,16 +33,16 @@ class Checkpoint8:
 
     @property
     def device(self) -> torch.device:
-        return self.codes.device
+        return self.data.device
 
     @property
     def nbytes(self) -> int:
-        return self.codes.numel() + self.scales.numel()
+        return self.data.numel()
 
     def restore(self, dtype: torch.dtype | None = None) -> Tensor:
         """The values the codes stand for, in the dtype of what was saved or another one (exact in fp32 and bf16)."""
-        return ops.checkpoint8_restore(self.codes, self.scales, self.fmt, self.rows, self.columns,
-                                       self.dtype if dtype is None else dtype).reshape(self.shape)
+        out = ops.checkpoint8_restore(self.data, self.fmt, self.rows, self.columns, self.dtype if dtype is None else dtype)
+        return out if len(self.shape) == 2 else out.reshape(self.shape)
 
 
 def checkpoint8(x: Tensor, fmt: str = "int8", *, keep_sign: bool = False) -> Checkpoint8:
@@ -48,13 +50,12 @@ def checkpoint8(x: Tensor, fmt: str = "int8", *, keep_sign: bool = False) -> Che
     fmt: "int8" or "e4m3". keep_sign: a value other than zero never becomes zero (a ReLU's mask survives)."""
     if x.ndim < 1:
         raise ValueError("checkpoint8: expected (..., D), got a scalar")
-    codes, scales = ops.checkpoint8_save(as_rows(x.detach()), fmt, keep_sign)
-    return Checkpoint8(codes, scales, fmt, x.shape, x.dtype)
+    return Checkpoint8(ops.checkpoint8_save(as_rows(x), fmt, keep_sign), fmt, x.shape, x.dtype)
 
 
 def as_rows(t: Tensor) -> Tensor:
-    """(..., D) as (tokens, D) with columns next to each other: a view where the strides allow one."""
-    t = t.reshape(t.shape[:-1].numel(), t.shape[-1])
-    if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
-        t = t.contiguous()
-    return t
+    """(..., D) as (tokens, D) with columns next to each other: a view where the strides allow one. Detached."""
+    t = t.detach()
+    if t.ndim != 2:
+        t = t.reshape(t.shape[:-1].numel(), t.shape[-1])
+    return t if ops.is_rows(t) else t.contiguous()

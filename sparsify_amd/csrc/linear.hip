@@ -1,8 +1,7 @@
 // A dense product with bias, activation and residual in its epilogue, and its gradients:
-//     y = act(x W^T + b) + r           (sphip_linear)
-//     dz = g act'(z), db = sum_n dz    (sphip_linear_grad_preact)
-//     dx = dz W                        (sphip_linear_grad_input)
-//     dW = dz^T x                      (sphip_linear_grad_weight; x as it is or an 8-bit checkpoint of it)
+//     y = act(x W^T + b) + r                                            (sphip_linear)
+//     dz = g act'(z), db = sum_n dz, dx = dz W, dW = dz^T x             (sphip_linear_backward)
+// x and z as they are or as 8-bit checkpoints (checkpoint8.hip).
 // The skip connection of a transcoder (sparsify/sparse_coder.py:219-222) is the first user.
 //
 // All three products are C[n, m] = sum_k A(n, k) B(m, k); what differs is which index of an operand is contiguous in
@@ -14,8 +13,7 @@
 // (v_perm: half an instruction per element), so one LDS image and one inner loop serve every combination.
 // Loads are unaligned-tolerant vectors; only the last chunk of a row or the last rows of a matrix take element loads.
 // Few tiles: the K range is split over workgroups, fp32 partial tiles are joined in a fixed order by a second kernel.
-#include "codes8.hpp"
-#include "epilogue.hpp"
+#include "linear.hpp"
 
 namespace sphip {
 
@@ -23,19 +21,6 @@ typedef __bf16 lbf16x8 __attribute__((ext_vector_type(8)));
 typedef float lf32x2 __attribute__((ext_vector_type(2)));
 typedef float lf32x4 __attribute__((ext_vector_type(4)));
 typedef float lf32x16 __attribute__((ext_vector_type(16)));
-
-// how element (row, k) of an operand is found
-enum { OP_ROWS = 0,      // p[row * ld + k]
-       OP_COLS = 1,      // p[k * ld + row]
-       OP_COLS_I8 = 2,   // 8-bit codes at p[k * ld + row], scale byte at scales[(k / 32) * ld + row] (checkpoint8.hip)
-       OP_COLS_E4M3 = 3 };
-
-struct Operand {
-    const void* p;
-    const uint8_t* scales;
-    int64_t ld;
-    int rows;
-};
 
 constexpr int LT = 128;                 // tile rows of either operand
 constexpr int LCH = 8;                  // 16-byte chunks of K per row and step
@@ -208,28 +193,17 @@ __device__ __forceinline__ void mma_step(const uint4& a, const uint4& b, lf32x16
     c = __builtin_amdgcn_mfma_f32_32x32x2f32(fa[3], fb[3], c, 0, 0, 0);
 }
 
-struct TileGrid {
-    int tilesM, tilesN, splits, steps_per;      // steps_per: K steps of one split
-    float* part;                                // [splits][N][Mp] fp32 partial sums, Mp = M rounded up to 4; splits > 1
-};
-
 // B (rows m) is the MFMA's first operand: a lane then holds 4 consecutive m of one n per accumulator quad, i.e. vector
 // stores along a row of C.
 template <typename T, int MODE_A, int MODE_B>
-__global__ __launch_bounds__(256, 2) void linear_tile_kernel(Operand A, Operand B, Epilogue epi, int64_t K, TileGrid g) {
+__global__ __launch_bounds__(256, 2) void linear_tile_kernel(Operand A, Operand B, Epilogue epi, int64_t K, int64_t KB, TileGrid g) {
     constexpr int E = Chunk<T>::E, STEP = LCH * E;
     __shared__ uint4 lds[2][2][LT * LCH];       // [buffer][B | A]
 
-    // workgroup -> (split, tile): each XCD (workgroup id mod 8) walks a contiguous range, 8-tall bands of tiles
-    const unsigned nb = gridDim.x, xcd = blockIdx.x & 7, slot = blockIdx.x >> 3;
-    const unsigned q8 = nb >> 3, r8 = nb & 7;
-    const unsigned L = (xcd < r8 ? xcd * (q8 + 1) : r8 * (q8 + 1) + (xcd - r8) * q8) + slot;
-    const unsigned tiles = (unsigned)g.tilesM * (unsigned)g.tilesN;
-    const unsigned split = L / tiles, Lt = L % tiles;
-    const unsigned band = 8u * (unsigned)g.tilesN, gi = Lt / band, within = Lt % band;
-    const unsigned gsize = min((unsigned)g.tilesM - gi * 8, 8u);
-    const int m0 = (int)(gi * 8 + within % gsize) * LT, n0 = (int)(within / gsize) * LT;
-
+    unsigned split;
+    int tm, tn;
+    tile_of(g, split, tm, tn);
+    const int m0 = tm * LT, n0 = tn * LT;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int wm = wave >> 1, wn = wave & 1, r = lane & 31, h = lane >> 5;
     const int step0 = (int)split * g.steps_per;
@@ -245,7 +219,7 @@ __global__ __launch_bounds__(256, 2) void linear_tile_kernel(Operand A, Operand 
 #pragma unroll
             for (int j = 0; j < 16; ++j) acc[mi][ni][j] = 0.f;
 
-    sb.fetch(B, m0, (int64_t)step0 * STEP, K, tid);
+    sb.fetch(B, m0, (int64_t)step0 * STEP, KB, tid);
     sa.fetch(A, n0, (int64_t)step0 * STEP, K, tid);
     sb.put(lds[0][0], tid);
     sa.put(lds[0][1], tid);
@@ -253,7 +227,7 @@ __global__ __launch_bounds__(256, 2) void linear_tile_kernel(Operand A, Operand 
     for (int s = 0; s < steps; ++s) {
         const int buf = s & 1;
         if (s + 1 < steps) {
-            sb.fetch(B, m0, (int64_t)(step0 + s + 1) * STEP, K, tid);
+            sb.fetch(B, m0, (int64_t)(step0 + s + 1) * STEP, KB, tid);
             sa.fetch(A, n0, (int64_t)(step0 + s + 1) * STEP, K, tid);
         }
 #pragma unroll
@@ -325,35 +299,53 @@ static int split_count(int64_t N, int64_t M, int64_t steps) {
     if (s > steps / 4) s = steps / 4;
     return s < 1 ? 1 : (int)s;
 }
-static size_t split_bytes(int64_t N, int64_t M, int64_t K) {
-    // (a K step is 64 bf16 or 32 fp32 elements: the latter has more steps and so at least as many splits)
-    const int s = split_count(N, M, cdiv(K, 32));
-    return s > 1 ? (size_t)s * N * ((M + 3) / 4 * 4) * 4 : 0;
+static size_t part_bytes(int64_t N, int64_t M, int splits) {
+    return splits > 1 ? (size_t)splits * N * ((M + 3) / 4 * 4) * 4 : 0;
+}
+// the most a product needs for its partial tiles, whichever kernel takes it
+static size_t split_bytes(int dtype, int64_t N, int64_t M, int64_t K) {
+    const size_t a = part_bytes(N, M, split_count(N, M, cdiv(K, dtype == SPHIP_BF16 ? 64 : 32)));
+    const size_t b = dtype == SPHIP_BF16 ? part_bytes(N, M, linear256_splits(N, M, cdiv(K, 64) * 64)) : 0;
+    return a > b ? a : b;
+}
+
+// Whether an (N, M) product over K is worth the 256 x 256 kernel (bf16): it has to fill most of the 256 compute units with
+// one workgroup each.
+static bool wants256(int64_t N, int64_t M, int64_t K) {
+    const int64_t tiles = cdiv(N, 256) * cdiv(M, 256);
+    return tiles * linear256_splits(N, M, K) >= 160;
 }
 
 template <typename T, int MODE_A, int MODE_B>
-static int launch_tiles(const char* what, const Operand& A, const Operand& B, const Epilogue& epi, int64_t K, void* ws,
-                        size_t ws_bytes, hipStream_t s) {
+static int launch_product(const char* what, const Operand& A, const Operand& B, const Epilogue& epi, int64_t K, int64_t KB,
+                          void* ws, size_t ws_bytes, hipStream_t s) {
     constexpr int STEP = LCH * Chunk<T>::E;
-    const int64_t N = A.rows, M = B.rows, steps = cdiv(K, STEP);
+    const int64_t N = A.rows, M = B.rows;
+    const bool big = sizeof(T) == 2 && wants256(N, M, K) && linear256_takes(MODE_A, MODE_B, A, B, K);
+    const int tile = big ? 256 : LT;
+    const int64_t steps = cdiv(K, STEP);
     TileGrid g;
-    g.tilesM = (int)cdiv(M, LT), g.tilesN = (int)cdiv(N, LT);
-    const int want = split_count(N, M, steps);
+    g.tilesM = (int)cdiv(M, tile), g.tilesN = (int)cdiv(N, tile);
+    const int want = big ? linear256_splits(N, M, K) : split_count(N, M, steps);
     g.steps_per = (int)cdiv(steps, want);
     g.splits = (int)cdiv(steps, g.steps_per);
     g.part = (float*)ws;
     if (g.splits > 1) {
-        const size_t need = (size_t)g.splits * N * ((M + 3) / 4 * 4) * 4;
+        const size_t need = part_bytes(N, M, g.splits);
         SPHIP_REQUIRE(ws != nullptr && ws_bytes >= need && ((uintptr_t)ws & 15) == 0, SPHIP_EWORKSPACE,
                       "%s: workspace of %zu bytes, needs %zu, 16-byte aligned", what, ws_bytes, need);
     }
-    const int64_t nblocks = (int64_t)g.tilesM * g.tilesN * g.splits;
-    SPHIP_REQUIRE(nblocks < (1ll << 31), SPHIP_EUNSUPPORTED, "%s: grid too large", what);
-    hipLaunchKernelGGL((linear_tile_kernel<T, MODE_A, MODE_B>), dim3((unsigned)nblocks), dim3(256), 0, s, A, B, epi, K, g);
-    SPHIP_CHECK_LAUNCH(what);
+    const int64_t nblocks = (int64_t)g.tilesM * g.tilesN * g.splits, threads = N * ((M + 3) / 4);
+    SPHIP_REQUIRE(nblocks < (1ll << 31) && (g.splits == 1 || cdiv(threads, 256) < (1ll << 31)), SPHIP_EUNSUPPORTED,
+                  "%s: grid too large", what);
+    if (big) {
+        const int st = launch_linear256(what, MODE_A, MODE_B, A, B, epi, K, KB, g, s);
+        if (st != SPHIP_OK) return st;
+    } else {
+        hipLaunchKernelGGL((linear_tile_kernel<T, MODE_A, MODE_B>), dim3((unsigned)nblocks), dim3(256), 0, s, A, B, epi, K, KB, g);
+        SPHIP_CHECK_LAUNCH(what);
+    }
     if (g.splits > 1) {
-        const int64_t threads = N * ((M + 3) / 4);
-        SPHIP_REQUIRE(cdiv(threads, 256) < (1ll << 31), SPHIP_EUNSUPPORTED, "%s: grid too large", what);
         hipLaunchKernelGGL(linear_join_kernel, dim3((unsigned)cdiv(threads, 256)), dim3(256), 0, s, g.part, epi, N, (int)M,
                            g.splits);
         SPHIP_CHECK_LAUNCH(what);
@@ -458,24 +450,34 @@ static bool aligned_elem(const void* p, int dt) { return ((uintptr_t)p & (dtype_
 
 }  // namespace sphip
 
+using namespace sphip;
+
 #define SPHIP_LINEAR_SIZES(what)                                                                                        \
     SPHIP_REQUIRE(N > 0 && D > 0 && M > 0, SPHIP_EINVAL, what ": empty shape N=%lld D=%lld M=%lld", (long long)N,        \
                   (long long)D, (long long)M);                                                                          \
     SPHIP_REQUIRE(N < (1ll << 31) - 256 && D < (1ll << 31) - 256 && M < (1ll << 31) - 256, SPHIP_EUNSUPPORTED,           \
                   what ": dimension exceeds int32")
 
-extern "C" size_t sphip_linear_workspace_bytes(int64_t N, int64_t D, int64_t M) {
-    if (N <= 0 || D <= 0 || M <= 0) return 0;
-    return sphip::split_bytes(N, M, D);
+static bool is_codes(int kind) { return kind == SPHIP_INT8 || kind == SPHIP_E4M3; }
+static bool codes_ok(const void* codes, const void* scales, int64_t ld, int64_t cols) {
+    return scales && ld >= cols && ld % 16 == 0 && ((uintptr_t)codes & 15) == 0 && ((uintptr_t)scales & 15) == 0;
+}
+static size_t up256(size_t b) { return (b + 255) / 256 * 256; }
+
+// workspace: partial tiles | z in fp32 on its way into 8 bits
+extern "C" size_t sphip_linear_workspace_bytes(int dtype, int z_kind, int64_t N, int64_t D, int64_t M) {
+    if (N <= 0 || D <= 0 || M <= 0 || !valid_dtype(dtype)) return 0;
+    return up256(split_bytes(dtype, N, M, D)) + (is_codes(z_kind) ? (size_t)N * (cdiv(M, 4) * 4) * 4 : 0);
 }
 
 extern "C" int sphip_linear(const void* x, int64_t ldx, const void* W, int64_t ldw, int dtype, const void* bias,
                             int bias_dtype, int act, const void* residual, int res_dtype, int64_t ldr, void* out,
-                            int out_dtype, int64_t ldo, void* z, int z_dtype, int64_t ldz, int64_t N, int64_t D, int64_t M,
-                            void* ws, size_t ws_bytes, void* stream) {
-    using namespace sphip;
+                            int out_dtype, int64_t ldo, void* z, int z_kind, uint8_t* z_scales, int64_t ldz, uint8_t* x_codes,
+                            uint8_t* x_scales, int x_fmt, int64_t ldq, int64_t N, int64_t D, int64_t M, void* ws,
+                            size_t ws_bytes, void* stream) {
+    const bool zc = z && is_codes(z_kind);
     SPHIP_REQUIRE(valid_dtype(dtype) && valid_dtype(out_dtype) && (!bias || valid_dtype(bias_dtype)) &&
-                      (!residual || valid_dtype(res_dtype)) && (!z || valid_dtype(z_dtype)),
+                      (!residual || valid_dtype(res_dtype)) && (!z || zc || valid_dtype(z_kind)) && (!x_codes || is_codes(x_fmt)),
                   SPHIP_EINVAL, "linear: bad dtype");
     SPHIP_REQUIRE(valid_act(act), SPHIP_EINVAL, "linear: bad activation %d", act);
     SPHIP_REQUIRE(x && W && out, SPHIP_EINVAL, "linear: null pointer");
@@ -484,122 +486,144 @@ extern "C" int sphip_linear(const void* x, int64_t ldx, const void* W, int64_t l
                   "linear: a row stride is shorter than its row");
     SPHIP_REQUIRE(aligned_elem(x, dtype) && aligned_elem(W, dtype) && aligned_elem(out, out_dtype) &&
                       (!bias || aligned_elem(bias, bias_dtype)) && (!residual || aligned_elem(residual, res_dtype)) &&
-                      (!z || aligned_elem(z, z_dtype)),
+                      (!z || zc || aligned_elem(z, z_kind)),
                   SPHIP_EINVAL, "linear: a pointer is not aligned to its element");
+    SPHIP_REQUIRE((!zc || codes_ok(z, z_scales, ldz, M)) && (!x_codes || codes_ok(x_codes, x_scales, ldq, D)), SPHIP_EINVAL,
+                  "linear: codes and scales need 16-byte aligned rows of at least their columns");
+    const size_t part = up256(split_bytes(dtype, N, M, D)), ldt = (size_t)cdiv(M, 4) * 4;
+    SPHIP_REQUIRE(!zc || (ws && ((uintptr_t)ws & 15) == 0 && ws_bytes >= part + (size_t)N * ldt * 4), SPHIP_EWORKSPACE,
+                  "linear: workspace of %zu bytes, needs %zu, 16-byte aligned", ws_bytes, part + (size_t)N * ldt * 4);
+    hipStream_t s = (hipStream_t)stream;
     Epilogue e;
     e.bias = bias, e.bias_dt = bias_dtype, e.res = residual, e.res_dt = res_dtype, e.ldr = ldr;
-    e.out = out, e.out_dt = out_dtype, e.ldo = ldo, e.z = z, e.z_dt = z_dtype, e.ldz = ldz, e.act = act;
+    e.out = out, e.out_dt = out_dtype, e.ldo = ldo, e.act = act;
+    if (zc) e.z = (char*)ws + part, e.z_dt = SPHIP_F32, e.ldz = (int64_t)ldt;
+    else e.z = z, e.z_dt = z_kind, e.ldz = ldz;
     set_vec(e);
     const Operand A = {x, nullptr, ldx, (int)N}, B = {W, nullptr, ldw, (int)M};
-    if (dtype == SPHIP_BF16)
-        return launch_tiles<bf16_t, OP_ROWS, OP_ROWS>("linear", A, B, e, D, ws, ws_bytes, (hipStream_t)stream);
-    return launch_tiles<float, OP_ROWS, OP_ROWS>("linear", A, B, e, D, ws, ws_bytes, (hipStream_t)stream);
+    int st = dtype == SPHIP_BF16 ? launch_product<bf16_t, OP_ROWS, OP_ROWS>("linear", A, B, e, D, D, ws, ws_bytes, s)
+                                 : launch_product<float, OP_ROWS, OP_ROWS>("linear", A, B, e, D, D, ws, ws_bytes, s);
+    if (st == SPHIP_OK && zc)
+        st = sphip_checkpoint8_save(e.z, SPHIP_F32, e.ldz, z_kind, act == SPHIP_ACT_RELU, (uint8_t*)z, z_scales, ldz, N, M, s);
+    if (st == SPHIP_OK && x_codes) st = sphip_checkpoint8_save(x, dtype, ldx, x_fmt, 0, x_codes, x_scales, ldq, N, D, s);
+    return st;
 }
 
-extern "C" size_t sphip_linear_grad_preact_workspace_bytes(int64_t N, int64_t M) {
-    return N > 0 && M > 0 ? (size_t)sphip::cdiv(N, 32) * M * 4 : 0;
+// workspace: dz | column sums of 32-row groups | x restored (8-bit x in the 256 x 256 kernel) | partial tiles of a product
+struct BackwardSpace {
+    size_t dz, sums, xr, part, total;
+};
+static int64_t dz_stride(int dtype, int64_t M) { return dtype == SPHIP_BF16 ? cdiv(M, 64) * 64 : cdiv(M, 4) * 4; }
+static BackwardSpace backward_space(int dtype, int x_kind, int want_dx, int want_dw, int want_db, int64_t N, int64_t D, int64_t M) {
+    BackwardSpace b;
+    const bool products = want_dx || want_dw;
+    b.dz = products ? up256((size_t)N * dz_stride(dtype, M) * dtype_size(dtype)) : 0;
+    b.sums = want_db ? up256((size_t)cdiv(N, 32) * M * 4) : 0;
+    b.xr = want_dw && dtype == SPHIP_BF16 && is_codes(x_kind) && wants256(M, D, N) ? up256((size_t)N * (cdiv(D, 16) * 16) * 2) : 0;
+    const size_t p1 = want_dx ? split_bytes(dtype, N, D, cdiv(M, 64) * 64) : 0, p2 = want_dw ? split_bytes(dtype, M, D, N) : 0;
+    b.part = p1 > p2 ? p1 : p2;
+    b.total = b.dz + b.sums + b.xr + b.part;
+    return b;
 }
 
-extern "C" int sphip_linear_grad_preact(const void* g, int g_dtype, int64_t ldg, const void* z, int z_kind,
-                                        const uint8_t* z_scales, int64_t ldz, int act, void* dz, int dz_dtype,
-                                        int64_t lddz, void* db, int db_dtype, int64_t N, int64_t M, void* ws,
-                                        size_t ws_bytes, void* stream) {
-    using namespace sphip;
-    SPHIP_REQUIRE(valid_dtype(g_dtype) && (!dz || valid_dtype(dz_dtype)) && (!db || valid_dtype(db_dtype)), SPHIP_EINVAL,
-                  "linear_grad_preact: bad dtype");
-    SPHIP_REQUIRE(valid_act(act), SPHIP_EINVAL, "linear_grad_preact: bad activation %d", act);
-    SPHIP_REQUIRE(g && (dz || db), SPHIP_EINVAL, "linear_grad_preact: null pointer");
-    SPHIP_REQUIRE(N > 0 && M > 0 && N < (1ll << 31) - 256 && M < (1ll << 31) - 256, SPHIP_EINVAL,
-                  "linear_grad_preact: bad shape N=%lld M=%lld", (long long)N, (long long)M);
-    const bool codes = z_kind == SPHIP_INT8 || z_kind == SPHIP_E4M3;
-    if (act != SPHIP_ACT_NONE) {
-        SPHIP_REQUIRE(z && (codes ? z_scales != nullptr : valid_dtype(z_kind)), SPHIP_EINVAL,
-                      "linear_grad_preact: an activation needs z (values, or codes with scales)");
-        SPHIP_REQUIRE(ldz >= M && (!codes || (ldz % 16 == 0 && ((uintptr_t)z & 3) == 0 && ((uintptr_t)z_scales & 3) == 0)),
-                      SPHIP_EINVAL, "linear_grad_preact: bad row stride or alignment of z");
+extern "C" size_t sphip_linear_backward_workspace_bytes(int dtype, int x_kind, int want_dx, int want_dw, int want_db, int64_t N,
+                                                        int64_t D, int64_t M) {
+    if (N <= 0 || D <= 0 || M <= 0 || !valid_dtype(dtype)) return 0;
+    return backward_space(dtype, x_kind, want_dx, want_dw, want_db, N, D, M).total;
+}
+
+template <typename T>
+static int backward_products(const Operand& dz, const void* W, int64_t ldw, const void* x, int x_kind, const uint8_t* x_scales,
+                             int64_t ldx, void* dx, int dx_dtype, int64_t lddx, void* dW, int dw_dtype, int64_t lddw, int64_t N,
+                             int64_t D, int64_t M, bool padded, void* xr, void* part, size_t part_size, hipStream_t s) {
+    if (dx) {
+        Epilogue e;
+        e.out = dx, e.out_dt = dx_dtype, e.ldo = lddx;
+        set_vec(e);
+        const Operand A = {dz.p, nullptr, dz.ld, (int)N}, B = {W, nullptr, ldw, (int)D};
+        const int st = launch_product<T, OP_ROWS, OP_COLS>("linear_backward(dx)", A, B, e, padded ? dz.ld : M, M, part, part_size, s);
+        if (st != SPHIP_OK) return st;
     }
-    SPHIP_REQUIRE(ldg >= M && (!dz || (lddz >= M && lddz % 4 == 0)), SPHIP_EINVAL, "linear_grad_preact: bad row stride");
-    SPHIP_REQUIRE(aligned_elem(g, g_dtype) && (!dz || ((uintptr_t)dz & 15) == 0) && (!db || aligned_elem(db, db_dtype)) &&
-                      (act == SPHIP_ACT_NONE || codes || aligned_elem(z, z_kind)),
-                  SPHIP_EINVAL, "linear_grad_preact: misaligned pointer");
-    const int64_t P = cdiv(N, 32);
-    if (db) {
-        const size_t need = (size_t)P * M * 4;
-        SPHIP_REQUIRE(ws && ws_bytes >= need && ((uintptr_t)ws & 15) == 0, SPHIP_EWORKSPACE,
-                      "linear_grad_preact: workspace of %zu bytes, needs %zu, 16-byte aligned", ws_bytes, need);
-    }
-    PreactArgs a;
-    a.g = g, a.z = z, a.scales = z_scales, a.dz = dz, a.part = db ? (float*)ws : nullptr;
-    a.ldg = ldg, a.ldz = ldz, a.lddz = lddz, a.g_dt = g_dtype, a.z_kind = z_kind, a.dz_dt = dz_dtype, a.act = act;
-    a.vec = aligned4(g, g_dtype, ldg) && (act == SPHIP_ACT_NONE || codes || aligned4(z, z_kind, ldz));
-    const int64_t quads = (dz ? lddz : M + 3) / 4, blocks = cdiv(P * quads, 256);
-    SPHIP_REQUIRE(blocks < (1ll << 31), SPHIP_EUNSUPPORTED, "linear_grad_preact: grid too large");
-    hipStream_t s = (hipStream_t)stream;
-    hipLaunchKernelGGL(linear_preact_kernel, dim3((unsigned)blocks), dim3(256), 0, s, a, N, (int)M);
-    SPHIP_CHECK_LAUNCH("linear_grad_preact");
-    if (db) {
-        hipLaunchKernelGGL(linear_bias_grad_kernel, dim3((unsigned)cdiv(M, 64)), dim3(1024), 0, s, (const float*)ws, P, (int)M,
-                           db, db_dtype);
-        SPHIP_CHECK_LAUNCH("linear_grad_preact(db)");
-    }
-    return SPHIP_OK;
-}
-
-extern "C" size_t sphip_linear_grad_input_workspace_bytes(int64_t N, int64_t D, int64_t M) {
-    if (N <= 0 || D <= 0 || M <= 0) return 0;
-    return sphip::split_bytes(N, D, M);
-}
-
-extern "C" int sphip_linear_grad_input(const void* dz, int64_t lddz, const void* W, int64_t ldw, int dtype, void* dx,
-                                       int dx_dtype, int64_t lddx, int64_t N, int64_t D, int64_t M, void* ws,
-                                       size_t ws_bytes, void* stream) {
-    using namespace sphip;
-    SPHIP_REQUIRE(valid_dtype(dtype) && valid_dtype(dx_dtype), SPHIP_EINVAL, "linear_grad_input: bad dtype");
-    SPHIP_REQUIRE(dz && W && dx, SPHIP_EINVAL, "linear_grad_input: null pointer");
-    SPHIP_LINEAR_SIZES("linear_grad_input");
-    SPHIP_REQUIRE(lddz >= M && ldw >= D && lddx >= D, SPHIP_EINVAL, "linear_grad_input: a row stride is shorter than its row");
-    SPHIP_REQUIRE(aligned_elem(dz, dtype) && aligned_elem(W, dtype) && aligned_elem(dx, dx_dtype), SPHIP_EINVAL,
-                  "linear_grad_input: a pointer is not aligned to its element");
-    Epilogue e;
-    e.out = dx, e.out_dt = dx_dtype, e.ldo = lddx;
-    set_vec(e);
-    const Operand A = {dz, nullptr, lddz, (int)N}, B = {W, nullptr, ldw, (int)D};
-    if (dtype == SPHIP_BF16)
-        return launch_tiles<bf16_t, OP_ROWS, OP_COLS>("linear_grad_input", A, B, e, M, ws, ws_bytes, (hipStream_t)stream);
-    return launch_tiles<float, OP_ROWS, OP_COLS>("linear_grad_input", A, B, e, M, ws, ws_bytes, (hipStream_t)stream);
-}
-
-extern "C" size_t sphip_linear_grad_weight_workspace_bytes(int64_t N, int64_t D, int64_t M) {
-    if (N <= 0 || D <= 0 || M <= 0) return 0;
-    return sphip::split_bytes(M, D, N);
-}
-
-extern "C" int sphip_linear_grad_weight(const void* dz, int64_t lddz, int dtype, const void* x, const uint8_t* x_scales,
-                                        int x_kind, int64_t ldx, void* dW, int dw_dtype, int64_t lddw, int64_t N, int64_t D,
-                                        int64_t M, void* ws, size_t ws_bytes, void* stream) {
-    using namespace sphip;
-    SPHIP_REQUIRE(valid_dtype(dtype) && valid_dtype(dw_dtype), SPHIP_EINVAL, "linear_grad_weight: bad dtype");
-    const bool codes = x_kind == SPHIP_INT8 || x_kind == SPHIP_E4M3;
-    SPHIP_REQUIRE(codes || x_kind == dtype, SPHIP_EINVAL, "linear_grad_weight: x must be of dz's type or 8-bit codes");
-    SPHIP_REQUIRE(dz && x && dW && (!codes || x_scales), SPHIP_EINVAL, "linear_grad_weight: null pointer");
-    SPHIP_LINEAR_SIZES("linear_grad_weight");
-    SPHIP_REQUIRE(lddz >= M && ldx >= D && lddw >= D, SPHIP_EINVAL, "linear_grad_weight: a row stride is shorter than its row");
-    SPHIP_REQUIRE(!codes || (ldx % 16 == 0 && ((uintptr_t)x & 15) == 0 && ((uintptr_t)x_scales & 15) == 0), SPHIP_EINVAL,
-                  "linear_grad_weight: codes need 16-byte aligned rows");
-    SPHIP_REQUIRE(aligned_elem(dz, dtype) && (codes || aligned_elem(x, dtype)) && aligned_elem(dW, dw_dtype), SPHIP_EINVAL,
-                  "linear_grad_weight: a pointer is not aligned to its element");
+    if (!dW) return SPHIP_OK;
+    const char* what = "linear_backward(dW)";
     Epilogue e;
     e.out = dW, e.out_dt = dw_dtype, e.ldo = lddw;
     set_vec(e);
-    const Operand A = {dz, nullptr, lddz, (int)M}, B = {x, x_scales, ldx, (int)D};
-    hipStream_t s = (hipStream_t)stream;
-    const char* what = "linear_grad_weight";
-    if (dtype == SPHIP_BF16) {
-        if (x_kind == SPHIP_INT8) return launch_tiles<bf16_t, OP_COLS, OP_COLS_I8>(what, A, B, e, N, ws, ws_bytes, s);
-        if (x_kind == SPHIP_E4M3) return launch_tiles<bf16_t, OP_COLS, OP_COLS_E4M3>(what, A, B, e, N, ws, ws_bytes, s);
-        return launch_tiles<bf16_t, OP_COLS, OP_COLS>(what, A, B, e, N, ws, ws_bytes, s);
+    const Operand A = {dz.p, nullptr, dz.ld, (int)M};
+    Operand B = {x, x_scales, ldx, (int)D};
+    if (xr != nullptr) {
+        const Operand R = {xr, nullptr, cdiv(D, 16) * 16, (int)D};
+        if (linear256_takes(OP_COLS, OP_COLS, A, R, N)) {
+            const int st = sphip_checkpoint8_restore((const uint8_t*)x, x_scales, ldx, x_kind, xr, SPHIP_BF16, R.ld, N, D, s);
+            if (st != SPHIP_OK) return st;
+            B = R;
+            x_kind = SPHIP_BF16;
+        }
     }
-    if (x_kind == SPHIP_INT8) return launch_tiles<float, OP_COLS, OP_COLS_I8>(what, A, B, e, N, ws, ws_bytes, s);
-    if (x_kind == SPHIP_E4M3) return launch_tiles<float, OP_COLS, OP_COLS_E4M3>(what, A, B, e, N, ws, ws_bytes, s);
-    return launch_tiles<float, OP_COLS, OP_COLS>(what, A, B, e, N, ws, ws_bytes, s);
+    if (x_kind == SPHIP_INT8) return launch_product<T, OP_COLS, OP_COLS_I8>(what, A, B, e, N, N, part, part_size, s);
+    if (x_kind == SPHIP_E4M3) return launch_product<T, OP_COLS, OP_COLS_E4M3>(what, A, B, e, N, N, part, part_size, s);
+    return launch_product<T, OP_COLS, OP_COLS>(what, A, B, e, N, N, part, part_size, s);
+}
+
+extern "C" int sphip_linear_backward(const void* g, int g_dtype, int64_t ldg, const void* W, int64_t ldw, int dtype, int act,
+                                     const void* z, int z_kind, const uint8_t* z_scales, int64_t ldz, const void* x, int x_kind,
+                                     const uint8_t* x_scales, int64_t ldx, void* dx, int dx_dtype, int64_t lddx, void* dW,
+                                     int dw_dtype, int64_t lddw, void* db, int db_dtype, int64_t N, int64_t D, int64_t M,
+                                     void* ws, size_t ws_bytes, void* stream) {
+    SPHIP_REQUIRE(valid_dtype(dtype) && valid_dtype(g_dtype) && (!dx || valid_dtype(dx_dtype)) && (!dW || valid_dtype(dw_dtype)) &&
+                      (!db || valid_dtype(db_dtype)),
+                  SPHIP_EINVAL, "linear_backward: bad dtype");
+    SPHIP_REQUIRE(valid_act(act), SPHIP_EINVAL, "linear_backward: bad activation %d", act);
+    SPHIP_LINEAR_SIZES("linear_backward");
+    SPHIP_REQUIRE(g && (dx || dW || db) && (!dx || W) && (!dW || x), SPHIP_EINVAL, "linear_backward: null pointer");
+    const bool zc = is_codes(z_kind), xc = is_codes(x_kind);
+    SPHIP_REQUIRE(act == SPHIP_ACT_NONE || (z && (zc || valid_dtype(z_kind))), SPHIP_EINVAL,
+                  "linear_backward: an activation needs z (values, or codes with scales)");
+    SPHIP_REQUIRE(!dW || xc || x_kind == dtype, SPHIP_EINVAL, "linear_backward: x must be of the product's type or 8-bit codes");
+    SPHIP_REQUIRE(ldg >= M && (!dx || (ldw >= D && lddx >= D)) && (!dW || (ldx >= D && lddw >= D)) &&
+                      (act == SPHIP_ACT_NONE || ldz >= M),
+                  SPHIP_EINVAL, "linear_backward: a row stride is shorter than its row");
+    SPHIP_REQUIRE((act == SPHIP_ACT_NONE || !zc || codes_ok(z, z_scales, ldz, M)) && (!dW || !xc || codes_ok(x, x_scales, ldx, D)),
+                  SPHIP_EINVAL, "linear_backward: codes and scales need 16-byte aligned rows of at least their columns");
+    SPHIP_REQUIRE(aligned_elem(g, g_dtype) && (!dx || (aligned_elem(W, dtype) && aligned_elem(dx, dx_dtype))) &&
+                      (!dW || ((xc || aligned_elem(x, dtype)) && aligned_elem(dW, dw_dtype))) && (!db || aligned_elem(db, db_dtype)) &&
+                      (act == SPHIP_ACT_NONE || zc || aligned_elem(z, z_kind)),
+                  SPHIP_EINVAL, "linear_backward: a pointer is not aligned to its element");
+    const BackwardSpace sp = backward_space(dtype, x_kind, dx != nullptr, dW != nullptr, db != nullptr, N, D, M);
+    SPHIP_REQUIRE(sp.total == 0 || (ws && ((uintptr_t)ws & 15) == 0 && ws_bytes >= sp.total), SPHIP_EWORKSPACE,
+                  "linear_backward: workspace of %zu bytes, needs %zu, 16-byte aligned", ws_bytes, sp.total);
+    hipStream_t s = (hipStream_t)stream;
+    char* w = (char*)ws;
+    float* sums = (float*)(w + sp.dz);
+    // Without an activation the incoming gradient is dz. It is copied (into the product's dtype, rows padded to 64) only
+    // where it does not have that dtype, or where a large product needs the padding.
+    const bool products = dx || dW;
+    bool direct = act == SPHIP_ACT_NONE && g_dtype == dtype;
+    if (direct && dtype == SPHIP_BF16 && (M % 64 != 0 || ldg % 8 != 0 || ((uintptr_t)g & 15) != 0))
+        direct = !((dx && wants256(N, D, cdiv(M, 64) * 64)) || (dW && wants256(M, D, N)));
+    Operand dz = {g, nullptr, ldg, (int)N};
+    if (products && !direct) dz.p = w, dz.ld = dz_stride(dtype, M);
+    if (db || (products && !direct)) {
+        PreactArgs a;
+        a.g = g, a.z = z, a.scales = z_scales, a.dz = products && !direct ? w : nullptr, a.part = db ? sums : nullptr;
+        a.ldg = ldg, a.ldz = ldz, a.lddz = dz.ld, a.g_dt = g_dtype, a.z_kind = z_kind, a.dz_dt = dtype, a.act = act;
+        a.vec = aligned4(g, g_dtype, ldg) && (act == SPHIP_ACT_NONE || zc || aligned4(z, z_kind, ldz));
+        const int64_t P = cdiv(N, 32), quads = (a.dz ? a.lddz : M + 3) / 4, blocks = cdiv(P * quads, 256);
+        SPHIP_REQUIRE(blocks < (1ll << 31), SPHIP_EUNSUPPORTED, "linear_backward: grid too large");
+        hipLaunchKernelGGL(linear_preact_kernel, dim3((unsigned)blocks), dim3(256), 0, s, a, N, (int)M);
+        SPHIP_CHECK_LAUNCH("linear_backward(dz)");
+        if (db) {
+            hipLaunchKernelGGL(linear_bias_grad_kernel, dim3((unsigned)cdiv(M, 64)), dim3(1024), 0, s, (const float*)sums, P,
+                               (int)M, db, db_dtype);
+            SPHIP_CHECK_LAUNCH("linear_backward(db)");
+        }
+    }
+    if (!products) return SPHIP_OK;
+    void* xr = sp.xr ? w + sp.dz + sp.sums : nullptr;
+    void* part = w + sp.dz + sp.sums + sp.xr;
+    if (dtype == SPHIP_BF16)
+        return backward_products<bf16_t>(dz, W, ldw, x, x_kind, x_scales, ldx, dx, dx_dtype, lddx, dW, dw_dtype, lddw, N, D, M,
+                                         !direct, xr, part, sp.part, s);
+    return backward_products<float>(dz, W, ldw, x, x_kind, x_scales, ldx, dx, dx_dtype, lddx, dW, dw_dtype, lddw, N, D, M, false,
+                                    xr, part, sp.part, s);
 }

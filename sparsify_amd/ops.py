@@ -6,6 +6,7 @@ host and then passes raw pointers; nothing in this module computes with torch op
 """
 from __future__ import annotations
 
+import functools
 import os
 
 import torch
@@ -1261,32 +1262,30 @@ ACTIVATIONS = tuple(_lib.ACTIVATIONS)
 CODE_GROUP = 32                     # tokens that share a scale in an 8-bit checkpoint
 
 
+def is_rows(t: Tensor) -> bool:
+    """Whether a 2-D tensor has its columns next to each other and rows that do not overlap (any row stride)."""
+    n, d = t.shape
+    s0, s1 = t.stride()
+    return (s1 == 1 or d <= 1) and (s0 >= d or n <= 1)
+
+
 def _rows(t: Tensor, name: str, shape: tuple | None = None, like: Tensor | None = None) -> Tensor:
     """A (rows, columns) tensor these ops take: on the GPU, fp32 or bf16, columns next to each other, any row stride."""
     if not t.is_cuda:
         raise RuntimeError(f"{name} is on {t.device}: sparsify_amd runs on the MI355X HIP path only (no CPU fallback)")
     _dt(t)
-    if t.ndim != 2 or (shape is not None and tuple(t.shape) != shape):
+    if t.ndim != 2 or (shape is not None and t.shape != shape):
         raise ValueError(f"{name}: expected {'2 dims' if shape is None else shape}, got shape {tuple(t.shape)}")
     if like is not None and t.device != like.device:
         raise ValueError(f"{name} is on {t.device}, the others on {like.device}")
-    if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+    if not is_rows(t):
         raise ValueError(f"{name} must have its columns next to each other and rows that do not overlap "
                          f"(strides {t.stride()} for shape {tuple(t.shape)})")
     return t
 
 
 def _ld(t: Tensor) -> int:
-    return max(t.stride(0), t.shape[1]) if t.shape[0] > 1 else t.shape[1]
-
-
-def _vector(t: Tensor | None, name: str, n: int, like: Tensor) -> Tensor | None:
-    if t is not None:
-        _req(t, name, ndim=1)
-        _dt(t)
-        if t.shape[0] != n or t.device != like.device:
-            raise ValueError(f"{name}: expected ({n},) on {like.device}, got {tuple(t.shape)} on {t.device}")
-    return t
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
 def _call(what: str, t: Tensor, *args) -> None:
@@ -1298,27 +1297,55 @@ def _call(what: str, t: Tensor, *args) -> None:
     else:
         with torch.cuda.device(t.device):
             st = fn(*args, _stream(t))
-    check(st, what)
+    if st:
+        check(st, what)
     timer.stop(ev, t)
 
 
 def _scratch(t: Tensor, nbytes: int) -> Tensor | None:
     """Scratch of one call. From the allocator each time (stream-ordered; inside a graph capture it belongs to that
     graph), not from the per-stream workspaces: two captured graphs may replay at once."""
-    return torch.empty(nbytes, dtype=torch.uint8, device=t.device) if nbytes else None
+    return t.new_empty((nbytes,), dtype=torch.uint8) if nbytes else None
+
+
+@functools.lru_cache(maxsize=1024)
+def _linear_bytes(*args) -> int:
+    return _lib.load().sphip_linear_workspace_bytes(*args)
+
+
+@functools.lru_cache(maxsize=1024)
+def _linear_backward_bytes(*args) -> int:
+    return _lib.load().sphip_linear_backward_workspace_bytes(*args)
 
 
 def _act(activation: str) -> int:
-    if activation not in _lib.ACTIVATIONS:
+    act = _lib.ACTIVATIONS.get(activation)
+    if act is None:
         raise ValueError(f"Unknown activation: {activation!r} (one of {ACTIVATIONS})")
-    return _lib.ACTIVATIONS[activation]
+    return act
+
+
+def _code(fmt: str) -> int:
+    code = _lib.CODES.get(fmt)
+    if code is None:
+        raise ValueError(f"Unknown 8-bit format: {fmt!r} (one of {tuple(_lib.CODES)})")
+    return code
+
+
+def _new_codes(t: Tensor, N: int, D: int):
+    """(buffer, address of the scales, row stride) of an (N, D) checkpoint: uint8 (33 G, ldq), G = ceil(N / 32) groups; the
+    codes of 32 G tokens, then a row of scales per group."""
+    groups, ldq = -(-N // CODE_GROUP), -(-D // 16) * 16
+    data = t.new_empty((33 * groups, ldq), dtype=torch.uint8)
+    return data, data.data_ptr() + CODE_GROUP * groups * ldq, ldq
 
 
 def linear(x: Tensor, W: Tensor, bias: Tensor | None = None, residual: Tensor | None = None, activation: str = "none",
-           out_dtype: torch.dtype | None = None, z_dtype: torch.dtype | None = None):
-    """act(x @ W.T + bias) + residual in one pass, one rounding at the end; (out, z), z = x @ W.T + bias as z_dtype or
-    None. x (N, D) and W (M, D) of one dtype, bias (M) and residual (N, M) of either; out_dtype defaults to the wider of
-    x's and residual's. (sparse_coder.py:219-222: sae_out += x @ W_skip.mT)"""
+           out_dtype: torch.dtype | None = None, keep_z: torch.dtype | str | None = None, keep_x: str | None = None):
+    """(out, z, codes of x): out = act(x @ W.T + bias) + residual in one pass, one rounding at the end. x (N, D) and W (M, D)
+    of one dtype, bias (M) and residual (N, M) of either; out_dtype defaults to the wider of x's and residual's.
+    keep_z: a dtype, or an 8-bit format, in which z = x @ W.T + bias is kept for linear_backward; keep_x: an 8-bit format
+    for x. Kept 8-bit data is a checkpoint buffer (checkpoint8_save). (sparse_coder.py:219-222: sae_out += x @ W_skip.mT)"""
     act = _act(activation)
     _rows(x, "x")
     N, D = x.shape
@@ -1326,141 +1353,107 @@ def linear(x: Tensor, W: Tensor, bias: Tensor | None = None, residual: Tensor | 
     M = W.shape[0]
     if W.shape[1] != D or W.dtype != x.dtype:
         raise ValueError(f"linear: x {tuple(x.shape)} {x.dtype} does not go with weight {tuple(W.shape)} {W.dtype}")
-    _vector(bias, "bias", M, x)
+    if bias is not None:
+        _req(bias, "bias", ndim=1)
+        if bias.shape[0] != M or bias.device != x.device:
+            raise ValueError(f"bias: expected ({M},) on {x.device}, got {tuple(bias.shape)} on {bias.device}")
     if residual is not None:
         _rows(residual, "residual", (N, M), like=x)
-    if out_dtype is None:
-        out_dtype = x.dtype if residual is None else torch.promote_types(x.dtype, residual.dtype)
-    out = torch.empty(N, M, dtype=out_dtype, device=x.device)
-    z = None if z_dtype is None else torch.empty(N, M, dtype=z_dtype, device=x.device)
+        if out_dtype is None:
+            out_dtype = torch.promote_types(x.dtype, residual.dtype)
+    out = x.new_empty((N, M), dtype=out_dtype)
+    z = codes = z_scales = x_scales = None
+    z_kind = x_fmt = z_ld = x_ld = 0
+    if isinstance(keep_z, str):
+        z_kind = _code(keep_z)
+        z, z_scales, z_ld = _new_codes(x, N, M)
+    elif keep_z is not None:
+        z, z_ld = x.new_empty((N, M), dtype=keep_z), M
+        z_kind = _dt(z)
+    if keep_x is not None:
+        x_fmt = _code(keep_x)
+        codes, x_scales, x_ld = _new_codes(x, N, D)
     if N == 0:
-        return out, z
-    nws = _lib.load().sphip_linear_workspace_bytes(N, D, M)
+        return out, z, codes
+    dt = _dt(x)
+    nws = _linear_bytes(dt, z_kind, N, D, M)
     ws = _scratch(x, nws)
-    _call("sphip_linear", x, x.data_ptr(), _ld(x), W.data_ptr(), _ld(W), _dt(x), _ptr(bias), 0 if bias is None else _dt(bias),
+    _call("sphip_linear", x, x.data_ptr(), _ld(x), W.data_ptr(), _ld(W), dt, _ptr(bias), 0 if bias is None else _dt(bias),
           act, _ptr(residual), 0 if residual is None else _dt(residual), 0 if residual is None else _ld(residual),
-          out.data_ptr(), _dt(out), M, _ptr(z), 0 if z is None else _dt(z), M, N, D, M, _ptr(ws), nws)
-    return out, z
+          out.data_ptr(), _dt(out), M, _ptr(z), z_kind, z_scales, z_ld, _ptr(codes), x_scales, x_fmt, x_ld, N, D, M, _ptr(ws), nws)
+    return out, z, codes
 
 
-def linear_grad_preact(g: Tensor, z, activation: str, dz_dtype: torch.dtype | None, db_dtype: torch.dtype | None):
-    """(dz, db): dz = g * act'(z) as dz_dtype with rows padded to a multiple of 8 columns (the returned tensor is the
-    (N, M) view), db its column sums; a dtype of None leaves that output out. z: a tensor, a Checkpoint8, or None
-    (activation "none")."""
+def _kept(t: Tensor, fmt: str | None, name: str, N: int, D: int, like: Tensor):
+    """(address, kind, address of the scales, row stride) of something linear kept."""
+    if fmt is None:
+        _rows(t, name, (N, D), like=like)
+        return t.data_ptr(), _dt(t), None, _ld(t)
+    groups, ldq = -(-N // CODE_GROUP), -(-D // 16) * 16
+    _req(t, name, torch.uint8, 2)
+    if t.shape != (33 * groups, ldq) or t.device != like.device:
+        raise ValueError(f"{name}: an {fmt} checkpoint of {N} x {D} values is uint8 {(33 * groups, ldq)} on {like.device}, "
+                         f"got {tuple(t.shape)} on {t.device}")
+    return t.data_ptr(), _code(fmt), t.data_ptr() + CODE_GROUP * groups * ldq, ldq
+
+
+def linear_backward(g: Tensor, W: Tensor, z: Tensor | None, x: Tensor | None, activation: str = "none", *,
+                    z_fmt: str | None = None, x_fmt: str | None = None, dx_dtype: torch.dtype | None = None,
+                    dw_dtype: torch.dtype | None = None, db_dtype: torch.dtype | None = None):
+    """(dx, dW, db) of linear from g = dL/dout (N, M): dz = g act'(z), dx = dz @ W, dW = dz.T @ x, db = dz.sum(0); a dtype
+    of None leaves that one out. z and x: tensors, or checkpoint buffers (z_fmt / x_fmt) that are read as they are. The
+    products run in W's dtype (dz rounded to it once), db sums dz unrounded; every sum has a fixed order."""
     act = _act(activation)
     _rows(g, "grad")
     N, M = g.shape
-    codes = z is not None and not isinstance(z, Tensor)
-    if act and z is None:
-        raise ValueError(f"linear_grad_preact: activation {activation!r} needs z")
-    if codes:
-        _codes_of(z, (N, M), g)
-    elif z is not None:
-        _rows(z, "z", (N, M), like=g)
-    ld = -(-M // 8) * 8
-    dz = None if dz_dtype is None else torch.empty(N, ld, dtype=dz_dtype, device=g.device)
-    db = None if db_dtype is None else torch.empty(M, dtype=db_dtype, device=g.device)
-    if N == 0:
-        return (None if dz is None else dz[:, :M]), (None if db is None else db.zero_())
-    if dz is None and db is None:
-        return None, None
-    nws = _lib.load().sphip_linear_grad_preact_workspace_bytes(N, M) if db is not None else 0
-    ws = _scratch(g, nws)
-    if not act:
-        zargs = (None, 0, None, 0)
-    elif codes:
-        zargs = (z.codes.data_ptr(), _lib.CODES[z.fmt], z.scales.data_ptr(), z.codes.shape[1])
-    else:
-        zargs = (z.data_ptr(), _dt(z), None, _ld(z))
-    _call("sphip_linear_grad_preact", g, g.data_ptr(), _dt(g), _ld(g), *zargs, act, _ptr(dz), 0 if dz is None else _dt(dz), ld,
-          _ptr(db), 0 if db is None else _dt(db), N, M, _ptr(ws), nws)
-    return (None if dz is None else dz[:, :M]), db
-
-
-def linear_grad_input(dz: Tensor, W: Tensor, out_dtype: torch.dtype) -> Tensor:
-    """dz @ W: dz (N, M), W (M, D) of one dtype."""
-    _rows(dz, "dz")
-    _rows(W, "weight", like=dz)
-    N, M = dz.shape
+    _rows(W, "weight", like=g)
     D = W.shape[1]
-    if W.shape[0] != M or W.dtype != dz.dtype:
-        raise ValueError(f"linear_grad_input: dz {tuple(dz.shape)} {dz.dtype} does not go with weight {tuple(W.shape)} {W.dtype}")
-    dx = torch.empty(N, D, dtype=out_dtype, device=dz.device)
+    dt = _dt(W)
+    if W.shape[0] != M:
+        raise ValueError(f"linear_backward: grad {tuple(g.shape)} does not go with weight {tuple(W.shape)}")
+    zargs = xargs = (None, 0, None, 0)
+    if act:
+        if z is None:
+            raise ValueError(f"linear_backward: activation {activation!r} needs z")
+        zargs = _kept(z, z_fmt, "z", N, M, g)
+    if dw_dtype is not None:
+        if x is None or (x_fmt is None and x.dtype != W.dtype):
+            raise ValueError("linear_backward: the weight's gradient needs x, in the weight's dtype or 8 bits")
+        xargs = _kept(x, x_fmt, "x", N, D, g)
+    dx = None if dx_dtype is None else g.new_empty((N, D), dtype=dx_dtype)
+    dW = None if dw_dtype is None else g.new_empty((M, D), dtype=dw_dtype)
+    db = None if db_dtype is None else g.new_empty((M,), dtype=db_dtype)
     if N == 0:
-        return dx
-    nws = _lib.load().sphip_linear_grad_input_workspace_bytes(N, D, M)
-    ws = _scratch(dz, nws)
-    _call("sphip_linear_grad_input", dz, dz.data_ptr(), _ld(dz), W.data_ptr(), _ld(W), _dt(dz), dx.data_ptr(), _dt(dx), D, N, D,
-          M, _ptr(ws), nws)
-    return dx
-
-
-def linear_grad_weight(dz: Tensor, x, out_dtype: torch.dtype) -> Tensor:
-    """dz.T @ x: dz (N, M), x (N, D) a tensor of the same dtype or a Checkpoint8, whose codes the product reads as they are."""
-    _rows(dz, "dz")
-    N, M = dz.shape
-    if isinstance(x, Tensor):
-        _rows(x, "x", like=dz)
-        if x.shape[0] != N or x.dtype != dz.dtype:
-            raise ValueError(f"linear_grad_weight: dz {tuple(dz.shape)} {dz.dtype} does not go with x {tuple(x.shape)} {x.dtype}")
-        D = x.shape[1]
-        xargs = (x.data_ptr(), None, _dt(x), _ld(x))
-    else:
-        D = x.columns
-        _codes_of(x, (N, D), dz)
-        xargs = (x.codes.data_ptr(), x.scales.data_ptr(), _lib.CODES[x.fmt], x.codes.shape[1])
-    dW = torch.empty(M, D, dtype=out_dtype, device=dz.device)
-    if N == 0:
-        return dW.zero_()
-    nws = _lib.load().sphip_linear_grad_weight_workspace_bytes(N, D, M)
-    ws = _scratch(dz, nws)
-    _call("sphip_linear_grad_weight", dz, dz.data_ptr(), _ld(dz), _dt(dz), *xargs, dW.data_ptr(), _dt(dW), D, N, D, M,
-          _ptr(ws), nws)
-    return dW
+        return dx, None if dW is None else dW.zero_(), None if db is None else db.zero_()
+    if dx is None and dW is None and db is None:
+        return None, None, None
+    nws = _linear_backward_bytes(dt, xargs[1], dx is not None, dW is not None, db is not None, N, D, M)
+    ws = _scratch(g, nws)
+    _call("sphip_linear_backward", g, g.data_ptr(), _dt(g), _ld(g), W.data_ptr(), _ld(W), dt, act, *zargs, *xargs,
+          _ptr(dx), 0 if dx is None else _dt(dx), D, _ptr(dW), 0 if dW is None else _dt(dW), D, _ptr(db),
+          0 if db is None else _dt(db), N, D, M, _ptr(ws), nws)
+    return dx, dW, db
 
 
 # ------------------------------------------------------------------ 8-bit checkpoints (checkpoint8.hip)
-def _codes_of(c, shape: tuple, like: Tensor) -> None:
-    if (c.rows, c.columns) != shape:
-        raise ValueError(f"the checkpoint holds {c.rows} x {c.columns} values, expected {shape[0]} x {shape[1]}")
-    if c.codes.device != like.device:
-        raise ValueError(f"the checkpoint is on {c.codes.device}, the others on {like.device}")
-
-
-def _code(fmt: str) -> int:
-    if fmt not in _lib.CODES:
-        raise ValueError(f"Unknown 8-bit format: {fmt!r} (one of {tuple(_lib.CODES)})")
-    return _lib.CODES[fmt]
-
-
-def checkpoint8_save(x: Tensor, fmt: str, keep_sign: bool = False):
-    """(codes, scales) of x (N, D): uint8 (32 ceil(N/32), ldq) and (ceil(N/32), ldq), ldq = D rounded up to 16."""
+def checkpoint8_save(x: Tensor, fmt: str, keep_sign: bool = False) -> Tensor:
+    """x (N, D) in 8 bits: uint8 (33 G, ldq), G = ceil(N / 32), ldq = D rounded up to 16; 32 G rows of codes, G of scales."""
     code = _code(fmt)
     _rows(x, "x")
     N, D = x.shape
-    groups, ldq = -(-N // CODE_GROUP), -(-D // 16) * 16
-    codes = torch.empty(groups * CODE_GROUP, ldq, dtype=torch.uint8, device=x.device)
-    scales = torch.empty(groups, ldq, dtype=torch.uint8, device=x.device)
-    if x.numel():
-        _call("sphip_checkpoint8_save", x, x.data_ptr(), _dt(x), _ld(x), code, int(keep_sign), codes.data_ptr(),
-              scales.data_ptr(), ldq, N, D)
-    return codes, scales
+    data, scales, ldq = _new_codes(x, N, D)
+    if N and D:
+        _call("sphip_checkpoint8_save", x, x.data_ptr(), _dt(x), _ld(x), code, int(keep_sign), data.data_ptr(), scales, ldq, N, D)
+    return data
 
 
-def checkpoint8_restore(codes: Tensor, scales: Tensor, fmt: str, rows: int, columns: int, dtype: torch.dtype) -> Tensor:
-    """The (rows, columns) values the codes stand for (exact in either dtype)."""
-    code = _code(fmt)
-    _req(codes, "codes", torch.uint8, 2)
-    _req(scales, "scales", torch.uint8, 2)
-    groups = -(-rows // CODE_GROUP)
-    if (codes.shape[0] != groups * CODE_GROUP or tuple(scales.shape) != (groups, codes.shape[1])
-            or codes.shape[1] % 16 or not 0 <= columns <= codes.shape[1] or scales.device != codes.device):
-        raise ValueError(f"checkpoint8_restore: codes {tuple(codes.shape)} and scales {tuple(scales.shape)} do not hold "
-                         f"{rows} x {columns} values")
-    out = torch.empty(rows, columns, dtype=dtype, device=codes.device)
-    if out.numel():
-        _call("sphip_checkpoint8_restore", codes, codes.data_ptr(), scales.data_ptr(), codes.shape[1], code, out.data_ptr(),
-              _dt(out), columns, rows, columns)
+def checkpoint8_restore(data: Tensor, fmt: str, rows: int, columns: int, dtype: torch.dtype) -> Tensor:
+    """The (rows, columns) values a checkpoint buffer stands for (exact in either dtype)."""
+    addr, code, scales, ldq = _kept(data, fmt, "checkpoint", rows, columns, data)
+    out = data.new_empty((rows, columns), dtype=dtype)
+    dt = _dt(out)
+    if rows and columns:
+        _call("sphip_checkpoint8_restore", data, addr, scales, ldq, code, out.data_ptr(), dt, columns, rows, columns)
     return out
 
 

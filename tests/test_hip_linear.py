@@ -144,12 +144,12 @@ def test_forward_writes_its_rows_only(device):
             xc, Wc, bc = cuda(x, W, b)
             out = torch.full((N + 2, M + 5), 7.0, dtype=dtype, device="cuda")
             z = torch.full((N + 2, M + 3), 7.0, device="cuda")
-            nws = lib.sphip_linear_workspace_bytes(N, D, M)
-            ws = torch.empty(max(nws, 16), dtype=torch.uint8, device="cuda")
             dt = _lib.BF16 if dtype == torch.bfloat16 else _lib.F32
+            nws = lib.sphip_linear_workspace_bytes(dt, _lib.F32, N, D, M)
+            ws = torch.empty(max(nws, 16), dtype=torch.uint8, device="cuda")
             _lib.check(lib.sphip_linear(xc.data_ptr(), D, Wc.data_ptr(), D, dt, bc.data_ptr(), dt, 1, None, 0, 0,
-                                        out[1:].data_ptr(), dt, M + 5, z[1:].data_ptr(), _lib.F32, M + 3, N, D, M, ws.data_ptr(),
-                                        nws, torch.cuda.current_stream().cuda_stream), "sphip_linear")
+                                        out[1:].data_ptr(), dt, M + 5, z[1:].data_ptr(), _lib.F32, None, M + 3, None, None,
+                                        0, 0, N, D, M, ws.data_ptr(), nws, torch.cuda.current_stream().cuda_stream), "sphip_linear")
             y, tol, zz, ez = forward64(x, W, b, None, "relu", dtype)
             assert_within(out[1:N + 1, :M], y, tol)
             assert_within(z[1:N + 1, :M], zz, ez + HALF[torch.float32] * zz.abs() + TINY)
@@ -312,11 +312,16 @@ def test_backward(device, N, D, M, dtype, fmt):
         g = torch.randn(N, M, generator=torch.Generator().manual_seed(i)).to(y.dtype)
         grads = torch.autograd.grad(y, [t for t in leaves if t is not None], g.cuda())
         # what the backward kept
-        zk = ops.linear(xc.detach(), Wc.detach(), None if bc is None else bc.detach(),
-                        None if rc is None else rc.detach(), act, z_dtype=torch.float32 if fmt else dtype)[1]
-        zhat = (checkpoint8(zk, fmt, keep_sign=act == "relu").restore() if fmt else zk).double().cpu()
-        if act == "relu":
-            assert torch.equal(torch.sign(zhat), torch.sign(zk.double().cpu()))
+        args = (xc.detach(), Wc.detach(), None if bc is None else bc.detach(), None if rc is None else rc.detach(), act)
+        zk = ops.linear(*args, keep_z=torch.float32 if fmt else dtype)[1]
+        zhat = zk.double().cpu()
+        if fmt:
+            _, zc, xcodes = ops.linear(*args, keep_z=fmt, keep_x=fmt)
+            zhat = ops.checkpoint8_restore(zc, fmt, N, M, torch.float32).double().cpu()
+            assert torch.equal(zhat, codes64(zk.cpu(), fmt, act == "relu"))
+            assert torch.equal(xcodes[:, :D], checkpoint8(xc, fmt).data[:, :D])
+            if act == "relu":
+                assert torch.equal(torch.sign(zhat), torch.sign(zk.double().cpu()))
         xhat = codes64(x, fmt) if fmt else x
         want = backward64(x, W, b, act, g, zhat, xhat, dtype, dtype, 0.0)
         names = [n for n, t in zip("xWbr", leaves) if t is not None]

@@ -15,7 +15,8 @@ def lib():
 
 def linear(**kw):
     a = dict(x=P, ldx=64, W=P, ldw=64, dtype=BF16, bias=None, bias_dtype=0, act=0, res=None, res_dtype=0, ldr=0, out=P,
-             out_dtype=BF16, ldo=32, z=None, z_dtype=0, ldz=0, N=8, D=64, M=32, ws=None, nws=0)
+             out_dtype=BF16, ldo=32, z=None, z_kind=0, z_scales=None, ldz=0, xc=None, xs=None, x_fmt=0, ldq=0, N=8, D=64, M=32,
+             ws=None, nws=0)
     assert set(kw) <= set(a)
     return lib().sphip_linear(*{**a, **kw}.values(), None)
 
@@ -29,44 +30,46 @@ def linear(**kw):
     (dict(ldo=31), EINVAL, b"stride"), (dict(res=P, ldr=31), EINVAL, b"stride"), (dict(z=P, ldz=8), EINVAL, b"stride"),
     (dict(x=P + 1), EINVAL, b"aligned"), (dict(out=P + 2, out_dtype=F32), EINVAL, b"aligned"),
     (dict(bias=P + 1, bias_dtype=BF16), EINVAL, b"aligned"), (dict(D=4096, ldx=4096, ldw=4096), EWORKSPACE, b"workspace"),
-    (dict(D=4096, ldx=4096, ldw=4096, ws=P + 4, nws=1 << 30), EWORKSPACE, b"aligned")])
+    (dict(D=4096, ldx=4096, ldw=4096, ws=P + 4, nws=1 << 30), EWORKSPACE, b"aligned"),
+    (dict(z=P, z_kind=9, ldz=32), EINVAL, b"dtype"), (dict(z=P, z_kind=INT8, ldz=32), EINVAL, b"codes"),
+    (dict(z=P, z_kind=E4M3, z_scales=P, ldz=40), EINVAL, b"codes"), (dict(z=P + 8, z_kind=INT8, z_scales=P, ldz=32), EINVAL, b"codes"),
+    (dict(z=P, z_kind=INT8, z_scales=P, ldz=32), EWORKSPACE, b"workspace"), (dict(xc=P, x_fmt=BF16), EINVAL, b"dtype"),
+    (dict(xc=P, x_fmt=INT8, ldq=64), EINVAL, b"codes"), (dict(xc=P, xs=P, x_fmt=INT8, ldq=48), EINVAL, b"codes")])
 def test_linear_entry(kw, status, word):
     assert linear(**kw) == status and word in lib().sphip_last_error()
 
 
-def test_gradient_entries():
+def backward(**kw):
+    a = dict(g=P, g_dtype=BF16, ldg=32, W=P, ldw=64, dtype=BF16, act=0, z=None, z_kind=0, z_scales=None, ldz=0, x=P, x_kind=BF16,
+             x_scales=None, ldx=64, dx=P, dx_dtype=BF16, lddx=64, dW=P, dw_dtype=BF16, lddw=64, db=None, db_dtype=0, N=8, D=64, M=32,
+             ws=None, nws=0)
+    assert set(kw) <= set(a)
+    return lib().sphip_linear_backward(*{**a, **kw}.values(), None)
+
+
+@pytest.mark.parametrize("kw,status,word", [
+    (dict(g=None), EINVAL, b"null"), (dict(W=None), EINVAL, b"null"), (dict(x=None), EINVAL, b"null"),
+    (dict(dx=None, dW=None), EINVAL, b"null"), (dict(dtype=5), EINVAL, b"dtype"), (dict(g_dtype=INT8), EINVAL, b"dtype"),
+    (dict(db=P, db_dtype=3), EINVAL, b"dtype"), (dict(act=4), EINVAL, b"activation"), (dict(act=2), EINVAL, b"needs z"),
+    (dict(act=2, z=P, z_kind=5, ldz=32), EINVAL, b"needs z"), (dict(act=2, z=P, z_kind=F32, ldz=31), EINVAL, b"stride"),
+    (dict(act=1, z=P, z_kind=INT8, ldz=32), EINVAL, b"codes"), (dict(act=1, z=P, z_kind=INT8, z_scales=P, ldz=40), EINVAL, b"codes"),
+    (dict(x_kind=F32), EINVAL, b"product's type"), (dict(x_kind=18), EINVAL, b"product's type"), (dict(x_kind=E4M3), EINVAL, b"codes"),
+    (dict(x_kind=INT8, x_scales=P, ldx=72), EINVAL, b"codes"), (dict(x=P + 4, x_kind=INT8, x_scales=P), EINVAL, b"codes"),
+    (dict(ldg=31), EINVAL, b"stride"), (dict(ldw=63), EINVAL, b"stride"), (dict(lddx=63), EINVAL, b"stride"),
+    (dict(ldx=63), EINVAL, b"stride"), (dict(lddw=1), EINVAL, b"stride"), (dict(dx=P + 1), EINVAL, b"aligned"),
+    (dict(g=P + 2, g_dtype=F32), EINVAL, b"aligned"), (dict(N=0), EINVAL, b"empty"), (dict(M=1 << 31, ldg=1 << 31), EUNSUPPORTED, b"int32"),
+    (dict(), EWORKSPACE, b"workspace"), (dict(ws=P + 8, nws=1 << 30), EWORKSPACE, b"aligned"),
+    (dict(dx=None, dW=None, db=P, db_dtype=F32), EWORKSPACE, b"workspace")])
+def test_backward_entry(kw, status, word):
+    assert backward(**kw) == status and word in lib().sphip_last_error()
+
+
+def test_workspace_queries():
     L = lib()
-
-    def preact(g=P, g_dtype=BF16, ldg=32, z=None, kind=0, sc=None, ldz=0, act=0, dz=P, dz_dtype=BF16, lddz=32, db=None, db_dtype=0,
-               N=8, M=32, ws=None, nws=0):
-        return L.sphip_linear_grad_preact(g, g_dtype, ldg, z, kind, sc, ldz, act, dz, dz_dtype, lddz, db, db_dtype, N, M, ws, nws, None)
-
-    for kw, st in [(dict(g=None), EINVAL), (dict(dz=None), EINVAL), (dict(act=9), EINVAL), (dict(act=2), EINVAL),
-                   (dict(act=2, z=P, kind=5, ldz=32), EINVAL), (dict(act=2, z=P, kind=INT8, ldz=32), EINVAL),
-                   (dict(act=2, z=P, kind=INT8, sc=P, ldz=40), EINVAL), (dict(act=2, z=P, kind=F32, ldz=31), EINVAL),
-                   (dict(lddz=33), EINVAL), (dict(lddz=28), EINVAL), (dict(ldg=8), EINVAL), (dict(dz=P + 8), EINVAL),
-                   (dict(N=0), EINVAL), (dict(db=P, db_dtype=F32), EWORKSPACE), (dict(db=P, db_dtype=3), EINVAL)]:
-        assert preact(**kw) == st, kw
-
-    def gin(dz=P, lddz=32, W=P, ldw=64, dtype=BF16, dx=P, dx_dtype=BF16, lddx=64, N=8, D=64, M=32, ws=None, nws=0):
-        return L.sphip_linear_grad_input(dz, lddz, W, ldw, dtype, dx, dx_dtype, lddx, N, D, M, ws, nws, None)
-
-    for kw, st in [(dict(dz=None), EINVAL), (dict(W=None), EINVAL), (dict(dx=None), EINVAL), (dict(dtype=16), EINVAL),
-                   (dict(lddz=31), EINVAL), (dict(ldw=63), EINVAL), (dict(lddx=63), EINVAL), (dict(M=0), EINVAL),
-                   (dict(D=1 << 31, ldw=1 << 31, lddx=1 << 31), EUNSUPPORTED), (dict(dx=P + 1), EINVAL),
-                   (dict(M=4096, lddz=4096), EWORKSPACE)]:
-        assert gin(**kw) == st, kw
-
-    def gw(dz=P, lddz=32, dtype=BF16, x=P, sc=None, kind=BF16, ldx=64, dW=P, dw_dtype=BF16, lddw=64, N=8, D=64, M=32, ws=None, nws=0):
-        return L.sphip_linear_grad_weight(dz, lddz, dtype, x, sc, kind, ldx, dW, dw_dtype, lddw, N, D, M, ws, nws, None)
-
-    for kw, st in [(dict(dz=None), EINVAL), (dict(x=None), EINVAL), (dict(dW=None), EINVAL), (dict(kind=F32), EINVAL),
-                   (dict(kind=INT8), EINVAL), (dict(kind=E4M3, sc=P, ldx=72), EINVAL), (dict(kind=INT8, sc=P + 4), EINVAL),
-                   (dict(kind=18, sc=P), EINVAL), (dict(lddz=1), EINVAL), (dict(ldx=63), EINVAL), (dict(lddw=63), EINVAL),
-                   (dict(N=0), EINVAL), (dict(N=1 << 20), EWORKSPACE)]:
-        assert gw(**kw) == st, kw
-    assert L.sphip_linear_workspace_bytes(0, 8, 8) == 0 and L.sphip_linear_workspace_bytes(8, -1, 8) == 0
-    assert L.sphip_linear_grad_weight_workspace_bytes(1 << 20, 64, 32) > 0
+    assert L.sphip_linear_workspace_bytes(BF16, 0, 0, 8, 8) == 0 and L.sphip_linear_workspace_bytes(9, 0, 8, 8, 8) == 0
+    assert L.sphip_linear_workspace_bytes(BF16, INT8, 8, 64, 32) >= 8 * 32 * 4
+    assert L.sphip_linear_backward_workspace_bytes(BF16, INT8, 0, 0, 1, 64, 64, 32) == 2 * 32 * 4
+    assert L.sphip_linear_backward_workspace_bytes(F32, F32, 1, 1, 1, 8, -1, 32) == 0
 
 
 def test_checkpoint_entries():
@@ -112,8 +115,7 @@ def test_python_surface_refuses_on_the_host():
         fused_linear(x, W, residual=torch.randn(5))
     with pytest.raises(ValueError, match="scalar"):
         checkpoint8(torch.tensor(1.0))
-    codes, scales = torch.zeros(32, 16, dtype=torch.uint8), torch.zeros(1, 16, dtype=torch.uint8)
-    c = Checkpoint8(codes, scales, "int8", (3, 8), torch.float32)
+    c = Checkpoint8(torch.zeros(33, 16, dtype=torch.uint8), "int8", (3, 8), torch.float32)
     assert c.rows == 3 and c.columns == 8 and c.nbytes == 33 * 16
     with pytest.raises(ValueError, match="checkpoint holds"):
         fused_linear(x, W, checkpoint=c)
