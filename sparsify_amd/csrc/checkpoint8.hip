@@ -189,11 +189,11 @@ extern "C" int sphip_checkpoint8_save(const void* x, int dtype, int64_t ldx, int
     SPHIP_REQUIRE(ldx >= D, SPHIP_EINVAL, "checkpoint8_save: ldx is shorter than a row");
     hipStream_t s = (hipStream_t)stream;
     const int64_t groups = cdiv(N, 32);
-    const int V = dtype == SPHIP_BF16 ? 8 : 4;
+    const int V = dtype == SPHIP_BF16 ? 4 : 2;
     const int64_t blocks = cdiv(groups * (ldq / V), 256);
     SPHIP_REQUIRE(blocks < (1ll << 31), SPHIP_EUNSUPPORTED, "checkpoint8_save: grid too large");
-    if (dtype == SPHIP_BF16) launch_save<bf16_t, 8>(x, ldx, fmt, keep_sign, codes, scales, ldq, N, D, (unsigned)blocks, s);
-    else launch_save<float, 4>(x, ldx, fmt, keep_sign, codes, scales, ldq, N, D, (unsigned)blocks, s);
+    if (dtype == SPHIP_BF16) launch_save<bf16_t, 4>(x, ldx, fmt, keep_sign, codes, scales, ldq, N, D, (unsigned)blocks, s);
+    else launch_save<float, 2>(x, ldx, fmt, keep_sign, codes, scales, ldq, N, D, (unsigned)blocks, s);
     SPHIP_CHECK_LAUNCH("checkpoint8_save");
     return SPHIP_OK;
 }

@@ -14,6 +14,7 @@
 // Loads are unaligned-tolerant vectors; only the last chunk of a row or the last rows of a matrix take element loads.
 // Few tiles: the K range is split over workgroups, fp32 partial tiles are joined in a fixed order by a second kernel.
 #include "linear.hpp"
+#include <stdlib.h>
 
 namespace sphip {
 
@@ -310,8 +311,10 @@ static size_t split_bytes(int dtype, int64_t N, int64_t M, int64_t K) {
 }
 
 // Whether an (N, M) product over K is worth the 256 x 256 kernel (bf16): it has to fill most of the 256 compute units with
-// one workgroup each.
+// one workgroup each. SPHIP_GEMM=128|256 forces a kernel (tests), as for the encoder.
 static bool wants256(int64_t N, int64_t M, int64_t K) {
+    const char* force = getenv("SPHIP_GEMM");
+    if (force) return force[0] == '2';
     const int64_t tiles = cdiv(N, 256) * cdiv(M, 256);
     return tiles * linear256_splits(N, M, K) >= 160;
 }
@@ -361,70 +364,114 @@ static void set_vec(Epilogue& e) {
             (e.res == nullptr || aligned4(e.res, e.res_dt, e.ldr)) && (e.z == nullptr || aligned4(e.z, e.z_dt, e.ldz));
 }
 
-// ---- dz = g act'(z) and its column sums. A thread owns 4 columns of one 32-row group (the group one scale of an 8-bit
-// z covers); its 32 rows' sum goes to part[group][M], added up in group order by the second kernel.
+// ---- dz = g act'(z) and its column sums. A thread owns 16 bytes of g's columns (4 fp32 or 8 bf16) of `per` rows, 8 rows
+// of loads in flight; its rows' sums go to part[row chunk][M], added up in order by the second kernel. per = 32 (the group
+// one scale of an 8-bit z covers) or, where that leaves the chip empty, 8.
 struct PreactArgs {
     const void* g;
-    const void* z;                 // values (z_kind = a dtype) or codes (SPHIP_INT8 / SPHIP_E4M3), row stride ldz
+    const void* z;                 // values or codes, row stride ldz
     const uint8_t* scales;
     void* dz;                      // row stride lddz (zeros in [M, lddz)), or null
-    float* part;                   // [ceil(N / 32)][M], or null
+    float* part;                   // [ceil(N / per)][M], or null
     int64_t ldg, ldz, lddz;
-    int g_dt, z_kind, dz_dt, act, vec;
+    int dz_dt, act, per;
 };
 
+template <int V> __device__ __forceinline__ void load_row(const bf16_t* p, int n, float (&v)[V]) {
+    unsigned w[V / 2];
+    if (n >= V) __builtin_memcpy(w, p, V * 2);
+    else
+#pragma unroll
+        for (int j = 0; j < V; ++j) w[j >> 1] = (j & 1 ? w[j >> 1] : 0u) | (j < n ? (unsigned)p[j] << ((j & 1) * 16) : 0u);
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] = __uint_as_float(j & 1 ? w[j >> 1] & 0xffff0000u : w[j >> 1] << 16);
+}
+template <int V> __device__ __forceinline__ void load_row(const float* p, int n, float (&v)[V]) {
+    if (n >= V) __builtin_memcpy(v, p, V * 4);
+    else
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] = j < n ? p[j] : 0.f;
+}
+
+// ZK: SPHIP_F32, SPHIP_BF16, SPHIP_INT8, SPHIP_E4M3, or -1: no activation, z is not read
+template <typename TG, int ZK>
 __global__ __launch_bounds__(256) void linear_preact_kernel(PreactArgs a, int64_t N, int M) {
-    const int quads = (int)(a.dz != nullptr ? a.lddz : (M + 3)) >> 2;
+    constexpr int V = 16 / sizeof(TG), B = 8;
+    const int pieces = (int)((a.dz != nullptr ? a.lddz : M) + V - 1) / V;
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int64_t grp = i / quads;
-    const int m = (int)(i % quads) * 4;
-    if (grp * 32 >= N) return;
-    const int n_rows = (int)min((int64_t)32, N - grp * 32);
-    const int cols = min(4, M - m);                        // <= 0: padding columns of dz
-    float sc[4] = {0.f, 0.f, 0.f, 0.f}, sum[4] = {0.f, 0.f, 0.f, 0.f};
-    const bool codes = a.z_kind >= SPHIP_INT8 && a.act != SPHIP_ACT_NONE;
-    if (codes && cols > 0) {
-        const unsigned s4 = *reinterpret_cast<const unsigned*>(a.scales + grp * a.ldz + m);
+    const int64_t chunk = i / pieces, r0 = chunk * a.per;
+    if (r0 >= N) return;
+    const int m = (int)(i % pieces) * V, cols = min(V, M - m);            // <= 0: padding columns of dz
+    const int64_t r1 = min(N, r0 + a.per);
+    float sc[V], sum[V];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) sc[j] = scale_value((s4 >> (8 * j)) & 0xffu);
+    for (int j = 0; j < V; ++j) sum[j] = 0.f, sc[j] = 0.f;
+    if ((ZK == SPHIP_INT8 || ZK == SPHIP_E4M3) && cols > 0) {
+        uint8_t s8[V];                                                    // (rows of codes are padded to 16: whole pieces)
+        __builtin_memcpy(s8, a.scales + (r0 >> 5) * a.ldz + m, V);
+#pragma unroll
+        for (int j = 0; j < V; ++j) sc[j] = scale_value(s8[j]);
     }
-#pragma unroll 4
-    for (int t = 0; t < n_rows; ++t) {
-        const int64_t n = grp * 32 + t;
-        float v[4] = {0.f, 0.f, 0.f, 0.f}, z[4] = {0.f, 0.f, 0.f, 0.f};
-        if (cols == 4 && a.vec) {
-            load4_as_f32(a.g, a.g_dt, n * a.ldg + m, v);
-        } else {
+    for (int64_t rb = r0; rb < r1; rb += B) {
+        float v[B][V], z[B][V];
+        unsigned q[B][V / 4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (j < cols) v[j] = load_as_f32(a.g, a.g_dt, n * a.ldg + m + j);
+        for (int t = 0; t < B; ++t) {
+            const int n = rb + t < r1 ? cols : 0;
+            load_row<V>((const TG*)a.g + (rb + t) * a.ldg + m, n, v[t]);
+            if (ZK == SPHIP_F32) load_row<V>((const float*)a.z + (rb + t) * a.ldz + m, n, z[t]);
+            if (ZK == SPHIP_BF16) load_row<V>((const bf16_t*)a.z + (rb + t) * a.ldz + m, n, z[t]);
+            if (ZK == SPHIP_INT8 || ZK == SPHIP_E4M3) {
+#pragma unroll
+                for (int j = 0; j < V / 4; ++j) q[t][j] = 0;
+                if (n > 0) __builtin_memcpy(q[t], (const uint8_t*)a.z + (rb + t) * a.ldz + m, V);
+            }
         }
-        if (a.act != SPHIP_ACT_NONE) {
-            if (codes) {
-                if (cols > 0) {
-                    const unsigned w = *reinterpret_cast<const unsigned*>((const uint8_t*)a.z + n * a.ldz + m);
-                    if (a.z_kind == SPHIP_INT8) code_values<SPHIP_INT8>(w, sc, z);
-                    else code_values<SPHIP_E4M3>(w, sc, z);
-                }
-            } else if (cols == 4 && a.vec) {
-                load4_as_f32(a.z, a.z_kind, n * a.ldz + m, z);
-            } else {
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (j < cols) z[j] = load_as_f32(a.z, a.z_kind, n * a.ldz + m + j);
+        for (int t = 0; t < B; ++t) {
+            if (rb + t >= r1) break;
+            if (ZK >= 0) {
+                if (ZK == SPHIP_INT8 || ZK == SPHIP_E4M3) {
+#pragma unroll
+                    for (int j = 0; j < V / 4; ++j) {
+                        const float s4[4] = {sc[4 * j], sc[4 * j + 1], sc[4 * j + 2], sc[4 * j + 3]};
+                        float o[4];
+                        code_values<ZK == SPHIP_INT8 ? SPHIP_INT8 : SPHIP_E4M3>(q[t][j], s4, o);
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) z[t][4 * j + c] = o[c];
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < V; ++j) v[t][j] = j < cols ? v[t][j] * act_slope(z[t][j], a.act) : 0.f;
             }
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (j < cols) v[j] *= act_slope(z[j], a.act);
-        }
+            for (int j = 0; j < V; ++j) sum[j] += v[t][j];
+            if (a.dz != nullptr) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) sum[j] += v[j];
-        if (a.dz != nullptr) store4_from_f32(a.dz, a.dz_dt, n * a.lddz + m, v);
+                for (int j = 0; j < V; j += 4) {
+                    const float o[4] = {v[t][j], v[t][j + 1], v[t][j + 2], v[t][j + 3]};
+                    if (m + j < a.lddz) store4_from_f32(a.dz, a.dz_dt, (rb + t) * a.lddz + m + j, o);
+                }
+            }
+        }
     }
     if (a.part != nullptr)
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (j < cols) a.part[grp * M + m + j] = sum[j];
+        for (int j = 0; j < V; ++j)
+            if (j < cols) a.part[chunk * M + m + j] = sum[j];
+}
+
+static int preact_rows(int64_t N, int64_t M) { return N * M < (4ll << 20) ? 8 : 32; }
+
+template <typename TG> static void launch_preact(const PreactArgs& a, int z_kind, int64_t N, int64_t M, hipStream_t s) {
+    constexpr int V = 16 / sizeof(TG);
+    const int64_t pieces = cdiv(a.dz != nullptr ? a.lddz : M, V);
+    const dim3 grid((unsigned)cdiv(cdiv(N, a.per) * pieces, 256)), block(256);
+    if (a.act == SPHIP_ACT_NONE) hipLaunchKernelGGL((linear_preact_kernel<TG, -1>), grid, block, 0, s, a, N, (int)M);
+    else if (z_kind == SPHIP_F32) hipLaunchKernelGGL((linear_preact_kernel<TG, SPHIP_F32>), grid, block, 0, s, a, N, (int)M);
+    else if (z_kind == SPHIP_BF16) hipLaunchKernelGGL((linear_preact_kernel<TG, SPHIP_BF16>), grid, block, 0, s, a, N, (int)M);
+    else if (z_kind == SPHIP_INT8) hipLaunchKernelGGL((linear_preact_kernel<TG, SPHIP_INT8>), grid, block, 0, s, a, N, (int)M);
+    else hipLaunchKernelGGL((linear_preact_kernel<TG, SPHIP_E4M3>), grid, block, 0, s, a, N, (int)M);
 }
 
 // column sums of part (P, M) in row order by 16 interleaved chains: 64 columns per workgroup of 1024 threads
@@ -509,7 +556,7 @@ extern "C" int sphip_linear(const void* x, int64_t ldx, const void* W, int64_t l
     return st;
 }
 
-// workspace: dz | column sums of 32-row groups | x restored (8-bit x in the 256 x 256 kernel) | partial tiles of a product
+// workspace: dz | column sums of row chunks | x restored (8-bit x in the 256 x 256 kernel) | partial tiles of a product
 struct BackwardSpace {
     size_t dz, sums, xr, part, total;
 };
@@ -518,7 +565,7 @@ static BackwardSpace backward_space(int dtype, int x_kind, int want_dx, int want
     BackwardSpace b;
     const bool products = want_dx || want_dw;
     b.dz = products ? up256((size_t)N * dz_stride(dtype, M) * dtype_size(dtype)) : 0;
-    b.sums = want_db ? up256((size_t)cdiv(N, 32) * M * 4) : 0;
+    b.sums = want_db ? up256((size_t)cdiv(N, preact_rows(N, M)) * M * 4) : 0;
     b.xr = want_dw && dtype == SPHIP_BF16 && is_codes(x_kind) && wants256(M, D, N) ? up256((size_t)N * (cdiv(D, 16) * 16) * 2) : 0;
     const size_t p1 = want_dx ? split_bytes(dtype, N, D, cdiv(M, 64) * 64) : 0, p2 = want_dw ? split_bytes(dtype, M, D, N) : 0;
     b.part = p1 > p2 ? p1 : p2;
@@ -606,15 +653,15 @@ extern "C" int sphip_linear_backward(const void* g, int g_dtype, int64_t ldg, co
     if (db || (products && !direct)) {
         PreactArgs a;
         a.g = g, a.z = z, a.scales = z_scales, a.dz = products && !direct ? w : nullptr, a.part = db ? sums : nullptr;
-        a.ldg = ldg, a.ldz = ldz, a.lddz = dz.ld, a.g_dt = g_dtype, a.z_kind = z_kind, a.dz_dt = dtype, a.act = act;
-        a.vec = aligned4(g, g_dtype, ldg) && (act == SPHIP_ACT_NONE || zc || aligned4(z, z_kind, ldz));
-        const int64_t P = cdiv(N, 32), quads = (a.dz ? a.lddz : M + 3) / 4, blocks = cdiv(P * quads, 256);
-        SPHIP_REQUIRE(blocks < (1ll << 31), SPHIP_EUNSUPPORTED, "linear_backward: grid too large");
-        hipLaunchKernelGGL(linear_preact_kernel, dim3((unsigned)blocks), dim3(256), 0, s, a, N, (int)M);
+        a.ldg = ldg, a.ldz = ldz, a.lddz = dz.ld, a.dz_dt = dtype, a.act = act, a.per = preact_rows(N, M);
+        SPHIP_REQUIRE(cdiv(cdiv(N, a.per) * cdiv(dz.ld > M ? dz.ld : M, 4), 256) < (1ll << 31), SPHIP_EUNSUPPORTED,
+                      "linear_backward: grid too large");
+        if (g_dtype == SPHIP_BF16) launch_preact<bf16_t>(a, z_kind, N, M, s);
+        else launch_preact<float>(a, z_kind, N, M, s);
         SPHIP_CHECK_LAUNCH("linear_backward(dz)");
         if (db) {
-            hipLaunchKernelGGL(linear_bias_grad_kernel, dim3((unsigned)cdiv(M, 64)), dim3(1024), 0, s, (const float*)sums, P,
-                               (int)M, db, db_dtype);
+            hipLaunchKernelGGL(linear_bias_grad_kernel, dim3((unsigned)cdiv(M, 64)), dim3(1024), 0, s, (const float*)sums,
+                               cdiv(N, a.per), (int)M, db, db_dtype);
             SPHIP_CHECK_LAUNCH("linear_backward(db)");
         }
     }

@@ -120,8 +120,10 @@ template <int MODE, int WHICH> struct Source {
             const int kr = tid >> LOG, f = (kr & 3) + 4 * ((kr >> 3) & 1);
             const int c = (tid & ((1 << LOG) - 1)) ^ (2 * f);
             const int col = WHICH == 0 ? c * 8 : (c >> 3) * 128 + (c & 7) * 8;
+            // (the end rounded up to a piece: a dword that crosses the end reads as zero, with it the last of an odd number
+            // of rows; rows are 16-byte aligned, so the piece is the one that holds the last element)
             rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)(p + k0 * o.ld + row0), 0,
-                                                     (int)(K > k0 ? (unsigned)(K - 1 - k0) * ld2 + (unsigned)(o.rows - row0) * 2u : 0u),
+                                                     (int)(K > k0 ? (unsigned)(K - 1 - k0) * ld2 + ((unsigned)(o.rows - row0) * 2u + 15u) / 16u * 16u : 0u),
                                                      0x00020000);
             voff = (unsigned)kr * ld2 + (unsigned)col * 2u;
             piece = (512u >> LOG) * ld2;
@@ -250,11 +252,34 @@ __global__ __launch_bounds__(512, 2) void linear256_kernel(Operand A, Operand B,
     if (wm == 0) segment_barrier();          // matches the stagger barrier of the other group
 
     // ---- epilogue. A lane holds 4 consecutive m of one n per accumulator; each wave turns its 64 x 128 part in two halves
-    // of 64 x 64 through a private LDS area (the operand image is dead), so that 16 lanes store 64 consecutive m of a row.
+    // of 64 x 64 through a private LDS area (the operand image is dead), so that 16 lanes store 64 consecutive m of a row
+    // and a lane keeps its m: one bias load per half. The half's 16 residual pieces are all in flight before the first is
+    // used (one workgroup runs per compute unit: nothing else hides their latency). Residual and result bypass L2, which
+    // holds the operands.
     const int N = A.rows, M = B.rows, Mp = (M + 3) & ~3;
     char* const stage = smem + wave * OUT_WAVE;
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
+        const int m = m0 + wm * 128 + half * 64 + r16 * 4, nb = n0 + wn * 64 + q4;
+        const bool whole = g.splits == 1 && epi.vec && m + 3 < M;
+        w4_t res[16];
+        float bias[4] = {0.f, 0.f, 0.f, 0.f};
+        if (whole && epi.res != nullptr) {
+            if (epi.res_dt == SPHIP_F32) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (nb + 4 * i < N)
+                        res[i] = __builtin_nontemporal_load((const w4_t*)((const float*)epi.res + (int64_t)(nb + 4 * i) * epi.ldr + m));
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (nb + 4 * i < N) {
+                        const w2_t r = __builtin_nontemporal_load((const w2_t*)((const bf16_t*)epi.res + (int64_t)(nb + 4 * i) * epi.ldr + m));
+                        res[i] = (w4_t){r.x << 16, r.x & 0xffff0000u, r.y << 16, r.y & 0xffff0000u};
+                    }
+            }
+        }
+        if (whole && epi.bias != nullptr) load4_as_f32(epi.bias, epi.bias_dt, m, bias);
 #pragma unroll
         for (int mt = 0; mt < 4; ++mt)
 #pragma unroll
@@ -263,15 +288,41 @@ __global__ __launch_bounds__(512, 2) void linear256_kernel(Operand A, Operand B,
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-        const int m = m0 + wm * 128 + half * 64 + r16 * 4;
+        if (whole) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int n = nb + 4 * i;
+                if (n >= N) continue;
+                const float4 c = *reinterpret_cast<const float4*>(stage + (i * 4 + q4) * OUT_ROW + r16 * 16);
+                float v[4] = {c.x + bias[0], c.y + bias[1], c.z + bias[2], c.w + bias[3]};
+                if (epi.z != nullptr) store4_from_f32(epi.z, epi.z_dt, n * epi.ldz + m, v);
+                if (epi.act != SPHIP_ACT_NONE) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v[j] = act_value(v[j], epi.act);
+                }
+                if (epi.res != nullptr) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v[j] += __uint_as_float(res[i][j]);
+                }
+                if (epi.out_dt == SPHIP_F32) {
+                    const acc4_t o = {v[0], v[1], v[2], v[3]};
+                    __builtin_nontemporal_store(o, (acc4_t*)((float*)epi.out + n * epi.ldo + m));
+                } else {
+                    const w2_t o = {(unsigned)f32_to_bf16(v[0]) | ((unsigned)f32_to_bf16(v[1]) << 16),
+                                    (unsigned)f32_to_bf16(v[2]) | ((unsigned)f32_to_bf16(v[3]) << 16)};
+                    __builtin_nontemporal_store(o, (w2_t*)((bf16_t*)epi.out + n * epi.ldo + m));
+                }
+            }
+        } else if (m < M) {
 #pragma unroll 4
-        for (int i = 0; i < 16; ++i) {
-            const int row = i * 4 + q4, n = n0 + wn * 64 + row;
-            const float4 c = *reinterpret_cast<const float4*>(stage + row * OUT_ROW + r16 * 16);
-            if (n >= N || m >= M) continue;
-            float v[4] = {c.x, c.y, c.z, c.w};
-            if (g.splits > 1) *reinterpret_cast<float4*>(g.part + ((int64_t)split * N + n) * Mp + m) = c;
-            else epilogue4(epi, n, m, M, v);
+            for (int i = 0; i < 16; ++i) {
+                const int n = nb + 4 * i;
+                if (n >= N) continue;
+                const float4 c = *reinterpret_cast<const float4*>(stage + (i * 4 + q4) * OUT_ROW + r16 * 16);
+                float v[4] = {c.x, c.y, c.z, c.w};
+                if (g.splits > 1) *reinterpret_cast<float4*>(g.part + ((int64_t)split * N + n) * Mp + m) = c;
+                else epilogue4(epi, n, m, M, v);
+            }
         }
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();

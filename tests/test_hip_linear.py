@@ -374,6 +374,38 @@ def test_gradient_against_differences(device, act, fmt):
         assert abs(float(got - num)) <= float(trunc + noise + kept) + 1e-3, (i, float(got), float(num))
 
 
+@pytest.mark.parametrize("N,D,M", [(256, 64, 256), (300, 128, 520), (1000, 192, 704), (64, 1024, 136), (257, 256, 255), (1030, 320, 1000),
+                                   (2048, 128, 257), (1, 64, 64)])
+def test_the_256_tile_kernel(device, monkeypatch, N, D, M):
+    """The large-shape kernel on small and ragged shapes (SPHIP_GEMM=256): forward, and both gradient products with their
+    K-strided operands, split over K and whole, against the definition."""
+    from sparsify_amd import ops
+    monkeypatch.setenv("SPHIP_GEMM", "256")
+    ops._linear_bytes.cache_clear(), ops._linear_backward_bytes.cache_clear()
+    try:
+        for i, (act, fmt) in enumerate([("none", "int8"), ("gelu", None), ("relu", "e4m3"), ("silu", "int8")]):
+            res = [None, torch.float32, torch.bfloat16, None][i]
+            x, W, b, r = make(N, D, M, torch.bfloat16, N + i, bias=i != 1, res=res)
+            out_dtype = torch.bfloat16 if res is None else res
+            xc, Wc, bc, rc = cuda(x, W, b, r)
+            y, zk, _ = ops.linear(xc, Wc, bc, rc, act, keep_z=torch.float32)
+            want, tol, z, ez = forward64(x, W, b, r, act, out_dtype)
+            assert_within(y, want, tol, f"y {act}")
+            assert_within(zk, z, ez + HALF[torch.float32] * z.abs() + TINY, f"z {act}")
+            _, zq, xq = ops.linear(xc, Wc, bc, rc, act, keep_z=fmt or torch.bfloat16, keep_x=fmt)
+            zhat = ops.checkpoint8_restore(zq, fmt, N, M, torch.float32) if fmt else zq
+            g = torch.randn(N, M, generator=torch.Generator().manual_seed(i)).to(out_dtype)
+            dx, dW, db = ops.linear_backward(g.cuda(), Wc, zq, xq if fmt else xc, act, z_fmt=fmt, x_fmt=fmt,
+                                             dx_dtype=torch.bfloat16, dw_dtype=torch.bfloat16, db_dtype=torch.bfloat16)
+            ref = backward64(x, W, torch.zeros(M, dtype=torch.bfloat16), act, g, zhat.double().cpu(),
+                             codes64(x, fmt) if fmt else x, torch.bfloat16, torch.bfloat16, 0.0)
+            for n, got in (("x", dx), ("W", dW), ("b", db)):
+                assert_within(got, *ref[n], f"d{n} {act} {N}x{D}x{M}")
+    finally:
+        monkeypatch.undo()
+        ops._linear_bytes.cache_clear(), ops._linear_backward_bytes.cache_clear()
+
+
 def test_only_the_asked_gradients_and_reuse(device):
     from sparsify_amd import checkpoint8, fused_linear
     x, W, b, r = cuda(*make(200, 96, 64, torch.bfloat16, 4, res=torch.float32))
