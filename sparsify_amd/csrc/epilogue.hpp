@@ -31,6 +31,20 @@ __device__ __forceinline__ float act_value(float z, int act) {
     return z;
 }
 
+// four at once, the choice of activation outside
+__device__ __forceinline__ void act_value4(float (&v)[4], int act) {
+    if (act == SPHIP_ACT_RELU) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = act_value(v[j], SPHIP_ACT_RELU);
+    } else if (act == SPHIP_ACT_GELU) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = act_value(v[j], SPHIP_ACT_GELU);
+    } else if (act == SPHIP_ACT_SILU) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = act_value(v[j], SPHIP_ACT_SILU);
+    }
+}
+
 __device__ __forceinline__ float act_slope(float z, int act) {
     if (act == SPHIP_ACT_RELU) return z > 0.f ? 1.f : (z != z ? z : 0.f);
     if (act == SPHIP_ACT_SILU) {
@@ -57,19 +71,29 @@ struct Epilogue {
     int64_t ldr = 0, ldo = 0, ldz = 0;
     int bias_dt = 0, res_dt = 0, out_dt = 0, z_dt = 0;
     int act = 0;
-    int vec = 0;                      // every row of res / out / z / bias takes 4-element vector accesses
 };
 
+// four consecutive elements at any element-aligned address (the hardware splits what is not 8- or 16-byte aligned; still
+// one instruction where element accesses would be four)
+typedef unsigned u2_any __attribute__((ext_vector_type(2), aligned(2)));
+typedef unsigned u4_any __attribute__((ext_vector_type(4), aligned(4)));
+
 __device__ __forceinline__ void load4_as_f32(const void* p, int dt, int64_t i, float (&v)[4]) {
-    const float4 t = dt == SPHIP_BF16 ? load4((const bf16_t*)p + i) : load4((const float*)p + i);
-    v[0] = t.x, v[1] = t.y, v[2] = t.z, v[3] = t.w;
+    if (dt == SPHIP_BF16) {
+        const u2_any u = *(const u2_any*)((const bf16_t*)p + i);
+        v[0] = __uint_as_float(u.x << 16), v[1] = __uint_as_float(u.x & 0xffff0000u);
+        v[2] = __uint_as_float(u.y << 16), v[3] = __uint_as_float(u.y & 0xffff0000u);
+    } else {
+        const u4_any u = *(const u4_any*)((const float*)p + i);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = __uint_as_float(u[j]);
+    }
 }
 __device__ __forceinline__ void store4_from_f32(void* p, int dt, int64_t i, const float (&v)[4]) {
     if (dt == SPHIP_BF16)
-        *reinterpret_cast<uint2*>((bf16_t*)p + i) =
-            make_uint2((unsigned)f32_to_bf16(v[0]) | ((unsigned)f32_to_bf16(v[1]) << 16),
-                       (unsigned)f32_to_bf16(v[2]) | ((unsigned)f32_to_bf16(v[3]) << 16));
-    else *reinterpret_cast<float4*>((float*)p + i) = make_float4(v[0], v[1], v[2], v[3]);
+        *(u2_any*)((bf16_t*)p + i) = (u2_any){(unsigned)f32_to_bf16(v[0]) | ((unsigned)f32_to_bf16(v[1]) << 16),
+                                              (unsigned)f32_to_bf16(v[2]) | ((unsigned)f32_to_bf16(v[3]) << 16)};
+    else *(u4_any*)((float*)p + i) = (u4_any){__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
 }
 __device__ __forceinline__ void store_from_f32(void* p, int dt, int64_t i, float v) {
     if (dt == SPHIP_BF16) ((bf16_t*)p)[i] = f32_to_bf16(v);
@@ -78,7 +102,7 @@ __device__ __forceinline__ void store_from_f32(void* p, int dt, int64_t i, float
 
 // outputs (n, m .. m + 3) of the accumulated product v; columns past M are left alone
 __device__ __forceinline__ void epilogue4(const Epilogue& e, int64_t n, int m, int M, float (&v)[4]) {
-    if (e.vec && m + 3 < M) {
+    if (m + 3 < M) {
         if (e.bias != nullptr) {
             float b[4];
             load4_as_f32(e.bias, e.bias_dt, m, b);
@@ -86,10 +110,7 @@ __device__ __forceinline__ void epilogue4(const Epilogue& e, int64_t n, int m, i
             for (int j = 0; j < 4; ++j) v[j] += b[j];
         }
         if (e.z != nullptr) store4_from_f32(e.z, e.z_dt, n * e.ldz + m, v);
-        if (e.act != SPHIP_ACT_NONE) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = act_value(v[j], e.act);
-        }
+        act_value4(v, e.act);
         if (e.res != nullptr) {
             float r[4];
             load4_as_f32(e.res, e.res_dt, n * e.ldr + m, r);
@@ -100,7 +121,7 @@ __device__ __forceinline__ void epilogue4(const Epilogue& e, int64_t n, int m, i
         return;
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < 3; ++j) {
         if (m + j >= M) continue;
         float t = v[j];
         if (e.bias != nullptr) t += load_as_f32(e.bias, e.bias_dt, m + j);

@@ -19,7 +19,6 @@
 namespace sphip {
 
 typedef __bf16 lbf16x8 __attribute__((ext_vector_type(8)));
-typedef float lf32x2 __attribute__((ext_vector_type(2)));
 typedef float lf32x4 __attribute__((ext_vector_type(4)));
 typedef float lf32x16 __attribute__((ext_vector_type(16)));
 
@@ -251,26 +250,19 @@ __global__ __launch_bounds__(256, 2) void linear_tile_kernel(Operand A, Operand 
         __syncthreads();
     }
 
+    // 4 consecutive m of one n per accumulator quad: 32 n x 64 m per wave and pass through its part of the (dead) image
     const int N = A.rows, M = B.rows;
-    const int Mp = (M + 3) & ~3;
+    char* const stage = reinterpret_cast<char*>(lds) + wave * 32 * OUT_ROW;
 #pragma unroll
-    for (int mi = 0; mi < 2; ++mi)
+    for (int ni = 0; ni < 2; ++ni) {
 #pragma unroll
-        for (int qd = 0; qd < 4; ++qd) {
-            const int m = m0 + wm * 64 + mi * 32 + 8 * qd + 4 * h;
-            if (m >= M) continue;
+        for (int mi = 0; mi < 2; ++mi)
 #pragma unroll
-            for (int ni = 0; ni < 2; ++ni) {
-                const int n = n0 + wn * 64 + ni * 32 + r;
-                if (n >= N) continue;
-                float v[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) v[j] = acc[mi][ni][4 * qd + j];
-                if (g.splits > 1)
-                    *reinterpret_cast<float4*>(g.part + ((int64_t)split * N + n) * Mp + m) = make_float4(v[0], v[1], v[2], v[3]);
-                else epilogue4(epi, n, m, M, v);
-            }
-        }
+            for (int qd = 0; qd < 4; ++qd)
+                *reinterpret_cast<float4*>(stage + r * OUT_ROW + (mi * 32 + 8 * qd + 4 * h) * 4) =
+                    make_float4(acc[mi][ni][4 * qd], acc[mi][ni][4 * qd + 1], acc[mi][ni][4 * qd + 2], acc[mi][ni][4 * qd + 3]);
+        finish_rows<32>(stage, epi, g, split, n0 + wn * 64 + ni * 32, m0 + wm * 64, N, M, lane);
+    }
 }
 
 // Sum of the splits' partial tiles in split order, then the epilogue. One thread per 4 outputs.
@@ -303,33 +295,44 @@ static int split_count(int64_t N, int64_t M, int64_t steps) {
 static size_t part_bytes(int64_t N, int64_t M, int splits) {
     return splits > 1 ? (size_t)splits * N * ((M + 3) / 4 * 4) * 4 : 0;
 }
-// the most a product needs for its partial tiles, whichever kernel takes it
-static size_t split_bytes(int dtype, int64_t N, int64_t M, int64_t K) {
-    const size_t a = part_bytes(N, M, split_count(N, M, cdiv(K, dtype == SPHIP_BF16 ? 64 : 32)));
-    const size_t b = dtype == SPHIP_BF16 ? part_bytes(N, M, linear256_splits(N, M, cdiv(K, 64) * 64)) : 0;
-    return a > b ? a : b;
+// Which kernel a bf16 product of these sizes goes to if its operands are such that LDS-DMA can fetch them.
+enum { BY_TILES = 0, BY_128 = 1, BY_256 = 2 };
+static int kernel_for(int64_t N, int64_t M) {
+    // SPHIP_LINEAR=tile|128|256 forces a kernel (tests, A/B runs)
+    const char* force = getenv("SPHIP_LINEAR");
+    if (force) return force[0] == '2' ? BY_256 : force[0] == '1' ? BY_128 : BY_TILES;
+    // The 256 x 256 kernel where its tiles fill most of the 256 compute units once: 16384 x 1024 x 4096 takes 101 us against
+    // 118 with 128 x 128 tiles, 8192 x 2048 x 2048 56 against 68. Below, splitting K for the large tile costs more than the
+    // smaller tile does: 1000 x 4096 x 4096 (64 large tiles) 47 us against 41, 2048^3 37 against 25.
+    return cdiv(N, 256) * cdiv(M, 256) >= 160 ? BY_256 : BY_128;
+}
+static int splits_of(int by, int64_t N, int64_t M, int64_t K) {
+    return by == BY_256 ? 1 : by == BY_128 ? linear128_splits(N, M, K) : split_count(N, M, cdiv(K, 64));
 }
 
-// Whether an (N, M) product over K is worth the 256 x 256 kernel (bf16): it has to fill most of the 256 compute units with
-// one workgroup each. SPHIP_GEMM=128|256 forces a kernel (tests), as for the encoder.
-static bool wants256(int64_t N, int64_t M, int64_t K) {
-    const char* force = getenv("SPHIP_GEMM");
-    if (force) return force[0] == '2';
-    const int64_t tiles = cdiv(N, 256) * cdiv(M, 256);
-    return tiles * linear256_splits(N, M, K) >= 160;
+// the most a product needs for its partial tiles, whichever kernel takes it
+static size_t split_bytes(int dtype, int64_t N, int64_t M, int64_t K) {
+    if (dtype != SPHIP_BF16) return part_bytes(N, M, split_count(N, M, cdiv(K, 32)));
+    const int64_t Kp = cdiv(K, 64) * 64;
+    const size_t a = part_bytes(N, M, split_count(N, M, cdiv(K, 64))), b = part_bytes(N, M, splits_of(kernel_for(N, M), N, M, Kp));
+    return a > b ? a : b;
 }
 
 template <typename T, int MODE_A, int MODE_B>
 static int launch_product(const char* what, const Operand& A, const Operand& B, const Epilogue& epi, int64_t K, int64_t KB,
                           void* ws, size_t ws_bytes, hipStream_t s) {
-    constexpr int STEP = LCH * Chunk<T>::E;
     const int64_t N = A.rows, M = B.rows;
-    const bool big = sizeof(T) == 2 && wants256(N, M, K) && linear256_takes(MODE_A, MODE_B, A, B, K);
-    const int tile = big ? 256 : LT;
-    const int64_t steps = cdiv(K, STEP);
+    int by = BY_TILES;
+    if (sizeof(T) == 2 && MODE_B <= OP_COLS) {
+        by = kernel_for(N, M);
+        if (by == BY_256 && !linear256_takes(MODE_A, MODE_B, A, B, K)) by = BY_TILES;
+        if (by == BY_128 && !linear128_takes(MODE_A, MODE_B, A, B, K)) by = BY_TILES;
+    }
+    const int tile = by == BY_256 ? 256 : 128;
+    const int64_t steps = cdiv(K, LCH * Chunk<T>::E);
     TileGrid g;
     g.tilesM = (int)cdiv(M, tile), g.tilesN = (int)cdiv(N, tile);
-    const int want = big ? linear256_splits(N, M, K) : split_count(N, M, steps);
+    const int want = by == BY_TILES ? split_count(N, M, steps) : splits_of(by, N, M, K);
     g.steps_per = (int)cdiv(steps, want);
     g.splits = (int)cdiv(steps, g.steps_per);
     g.part = (float*)ws;
@@ -341,8 +344,9 @@ static int launch_product(const char* what, const Operand& A, const Operand& B, 
     const int64_t nblocks = (int64_t)g.tilesM * g.tilesN * g.splits, threads = N * ((M + 3) / 4);
     SPHIP_REQUIRE(nblocks < (1ll << 31) && (g.splits == 1 || cdiv(threads, 256) < (1ll << 31)), SPHIP_EUNSUPPORTED,
                   "%s: grid too large", what);
-    if (big) {
-        const int st = launch_linear256(what, MODE_A, MODE_B, A, B, epi, K, KB, g, s);
+    if (by != BY_TILES) {
+        const int st = by == BY_256 ? launch_linear256(what, MODE_A, MODE_B, A, B, epi, K, KB, g, s)
+                                    : launch_linear128(what, MODE_A, MODE_B, A, B, epi, K, KB, g, s);
         if (st != SPHIP_OK) return st;
     } else {
         hipLaunchKernelGGL((linear_tile_kernel<T, MODE_A, MODE_B>), dim3((unsigned)nblocks), dim3(256), 0, s, A, B, epi, K, KB, g);
@@ -356,25 +360,43 @@ static int launch_product(const char* what, const Operand& A, const Operand& B, 
     return SPHIP_OK;
 }
 
-static inline bool aligned4(const void* p, int dt, int64_t ld) {
-    return ((uintptr_t)p % (4 * dtype_size(dt))) == 0 && ld % 4 == 0;
+// bf16 rows copied to a 16-byte aligned stride that is a multiple of 64, zeros behind them: what LDS-DMA asks of an operand
+__global__ __launch_bounds__(256) void linear_pack_kernel(const bf16_t* __restrict__ src, int64_t ld, int rows, int cols,
+                                                          bf16_t* __restrict__ dst, int pieces) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t row = i / pieces;
+    if (row >= rows) return;
+    const int c = (int)(i % pieces) * 8;
+    *reinterpret_cast<uint4*>(dst + i * 8) = Chunk<bf16_t>::load(src + row * ld + c, cols - c);
 }
-static void set_vec(Epilogue& e) {
-    e.vec = aligned4(e.out, e.out_dt, e.ldo) && (e.bias == nullptr || aligned4(e.bias, e.bias_dt, 0)) &&
-            (e.res == nullptr || aligned4(e.res, e.res_dt, e.ldr)) && (e.z == nullptr || aligned4(e.z, e.z_dt, e.ldz));
+static int64_t packed_ld(int64_t cols) { return cdiv(cols, 64) * 64; }
+static int pack_rows(const char* what, Operand& o, int64_t rows, int64_t cols, void* dst, hipStream_t s) {
+    const int64_t ld = packed_ld(cols), threads = rows * (ld / 8);
+    SPHIP_REQUIRE(cdiv(threads, 256) < (1ll << 31), SPHIP_EUNSUPPORTED, "%s: grid too large", what);
+    hipLaunchKernelGGL(linear_pack_kernel, dim3((unsigned)cdiv(threads, 256)), dim3(256), 0, s, (const bf16_t*)o.p, o.ld, (int)rows,
+                       (int)cols, (bf16_t*)dst, (int)(ld / 8));
+    SPHIP_CHECK_LAUNCH(what);
+    o.p = dst, o.ld = ld;
+    return SPHIP_OK;
+}
+// Whether a bf16 product is worth copying an operand whose rows LDS-DMA cannot fetch (they do not start at multiples of 16
+// bytes, or K is no multiple of 64)
+static bool worth_packing(int64_t N, int64_t M, int64_t K) {
+    const char* force = getenv("SPHIP_LINEAR");
+    return force ? force[0] != 't' : N * M * K >= (1ll << 27);
 }
 
-// ---- dz = g act'(z) and its column sums. A thread owns 16 bytes of g's columns (4 fp32 or 8 bf16) of `per` rows, 8 rows
-// of loads in flight; its rows' sums go to part[row chunk][M], added up in order by the second kernel. per = 32 (the group
-// one scale of an 8-bit z covers) or, where that leaves the chip empty, 8.
+// ---- dz = g act'(z) and its column sums. A workgroup takes 32 rows (the group one scale of an 8-bit z covers) of 32 x 16
+// bytes of columns: 32 lanes side by side, 8 rows at a time, every thread 4 rows whose loads are all in flight; the 8 row
+// sums of a column meet in LDS and go to part[row group][M], added up in order by the second kernel.
 struct PreactArgs {
     const void* g;
     const void* z;                 // values or codes, row stride ldz
     const uint8_t* scales;
     void* dz;                      // row stride lddz (zeros in [M, lddz)), or null
-    float* part;                   // [ceil(N / per)][M], or null
+    float* part;                   // [ceil(N / 32)][M], or null
     int64_t ldg, ldz, lddz;
-    int dz_dt, act, per;
+    int dz_dt, act, strips;        // strips: workgroups side by side along a row
 };
 
 template <int V> __device__ __forceinline__ void load_row(const bf16_t* p, int n, float (&v)[V]) {
@@ -396,82 +418,85 @@ template <int V> __device__ __forceinline__ void load_row(const float* p, int n,
 // ZK: SPHIP_F32, SPHIP_BF16, SPHIP_INT8, SPHIP_E4M3, or -1: no activation, z is not read
 template <typename TG, int ZK>
 __global__ __launch_bounds__(256) void linear_preact_kernel(PreactArgs a, int64_t N, int M) {
-    constexpr int V = 16 / sizeof(TG), B = 8;
-    const int pieces = (int)((a.dz != nullptr ? a.lddz : M) + V - 1) / V;
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int64_t chunk = i / pieces, r0 = chunk * a.per;
-    if (r0 >= N) return;
-    const int m = (int)(i % pieces) * V, cols = min(V, M - m);            // <= 0: padding columns of dz
-    const int64_t r1 = min(N, r0 + a.per);
-    float sc[V], sum[V];
+    constexpr int V = 16 / sizeof(TG), B = 4;
+    constexpr bool CODES = ZK == SPHIP_INT8 || ZK == SPHIP_E4M3;
+    __shared__ float red[8][32 * V];
+    const int cl = threadIdx.x & 31, rl = threadIdx.x >> 5;
+    const int64_t grp = blockIdx.x / (unsigned)a.strips, r0 = grp * 32 + rl;
+    const int m = ((int)(blockIdx.x % (unsigned)a.strips) * 32 + cl) * V, cols = min(V, M - m);    // <= 0: padding of dz
+    float sum[V], v[B][V], z[B][V];
+    unsigned q[B][V / 4];
+    uint8_t s8[V];
 #pragma unroll
-    for (int j = 0; j < V; ++j) sum[j] = 0.f, sc[j] = 0.f;
-    if ((ZK == SPHIP_INT8 || ZK == SPHIP_E4M3) && cols > 0) {
-        uint8_t s8[V];                                                    // (rows of codes are padded to 16: whole pieces)
-        __builtin_memcpy(s8, a.scales + (r0 >> 5) * a.ldz + m, V);
+    for (int j = 0; j < V; ++j) sum[j] = 0.f, s8[j] = 0;
+    if (CODES && cols > 0) __builtin_memcpy(s8, a.scales + grp * a.ldz + m, V);      // (code rows are padded to 16: whole pieces)
 #pragma unroll
-        for (int j = 0; j < V; ++j) sc[j] = scale_value(s8[j]);
+    for (int t = 0; t < B; ++t) {
+        const int64_t row = r0 + 8 * t;
+        const int n = row < N ? cols : 0;
+        load_row<V>((const TG*)a.g + row * a.ldg + m, n, v[t]);
+        if (ZK == SPHIP_F32) load_row<V>((const float*)a.z + row * a.ldz + m, n, z[t]);
+        if (ZK == SPHIP_BF16) load_row<V>((const bf16_t*)a.z + row * a.ldz + m, n, z[t]);
+        if (CODES) {
+#pragma unroll
+            for (int j = 0; j < V / 4; ++j) q[t][j] = 0;
+            if (n > 0) __builtin_memcpy(q[t], (const uint8_t*)a.z + row * a.ldz + m, V);
+        }
     }
-    for (int64_t rb = r0; rb < r1; rb += B) {
-        float v[B][V], z[B][V];
-        unsigned q[B][V / 4];
 #pragma unroll
-        for (int t = 0; t < B; ++t) {
-            const int n = rb + t < r1 ? cols : 0;
-            load_row<V>((const TG*)a.g + (rb + t) * a.ldg + m, n, v[t]);
-            if (ZK == SPHIP_F32) load_row<V>((const float*)a.z + (rb + t) * a.ldz + m, n, z[t]);
-            if (ZK == SPHIP_BF16) load_row<V>((const bf16_t*)a.z + (rb + t) * a.ldz + m, n, z[t]);
-            if (ZK == SPHIP_INT8 || ZK == SPHIP_E4M3) {
+    for (int t = 0; t < B; ++t) {
+        const int64_t row = r0 + 8 * t;
+        if (CODES) {
 #pragma unroll
-                for (int j = 0; j < V / 4; ++j) q[t][j] = 0;
-                if (n > 0) __builtin_memcpy(q[t], (const uint8_t*)a.z + (rb + t) * a.ldz + m, V);
+            for (int j = 0; j < V / 4; ++j) {
+                const float s4[4] = {scale_value(s8[4 * j]), scale_value(s8[4 * j + 1]), scale_value(s8[4 * j + 2]), scale_value(s8[4 * j + 3])};
+                float o[4];
+                code_values<ZK == SPHIP_INT8 ? SPHIP_INT8 : SPHIP_E4M3>(q[t][j], s4, o);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) z[t][4 * j + c] = o[c];
             }
         }
+        if (row >= N) continue;
 #pragma unroll
-        for (int t = 0; t < B; ++t) {
-            if (rb + t >= r1) break;
-            if (ZK >= 0) {
-                if (ZK == SPHIP_INT8 || ZK == SPHIP_E4M3) {
+        for (int j = 0; j < V; ++j) {
+            if (ZK >= 0) v[t][j] = j < cols ? v[t][j] * act_slope(z[t][j], a.act) : 0.f;
+            sum[j] += v[t][j];
+        }
+        if (a.dz != nullptr) {
 #pragma unroll
-                    for (int j = 0; j < V / 4; ++j) {
-                        const float s4[4] = {sc[4 * j], sc[4 * j + 1], sc[4 * j + 2], sc[4 * j + 3]};
-                        float o[4];
-                        code_values<ZK == SPHIP_INT8 ? SPHIP_INT8 : SPHIP_E4M3>(q[t][j], s4, o);
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) z[t][4 * j + c] = o[c];
-                    }
-                }
-#pragma unroll
-                for (int j = 0; j < V; ++j) v[t][j] = j < cols ? v[t][j] * act_slope(z[t][j], a.act) : 0.f;
-            }
-#pragma unroll
-            for (int j = 0; j < V; ++j) sum[j] += v[t][j];
-            if (a.dz != nullptr) {
-#pragma unroll
-                for (int j = 0; j < V; j += 4) {
-                    const float o[4] = {v[t][j], v[t][j + 1], v[t][j + 2], v[t][j + 3]};
-                    if (m + j < a.lddz) store4_from_f32(a.dz, a.dz_dt, (rb + t) * a.lddz + m + j, o);
-                }
+            for (int j = 0; j < V; j += 4) {
+                const float o[4] = {v[t][j], v[t][j + 1], v[t][j + 2], v[t][j + 3]};
+                if (m + j < a.lddz) store4_from_f32(a.dz, a.dz_dt, row * a.lddz + m + j, o);
             }
         }
     }
-    if (a.part != nullptr)
+    if (a.part == nullptr) return;
 #pragma unroll
-        for (int j = 0; j < V; ++j)
-            if (j < cols) a.part[chunk * M + m + j] = sum[j];
+    for (int j = 0; j < V; ++j) red[rl][cl * V + j] = sum[j];
+    __syncthreads();
+    for (int c = threadIdx.x; c < 32 * V; c += 256) {
+        const int col = (int)(blockIdx.x % (unsigned)a.strips) * 32 * V + c;
+        if (col >= M) continue;
+        float t = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) t += red[i][c];
+        a.part[grp * M + col] = t;
+    }
 }
 
-static int preact_rows(int64_t N, int64_t M) { return N * M < (4ll << 20) ? 8 : 32; }
-
-template <typename TG> static void launch_preact(const PreactArgs& a, int z_kind, int64_t N, int64_t M, hipStream_t s) {
+template <typename TG> static int launch_preact(PreactArgs& a, int z_kind, int64_t N, int64_t M, hipStream_t s) {
     constexpr int V = 16 / sizeof(TG);
-    const int64_t pieces = cdiv(a.dz != nullptr ? a.lddz : M, V);
-    const dim3 grid((unsigned)cdiv(cdiv(N, a.per) * pieces, 256)), block(256);
+    const int64_t strips = cdiv(a.dz != nullptr ? a.lddz : M, 32 * V), blocks = cdiv(N, 32) * strips;
+    SPHIP_REQUIRE(blocks < (1ll << 31), SPHIP_EUNSUPPORTED, "linear_backward: grid too large");
+    a.strips = (int)strips;
+    const dim3 grid((unsigned)blocks), block(256);
     if (a.act == SPHIP_ACT_NONE) hipLaunchKernelGGL((linear_preact_kernel<TG, -1>), grid, block, 0, s, a, N, (int)M);
     else if (z_kind == SPHIP_F32) hipLaunchKernelGGL((linear_preact_kernel<TG, SPHIP_F32>), grid, block, 0, s, a, N, (int)M);
     else if (z_kind == SPHIP_BF16) hipLaunchKernelGGL((linear_preact_kernel<TG, SPHIP_BF16>), grid, block, 0, s, a, N, (int)M);
     else if (z_kind == SPHIP_INT8) hipLaunchKernelGGL((linear_preact_kernel<TG, SPHIP_INT8>), grid, block, 0, s, a, N, (int)M);
     else hipLaunchKernelGGL((linear_preact_kernel<TG, SPHIP_E4M3>), grid, block, 0, s, a, N, (int)M);
+    SPHIP_CHECK_LAUNCH("linear_backward(dz)");
+    return SPHIP_OK;
 }
 
 // column sums of part (P, M) in row order by 16 interleaved chains: 64 columns per workgroup of 1024 threads
@@ -511,10 +536,21 @@ static bool codes_ok(const void* codes, const void* scales, int64_t ld, int64_t 
 }
 static size_t up256(size_t b) { return (b + 255) / 256 * 256; }
 
-// workspace: partial tiles | z in fp32 on its way into 8 bits
+// workspace: partial tiles | z in fp32 on its way into 8 bits | x and W packed (D no multiple of 64)
+struct ForwardSpace {
+    size_t part, z, pack, total;
+};
+static ForwardSpace forward_space(int dtype, int z_kind, int64_t N, int64_t D, int64_t M) {
+    ForwardSpace f;
+    f.part = up256(split_bytes(dtype, N, M, D));
+    f.z = is_codes(z_kind) ? up256((size_t)N * (cdiv(M, 4) * 4) * 4) : 0;
+    f.pack = dtype == SPHIP_BF16 && D % 64 != 0 && worth_packing(N, M, D) ? (size_t)(N + M) * packed_ld(D) * 2 : 0;
+    f.total = f.part + f.z + f.pack;
+    return f;
+}
 extern "C" size_t sphip_linear_workspace_bytes(int dtype, int z_kind, int64_t N, int64_t D, int64_t M) {
     if (N <= 0 || D <= 0 || M <= 0 || !valid_dtype(dtype)) return 0;
-    return up256(split_bytes(dtype, N, M, D)) + (is_codes(z_kind) ? (size_t)N * (cdiv(M, 4) * 4) * 4 : 0);
+    return forward_space(dtype, z_kind, N, D, M).total;
 }
 
 extern "C" int sphip_linear(const void* x, int64_t ldx, const void* W, int64_t ldw, int dtype, const void* bias,
@@ -537,39 +573,49 @@ extern "C" int sphip_linear(const void* x, int64_t ldx, const void* W, int64_t l
                   SPHIP_EINVAL, "linear: a pointer is not aligned to its element");
     SPHIP_REQUIRE((!zc || codes_ok(z, z_scales, ldz, M)) && (!x_codes || codes_ok(x_codes, x_scales, ldq, D)), SPHIP_EINVAL,
                   "linear: codes and scales need 16-byte aligned rows of at least their columns");
-    const size_t part = up256(split_bytes(dtype, N, M, D)), ldt = (size_t)cdiv(M, 4) * 4;
-    SPHIP_REQUIRE(!zc || (ws && ((uintptr_t)ws & 15) == 0 && ws_bytes >= part + (size_t)N * ldt * 4), SPHIP_EWORKSPACE,
-                  "linear: workspace of %zu bytes, needs %zu, 16-byte aligned", ws_bytes, part + (size_t)N * ldt * 4);
+    const ForwardSpace f = forward_space(dtype, zc ? z_kind : SPHIP_F32, N, D, M);
+    SPHIP_REQUIRE(f.total == 0 || (ws && ((uintptr_t)ws & 15) == 0 && ws_bytes >= f.total), SPHIP_EWORKSPACE,
+                  "linear: workspace of %zu bytes, needs %zu, 16-byte aligned", ws_bytes, f.total);
     hipStream_t s = (hipStream_t)stream;
     Epilogue e;
     e.bias = bias, e.bias_dt = bias_dtype, e.res = residual, e.res_dt = res_dtype, e.ldr = ldr;
     e.out = out, e.out_dt = out_dtype, e.ldo = ldo, e.act = act;
-    if (zc) e.z = (char*)ws + part, e.z_dt = SPHIP_F32, e.ldz = (int64_t)ldt;
+    if (zc) e.z = (char*)ws + f.part, e.z_dt = SPHIP_F32, e.ldz = cdiv(M, 4) * 4;
     else e.z = z, e.z_dt = z_kind, e.ldz = ldz;
-    set_vec(e);
-    const Operand A = {x, nullptr, ldx, (int)N}, B = {W, nullptr, ldw, (int)M};
-    int st = dtype == SPHIP_BF16 ? launch_product<bf16_t, OP_ROWS, OP_ROWS>("linear", A, B, e, D, D, ws, ws_bytes, s)
-                                 : launch_product<float, OP_ROWS, OP_ROWS>("linear", A, B, e, D, D, ws, ws_bytes, s);
+    Operand A = {x, nullptr, ldx, (int)N}, B = {W, nullptr, ldw, (int)M};
+    int64_t K = D;
+    int st = SPHIP_OK;
+    if (f.pack) {
+        K = packed_ld(D);
+        char* to = (char*)ws + f.part + f.z;
+        st = pack_rows("linear", A, N, D, to, s);
+        if (st == SPHIP_OK) st = pack_rows("linear", B, M, D, to + (size_t)N * K * 2, s);
+        if (st != SPHIP_OK) return st;
+    }
+    st = dtype == SPHIP_BF16 ? launch_product<bf16_t, OP_ROWS, OP_ROWS>("linear", A, B, e, K, K, ws, f.part, s)
+                             : launch_product<float, OP_ROWS, OP_ROWS>("linear", A, B, e, K, K, ws, f.part, s);
     if (st == SPHIP_OK && zc)
         st = sphip_checkpoint8_save(e.z, SPHIP_F32, e.ldz, z_kind, act == SPHIP_ACT_RELU, (uint8_t*)z, z_scales, ldz, N, M, s);
     if (st == SPHIP_OK && x_codes) st = sphip_checkpoint8_save(x, dtype, ldx, x_fmt, 0, x_codes, x_scales, ldq, N, D, s);
     return st;
 }
 
-// workspace: dz | column sums of row chunks | x restored (8-bit x in the 256 x 256 kernel) | partial tiles of a product
+// workspace: dz | column sums of 32-row groups | x as aligned bf16 rows (restored from codes, or packed) | W packed | partial
+// tiles of a product
 struct BackwardSpace {
-    size_t dz, sums, xr, part, total;
+    size_t dz, sums, x, w, part, total;
 };
-static int64_t dz_stride(int dtype, int64_t M) { return dtype == SPHIP_BF16 ? cdiv(M, 64) * 64 : cdiv(M, 4) * 4; }
+static int64_t dz_stride(int dtype, int64_t M) { return dtype == SPHIP_BF16 ? packed_ld(M) : cdiv(M, 4) * 4; }
 static BackwardSpace backward_space(int dtype, int x_kind, int want_dx, int want_dw, int want_db, int64_t N, int64_t D, int64_t M) {
     BackwardSpace b;
-    const bool products = want_dx || want_dw;
-    b.dz = products ? up256((size_t)N * dz_stride(dtype, M) * dtype_size(dtype)) : 0;
-    b.sums = want_db ? up256((size_t)cdiv(N, preact_rows(N, M)) * M * 4) : 0;
-    b.xr = want_dw && dtype == SPHIP_BF16 && is_codes(x_kind) && wants256(M, D, N) ? up256((size_t)N * (cdiv(D, 16) * 16) * 2) : 0;
-    const size_t p1 = want_dx ? split_bytes(dtype, N, D, cdiv(M, 64) * 64) : 0, p2 = want_dw ? split_bytes(dtype, M, D, N) : 0;
+    const bool bf = dtype == SPHIP_BF16;
+    b.dz = want_dx || want_dw ? up256((size_t)N * dz_stride(dtype, M) * dtype_size(dtype)) : 0;
+    b.sums = want_db ? up256((size_t)cdiv(N, 32) * M * 4) : 0;
+    b.x = want_dw && bf && worth_packing(M, D, N) && (is_codes(x_kind) || D % 8 != 0) ? up256((size_t)N * packed_ld(D) * 2) : 0;
+    b.w = want_dx && bf && worth_packing(N, D, M) && D % 8 != 0 ? up256((size_t)M * packed_ld(D) * 2) : 0;
+    const size_t p1 = want_dx ? split_bytes(dtype, N, D, M) : 0, p2 = want_dw ? split_bytes(dtype, M, D, N) : 0;
     b.part = p1 > p2 ? p1 : p2;
-    b.total = b.dz + b.sums + b.xr + b.part;
+    b.total = b.dz + b.sums + b.x + b.w + b.part;
     return b;
 }
 
@@ -582,34 +628,40 @@ extern "C" size_t sphip_linear_backward_workspace_bytes(int dtype, int x_kind, i
 template <typename T>
 static int backward_products(const Operand& dz, const void* W, int64_t ldw, const void* x, int x_kind, const uint8_t* x_scales,
                              int64_t ldx, void* dx, int dx_dtype, int64_t lddx, void* dW, int dw_dtype, int64_t lddw, int64_t N,
-                             int64_t D, int64_t M, bool padded, void* xr, void* part, size_t part_size, hipStream_t s) {
+                             int64_t D, int64_t M, bool padded, char* ws, const BackwardSpace& sp, hipStream_t s) {
+    char *xs = ws + sp.dz + sp.sums, *wsp = xs + sp.x, *part = wsp + sp.w;
     if (dx) {
+        const char* what = "linear_backward(dx)";
         Epilogue e;
         e.out = dx, e.out_dt = dx_dtype, e.ldo = lddx;
-        set_vec(e);
-        const Operand A = {dz.p, nullptr, dz.ld, (int)N}, B = {W, nullptr, ldw, (int)D};
-        const int st = launch_product<T, OP_ROWS, OP_COLS>("linear_backward(dx)", A, B, e, padded ? dz.ld : M, M, part, part_size, s);
+            Operand A = {dz.p, nullptr, dz.ld, (int)N}, B = {W, nullptr, ldw, (int)D};
+        if (sp.w) {
+            const int st = pack_rows(what, B, M, D, wsp, s);
+            if (st != SPHIP_OK) return st;
+        }
+        const int st = launch_product<T, OP_ROWS, OP_COLS>(what, A, B, e, padded ? dz.ld : M, M, part, sp.part, s);
         if (st != SPHIP_OK) return st;
     }
     if (!dW) return SPHIP_OK;
     const char* what = "linear_backward(dW)";
     Epilogue e;
     e.out = dW, e.out_dt = dw_dtype, e.ldo = lddw;
-    set_vec(e);
     const Operand A = {dz.p, nullptr, dz.ld, (int)M};
     Operand B = {x, x_scales, ldx, (int)D};
-    if (xr != nullptr) {
-        const Operand R = {xr, nullptr, cdiv(D, 16) * 16, (int)D};
-        if (linear256_takes(OP_COLS, OP_COLS, A, R, N)) {
-            const int st = sphip_checkpoint8_restore((const uint8_t*)x, x_scales, ldx, x_kind, xr, SPHIP_BF16, R.ld, N, D, s);
-            if (st != SPHIP_OK) return st;
-            B = R;
-            x_kind = SPHIP_BF16;
+    if (sp.x) {
+        int st;
+        if (is_codes(x_kind)) {
+            const int64_t ld = packed_ld(D);
+            st = sphip_checkpoint8_restore((const uint8_t*)x, x_scales, ldx, x_kind, xs, SPHIP_BF16, ld, N, D, s);
+            B.p = xs, B.ld = ld, x_kind = SPHIP_BF16;
+        } else {
+            st = pack_rows(what, B, N, D, xs, s);
         }
+        if (st != SPHIP_OK) return st;
     }
-    if (x_kind == SPHIP_INT8) return launch_product<T, OP_COLS, OP_COLS_I8>(what, A, B, e, N, N, part, part_size, s);
-    if (x_kind == SPHIP_E4M3) return launch_product<T, OP_COLS, OP_COLS_E4M3>(what, A, B, e, N, N, part, part_size, s);
-    return launch_product<T, OP_COLS, OP_COLS>(what, A, B, e, N, N, part, part_size, s);
+    if (x_kind == SPHIP_INT8) return launch_product<T, OP_COLS, OP_COLS_I8>(what, A, B, e, N, N, part, sp.part, s);
+    if (x_kind == SPHIP_E4M3) return launch_product<T, OP_COLS, OP_COLS_E4M3>(what, A, B, e, N, N, part, sp.part, s);
+    return launch_product<T, OP_COLS, OP_COLS>(what, A, B, e, N, N, part, sp.part, s);
 }
 
 extern "C" int sphip_linear_backward(const void* g, int g_dtype, int64_t ldg, const void* W, int64_t ldw, int dtype, int act,
@@ -643,34 +695,33 @@ extern "C" int sphip_linear_backward(const void* g, int g_dtype, int64_t ldg, co
     char* w = (char*)ws;
     float* sums = (float*)(w + sp.dz);
     // Without an activation the incoming gradient is dz. It is copied (into the product's dtype, rows padded to 64) only
-    // where it does not have that dtype, or where a large product needs the padding.
+    // where it does not have that dtype, or where LDS-DMA could not fetch it as it is.
     const bool products = dx || dW;
     bool direct = act == SPHIP_ACT_NONE && g_dtype == dtype;
     if (direct && dtype == SPHIP_BF16 && (M % 64 != 0 || ldg % 8 != 0 || ((uintptr_t)g & 15) != 0))
-        direct = !((dx && wants256(N, D, cdiv(M, 64) * 64)) || (dW && wants256(M, D, N)));
+        direct = !((dx && worth_packing(N, D, M)) || (dW && worth_packing(M, D, N)));
     Operand dz = {g, nullptr, ldg, (int)N};
     if (products && !direct) dz.p = w, dz.ld = dz_stride(dtype, M);
-    if (db || (products && !direct)) {
+    if (products && !direct && !db && act == SPHIP_ACT_NONE && g_dtype == dtype && dtype == SPHIP_BF16) {
+        Operand o = {g, nullptr, ldg, (int)N};                  // a copy with padded rows is all there is to do
+        const int st = pack_rows("linear_backward(dz)", o, N, M, w, s);
+        if (st != SPHIP_OK) return st;
+    } else if (db || (products && !direct)) {
         PreactArgs a;
         a.g = g, a.z = z, a.scales = z_scales, a.dz = products && !direct ? w : nullptr, a.part = db ? sums : nullptr;
-        a.ldg = ldg, a.ldz = ldz, a.lddz = dz.ld, a.dz_dt = dtype, a.act = act, a.per = preact_rows(N, M);
-        SPHIP_REQUIRE(cdiv(cdiv(N, a.per) * cdiv(dz.ld > M ? dz.ld : M, 4), 256) < (1ll << 31), SPHIP_EUNSUPPORTED,
-                      "linear_backward: grid too large");
-        if (g_dtype == SPHIP_BF16) launch_preact<bf16_t>(a, z_kind, N, M, s);
-        else launch_preact<float>(a, z_kind, N, M, s);
-        SPHIP_CHECK_LAUNCH("linear_backward(dz)");
+        a.ldg = ldg, a.ldz = ldz, a.lddz = dz.ld, a.dz_dt = dtype, a.act = act;
+        const int st = g_dtype == SPHIP_BF16 ? launch_preact<bf16_t>(a, z_kind, N, M, s) : launch_preact<float>(a, z_kind, N, M, s);
+        if (st != SPHIP_OK) return st;
         if (db) {
             hipLaunchKernelGGL(linear_bias_grad_kernel, dim3((unsigned)cdiv(M, 64)), dim3(1024), 0, s, (const float*)sums,
-                               cdiv(N, a.per), (int)M, db, db_dtype);
+                               cdiv(N, 32), (int)M, db, db_dtype);
             SPHIP_CHECK_LAUNCH("linear_backward(db)");
         }
     }
     if (!products) return SPHIP_OK;
-    void* xr = sp.xr ? w + sp.dz + sp.sums : nullptr;
-    void* part = w + sp.dz + sp.sums + sp.xr;
     if (dtype == SPHIP_BF16)
         return backward_products<bf16_t>(dz, W, ldw, x, x_kind, x_scales, ldx, dx, dx_dtype, lddx, dW, dw_dtype, lddw, N, D, M,
-                                         !direct, xr, part, sp.part, s);
+                                         !direct, w, sp, s);
     return backward_products<float>(dz, W, ldw, x, x_kind, x_scales, ldx, dx, dx_dtype, lddx, dW, dw_dtype, lddw, N, D, M, false,
-                                    xr, part, sp.part, s);
+                                    w, sp, s);
 }

@@ -37,11 +37,107 @@ __device__ __forceinline__ void tile_of(const TileGrid& g, unsigned& split, int&
     tn = (int)(within / gsize);
 }
 
-// linear256.hip: whether the 256 x 256 kernel takes these operands, how it splits K, and its launch (bf16; the caller joins).
-// KB: rows of an OP_COLS B, which may be fewer than K (a multiple of 64 where A is OP_ROWS): B counts as zero from there on.
+typedef __bf16 b16x8_t __attribute__((ext_vector_type(8)));
+typedef float acc4_t __attribute__((ext_vector_type(4)));
+typedef unsigned w4_t __attribute__((ext_vector_type(4)));
+typedef unsigned w2_t __attribute__((ext_vector_type(2)));
+typedef void __attribute__((address_space(3)))* lds_t;
+
+// The tail the product's kernels share: ROWS x 64 values of C that a wave has put into its own LDS area [row][OUT_ROW bytes],
+// row r being n = n0 + r, leave so that 16 lanes store 64 consecutive m of a row. A lane keeps its m: one bias load. The
+// residual's pieces are all in flight before the first is used (little else hides their latency). Residual and result bypass
+// L2, which holds the operands. The activation is one rolled loop over LDS, not unrolled with the rest: inlined per output
+// quad it made kernels of 60 to 90 KB, more than the instruction cache holds.
+constexpr int OUT_ROW = 272;                       // 64 fp32 + 16 bytes
+template <int ROWS>
+__device__ __forceinline__ void finish_rows(char* stage, const Epilogue& epi, const TileGrid& g, unsigned split, int n0, int m0,
+                                            int N, int M, int lane) {
+    constexpr int P = ROWS / 4;                    // pieces of 4 outputs per lane
+    const int r16 = lane & 15, q4 = lane >> 4, Mp = (M + 3) & ~3;
+    const int m = m0 + r16 * 4, nb = n0 + q4, cols = M - m;
+    char* const mine = stage + q4 * OUT_ROW + r16 * 16;        // piece i is 4 OUT_ROW i further on
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    if (g.splits > 1) {
+#pragma unroll 4
+        for (int i = 0; i < P; ++i)
+            if (nb + 4 * i < N && cols > 0)
+                *reinterpret_cast<float4*>(g.part + ((int64_t)split * N + nb + 4 * i) * Mp + m) =
+                    *reinterpret_cast<const float4*>(mine + i * 4 * OUT_ROW);
+    } else if (cols >= 4) {
+        w4_t res[P];
+        if (epi.res != nullptr) {
+            if (epi.res_dt == SPHIP_F32) {
+#pragma unroll
+                for (int i = 0; i < P; ++i)
+                    if (nb + 4 * i < N)
+                        res[i] = __builtin_nontemporal_load((const u4_any*)((const float*)epi.res + (int64_t)(nb + 4 * i) * epi.ldr + m));
+            } else {
+#pragma unroll
+                for (int i = 0; i < P; ++i)
+                    if (nb + 4 * i < N) {
+                        const u2_any r = __builtin_nontemporal_load((const u2_any*)((const bf16_t*)epi.res + (int64_t)(nb + 4 * i) * epi.ldr + m));
+                        res[i] = (w4_t){r.x << 16, r.x & 0xffff0000u, r.y << 16, r.y & 0xffff0000u};
+                    }
+            }
+        }
+        if (epi.bias != nullptr || epi.act != SPHIP_ACT_NONE || epi.z != nullptr) {
+            float bias[4] = {0.f, 0.f, 0.f, 0.f};
+            if (epi.bias != nullptr) load4_as_f32(epi.bias, epi.bias_dt, m, bias);
+#pragma unroll 1
+            for (int i = 0; i < P; ++i) {
+                const int n = nb + 4 * i;
+                if (n >= N) break;
+                float4* at = reinterpret_cast<float4*>(mine + i * 4 * OUT_ROW);
+                const float4 c = *at;
+                float v[4] = {c.x + bias[0], c.y + bias[1], c.z + bias[2], c.w + bias[3]};
+                if (epi.z != nullptr) store4_from_f32(epi.z, epi.z_dt, n * epi.ldz + m, v);
+                act_value4(v, epi.act);
+                *at = make_float4(v[0], v[1], v[2], v[3]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            const int n = nb + 4 * i;
+            if (n >= N) continue;
+            const float4 c = *reinterpret_cast<const float4*>(mine + i * 4 * OUT_ROW);
+            float v[4] = {c.x, c.y, c.z, c.w};
+            if (epi.res != nullptr) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] += __uint_as_float(res[i][j]);
+            }
+            if (epi.out_dt == SPHIP_F32) {
+                const u4_any o = {__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
+                __builtin_nontemporal_store(o, (u4_any*)((float*)epi.out + n * epi.ldo + m));
+            } else {
+                const u2_any o = {(unsigned)f32_to_bf16(v[0]) | ((unsigned)f32_to_bf16(v[1]) << 16),
+                                  (unsigned)f32_to_bf16(v[2]) | ((unsigned)f32_to_bf16(v[3]) << 16)};
+                __builtin_nontemporal_store(o, (u2_any*)((bf16_t*)epi.out + n * epi.ldo + m));
+            }
+        }
+    } else if (cols > 0) {
+#pragma unroll 1
+        for (int i = 0; i < P; ++i) {
+            if (nb + 4 * i >= N) break;
+            const float4 c = *reinterpret_cast<const float4*>(mine + i * 4 * OUT_ROW);
+            float v[4] = {c.x, c.y, c.z, c.w};
+            epilogue4(epi, nb + 4 * i, m, M, v);
+        }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// The LDS-DMA kernels (bf16): whether they take these operands, how they split K, their launch (the caller joins). KB: rows
+// of an OP_COLS B, which may be fewer than K (a multiple of 64 where A is OP_ROWS): B counts as zero from there on.
 bool linear256_takes(int mode_a, int mode_b, const Operand& A, const Operand& B, int64_t K);
-int linear256_splits(int64_t N, int64_t M, int64_t K);
 int launch_linear256(const char* what, int mode_a, int mode_b, const Operand& A, const Operand& B, const Epilogue& epi, int64_t K,
+                     int64_t KB, const TileGrid& g, hipStream_t s);
+bool linear128_takes(int mode_a, int mode_b, const Operand& A, const Operand& B, int64_t K);
+int linear128_splits(int64_t N, int64_t M, int64_t K);
+int launch_linear128(const char* what, int mode_a, int mode_b, const Operand& A, const Operand& B, const Epilogue& epi, int64_t K,
                      int64_t KB, const TileGrid& g, hipStream_t s);
 
 }  // namespace sphip

@@ -1,0 +1,154 @@
+// The dense product's kernel for mid-size bf16 shapes: a 128 x 128 tile of C per workgroup of 4 waves (2 x 2 of 64 x 64
+// outputs), 64 of K per step, v_mfma_f32_16x16x32_bf16, operand tiles by LDS-DMA (images: linear_dma.hpp).
+//
+// STAGES buffers of 32 KiB, one barrier per step: at step t a wave waits for its own DMA of step t, passes the barrier
+// (everybody's step t has landed, everybody has read step t - 1), sends off the DMA of step t + STAGES - 1 into the buffer
+// just freed, reads its fragments and multiplies. With at most one workgroup per compute unit 4 buffers (these shapes are
+// short: their time is the latency of the loads), with more 2 buffers, so that two workgroups share a unit and cover each
+// other. (32 of K per step with 5 buffers of 16 KiB, two workgroups per unit: 8192 x 2048 x 2048 83 us against 70.)
+#include "linear_dma.hpp"
+
+namespace sphip {
+
+constexpr int T128 = 128, IMG_A = 0, IMG_B = 16384, STAGE = 32768;
+
+template <int MODE> struct Source128 {
+    __amdgpu_buffer_rsrc_t rsrc;
+    unsigned voff, piece, step;            // bytes: lane offset, between the 4 pieces of a step, between K steps
+    __device__ __forceinline__ void init(const Operand& o, int row0, int64_t k0, int64_t K, int tid) {
+        const bf16_t* p = (const bf16_t*)o.p;
+        const unsigned ld2 = (unsigned)o.ld * 2u;
+        if (MODE == OP_ROWS) {
+            const int hr = tid >> 3, ch = (tid & 7) ^ ((hr >> 1) & 7);
+            const int rows = min(T128, o.rows - row0);
+            rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)(p + (int64_t)row0 * o.ld + k0), 0,
+                                                     (int)((unsigned)(rows - 1) * ld2 + (unsigned)(K - k0) * 2u), 0x00020000);
+            voff = (unsigned)hr * ld2 + (unsigned)ch * 16u;
+            piece = 32u * ld2;
+            step = K64 * 2;
+        } else {
+            const int kr = tid >> 4, f = (kr & 3) + 4 * ((kr >> 3) & 1);
+            const int c = (tid & 15) ^ (2 * f);
+            // (the end rounded up to a piece, see linear256.hip)
+            rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)(p + k0 * o.ld + row0), 0,
+                                                     (int)(K > k0 ? (unsigned)(K - 1 - k0) * ld2 + ((unsigned)(o.rows - row0) * 2u + 15u) / 16u * 16u : 0u),
+                                                     0x00020000);
+            voff = (unsigned)kr * ld2 + (unsigned)c * 16u;
+            piece = 16u * ld2;
+            step = K64 * ld2;
+        }
+    }
+    __device__ __forceinline__ void dma(char* lds, int t) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_t)(lds + 4096 * i), 16, voff + (unsigned)t * step + (unsigned)i * piece, 0, 0, 0);
+    }
+};
+
+template <int MA, int MB, int STAGES>
+__global__ __launch_bounds__(256, STAGES == 2 ? 2 : 1) void linear128_kernel(Operand A, Operand B, Epilogue epi, int64_t K, int64_t KB,
+                                                                             TileGrid g) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    unsigned split;
+    int tm, tn;
+    tile_of(g, split, tm, tn);
+    const int m0 = tm * T128, n0 = tn * T128;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wm = wave >> 1, wn = wave & 1;
+    const int64_t k0 = (int64_t)split * g.steps_per * K64;
+    const int steps = (int)min((int64_t)g.steps_per, (K - k0 + K64 - 1) / K64);
+
+    Source128<MA> sa;
+    Source128<MB> sb;
+    sa.init(A, n0, k0, K, tid);
+    sb.init(B, m0, k0, KB, tid);
+    auto fetch = [&](int t, unsigned image) {      // 8 DMA instructions per wave
+        if (t >= steps) return;
+        char* dst = smem + image + wave * 1024;
+        sa.dma(dst + IMG_A, t);
+        sb.dma(dst + IMG_B, t);
+    };
+    const unsigned lds0 = (unsigned)(size_t)(lds_t)smem;
+    Frag<MA, 256> fa;
+    Frag<MB, 256> fb;
+    fa.init(lds0 + IMG_A, wn * 64, lane);
+    fb.init(lds0 + IMG_B, wm * 64, lane);
+    acc4_t acc[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = (acc4_t){0.f, 0.f, 0.f, 0.f};
+
+#pragma unroll
+    for (int t = 0; t < STAGES - 1; ++t) fetch(t, t * STAGE);
+    unsigned img = 0, freed = (STAGES - 1) * STAGE;            // buffers of step t and of step t - 1
+    for (int t = 0; t < steps; ++t) {
+        // step t has landed; the (at most STAGES - 2) steps after it that are on their way may still be out
+        const int later = min(STAGES - 2, steps - 1 - t);
+        if (later == 2) LIN_VMCNT(16);
+        else if (later == 1) LIN_VMCNT(8);
+        else LIN_VMCNT(0);
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+        fetch(t + STAGES - 1, freed);
+        fa.template read<0>(img);
+        fb.template read<0>(img);
+        fa.template read<1>(img);
+        fb.template read<1>(img);
+        constexpr int LATER = Frag<MA, 256>::READS + Frag<MB, 256>::READS;     // the counter holds 15 at most
+        fa.template wait<0, (LATER > 15 ? 15 : LATER)>();
+        fb.template wait<0, (LATER > 15 ? 15 : LATER)>();
+#pragma unroll
+        for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+            for (int nt = 0; nt < 4; ++nt)
+                acc[mt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb.get(mt, 0), fa.get(nt, 0), acc[mt][nt], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);         // these 16 MFMAs run while the other fragments arrive
+        fa.template wait<1, 0>();
+        fb.template wait<1, 0>();
+#pragma unroll
+        for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+            for (int nt = 0; nt < 4; ++nt)
+                acc[mt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb.get(mt, 1), fa.get(nt, 1), acc[mt][nt], 0, 0, 0);
+        freed = img;
+        img = img + STAGE == STAGES * STAGE ? 0 : img + STAGE;
+    }
+    __syncthreads();                               // the last step has been read: the buffers become the staging area
+    const int N = A.rows, M = B.rows;
+    char* const stage = smem + wave * 32 * OUT_ROW;
+    finish_tile<2>([&](int mt, int nt) { return acc[mt][nt]; }, stage, epi, g, split, n0 + wn * 64, m0 + wm * 64, N, M, lane);
+    finish_tile<2>([&](int mt, int nt) { return acc[mt][2 + nt]; }, stage, epi, g, split, n0 + wn * 64 + 32, m0 + wm * 64, N, M, lane);
+}
+
+bool linear128_takes(int mode_a, int mode_b, const Operand& A, const Operand& B, int64_t K) {
+    return dma_ok(mode_a, A, K, T128) && dma_ok(mode_b, B, K, T128);
+}
+
+// Splits of the K range, towards one workgroup per compute unit, 2 steps each at least: a split costs a round trip of the
+// fp32 partial tiles, a step about what its first load takes.
+int linear128_splits(int64_t N, int64_t M, int64_t K) {
+    const int64_t tiles = cdiv(N, T128) * cdiv(M, T128), steps = cdiv(K, K64);
+    int64_t s = 256 / tiles;
+    if (s > steps / 2) s = steps / 2;
+    return s < 1 ? 1 : (int)s;
+}
+
+int launch_linear128(const char* what, int mode_a, int mode_b, const Operand& A, const Operand& B, const Epilogue& epi, int64_t K,
+                     int64_t KB, const TileGrid& g, hipStream_t s) {
+    typedef void (*kern_t)(Operand, Operand, Epilogue, int64_t, int64_t, TileGrid);
+    const int64_t blocks = (int64_t)g.tilesM * g.tilesN * g.splits;
+    const int which = mode_a == OP_ROWS ? (mode_b == OP_ROWS ? 0 : 1) : 2, deep = blocks <= 256;
+    static const kern_t kerns[3][2] = {{linear128_kernel<OP_ROWS, OP_ROWS, 2>, linear128_kernel<OP_ROWS, OP_ROWS, 4>},
+                                       {linear128_kernel<OP_ROWS, OP_COLS, 2>, linear128_kernel<OP_ROWS, OP_COLS, 4>},
+                                       {linear128_kernel<OP_COLS, OP_COLS, 2>, linear128_kernel<OP_COLS, OP_COLS, 4>}};
+    const int lds = (deep ? 4 : 2) * STAGE;
+    SPHIP_REQUIRE(hipFuncSetAttribute((const void*)kerns[which][deep], hipFuncAttributeMaxDynamicSharedMemorySize, lds) == hipSuccess,
+                  SPHIP_ELAUNCH, "%s: cannot reserve %d bytes of LDS", what, lds);
+    hipLaunchKernelGGL(kerns[which][deep], dim3((unsigned)blocks), dim3(256), lds, s, A, B, epi, K, KB, g);
+    SPHIP_CHECK_LAUNCH(what);
+    return SPHIP_OK;
+}
+
+}  // namespace sphip

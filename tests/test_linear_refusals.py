@@ -68,7 +68,7 @@ def test_workspace_queries():
     L = lib()
     assert L.sphip_linear_workspace_bytes(BF16, 0, 0, 8, 8) == 0 and L.sphip_linear_workspace_bytes(9, 0, 8, 8, 8) == 0
     assert L.sphip_linear_workspace_bytes(BF16, INT8, 8, 64, 32) >= 8 * 32 * 4
-    assert L.sphip_linear_backward_workspace_bytes(BF16, INT8, 0, 0, 1, 64, 64, 32) == 8 * 32 * 4
+    assert L.sphip_linear_backward_workspace_bytes(BF16, INT8, 0, 0, 1, 64, 64, 32) == 2 * 32 * 4
     assert L.sphip_linear_backward_workspace_bytes(F32, F32, 1, 1, 1, 8, -1, 32) == 0
 
 
