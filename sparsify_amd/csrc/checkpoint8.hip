@@ -14,102 +14,98 @@
 // A group with an infinity or a NaN in it has scale byte 255 and restores as NaN throughout.
 // Codes (32 ceil(N/32), ldq) and scales (ceil(N/32), ldq), ldq a multiple of 16 >= D; padding rows and columns are zeros.
 //
-// Bound: HBM. One thread owns V columns of a group and holds its 32 rows in registers (32 independent loads in flight),
-// so x is read once: maximum, scale, codes.
+// Bound: HBM. A workgroup takes a group's 32 rows of 32 x 16 bytes of columns: 32 lanes side by side, every thread 4 rows,
+// all loads in flight at once; x is read once, its maxima meet in LDS. (A thread per column piece and all 32 rows, no LDS,
+// has an eighth of the threads: as fast at 65536 x 4096, 20 us against 8 at 5001 x 1111.)
 #include "codes8.hpp"
 
 namespace sphip {
 
-template <typename T, int V> struct Cols;                 // V columns of one row, raw bits
-template <int V> struct Cols<bf16_t, V> {
-    unsigned w[(V + 1) / 2];
-    __device__ __forceinline__ void load(const bf16_t* p, int n) {
-#pragma unroll
-        for (int j = 0; j < (V + 1) / 2; ++j) w[j] = 0;
-        if (n >= V) __builtin_memcpy(w, p, V * 2);
-        else
-#pragma unroll
-            for (int j = 0; j < V; ++j)
-                if (j < n) w[j >> 1] |= (unsigned)p[j] << ((j & 1) * 16);
-    }
-    __device__ __forceinline__ unsigned magnitude(int j) const { return (j & 1 ? w[j >> 1] & 0x7fff0000u : (w[j >> 1] << 16) & 0x7fff0000u); }
-    __device__ __forceinline__ float value(int j) const { return __uint_as_float(j & 1 ? w[j >> 1] & 0xffff0000u : w[j >> 1] << 16); }
-};
-template <int V> struct Cols<float, V> {
-    float w[V];
-    __device__ __forceinline__ void load(const float* p, int n) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) w[j] = 0.f;
-        if (n >= V) __builtin_memcpy(w, p, V * 4);
-        else
-#pragma unroll
-            for (int j = 0; j < V; ++j)
-                if (j < n) w[j] = p[j];
-    }
-    __device__ __forceinline__ unsigned magnitude(int j) const { return __float_as_uint(w[j]) & 0x7fffffffu; }
-    __device__ __forceinline__ float value(int j) const { return w[j]; }
+struct SaveArgs {
+    const void* x;
+    uint8_t *codes, *scales;
+    void* packed;                  // or null: also a copy of x, rows of ldp (a multiple of 64), zeros behind column D
+    int64_t ldx, ldq, ldp, N;
+    int D, strips, keep;           // strips: workgroups side by side along a row
 };
 
-// biased exponent byte of the group's scale from the bits of its largest magnitude
-template <int FMT> __device__ __forceinline__ unsigned scale_byte(unsigned top) {
-    if (top >= 0x7f800000u) return 255u;
-    // top = f 2^E: f 2^6 <= 127 (f 2^8 <= 448) for mantissas up to 1.984375 (1.75), one step coarser above
-    const unsigned most = FMT == SPHIP_INT8 ? 0x7e0000u : 0x600000u;
-    const int e = (int)(top >> 23) - (FMT == SPHIP_INT8 ? 6 : 8) + ((top & 0x7fffffu) > most ? 1 : 0);
-    return (unsigned)max(e, FMT == SPHIP_INT8 ? 1 : 10);
-}
-
-template <typename T, int V, int FMT, bool KEEP>
-__global__ __launch_bounds__(256) void checkpoint8_save_kernel(const T* __restrict__ x, int64_t ldx, uint8_t* __restrict__ codes,
-                                                               uint8_t* __restrict__ scales, int64_t ldq, int64_t N, int D) {
-    const int per_row = (int)(ldq / V);
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int64_t grp = i / per_row;
-    if (grp * 32 >= N) return;
-    const int c0 = (int)(i % per_row) * V;
-    const T* p = x + grp * 32 * ldx + c0;
-    Cols<T, V> v[32];
-    const int rows = (int)min((int64_t)32, N - grp * 32);
+template <typename T, int FMT>
+__global__ __launch_bounds__(256) void checkpoint8_save_kernel(SaveArgs a) {
+    constexpr int V = 16 / sizeof(T), W = 4;
+    __shared__ unsigned red[4][32 * V];
+    const int cl = threadIdx.x & 31, rl = threadIdx.x >> 5, wave = threadIdx.x >> 6;
+    const int64_t grp = blockIdx.x / (unsigned)a.strips, r0 = grp * 32 + rl;
+    const int c0 = ((int)(blockIdx.x % (unsigned)a.strips) * 32 + cl) * V, n = a.D - c0;
+    unsigned w[W][4];                                            // 4 rows of 16 bytes, raw
 #pragma unroll
-    for (int t = 0; t < 32; ++t) v[t].load(p + (int64_t)t * ldx, t < rows ? D - c0 : 0);
+    for (int t = 0; t < W; ++t) {
+        const int64_t row = r0 + 8 * t;
+        const T* p = (const T*)a.x + row * a.ldx + c0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[t][j] = 0;
+        if (row >= a.N || n <= 0) continue;
+        if (n >= V) {
+            __builtin_memcpy(w[t], p, 16);
+        } else if (sizeof(T) == 2) {
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+                if (j < n) w[t][j / 2] |= (unsigned)((const bf16_t*)p)[j] << ((j & 1) * 16);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (j < n) w[t][j] = ((const unsigned*)p)[j];
+        }
+    }
+    // element j of a row as fp32 bits
+    auto bits = [&](int t, int j) {
+        if (sizeof(T) == 4) return w[t][j % 4];
+        return j & 1 ? w[t][j / 2] & 0xffff0000u : w[t][j / 2] << 16;
+    };
     unsigned top[V];
 #pragma unroll
-    for (int j = 0; j < V; ++j) top[j] = 0;
+    for (int j = 0; j < V; ++j) {
+        top[j] = 0;
 #pragma unroll
-    for (int t = 0; t < 32; ++t)
+        for (int t = 0; t < W; ++t) top[j] = max(top[j], bits(t, j) & 0x7fffffffu);
+        top[j] = max(top[j], (unsigned)__shfl_xor((int)top[j], 32, 64));
+    }
+    if ((rl & 1) == 0)
 #pragma unroll
-        for (int j = 0; j < V; ++j) top[j] = max(top[j], v[t].magnitude(j));
+        for (int j = 0; j < V; j += 4) *reinterpret_cast<uint4*>(&red[wave][cl * V + j]) = make_uint4(top[j], top[j + 1], top[j + 2], top[j + 3]);
+    __syncthreads();
+    if (c0 >= max(a.ldq, a.packed != nullptr ? a.ldp : 0)) return;
     float inv[V];
     bool bad[V];
     uint8_t sb[V];
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-        const unsigned b = scale_byte<FMT>(top[j]);
-        sb[j] = (uint8_t)b;
-        bad[j] = b == 255u;
-        inv[j] = __uint_as_float((bad[j] ? 127u : 254u - b) << 23);          // 2^-e, a normal number: 1 <= b <= 249
-    }
-    __builtin_memcpy(scales + grp * ldq + c0, sb, V);
-    uint8_t* q = codes + grp * 32 * ldq + c0;
+    for (int j = 0; j < V; j += 4) {
+        uint4 m = *reinterpret_cast<const uint4*>(&red[0][cl * V + j]);
 #pragma unroll
-    for (int t = 0; t < 32; ++t) {
-        uint8_t o[V];
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const float a = v[t].value(j);
-            unsigned c;
-            if (FMT == SPHIP_INT8) {
-                // one rounding, to nearest even, by adding 1.5 2^23: the low byte is the two's complement code
-                c = __float_as_uint(fmaf(a, inv[j], 12582912.f)) & 0xffu;
-                if (KEEP && c == 0u && a != 0.f) c = a < 0.f ? 0xffu : 1u;
-            } else {
-                const float s = a * inv[j];
-                c = (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(s, s, 0, false) & 0xffu;
-                if (KEEP && (c & 0x7fu) == 0u && a != 0.f) c = a < 0.f ? 0x81u : 1u;
-            }
-            o[j] = (uint8_t)(bad[j] ? 0x7fu : c);                            // (not read: the scale is NaN)
+        for (int i = 1; i < 4; ++i) {
+            const uint4 o = *reinterpret_cast<const uint4*>(&red[i][cl * V + j]);
+            m = make_uint4(max(m.x, o.x), max(m.y, o.y), max(m.z, o.z), max(m.w, o.w));
         }
-        __builtin_memcpy(q + (int64_t)t * ldq, o, V);
+        const unsigned mv[4] = {m.x, m.y, m.z, m.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const unsigned b = scale_byte<FMT>(mv[i]);
+            sb[j + i] = (uint8_t)b, bad[j + i] = b == 255u, inv[j + i] = inverse_scale(b);
+        }
+    }
+    const bool in = c0 < a.ldq;
+    if (rl == 0 && in) __builtin_memcpy(a.scales + grp * a.ldq + c0, sb, V);
+#pragma unroll
+    for (int t = 0; t < W; ++t) {
+        const int64_t row = r0 + 8 * t;
+        if (in) {
+            uint8_t o[V];
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+                o[j] = (uint8_t)(bad[j] ? 0x7fu : code_of<FMT>(__uint_as_float(bits(t, j)), inv[j], a.keep != 0));
+            __builtin_memcpy(a.codes + row * a.ldq + c0, o, V);
+        }
+        if (a.packed != nullptr && row < a.N && c0 < a.ldp)
+            *reinterpret_cast<uint4*>((T*)a.packed + row * a.ldp + c0) = make_uint4(w[t][0], w[t][1], w[t][2], w[t][3]);
     }
 }
 
@@ -150,22 +146,6 @@ __global__ __launch_bounds__(256) void checkpoint8_restore_kernel(const uint8_t*
     }
 }
 
-template <typename T, int V>
-static void launch_save(const void* x, int64_t ldx, int fmt, int keep, uint8_t* codes, uint8_t* scales, int64_t ldq, int64_t N,
-                        int64_t D, unsigned blocks, hipStream_t s) {
-#define SPHIP_SAVE(F, KP)                                                                                            \
-    hipLaunchKernelGGL((checkpoint8_save_kernel<T, V, F, KP>), dim3(blocks), dim3(256), 0, s, (const T*)x, ldx, codes, \
-                       scales, ldq, N, (int)D)
-    if (fmt == SPHIP_INT8) {
-        if (keep) SPHIP_SAVE(SPHIP_INT8, true);
-        else SPHIP_SAVE(SPHIP_INT8, false);
-    } else {
-        if (keep) SPHIP_SAVE(SPHIP_E4M3, true);
-        else SPHIP_SAVE(SPHIP_E4M3, false);
-    }
-#undef SPHIP_SAVE
-}
-
 static int check_codes(const char* what, const void* codes, const void* scales, int64_t ldq, int fmt, int dtype, int64_t N,
                        int64_t D) {
     SPHIP_REQUIRE(valid_dtype(dtype), SPHIP_EINVAL, "%s: bad dtype %d", what, dtype);
@@ -178,6 +158,25 @@ static int check_codes(const char* what, const void* codes, const void* scales, 
     return SPHIP_OK;
 }
 
+// see linear.hpp
+int save_codes(const char* what, const void* x, int dtype, int64_t ldx, int fmt, int keep_sign, uint8_t* codes, uint8_t* scales,
+               int64_t ldq, void* packed, int64_t ldp, int64_t N, int64_t D, hipStream_t s) {
+    const int V = dtype == SPHIP_BF16 ? 8 : 4;
+    const int64_t strips = cdiv(packed && ldp > ldq ? ldp : ldq, 32 * V), blocks = cdiv(N, 32) * strips;
+    SPHIP_REQUIRE(blocks < (1ll << 31), SPHIP_EUNSUPPORTED, "%s: grid too large", what);
+    const SaveArgs a = {x, codes, scales, packed, ldx, ldq, ldp, N, (int)D, (int)strips, keep_sign};
+    const dim3 grid((unsigned)blocks), block(256);
+    if (dtype == SPHIP_BF16) {
+        if (fmt == SPHIP_INT8) hipLaunchKernelGGL((checkpoint8_save_kernel<bf16_t, SPHIP_INT8>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((checkpoint8_save_kernel<bf16_t, SPHIP_E4M3>), grid, block, 0, s, a);
+    } else {
+        if (fmt == SPHIP_INT8) hipLaunchKernelGGL((checkpoint8_save_kernel<float, SPHIP_INT8>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((checkpoint8_save_kernel<float, SPHIP_E4M3>), grid, block, 0, s, a);
+    }
+    SPHIP_CHECK_LAUNCH(what);
+    return SPHIP_OK;
+}
+
 }  // namespace sphip
 
 extern "C" int sphip_checkpoint8_save(const void* x, int dtype, int64_t ldx, int fmt, int keep_sign, uint8_t* codes,
@@ -187,15 +186,7 @@ extern "C" int sphip_checkpoint8_save(const void* x, int dtype, int64_t ldx, int
     if (st != SPHIP_OK) return st;
     SPHIP_REQUIRE(x && ((uintptr_t)x & (dtype_size(dtype) - 1)) == 0, SPHIP_EINVAL, "checkpoint8_save: null or misaligned x");
     SPHIP_REQUIRE(ldx >= D, SPHIP_EINVAL, "checkpoint8_save: ldx is shorter than a row");
-    hipStream_t s = (hipStream_t)stream;
-    const int64_t groups = cdiv(N, 32);
-    const int V = dtype == SPHIP_BF16 ? 4 : 2;
-    const int64_t blocks = cdiv(groups * (ldq / V), 256);
-    SPHIP_REQUIRE(blocks < (1ll << 31), SPHIP_EUNSUPPORTED, "checkpoint8_save: grid too large");
-    if (dtype == SPHIP_BF16) launch_save<bf16_t, 4>(x, ldx, fmt, keep_sign, codes, scales, ldq, N, D, (unsigned)blocks, s);
-    else launch_save<float, 2>(x, ldx, fmt, keep_sign, codes, scales, ldq, N, D, (unsigned)blocks, s);
-    SPHIP_CHECK_LAUNCH("checkpoint8_save");
-    return SPHIP_OK;
+    return save_codes("checkpoint8_save", x, dtype, ldx, fmt, keep_sign, codes, scales, ldq, nullptr, 0, N, D, (hipStream_t)stream);
 }
 
 extern "C" int sphip_checkpoint8_restore(const uint8_t* codes, const uint8_t* scales, int64_t ldq, int fmt, void* out,

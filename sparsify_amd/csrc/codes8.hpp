@@ -29,4 +29,29 @@ template <int FMT> __device__ __forceinline__ void code_values(unsigned w, float
     code_values<FMT>(w, s4, o);
 }
 
+// The other direction. Biased exponent byte of a group's scale from the bits of its largest magnitude (255: a NaN or an
+// infinity in it): the smallest that keeps top = f 2^E within the largest code, f 2^6 <= 127 (f 2^8 <= 448) up to a mantissa
+// of 1.984375 (1.75), one step coarser above.
+template <int FMT> __device__ __forceinline__ unsigned scale_byte(unsigned top) {
+    if (top >= 0x7f800000u) return 255u;
+    const unsigned most = FMT == SPHIP_INT8 ? 0x7e0000u : 0x600000u;
+    const int e = (int)(top >> 23) - (FMT == SPHIP_INT8 ? 6 : 8) + ((top & 0x7fffffu) > most ? 1 : 0);
+    return (unsigned)max(e, FMT == SPHIP_INT8 ? 1 : 10);
+}
+// 1 / scale, a normal number (1 <= byte <= 249)
+__device__ __forceinline__ float inverse_scale(unsigned byte) { return __uint_as_float((byte == 255u ? 127u : 254u - byte) << 23); }
+// code of a, given the inverse scale: a power of two, so that a * inv is exact and there is one rounding, to nearest even
+template <int FMT> __device__ __forceinline__ unsigned code_of(float a, float inv, bool keep_sign) {
+    unsigned c;
+    if (FMT == SPHIP_INT8) {
+        c = __float_as_uint(fmaf(a, inv, 12582912.f)) & 0xffu;               // 1.5 2^23: the low byte is the two's complement code
+        if (keep_sign && c == 0u && a != 0.f) c = a < 0.f ? 0xffu : 1u;
+    } else {
+        const float s = a * inv;
+        c = (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(s, s, 0, false) & 0xffu;
+        if (keep_sign && (c & 0x7fu) == 0u && a != 0.f) c = a < 0.f ? 0x81u : 1u;
+    }
+    return c;
+}
+
 }  // namespace sphip

@@ -67,7 +67,8 @@ struct Epilogue {
     const void* bias = nullptr;       // (M) or null
     const void* res = nullptr;        // (N, M), row stride ldr, or null
     void* out = nullptr;              // (N, M), row stride ldo
-    void* z = nullptr;                // (N, M), row stride ldz, or null: z + b before the activation
+    void* z = nullptr;                // (N, M), row stride ldz, or null: z + b before the activation, as values of z_dt
+    uint8_t* z_scales = nullptr;      // or, with scales, as codes of that format (whole tiles only: finish_rows)
     int64_t ldr = 0, ldo = 0, ldz = 0;
     int bias_dt = 0, res_dt = 0, out_dt = 0, z_dt = 0;
     int act = 0;
@@ -109,7 +110,7 @@ __device__ __forceinline__ void epilogue4(const Epilogue& e, int64_t n, int m, i
 #pragma unroll
             for (int j = 0; j < 4; ++j) v[j] += b[j];
         }
-        if (e.z != nullptr) store4_from_f32(e.z, e.z_dt, n * e.ldz + m, v);
+        if (e.z != nullptr && e.z_scales == nullptr) store4_from_f32(e.z, e.z_dt, n * e.ldz + m, v);
         act_value4(v, e.act);
         if (e.res != nullptr) {
             float r[4];
@@ -125,7 +126,7 @@ __device__ __forceinline__ void epilogue4(const Epilogue& e, int64_t n, int m, i
         if (m + j >= M) continue;
         float t = v[j];
         if (e.bias != nullptr) t += load_as_f32(e.bias, e.bias_dt, m + j);
-        if (e.z != nullptr) store_from_f32(e.z, e.z_dt, n * e.ldz + m + j, t);
+        if (e.z != nullptr && e.z_scales == nullptr) store_from_f32(e.z, e.z_dt, n * e.ldz + m + j, t);
         t = act_value(t, e.act);
         if (e.res != nullptr) t += load_as_f32(e.res, e.res_dt, n * e.ldr + m + j);
         store_from_f32(e.out, e.out_dt, n * e.ldo + m + j, t);

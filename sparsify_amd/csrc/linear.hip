@@ -261,26 +261,40 @@ __global__ __launch_bounds__(256, 2) void linear_tile_kernel(Operand A, Operand 
             for (int qd = 0; qd < 4; ++qd)
                 *reinterpret_cast<float4*>(stage + r * OUT_ROW + (mi * 32 + 8 * qd + 4 * h) * 4) =
                     make_float4(acc[mi][ni][4 * qd], acc[mi][ni][4 * qd + 1], acc[mi][ni][4 * qd + 2], acc[mi][ni][4 * qd + 3]);
-        finish_rows<32>(stage, epi, g, split, n0 + wn * 64 + ni * 32, m0 + wm * 64, N, M, lane);
+        Residual<32> res;
+        res.load(epi, g, n0 + wn * 64 + ni * 32, m0 + wm * 64, N, M, lane);
+        finish_rows<32>(stage, epi, g, split, n0 + wn * 64 + ni * 32, m0 + wm * 64, N, M, lane, res);
     }
 }
 
-// Sum of the splits' partial tiles in split order, then the epilogue. One thread per 4 outputs.
+// Sum of the splits' partial tiles, then the epilogue. One thread per 4 outputs, the splits in order; with many splits of a
+// small product 8 threads share an output, each taking every eighth split (LANES = 8), their sums added in order.
+template <int LANES>
 __global__ __launch_bounds__(256) void linear_join_kernel(const float* __restrict__ part, Epilogue epi, int64_t N, int M,
                                                           int splits) {
-    const int quads = (M + 3) >> 2;
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= N * quads) return;
-    const int64_t n = i / quads, stride = N * quads * 4;
-    const int m = (int)(i % quads) * 4;
-    const float* p = part + i * 4;
-    float4 t = load4(p);
-    float v[4] = {t.x, t.y, t.z, t.w};
-    for (int s = 1; s < splits; ++s) {
-        t = load4(p + s * stride);
-        v[0] += t.x, v[1] += t.y, v[2] += t.z, v[3] += t.w;
+    constexpr int OUTS = 256 / LANES;
+    __shared__ float4 red[LANES][OUTS];
+    const int quads = (M + 3) >> 2, lane = threadIdx.x / OUTS, o = threadIdx.x % OUTS;
+    const int64_t i = (int64_t)blockIdx.x * OUTS + o, total = N * quads;
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    if (i < total) {
+#pragma unroll 4
+        for (int s = lane; s < splits; s += LANES) {
+            const float4 t = load4(part + (s * total + i) * 4);
+            v[0] += t.x, v[1] += t.y, v[2] += t.z, v[3] += t.w;
+        }
     }
-    epilogue4(epi, n, m, M, v);
+    if (LANES > 1) {
+        red[lane][o] = make_float4(v[0], v[1], v[2], v[3]);
+        __syncthreads();
+        if (lane != 0) return;
+#pragma unroll
+        for (int l = 1; l < LANES; ++l) {
+            const float4 t = red[l][o];
+            v[0] += t.x, v[1] += t.y, v[2] += t.z, v[3] += t.w;
+        }
+    }
+    if (i < total) epilogue4(epi, i / quads, (int)(i % quads) * 4, M, v);
 }
 
 // How many ways the K range of an (N, M) product of `steps` K steps is split: none when the tiles fill the 256 compute
@@ -353,37 +367,57 @@ static int launch_product(const char* what, const Operand& A, const Operand& B, 
         SPHIP_CHECK_LAUNCH(what);
     }
     if (g.splits > 1) {
-        hipLaunchKernelGGL(linear_join_kernel, dim3((unsigned)cdiv(threads, 256)), dim3(256), 0, s, g.part, epi, N, (int)M,
-                           g.splits);
+        if (g.splits > 8 && threads < (1 << 17))
+            hipLaunchKernelGGL(linear_join_kernel<8>, dim3((unsigned)cdiv(threads, 32)), dim3(256), 0, s, g.part, epi, N, (int)M, g.splits);
+        else
+            hipLaunchKernelGGL(linear_join_kernel<1>, dim3((unsigned)cdiv(threads, 256)), dim3(256), 0, s, g.part, epi, N, (int)M, g.splits);
         SPHIP_CHECK_LAUNCH(what);
     }
     return SPHIP_OK;
 }
 
-// bf16 rows copied to a 16-byte aligned stride that is a multiple of 64, zeros behind them: what LDS-DMA asks of an operand
-__global__ __launch_bounds__(256) void linear_pack_kernel(const bf16_t* __restrict__ src, int64_t ld, int rows, int cols,
-                                                          bf16_t* __restrict__ dst, int pieces) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int64_t row = i / pieces;
-    if (row >= rows) return;
-    const int c = (int)(i % pieces) * 8;
-    *reinterpret_cast<uint4*>(dst + i * 8) = Chunk<bf16_t>::load(src + row * ld + c, cols - c);
+// bf16 rows copied to a 16-byte aligned stride that is a multiple of 64, zeros behind them: what LDS-DMA asks of an operand.
+// Up to two matrices in one launch.
+struct PackArgs {
+    const bf16_t* src[2];
+    bf16_t* dst[2];
+    int64_t ld[2], n[2];                   // n: 16-byte pieces of the copy
+    int cols[2], pieces[2];                // pieces per row
+};
+__global__ __launch_bounds__(256) void linear_pack_kernel(PackArgs a) {
+    int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int w = i >= a.n[0];
+    if (w) i -= a.n[0];
+    if (i >= a.n[w]) return;
+    const int64_t row = i / a.pieces[w];
+    const int c = (int)(i - row * a.pieces[w]) * 8;
+    *reinterpret_cast<uint4*>(a.dst[w] + i * 8) = Chunk<bf16_t>::load(a.src[w] + row * a.ld[w] + c, a.cols[w] - c);
 }
 static int64_t packed_ld(int64_t cols) { return cdiv(cols, 64) * 64; }
-static int pack_rows(const char* what, Operand& o, int64_t rows, int64_t cols, void* dst, hipStream_t s) {
-    const int64_t ld = packed_ld(cols), threads = rows * (ld / 8);
-    SPHIP_REQUIRE(cdiv(threads, 256) < (1ll << 31), SPHIP_EUNSUPPORTED, "%s: grid too large", what);
-    hipLaunchKernelGGL(linear_pack_kernel, dim3((unsigned)cdiv(threads, 256)), dim3(256), 0, s, (const bf16_t*)o.p, o.ld, (int)rows,
-                       (int)cols, (bf16_t*)dst, (int)(ld / 8));
-    SPHIP_CHECK_LAUNCH(what);
-    o.p = dst, o.ld = ld;
-    return SPHIP_OK;
-}
+struct Packing {
+    PackArgs a = {};
+    int count = 0;
+    void add(Operand& o, int64_t rows, int64_t cols, void* dst) {
+        const int64_t ld = packed_ld(cols);
+        a.src[count] = (const bf16_t*)o.p, a.dst[count] = (bf16_t*)dst, a.ld[count] = o.ld, a.cols[count] = (int)cols;
+        a.pieces[count] = (int)(ld / 8), a.n[count] = rows * (ld / 8);
+        ++count;
+        o.p = dst, o.ld = ld;
+    }
+    int launch(const char* what, hipStream_t s) {
+        if (count == 0) return SPHIP_OK;
+        const int64_t blocks = cdiv(a.n[0] + a.n[1], 256);
+        SPHIP_REQUIRE(blocks < (1ll << 31), SPHIP_EUNSUPPORTED, "%s: grid too large", what);
+        hipLaunchKernelGGL(linear_pack_kernel, dim3((unsigned)blocks), dim3(256), 0, s, a);
+        SPHIP_CHECK_LAUNCH(what);
+        return SPHIP_OK;
+    }
+};
 // Whether a bf16 product is worth copying an operand whose rows LDS-DMA cannot fetch (they do not start at multiples of 16
 // bytes, or K is no multiple of 64)
-static bool worth_packing(int64_t N, int64_t M, int64_t K) {
+static bool worth_packing(int64_t N, int64_t M, int64_t K, int least = 29) {
     const char* force = getenv("SPHIP_LINEAR");
-    return force ? force[0] != 't' : N * M * K >= (1ll << 27);
+    return force ? force[0] != 't' : N * M * K >= (1ll << least);
 }
 
 // ---- dz = g act'(z) and its column sums. A workgroup takes 32 rows (the group one scale of an 8-bit z covers) of 32 x 16
@@ -543,7 +577,7 @@ struct ForwardSpace {
 static ForwardSpace forward_space(int dtype, int z_kind, int64_t N, int64_t D, int64_t M) {
     ForwardSpace f;
     f.part = up256(split_bytes(dtype, N, M, D));
-    f.z = is_codes(z_kind) ? up256((size_t)N * (cdiv(M, 4) * 4) * 4) : 0;
+    f.z = is_codes(z_kind) && f.part ? up256((size_t)N * (cdiv(M, 4) * 4) * 4) : 0;      // (part: the K range may be split)
     f.pack = dtype == SPHIP_BF16 && D % 64 != 0 && worth_packing(N, M, D) ? (size_t)(N + M) * packed_ld(D) * 2 : 0;
     f.total = f.part + f.z + f.pack;
     return f;
@@ -580,23 +614,33 @@ extern "C" int sphip_linear(const void* x, int64_t ldx, const void* W, int64_t l
     Epilogue e;
     e.bias = bias, e.bias_dt = bias_dtype, e.res = residual, e.res_dt = res_dtype, e.ldr = ldr;
     e.out = out, e.out_dt = out_dtype, e.ldo = ldo, e.act = act;
-    if (zc) e.z = (char*)ws + f.part, e.z_dt = SPHIP_F32, e.ldz = cdiv(M, 4) * 4;
-    else e.z = z, e.z_dt = z_kind, e.ldz = ldz;
+    // z becomes codes in the epilogue itself, unless the K range is split: its partial sums then meet in the joining kernel,
+    // which has no groups of rows, and z takes the way over fp32
+    if (zc && f.z) e.z = (char*)ws + f.part, e.z_dt = SPHIP_F32, e.ldz = cdiv(M, 4) * 4;
+    else e.z = z, e.z_dt = z_kind, e.ldz = ldz, e.z_scales = zc ? z_scales : nullptr;
     Operand A = {x, nullptr, ldx, (int)N}, B = {W, nullptr, ldw, (int)M};
     int64_t K = D;
     int st = SPHIP_OK;
     if (f.pack) {
         K = packed_ld(D);
         char* to = (char*)ws + f.part + f.z;
-        st = pack_rows("linear", A, N, D, to, s);
-        if (st == SPHIP_OK) st = pack_rows("linear", B, M, D, to + (size_t)N * K * 2, s);
-        if (st != SPHIP_OK) return st;
+        Packing p;
+        if (x_codes) {                                          // x is read once for both
+            st = save_codes("linear", x, dtype, ldx, x_fmt, 0, x_codes, x_scales, ldq, to, K, N, D, s);
+            A.p = to, A.ld = K;
+        } else {
+            p.add(A, N, D, to);
+        }
+        p.add(B, M, D, to + (size_t)N * K * 2);
+        if (st == SPHIP_OK) st = p.launch("linear", s);
+    } else if (x_codes) {
+        st = save_codes("linear", x, dtype, ldx, x_fmt, 0, x_codes, x_scales, ldq, nullptr, 0, N, D, s);
     }
+    if (st != SPHIP_OK) return st;
     st = dtype == SPHIP_BF16 ? launch_product<bf16_t, OP_ROWS, OP_ROWS>("linear", A, B, e, K, K, ws, f.part, s)
                              : launch_product<float, OP_ROWS, OP_ROWS>("linear", A, B, e, K, K, ws, f.part, s);
-    if (st == SPHIP_OK && zc)
-        st = sphip_checkpoint8_save(e.z, SPHIP_F32, e.ldz, z_kind, act == SPHIP_ACT_RELU, (uint8_t*)z, z_scales, ldz, N, M, s);
-    if (st == SPHIP_OK && x_codes) st = sphip_checkpoint8_save(x, dtype, ldx, x_fmt, 0, x_codes, x_scales, ldq, N, D, s);
+    if (st == SPHIP_OK && zc && f.z)
+        st = save_codes("linear", e.z, SPHIP_F32, e.ldz, z_kind, act == SPHIP_ACT_RELU, (uint8_t*)z, z_scales, ldz, nullptr, 0, N, M, s);
     return st;
 }
 
@@ -611,7 +655,7 @@ static BackwardSpace backward_space(int dtype, int x_kind, int want_dx, int want
     const bool bf = dtype == SPHIP_BF16;
     b.dz = want_dx || want_dw ? up256((size_t)N * dz_stride(dtype, M) * dtype_size(dtype)) : 0;
     b.sums = want_db ? up256((size_t)cdiv(N, 32) * M * 4) : 0;
-    b.x = want_dw && bf && worth_packing(M, D, N) && (is_codes(x_kind) || D % 8 != 0) ? up256((size_t)N * packed_ld(D) * 2) : 0;
+    b.x = want_dw && bf && (is_codes(x_kind) ? worth_packing(M, D, N, 31) : D % 8 != 0 && worth_packing(M, D, N)) ? up256((size_t)N * packed_ld(D) * 2) : 0;
     b.w = want_dx && bf && worth_packing(N, D, M) && D % 8 != 0 ? up256((size_t)M * packed_ld(D) * 2) : 0;
     const size_t p1 = want_dx ? split_bytes(dtype, N, D, M) : 0, p2 = want_dw ? split_bytes(dtype, M, D, N) : 0;
     b.part = p1 > p2 ? p1 : p2;
@@ -629,16 +673,12 @@ template <typename T>
 static int backward_products(const Operand& dz, const void* W, int64_t ldw, const void* x, int x_kind, const uint8_t* x_scales,
                              int64_t ldx, void* dx, int dx_dtype, int64_t lddx, void* dW, int dw_dtype, int64_t lddw, int64_t N,
                              int64_t D, int64_t M, bool padded, char* ws, const BackwardSpace& sp, hipStream_t s) {
-    char *xs = ws + sp.dz + sp.sums, *wsp = xs + sp.x, *part = wsp + sp.w;
+    char *xs = ws + sp.dz + sp.sums, *part = xs + sp.x + sp.w;
     if (dx) {
         const char* what = "linear_backward(dx)";
         Epilogue e;
         e.out = dx, e.out_dt = dx_dtype, e.ldo = lddx;
-            Operand A = {dz.p, nullptr, dz.ld, (int)N}, B = {W, nullptr, ldw, (int)D};
-        if (sp.w) {
-            const int st = pack_rows(what, B, M, D, wsp, s);
-            if (st != SPHIP_OK) return st;
-        }
+            const Operand A = {dz.p, nullptr, dz.ld, (int)N}, B = {W, nullptr, ldw, (int)D};
         const int st = launch_product<T, OP_ROWS, OP_COLS>(what, A, B, e, padded ? dz.ld : M, M, part, sp.part, s);
         if (st != SPHIP_OK) return st;
     }
@@ -655,7 +695,9 @@ static int backward_products(const Operand& dz, const void* W, int64_t ldw, cons
             st = sphip_checkpoint8_restore((const uint8_t*)x, x_scales, ldx, x_kind, xs, SPHIP_BF16, ld, N, D, s);
             B.p = xs, B.ld = ld, x_kind = SPHIP_BF16;
         } else {
-            st = pack_rows(what, B, N, D, xs, s);
+            Packing p;
+            p.add(B, N, D, xs);
+            st = p.launch(what, s);
         }
         if (st != SPHIP_OK) return st;
     }
@@ -702,11 +744,20 @@ extern "C" int sphip_linear_backward(const void* g, int g_dtype, int64_t ldg, co
         direct = !((dx && worth_packing(N, D, M)) || (dW && worth_packing(M, D, N)));
     Operand dz = {g, nullptr, ldg, (int)N};
     if (products && !direct) dz.p = w, dz.ld = dz_stride(dtype, M);
-    if (products && !direct && !db && act == SPHIP_ACT_NONE && g_dtype == dtype && dtype == SPHIP_BF16) {
-        Operand o = {g, nullptr, ldg, (int)N};                  // a copy with padded rows is all there is to do
-        const int st = pack_rows("linear_backward(dz)", o, N, M, w, s);
-        if (st != SPHIP_OK) return st;
-    } else if (db || (products && !direct)) {
+    Packing pack;
+    if (sp.w) {
+        Operand o = {W, nullptr, ldw, (int)M};
+        pack.add(o, M, D, w + sp.dz + sp.sums + sp.x);
+        W = o.p, ldw = o.ld;
+    }
+    const bool copied = products && !direct && !db && act == SPHIP_ACT_NONE && g_dtype == dtype && dtype == SPHIP_BF16;
+    if (copied) {                                               // g with padded rows is all there is to do
+        Operand o = {g, nullptr, ldg, (int)N};
+        pack.add(o, N, M, w);
+    }
+    const int pst = pack.launch("linear_backward", s);
+    if (pst != SPHIP_OK) return pst;
+    if (!copied && (db || (products && !direct))) {
         PreactArgs a;
         a.g = g, a.z = z, a.scales = z_scales, a.dz = products && !direct ? w : nullptr, a.part = db ? sums : nullptr;
         a.ldg = ldg, a.ldz = ldz, a.lddz = dz.ld, a.dz_dt = dtype, a.act = act;

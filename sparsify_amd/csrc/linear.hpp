@@ -44,14 +44,77 @@ typedef unsigned w2_t __attribute__((ext_vector_type(2)));
 typedef void __attribute__((address_space(3)))* lds_t;
 
 // The tail the product's kernels share: ROWS x 64 values of C that a wave has put into its own LDS area [row][OUT_ROW bytes],
-// row r being n = n0 + r, leave so that 16 lanes store 64 consecutive m of a row. A lane keeps its m: one bias load. The
-// residual's pieces are all in flight before the first is used (little else hides their latency). Residual and result bypass
-// L2, which holds the operands. The activation is one rolled loop over LDS, not unrolled with the rest: inlined per output
-// quad it made kernels of 60 to 90 KB, more than the instruction cache holds.
+// row r being n = n0 + r, leave so that 16 lanes store 64 consecutive m of a row. A lane keeps its m: one bias load.
+// The activation and the 8-bit codes of z are rolled loops over LDS, not unrolled with the rest: inlined per output quad
+// they made kernels of 60 to 90 KB, more than the instruction cache holds. Residual and result bypass L2, which holds the
+// operands.
 constexpr int OUT_ROW = 272;                       // 64 fp32 + 16 bytes
+
+// the lane's residual pieces, all in flight before the first is used: little else hides their latency
+template <int ROWS> struct Residual {
+    w4_t v[ROWS / 4];
+    __device__ __forceinline__ void load(const Epilogue& epi, const TileGrid& g, int n0, int m0, int N, int M, int lane) {
+        const int m = m0 + (lane & 15) * 4, nb = n0 + (lane >> 4);
+        if (epi.res == nullptr || g.splits > 1 || m + 3 >= M) return;
+        if (epi.res_dt == SPHIP_F32) {
+#pragma unroll
+            for (int i = 0; i < ROWS / 4; ++i)
+                if (nb + 4 * i < N)
+                    v[i] = __builtin_nontemporal_load((const u4_any*)((const float*)epi.res + (int64_t)(nb + 4 * i) * epi.ldr + m));
+        } else {
+#pragma unroll
+            for (int i = 0; i < ROWS / 4; ++i)
+                if (nb + 4 * i < N) {
+                    const u2_any r = __builtin_nontemporal_load((const u2_any*)((const bf16_t*)epi.res + (int64_t)(nb + 4 * i) * epi.ldr + m));
+                    v[i] = (w4_t){r.x << 16, r.x & 0xffff0000u, r.y << 16, r.y & 0xffff0000u};
+                }
+        }
+    }
+};
+
+// z + bias of 32 staged rows (a group of the checkpoint) into 8-bit codes: the maxima of a lane's 4 columns over its 8 rows,
+// then over the 4 lanes that share them; padding rows and columns get zero codes
+template <int FMT>
+__device__ __forceinline__ void store_codes(char* mine, const Epilogue& epi, int nb, int m, int N, int M, const float (&bias)[4], int lane) {
+    unsigned top[4] = {0, 0, 0, 0};
+#pragma unroll 2
+    for (int i = 0; i < 8; ++i) {
+        const float4 c = *reinterpret_cast<const float4*>(mine + i * 4 * OUT_ROW);
+        const float v[4] = {c.x + bias[0], c.y + bias[1], c.z + bias[2], c.w + bias[3]};
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (nb + 4 * i < N && m + j < M) top[j] = max(top[j], __float_as_uint(v[j]) & 0x7fffffffu);
+    }
+    float inv[4];
+    unsigned scales = 0, bad = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        top[j] = max(top[j], (unsigned)__shfl_xor((int)top[j], 16, 64));
+        top[j] = max(top[j], (unsigned)__shfl_xor((int)top[j], 32, 64));
+        const unsigned b = scale_byte<FMT>(top[j]);
+        scales |= b << (8 * j);
+        bad |= b == 255u ? 0xffu << (8 * j) : 0u;
+        inv[j] = inverse_scale(b);
+    }
+    if (m >= epi.ldz || nb - (lane >> 4) >= N) return;
+    const int64_t grp = nb >> 5;
+    if (lane < 16) *reinterpret_cast<unsigned*>(epi.z_scales + grp * epi.ldz + m) = scales;
+    const bool keep = epi.act == SPHIP_ACT_RELU;
+#pragma unroll 2
+    for (int i = 0; i < 8; ++i) {
+        const float4 c = *reinterpret_cast<const float4*>(mine + i * 4 * OUT_ROW);
+        const float v[4] = {c.x + bias[0], c.y + bias[1], c.z + bias[2], c.w + bias[3]};
+        unsigned w = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (nb + 4 * i < N && m + j < M) w |= code_of<FMT>(v[j], inv[j], keep) << (8 * j);
+        *reinterpret_cast<unsigned*>((uint8_t*)epi.z + (int64_t)(nb + 4 * i) * epi.ldz + m) = (w & ~bad) | (bad & 0x7f7f7f7fu);
+    }
+}
+
 template <int ROWS>
 __device__ __forceinline__ void finish_rows(char* stage, const Epilogue& epi, const TileGrid& g, unsigned split, int n0, int m0,
-                                            int N, int M, int lane) {
+                                            int N, int M, int lane, const Residual<ROWS>& res) {
     constexpr int P = ROWS / 4;                    // pieces of 4 outputs per lane
     const int r16 = lane & 15, q4 = lane >> 4, Mp = (M + 3) & ~3;
     const int m = m0 + r16 * 4, nb = n0 + q4, cols = M - m;
@@ -65,70 +128,73 @@ __device__ __forceinline__ void finish_rows(char* stage, const Epilogue& epi, co
             if (nb + 4 * i < N && cols > 0)
                 *reinterpret_cast<float4*>(g.part + ((int64_t)split * N + nb + 4 * i) * Mp + m) =
                     *reinterpret_cast<const float4*>(mine + i * 4 * OUT_ROW);
-    } else if (cols >= 4) {
-        w4_t res[P];
-        if (epi.res != nullptr) {
-            if (epi.res_dt == SPHIP_F32) {
+    } else {
+        float bias[4] = {0.f, 0.f, 0.f, 0.f};
+        if (epi.bias != nullptr) {
+            if (cols >= 4) load4_as_f32(epi.bias, epi.bias_dt, m, bias);
+            else
 #pragma unroll
-                for (int i = 0; i < P; ++i)
-                    if (nb + 4 * i < N)
-                        res[i] = __builtin_nontemporal_load((const u4_any*)((const float*)epi.res + (int64_t)(nb + 4 * i) * epi.ldr + m));
-            } else {
+                for (int j = 0; j < 3; ++j)
+                    if (j < cols) bias[j] = load_as_f32(epi.bias, epi.bias_dt, m + j);
+        }
+        if (epi.z_scales != nullptr) {                          // (the whole wave: lanes exchange maxima)
 #pragma unroll
-                for (int i = 0; i < P; ++i)
-                    if (nb + 4 * i < N) {
-                        const u2_any r = __builtin_nontemporal_load((const u2_any*)((const bf16_t*)epi.res + (int64_t)(nb + 4 * i) * epi.ldr + m));
-                        res[i] = (w4_t){r.x << 16, r.x & 0xffff0000u, r.y << 16, r.y & 0xffff0000u};
-                    }
+            for (int h = 0; h < ROWS / 32; ++h) {
+                char* const at = mine + h * 32 * OUT_ROW;
+                if (epi.z_dt == SPHIP_INT8) store_codes<SPHIP_INT8>(at, epi, nb + 32 * h, m, N, M, bias, lane);
+                else store_codes<SPHIP_E4M3>(at, epi, nb + 32 * h, m, N, M, bias, lane);
             }
         }
-        if (epi.bias != nullptr || epi.act != SPHIP_ACT_NONE || epi.z != nullptr) {
-            float bias[4] = {0.f, 0.f, 0.f, 0.f};
-            if (epi.bias != nullptr) load4_as_f32(epi.bias, epi.bias_dt, m, bias);
-#pragma unroll 1
+        if (cols >= 4) {
+            if (epi.bias != nullptr || epi.act != SPHIP_ACT_NONE || epi.z != nullptr) {
+#pragma unroll 2
+                for (int i = 0; i < P; ++i) {
+                    const int n = nb + 4 * i;
+                    float4* at = reinterpret_cast<float4*>(mine + i * 4 * OUT_ROW);
+                    const float4 c = *at;
+                    float v[4] = {c.x + bias[0], c.y + bias[1], c.z + bias[2], c.w + bias[3]};
+                    if (epi.z != nullptr && epi.z_scales == nullptr && n < N) store4_from_f32(epi.z, epi.z_dt, n * epi.ldz + m, v);
+                    act_value4(v, epi.act);
+                    *at = make_float4(v[0], v[1], v[2], v[3]);
+                }
+            }
+#pragma unroll
             for (int i = 0; i < P; ++i) {
                 const int n = nb + 4 * i;
-                if (n >= N) break;
-                float4* at = reinterpret_cast<float4*>(mine + i * 4 * OUT_ROW);
-                const float4 c = *at;
-                float v[4] = {c.x + bias[0], c.y + bias[1], c.z + bias[2], c.w + bias[3]};
-                if (epi.z != nullptr) store4_from_f32(epi.z, epi.z_dt, n * epi.ldz + m, v);
-                act_value4(v, epi.act);
-                *at = make_float4(v[0], v[1], v[2], v[3]);
-            }
-        }
+                if (n >= N) continue;
+                const float4 c = *reinterpret_cast<const float4*>(mine + i * 4 * OUT_ROW);
+                float v[4] = {c.x, c.y, c.z, c.w};
+                if (epi.res != nullptr) {
 #pragma unroll
-        for (int i = 0; i < P; ++i) {
-            const int n = nb + 4 * i;
-            if (n >= N) continue;
-            const float4 c = *reinterpret_cast<const float4*>(mine + i * 4 * OUT_ROW);
-            float v[4] = {c.x, c.y, c.z, c.w};
-            if (epi.res != nullptr) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) v[j] += __uint_as_float(res[i][j]);
+                    for (int j = 0; j < 4; ++j) v[j] += __uint_as_float(res.v[i][j]);
+                }
+                if (epi.out_dt == SPHIP_F32) {
+                    const u4_any o = {__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
+                    __builtin_nontemporal_store(o, (u4_any*)((float*)epi.out + n * epi.ldo + m));
+                } else {
+                    const u2_any o = {(unsigned)f32_to_bf16(v[0]) | ((unsigned)f32_to_bf16(v[1]) << 16),
+                                      (unsigned)f32_to_bf16(v[2]) | ((unsigned)f32_to_bf16(v[3]) << 16)};
+                    __builtin_nontemporal_store(o, (u2_any*)((bf16_t*)epi.out + n * epi.ldo + m));
+                }
             }
-            if (epi.out_dt == SPHIP_F32) {
-                const u4_any o = {__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
-                __builtin_nontemporal_store(o, (u4_any*)((float*)epi.out + n * epi.ldo + m));
-            } else {
-                const u2_any o = {(unsigned)f32_to_bf16(v[0]) | ((unsigned)f32_to_bf16(v[1]) << 16),
-                                  (unsigned)f32_to_bf16(v[2]) | ((unsigned)f32_to_bf16(v[3]) << 16)};
-                __builtin_nontemporal_store(o, (u2_any*)((bf16_t*)epi.out + n * epi.ldo + m));
-            }
-        }
-    } else if (cols > 0) {
+        } else if (cols > 0) {
 #pragma unroll 1
-        for (int i = 0; i < P; ++i) {
-            if (nb + 4 * i >= N) break;
-            const float4 c = *reinterpret_cast<const float4*>(mine + i * 4 * OUT_ROW);
-            float v[4] = {c.x, c.y, c.z, c.w};
-            epilogue4(epi, nb + 4 * i, m, M, v);
+            for (int i = 0; i < P; ++i) {
+                if (nb + 4 * i >= N) break;
+                const float4 c = *reinterpret_cast<const float4*>(mine + i * 4 * OUT_ROW);
+                float v[4] = {c.x, c.y, c.z, c.w};
+                epilogue4(epi, nb + 4 * i, m, M, v);
+            }
         }
     }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
+
+// checkpoint8.hip: x (N, D) in 8 bits; with `packed` also a copy of it in rows of ldp elements, zeros behind column D
+int save_codes(const char* what, const void* x, int dtype, int64_t ldx, int fmt, int keep_sign, uint8_t* codes, uint8_t* scales,
+               int64_t ldq, void* packed, int64_t ldp, int64_t N, int64_t D, hipStream_t s);
 
 // The LDS-DMA kernels (bf16): whether they take these operands, how they split K, their launch (the caller joins). KB: rows
 // of an OP_COLS B, which may be fewer than K (a multiple of 64 where A is OP_ROWS): B counts as zero from there on.

@@ -11,6 +11,7 @@
 namespace sphip {
 
 constexpr int T128 = 128, IMG_A = 0, IMG_B = 16384, STAGE = 32768;
+constexpr int FINISH = 4 * 64 * OUT_ROW;            // the epilogue's staging: more than two stages, twice still within the LDS
 
 template <int MODE> struct Source128 {
     __amdgpu_buffer_rsrc_t rsrc;
@@ -79,6 +80,9 @@ __global__ __launch_bounds__(256, STAGES == 2 ? 2 : 1) void linear128_kernel(Ope
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[i][j] = (acc4_t){0.f, 0.f, 0.f, 0.f};
 
+    const int N = A.rows, M = B.rows;
+    Residual<64> res;                              // waits in registers until the product is done
+    res.load(epi, g, n0 + wn * 64, m0 + wm * 64, N, M, lane);
 #pragma unroll
     for (int t = 0; t < STAGES - 1; ++t) fetch(t, t * STAGE);
     unsigned img = 0, freed = (STAGES - 1) * STAGE;            // buffers of step t and of step t - 1
@@ -116,10 +120,8 @@ __global__ __launch_bounds__(256, STAGES == 2 ? 2 : 1) void linear128_kernel(Ope
         img = img + STAGE == STAGES * STAGE ? 0 : img + STAGE;
     }
     __syncthreads();                               // the last step has been read: the buffers become the staging area
-    const int N = A.rows, M = B.rows;
-    char* const stage = smem + wave * 32 * OUT_ROW;
-    finish_tile<2>([&](int mt, int nt) { return acc[mt][nt]; }, stage, epi, g, split, n0 + wn * 64, m0 + wm * 64, N, M, lane);
-    finish_tile<2>([&](int mt, int nt) { return acc[mt][2 + nt]; }, stage, epi, g, split, n0 + wn * 64 + 32, m0 + wm * 64, N, M, lane);
+    finish_tile<4>([&](int mt, int nt) { return acc[mt][nt]; }, smem + wave * 64 * OUT_ROW, epi, g, split, n0 + wn * 64, m0 + wm * 64,
+                   N, M, lane, res);
 }
 
 bool linear128_takes(int mode_a, int mode_b, const Operand& A, const Operand& B, int64_t K) {
@@ -143,7 +145,7 @@ int launch_linear128(const char* what, int mode_a, int mode_b, const Operand& A,
     static const kern_t kerns[3][2] = {{linear128_kernel<OP_ROWS, OP_ROWS, 2>, linear128_kernel<OP_ROWS, OP_ROWS, 4>},
                                        {linear128_kernel<OP_ROWS, OP_COLS, 2>, linear128_kernel<OP_ROWS, OP_COLS, 4>},
                                        {linear128_kernel<OP_COLS, OP_COLS, 2>, linear128_kernel<OP_COLS, OP_COLS, 4>}};
-    const int lds = (deep ? 4 : 2) * STAGE;
+    const int lds = deep ? 4 * STAGE : FINISH;
     SPHIP_REQUIRE(hipFuncSetAttribute((const void*)kerns[which][deep], hipFuncAttributeMaxDynamicSharedMemorySize, lds) == hipSuccess,
                   SPHIP_ELAUNCH, "%s: cannot reserve %d bytes of LDS", what, lds);
     hipLaunchKernelGGL(kerns[which][deep], dim3((unsigned)blocks), dim3(256), lds, s, A, B, epi, K, KB, g);

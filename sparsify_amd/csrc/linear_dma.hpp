@@ -76,14 +76,14 @@ template <int PITCH> struct Frag<OP_COLS, PITCH> {     // PITCH bytes per k row 
 // The 16x16 accumulators acc(mt, nt) of a wave (4 consecutive m of one n per lane), 16 NT rows of n, through its LDS area.
 template <int NT, typename Acc>
 __device__ __forceinline__ void finish_tile(Acc acc, char* stage, const Epilogue& epi, const TileGrid& g, unsigned split, int n0,
-                                            int m0, int N, int M, int lane) {
+                                            int m0, int N, int M, int lane, const Residual<NT * 16>& res) {
     const int r16 = lane & 15, q4 = lane >> 4;
 #pragma unroll
     for (int mt = 0; mt < 4; ++mt)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
             *reinterpret_cast<acc4_t*>(stage + (nt * 16 + r16) * OUT_ROW + (mt * 16 + q4 * 4) * 4) = acc(mt, nt);
-    finish_rows<NT * 16>(stage, epi, g, split, n0, m0, N, M, lane);
+    finish_rows<NT * 16>(stage, epi, g, split, n0, m0, N, M, lane, res);
 }
 
 // whether LDS-DMA can fetch an operand: 16-byte aligned rows, 32-bit byte offsets inside a tile's descriptor

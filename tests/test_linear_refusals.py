@@ -33,7 +33,7 @@ def linear(**kw):
     (dict(D=4096, ldx=4096, ldw=4096, ws=P + 4, nws=1 << 30), EWORKSPACE, b"aligned"),
     (dict(z=P, z_kind=9, ldz=32), EINVAL, b"dtype"), (dict(z=P, z_kind=INT8, ldz=32), EINVAL, b"codes"),
     (dict(z=P, z_kind=E4M3, z_scales=P, ldz=40), EINVAL, b"codes"), (dict(z=P + 8, z_kind=INT8, z_scales=P, ldz=32), EINVAL, b"codes"),
-    (dict(z=P, z_kind=INT8, z_scales=P, ldz=32), EWORKSPACE, b"workspace"), (dict(xc=P, x_fmt=BF16), EINVAL, b"dtype"),
+    (dict(z=P, z_kind=INT8, z_scales=P, ldz=32, D=4096, ldx=4096, ldw=4096), EWORKSPACE, b"workspace"), (dict(xc=P, x_fmt=BF16), EINVAL, b"dtype"),
     (dict(xc=P, x_fmt=INT8, ldq=64), EINVAL, b"codes"), (dict(xc=P, xs=P, x_fmt=INT8, ldq=48), EINVAL, b"codes")])
 def test_linear_entry(kw, status, word):
     assert linear(**kw) == status and word in lib().sphip_last_error()
@@ -67,7 +67,8 @@ def test_backward_entry(kw, status, word):
 def test_workspace_queries():
     L = lib()
     assert L.sphip_linear_workspace_bytes(BF16, 0, 0, 8, 8) == 0 and L.sphip_linear_workspace_bytes(9, 0, 8, 8, 8) == 0
-    assert L.sphip_linear_workspace_bytes(BF16, INT8, 8, 64, 32) >= 8 * 32 * 4
+    assert L.sphip_linear_workspace_bytes(BF16, INT8, 8, 4096, 32) >= L.sphip_linear_workspace_bytes(BF16, F32, 8, 4096, 32) + 8 * 32 * 4
+    assert L.sphip_linear_workspace_bytes(BF16, INT8, 8, 64, 32) == 0
     assert L.sphip_linear_backward_workspace_bytes(BF16, INT8, 0, 0, 1, 64, 64, 32) == 2 * 32 * 4
     assert L.sphip_linear_backward_workspace_bytes(F32, F32, 1, 1, 1, 8, -1, 32) == 0
 
