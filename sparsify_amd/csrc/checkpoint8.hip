@@ -74,11 +74,11 @@ __global__ __launch_bounds__(256) void checkpoint8_save_kernel(SaveArgs a) {
         for (int j = 0; j < V; j += 4) *reinterpret_cast<uint4*>(&red[wave][cl * V + j]) = make_uint4(top[j], top[j + 1], top[j + 2], top[j + 3]);
     __syncthreads();
     if (c0 >= max(a.ldq, a.packed != nullptr ? a.ldp : 0)) return;
-    float inv[V];
-    bool bad[V];
-    uint8_t sb[V];
+    float inv[V / 4][4];
+    unsigned bad[V / 4], sb[V / 4];
 #pragma unroll
     for (int j = 0; j < V; j += 4) {
+        bad[j / 4] = sb[j / 4] = 0;
         uint4 m = *reinterpret_cast<const uint4*>(&red[0][cl * V + j]);
 #pragma unroll
         for (int i = 1; i < 4; ++i) {
@@ -89,7 +89,7 @@ __global__ __launch_bounds__(256) void checkpoint8_save_kernel(SaveArgs a) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const unsigned b = scale_byte<FMT>(mv[i]);
-            sb[j + i] = (uint8_t)b, bad[j + i] = b == 255u, inv[j + i] = inverse_scale(b);
+            sb[j / 4] |= b << (8 * i), bad[j / 4] |= b == 255u ? 0xffu << (8 * i) : 0u, inv[j / 4][i] = inverse_scale(b);
         }
     }
     const bool in = c0 < a.ldq;
@@ -98,10 +98,13 @@ __global__ __launch_bounds__(256) void checkpoint8_save_kernel(SaveArgs a) {
     for (int t = 0; t < W; ++t) {
         const int64_t row = r0 + 8 * t;
         if (in) {
-            uint8_t o[V];
+            unsigned o[V / 4];
 #pragma unroll
-            for (int j = 0; j < V; ++j)
-                o[j] = (uint8_t)(bad[j] ? 0x7fu : code_of<FMT>(__uint_as_float(bits(t, j)), inv[j], a.keep != 0));
+            for (int j = 0; j < V; j += 4) {
+                const float v[4] = {__uint_as_float(bits(t, j)), __uint_as_float(bits(t, j + 1)), __uint_as_float(bits(t, j + 2)),
+                                    __uint_as_float(bits(t, j + 3))};
+                o[j / 4] = codes_of<FMT>(v, inv[j / 4], a.keep != 0, bad[j / 4]);
+            }
             __builtin_memcpy(a.codes + row * a.ldq + c0, o, V);
         }
         if (a.packed != nullptr && row < a.N && c0 < a.ldp)

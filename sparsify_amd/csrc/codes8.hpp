@@ -40,18 +40,30 @@ template <int FMT> __device__ __forceinline__ unsigned scale_byte(unsigned top) 
 }
 // 1 / scale, a normal number (1 <= byte <= 249)
 __device__ __forceinline__ float inverse_scale(unsigned byte) { return __uint_as_float((byte == 255u ? 127u : 254u - byte) << 23); }
-// code of a, given the inverse scale: a power of two, so that a * inv is exact and there is one rounding, to nearest even
-template <int FMT> __device__ __forceinline__ unsigned code_of(float a, float inv, bool keep_sign) {
-    unsigned c;
+// Codes of four values, given the inverse scales: powers of two, so that a * inv is exact and there is one rounding, to
+// nearest even. bad: 0xff in the bytes whose group is to read as NaN (their codes are not looked at; kept finite).
+template <int FMT> __device__ __forceinline__ unsigned codes_of(const float (&a)[4], const float (&inv)[4], bool keep_sign, unsigned bad) {
+    unsigned w;
     if (FMT == SPHIP_INT8) {
-        c = __float_as_uint(fmaf(a, inv, 12582912.f)) & 0xffu;               // 1.5 2^23: the low byte is the two's complement code
-        if (keep_sign && c == 0u && a != 0.f) c = a < 0.f ? 0xffu : 1u;
+        // + 1.5 2^23: the low byte is the two's complement code
+        unsigned c[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) c[j] = __float_as_uint(fmaf(a[j], inv[j], 12582912.f));
+        const unsigned lo = __builtin_amdgcn_perm(c[1], c[0], 0x0c0c0400u), hi = __builtin_amdgcn_perm(c[3], c[2], 0x04000c0cu);
+        w = lo | hi;
     } else {
-        const float s = a * inv;
-        c = (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(s, s, 0, false) & 0xffu;
-        if (keep_sign && (c & 0x7fu) == 0u && a != 0.f) c = a < 0.f ? 0x81u : 1u;
+        int t = __builtin_amdgcn_cvt_pk_fp8_f32(a[0] * inv[0], a[1] * inv[1], 0, false);
+        w = (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(a[2] * inv[2], a[3] * inv[3], t, true);
     }
-    return c;
+    if (keep_sign) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const unsigned c = (w >> (8 * j)) & (FMT == SPHIP_INT8 ? 0xffu : 0x7fu);
+            const unsigned least = FMT == SPHIP_INT8 ? (a[j] < 0.f ? 0xffu : 1u) : (a[j] < 0.f ? 0x81u : 1u);
+            if (c == 0u && a[j] != 0.f) w = (w & ~(0xffu << (8 * j))) | (least << (8 * j));
+        }
+    }
+    return (w & ~bad) | (bad & 0x7f7f7f7fu);
 }
 
 }  // namespace sphip

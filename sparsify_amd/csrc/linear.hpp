@@ -50,24 +50,49 @@ typedef void __attribute__((address_space(3)))* lds_t;
 // operands.
 constexpr int OUT_ROW = 272;                       // 64 fp32 + 16 bytes
 
-// the lane's residual pieces, all in flight before the first is used: little else hides their latency
+// The lane's residual pieces, raw, all in flight before the first is used: little else hides their latency. No branch and no
+// arithmetic between the loads (either would wait for them one by one): rows past the end load the last row again.
 template <int ROWS> struct Residual {
     w4_t v[ROWS / 4];
     __device__ __forceinline__ void load(const Epilogue& epi, const TileGrid& g, int n0, int m0, int N, int M, int lane) {
-        const int m = m0 + (lane & 15) * 4, nb = n0 + (lane >> 4);
-        if (epi.res == nullptr || g.splits > 1 || m + 3 >= M) return;
-        if (epi.res_dt == SPHIP_F32) {
+        const int m = m0 + (lane & 15) * 4, nb = n0 + (lane >> 4), cols = M - m;
+        if (epi.res == nullptr || g.splits > 1 || cols <= 0) return;
+        if (cols >= 4) {
+            if (epi.res_dt == SPHIP_F32) {
 #pragma unroll
-            for (int i = 0; i < ROWS / 4; ++i)
-                if (nb + 4 * i < N)
-                    v[i] = __builtin_nontemporal_load((const u4_any*)((const float*)epi.res + (int64_t)(nb + 4 * i) * epi.ldr + m));
+                for (int i = 0; i < ROWS / 4; ++i)
+                    v[i] = __builtin_nontemporal_load((const u4_any*)((const float*)epi.res + (int64_t)min(nb + 4 * i, N - 1) * epi.ldr + m));
+            } else {
+#pragma unroll
+                for (int i = 0; i < ROWS / 4; ++i) {
+                    const u2_any r = __builtin_nontemporal_load((const u2_any*)((const bf16_t*)epi.res + (int64_t)min(nb + 4 * i, N - 1) * epi.ldr + m));
+                    v[i].x = r.x, v[i].y = r.y;
+                }
+            }
+        } else if (epi.res_dt == SPHIP_F32) {      // the row's last, partial piece: missing columns load the last one again
+#pragma unroll
+            for (int i = 0; i < ROWS / 4; ++i) {
+                const unsigned* p = (const unsigned*)epi.res + (int64_t)min(nb + 4 * i, N - 1) * epi.ldr + m;
+                v[i].x = p[0], v[i].y = p[min(1, cols - 1)], v[i].z = p[cols - 1];
+            }
         } else {
 #pragma unroll
-            for (int i = 0; i < ROWS / 4; ++i)
-                if (nb + 4 * i < N) {
-                    const u2_any r = __builtin_nontemporal_load((const u2_any*)((const bf16_t*)epi.res + (int64_t)(nb + 4 * i) * epi.ldr + m));
-                    v[i] = (w4_t){r.x << 16, r.x & 0xffff0000u, r.y << 16, r.y & 0xffff0000u};
-                }
+            for (int i = 0; i < ROWS / 4; ++i) {
+                const bf16_t* p = (const bf16_t*)epi.res + (int64_t)min(nb + 4 * i, N - 1) * epi.ldr + m;
+                v[i].x = p[0], v[i].y = p[min(1, cols - 1)], v[i].z = p[cols - 1];
+            }
+        }
+    }
+    __device__ __forceinline__ void get(const Epilogue& epi, int i, int cols, float (&r)[4]) const {
+        if (epi.res_dt == SPHIP_F32) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) r[j] = __uint_as_float(v[i][j]);
+        } else if (cols >= 4) {
+            r[0] = __uint_as_float(v[i].x << 16), r[1] = __uint_as_float(v[i].x & 0xffff0000u);
+            r[2] = __uint_as_float(v[i].y << 16), r[3] = __uint_as_float(v[i].y & 0xffff0000u);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) r[j] = __uint_as_float(v[i][j] << 16);
         }
     }
 };
@@ -75,41 +100,35 @@ template <int ROWS> struct Residual {
 // z + bias of 32 staged rows (a group of the checkpoint) into 8-bit codes: the maxima of a lane's 4 columns over its 8 rows,
 // then over the 4 lanes that share them; padding rows and columns get zero codes
 template <int FMT>
-__device__ __forceinline__ void store_codes(char* mine, const Epilogue& epi, int nb, int m, int N, int M, const float (&bias)[4], int lane) {
-    unsigned top[4] = {0, 0, 0, 0};
-#pragma unroll 2
+__device__ __forceinline__ void store_codes(const char* mine, const Epilogue& epi, int nb, int m, int N, int M, const float (&bias)[4], int lane) {
+    float v[8][4];
+#pragma unroll
     for (int i = 0; i < 8; ++i) {
         const float4 c = *reinterpret_cast<const float4*>(mine + i * 4 * OUT_ROW);
-        const float v[4] = {c.x + bias[0], c.y + bias[1], c.z + bias[2], c.w + bias[3]};
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (nb + 4 * i < N && m + j < M) top[j] = max(top[j], __float_as_uint(v[j]) & 0x7fffffffu);
+        const bool in = nb + 4 * i < N;
+        v[i][0] = in && m < M ? c.x + bias[0] : 0.f, v[i][1] = in && m + 1 < M ? c.y + bias[1] : 0.f;
+        v[i][2] = in && m + 2 < M ? c.z + bias[2] : 0.f, v[i][3] = in && m + 3 < M ? c.w + bias[3] : 0.f;
     }
     float inv[4];
     unsigned scales = 0, bad = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        top[j] = max(top[j], (unsigned)__shfl_xor((int)top[j], 16, 64));
-        top[j] = max(top[j], (unsigned)__shfl_xor((int)top[j], 32, 64));
-        const unsigned b = scale_byte<FMT>(top[j]);
+        unsigned top = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i][j]) & 0x7fffffffu);
+        top = max(top, (unsigned)__shfl_xor((int)top, 16, 64));
+        top = max(top, (unsigned)__shfl_xor((int)top, 32, 64));
+        const unsigned b = scale_byte<FMT>(top);
         scales |= b << (8 * j);
         bad |= b == 255u ? 0xffu << (8 * j) : 0u;
         inv[j] = inverse_scale(b);
     }
     if (m >= epi.ldz || nb - (lane >> 4) >= N) return;
-    const int64_t grp = nb >> 5;
-    if (lane < 16) *reinterpret_cast<unsigned*>(epi.z_scales + grp * epi.ldz + m) = scales;
+    if (lane < 16) *reinterpret_cast<unsigned*>(epi.z_scales + (int64_t)(nb >> 5) * epi.ldz + m) = scales;
     const bool keep = epi.act == SPHIP_ACT_RELU;
-#pragma unroll 2
-    for (int i = 0; i < 8; ++i) {
-        const float4 c = *reinterpret_cast<const float4*>(mine + i * 4 * OUT_ROW);
-        const float v[4] = {c.x + bias[0], c.y + bias[1], c.z + bias[2], c.w + bias[3]};
-        unsigned w = 0;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (nb + 4 * i < N && m + j < M) w |= code_of<FMT>(v[j], inv[j], keep) << (8 * j);
-        *reinterpret_cast<unsigned*>((uint8_t*)epi.z + (int64_t)(nb + 4 * i) * epi.ldz + m) = (w & ~bad) | (bad & 0x7f7f7f7fu);
-    }
+    for (int i = 0; i < 8; ++i)
+        *reinterpret_cast<unsigned*>((uint8_t*)epi.z + (int64_t)(nb + 4 * i) * epi.ldz + m) = codes_of<FMT>(v[i], inv, keep, bad);
 }
 
 template <int ROWS>
@@ -138,36 +157,44 @@ __device__ __forceinline__ void finish_rows(char* stage, const Epilogue& epi, co
                     if (j < cols) bias[j] = load_as_f32(epi.bias, epi.bias_dt, m + j);
         }
         if (epi.z_scales != nullptr) {                          // (the whole wave: lanes exchange maxima)
-#pragma unroll
-            for (int h = 0; h < ROWS / 32; ++h) {
-                char* const at = mine + h * 32 * OUT_ROW;
-                if (epi.z_dt == SPHIP_INT8) store_codes<SPHIP_INT8>(at, epi, nb + 32 * h, m, N, M, bias, lane);
-                else store_codes<SPHIP_E4M3>(at, epi, nb + 32 * h, m, N, M, bias, lane);
+#pragma unroll 1
+            for (int h = 0; h < ROWS; h += 32) {
+                if (epi.z_dt == SPHIP_INT8) store_codes<SPHIP_INT8>(mine + h * OUT_ROW, epi, nb + h, m, N, M, bias, lane);
+                else store_codes<SPHIP_E4M3>(mine + h * OUT_ROW, epi, nb + h, m, N, M, bias, lane);
             }
         }
-        if (cols >= 4) {
-            if (epi.bias != nullptr || epi.act != SPHIP_ACT_NONE || epi.z != nullptr) {
+        if (epi.bias != nullptr || epi.act != SPHIP_ACT_NONE || epi.z != nullptr) {
+            const bool values = epi.z != nullptr && epi.z_scales == nullptr;
 #pragma unroll 2
-                for (int i = 0; i < P; ++i) {
-                    const int n = nb + 4 * i;
-                    float4* at = reinterpret_cast<float4*>(mine + i * 4 * OUT_ROW);
-                    const float4 c = *at;
-                    float v[4] = {c.x + bias[0], c.y + bias[1], c.z + bias[2], c.w + bias[3]};
-                    if (epi.z != nullptr && epi.z_scales == nullptr && n < N) store4_from_f32(epi.z, epi.z_dt, n * epi.ldz + m, v);
-                    act_value4(v, epi.act);
-                    *at = make_float4(v[0], v[1], v[2], v[3]);
-                }
-            }
-#pragma unroll
             for (int i = 0; i < P; ++i) {
                 const int n = nb + 4 * i;
-                if (n >= N) continue;
-                const float4 c = *reinterpret_cast<const float4*>(mine + i * 4 * OUT_ROW);
-                float v[4] = {c.x, c.y, c.z, c.w};
-                if (epi.res != nullptr) {
+                float4* at = reinterpret_cast<float4*>(mine + i * 4 * OUT_ROW);
+                const float4 c = *at;
+                float v[4] = {c.x + bias[0], c.y + bias[1], c.z + bias[2], c.w + bias[3]};
+                if (values && n < N) {
+                    if (cols >= 4) store4_from_f32(epi.z, epi.z_dt, n * epi.ldz + m, v);
+                    else
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) v[j] += __uint_as_float(res.v[i][j]);
+                        for (int j = 0; j < 3; ++j)
+                            if (j < cols) store_from_f32(epi.z, epi.z_dt, n * epi.ldz + m + j, v[j]);
                 }
+                act_value4(v, epi.act);
+                *at = make_float4(v[0], v[1], v[2], v[3]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            const int n = nb + 4 * i;
+            if (n >= N) continue;
+            const float4 c = *reinterpret_cast<const float4*>(mine + i * 4 * OUT_ROW);
+            float v[4] = {c.x, c.y, c.z, c.w};
+            if (epi.res != nullptr) {
+                float r[4];
+                res.get(epi, i, cols, r);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] += r[j];
+            }
+            if (cols >= 4) {
                 if (epi.out_dt == SPHIP_F32) {
                     const u4_any o = {__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
                     __builtin_nontemporal_store(o, (u4_any*)((float*)epi.out + n * epi.ldo + m));
@@ -176,14 +203,10 @@ __device__ __forceinline__ void finish_rows(char* stage, const Epilogue& epi, co
                                       (unsigned)f32_to_bf16(v[2]) | ((unsigned)f32_to_bf16(v[3]) << 16)};
                     __builtin_nontemporal_store(o, (u2_any*)((bf16_t*)epi.out + n * epi.ldo + m));
                 }
-            }
-        } else if (cols > 0) {
-#pragma unroll 1
-            for (int i = 0; i < P; ++i) {
-                if (nb + 4 * i >= N) break;
-                const float4 c = *reinterpret_cast<const float4*>(mine + i * 4 * OUT_ROW);
-                float v[4] = {c.x, c.y, c.z, c.w};
-                epilogue4(epi, nb + 4 * i, m, M, v);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 3; ++j)
+                    if (j < cols) store_from_f32(epi.out, epi.out_dt, n * epi.ldo + m + j, v[j]);
             }
         }
     }
