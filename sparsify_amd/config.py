@@ -93,6 +93,11 @@ class TrainConfig(_Serializable):
     multi-top-k) do not store the (tokens, latents) matrix: top-k from candidate lists the GEMM
     epilogue emits (csrc/lazy.hip). Same selection; 4 GiB less per 16384 tokens, about 3 % more
     forward time at the headline shape."""
+    checkpoint_8bit: Literal["int8", "e4m3"] | None = None
+    """(not in the reference) keep every coder's input between forward and backward in 8 bits, once for the encoder and the
+    skip connection (SparseCoder.checkpoint): half the bytes of a bf16 batch, a quarter of an fp32 one. What it saves adds
+    up where many coders wait for one backward pass, the end-to-end losses ("ce", "kl"). Gradients of encoder.weight and
+    W_skip are then those at the 8-bit values. Not with `shard_latents`."""
     save_every: int = 1000
     save_best: bool = False
     finetune: str | None = None
@@ -115,5 +120,9 @@ class TrainConfig(_Serializable):
         if self.shard_latents and (self.distribute_modules or self.loss_fn != "fvu" or self.sae.activation != "topk"):
             raise ValueError("`shard_latents` implements the top-k FVU step (with AuxK, multi-top-k and the skip "
                              "connection): no distribute_modules, ce / kl loss or groupmax")
+        if self.checkpoint_8bit not in (None, "int8", "e4m3"):
+            raise ValueError(f"checkpoint_8bit must be None, 'int8' or 'e4m3', got {self.checkpoint_8bit!r}")
+        if self.checkpoint_8bit is not None and self.shard_latents:
+            raise ValueError("`checkpoint_8bit` does not go with `shard_latents`")
         if not self.init_seeds:
             raise ValueError("Must specify at least one random seed.")

@@ -309,12 +309,17 @@ static int split_count(int64_t N, int64_t M, int64_t steps) {
 static size_t part_bytes(int64_t N, int64_t M, int splits) {
     return splits > 1 ? (size_t)splits * N * ((M + 3) / 4 * 4) * 4 : 0;
 }
+// SPHIP_LINEAR=tile|128|256|few forces a kernel (tests, A/B runs); read once per entry point
+static thread_local char g_forced = 0;
+static void read_forced() {
+    const char* e = getenv("SPHIP_LINEAR");
+    g_forced = e ? e[0] : 0;
+}
+
 // Which kernel a bf16 product of these sizes goes to if its operands are such that LDS-DMA can fetch them.
 enum { BY_TILES = 0, BY_128 = 1, BY_256 = 2 };
 static int kernel_for(int64_t N, int64_t M) {
-    // SPHIP_LINEAR=tile|128|256 forces a kernel (tests, A/B runs)
-    const char* force = getenv("SPHIP_LINEAR");
-    if (force) return force[0] == '2' ? BY_256 : force[0] == '1' ? BY_128 : BY_TILES;
+    if (g_forced) return g_forced == '2' ? BY_256 : g_forced == '1' ? BY_128 : BY_TILES;
     // The 256 x 256 kernel where its tiles fill most of the 256 compute units once: 16384 x 1024 x 4096 takes 101 us against
     // 118 with 128 x 128 tiles, 8192 x 2048 x 2048 56 against 68. Below, splitting K for the large tile costs more than the
     // smaller tile does: 1000 x 4096 x 4096 (64 large tiles) 47 us against 41, 2048^3 37 against 25.
@@ -416,8 +421,7 @@ struct Packing {
 // Whether a bf16 product is worth copying an operand whose rows LDS-DMA cannot fetch (they do not start at multiples of 16
 // bytes, or K is no multiple of 64)
 static bool worth_packing(int64_t N, int64_t M, int64_t K, int least = 29) {
-    const char* force = getenv("SPHIP_LINEAR");
-    return force ? force[0] != 't' : N * M * K >= (1ll << least);
+    return g_forced ? g_forced != 't' : N * M * K >= (1ll << least);
 }
 
 // ---- dz = g act'(z) and its column sums. A workgroup takes 32 rows (the group one scale of an 8-bit z covers) of 32 x 16
@@ -574,16 +578,27 @@ static size_t up256(size_t b) { return (b + 255) / 256 * 256; }
 struct ForwardSpace {
     size_t part, z, pack, total;
 };
+// Whether the forward product takes linear_few.hip. Its workgroups read x through the caches once each and share K among 8
+// waves only; the tile kernels stage x and split K further. bf16, us here / with 128 x 128 tiles: 1 x 4096 x 4096 7.2 / 10.4,
+// 16 x 4096 x 4096 9.7 / 11.1, 40 x 333 x 777 7.0 / 9.9, but 64 x 4096 x 4096 20 / 14 and 16 x 8192 x 256 16 / 7. fp32 (whose
+// tiles take 42 us at 1 x 4096 x 4096, here 12): but for a long K with few rows of W (16 x 8192 x 256 30 / 17).
+static bool few(int dtype, int64_t N, int64_t D, int64_t M) {
+    if (N > FEW || (g_forced && g_forced != 'f')) return false;
+    if (g_forced || dtype != SPHIP_BF16) return g_forced || D <= 4096 || M >= 2048;
+    return cdiv(N, 16) * 16 * D <= 65536 || (N <= 16 && M >= 4096);
+}
 static ForwardSpace forward_space(int dtype, int z_kind, int64_t N, int64_t D, int64_t M) {
     ForwardSpace f;
-    f.part = up256(split_bytes(dtype, N, M, D));
-    f.z = is_codes(z_kind) && f.part ? up256((size_t)N * (cdiv(M, 4) * 4) * 4) : 0;      // (part: the K range may be split)
-    f.pack = dtype == SPHIP_BF16 && D % 64 != 0 && worth_packing(N, M, D) ? (size_t)(N + M) * packed_ld(D) * 2 : 0;
+    const bool one = few(dtype, N, D, M);
+    f.part = one ? 0 : up256(split_bytes(dtype, N, M, D));
+    f.z = is_codes(z_kind) && (f.part || one) ? up256((size_t)N * (cdiv(M, 4) * 4) * 4) : 0;      // (no codes from a split K range or from few rows)
+    f.pack = dtype == SPHIP_BF16 && !one && D % 64 != 0 && worth_packing(N, M, D) ? (size_t)(N + M) * packed_ld(D) * 2 : 0;
     f.total = f.part + f.z + f.pack;
     return f;
 }
 extern "C" size_t sphip_linear_workspace_bytes(int dtype, int z_kind, int64_t N, int64_t D, int64_t M) {
     if (N <= 0 || D <= 0 || M <= 0 || !valid_dtype(dtype)) return 0;
+    read_forced();
     return forward_space(dtype, z_kind, N, D, M).total;
 }
 
@@ -607,6 +622,7 @@ extern "C" int sphip_linear(const void* x, int64_t ldx, const void* W, int64_t l
                   SPHIP_EINVAL, "linear: a pointer is not aligned to its element");
     SPHIP_REQUIRE((!zc || codes_ok(z, z_scales, ldz, M)) && (!x_codes || codes_ok(x_codes, x_scales, ldq, D)), SPHIP_EINVAL,
                   "linear: codes and scales need 16-byte aligned rows of at least their columns");
+    read_forced();
     const ForwardSpace f = forward_space(dtype, zc ? z_kind : SPHIP_F32, N, D, M);
     SPHIP_REQUIRE(f.total == 0 || (ws && ((uintptr_t)ws & 15) == 0 && ws_bytes >= f.total), SPHIP_EWORKSPACE,
                   "linear: workspace of %zu bytes, needs %zu, 16-byte aligned", ws_bytes, f.total);
@@ -615,7 +631,7 @@ extern "C" int sphip_linear(const void* x, int64_t ldx, const void* W, int64_t l
     e.bias = bias, e.bias_dt = bias_dtype, e.res = residual, e.res_dt = res_dtype, e.ldr = ldr;
     e.out = out, e.out_dt = out_dtype, e.ldo = ldo, e.act = act;
     // z becomes codes in the epilogue itself, unless the K range is split: its partial sums then meet in the joining kernel,
-    // which has no groups of rows, and z takes the way over fp32
+    // which has no groups of rows (nor has the kernel for few rows), and z takes the way over fp32
     if (zc && f.z) e.z = (char*)ws + f.part, e.z_dt = SPHIP_F32, e.ldz = cdiv(M, 4) * 4;
     else e.z = z, e.z_dt = z_kind, e.ldz = ldz, e.z_scales = zc ? z_scales : nullptr;
     Operand A = {x, nullptr, ldx, (int)N}, B = {W, nullptr, ldw, (int)M};
@@ -637,8 +653,9 @@ extern "C" int sphip_linear(const void* x, int64_t ldx, const void* W, int64_t l
         st = save_codes("linear", x, dtype, ldx, x_fmt, 0, x_codes, x_scales, ldq, nullptr, 0, N, D, s);
     }
     if (st != SPHIP_OK) return st;
-    st = dtype == SPHIP_BF16 ? launch_product<bf16_t, OP_ROWS, OP_ROWS>("linear", A, B, e, K, K, ws, f.part, s)
-                             : launch_product<float, OP_ROWS, OP_ROWS>("linear", A, B, e, K, K, ws, f.part, s);
+    st = few(dtype, N, D, M) ? launch_linear_few("linear", dtype, A, B, e, K, s)
+         : dtype == SPHIP_BF16 ? launch_product<bf16_t, OP_ROWS, OP_ROWS>("linear", A, B, e, K, K, ws, f.part, s)
+                               : launch_product<float, OP_ROWS, OP_ROWS>("linear", A, B, e, K, K, ws, f.part, s);
     if (st == SPHIP_OK && zc && f.z)
         st = save_codes("linear", e.z, SPHIP_F32, e.ldz, z_kind, act == SPHIP_ACT_RELU, (uint8_t*)z, z_scales, ldz, nullptr, 0, N, M, s);
     return st;
@@ -666,6 +683,7 @@ static BackwardSpace backward_space(int dtype, int x_kind, int want_dx, int want
 extern "C" size_t sphip_linear_backward_workspace_bytes(int dtype, int x_kind, int want_dx, int want_dw, int want_db, int64_t N,
                                                         int64_t D, int64_t M) {
     if (N <= 0 || D <= 0 || M <= 0 || !valid_dtype(dtype)) return 0;
+    read_forced();
     return backward_space(dtype, x_kind, want_dx, want_dw, want_db, N, D, M).total;
 }
 
@@ -730,6 +748,7 @@ extern "C" int sphip_linear_backward(const void* g, int g_dtype, int64_t ldg, co
                       (!dW || ((xc || aligned_elem(x, dtype)) && aligned_elem(dW, dw_dtype))) && (!db || aligned_elem(db, db_dtype)) &&
                       (act == SPHIP_ACT_NONE || zc || aligned_elem(z, z_kind)),
                   SPHIP_EINVAL, "linear_backward: a pointer is not aligned to its element");
+    read_forced();
     const BackwardSpace sp = backward_space(dtype, x_kind, dx != nullptr, dW != nullptr, db != nullptr, N, D, M);
     SPHIP_REQUIRE(sp.total == 0 || (ws && ((uintptr_t)ws & 15) == 0 && ws_bytes >= sp.total), SPHIP_EWORKSPACE,
                   "linear_backward: workspace of %zu bytes, needs %zu, 16-byte aligned", ws_bytes, sp.total);

@@ -18,6 +18,19 @@ struct Operand {
     int rows;
 };
 
+// hipFuncAttributeMaxDynamicSharedMemorySize of a kernel, set once per device (`done`: a bit per device, one word a kernel)
+static inline bool reserve_lds(const void* kernel, int bytes, uint64_t& done) {
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev > 63) return false;
+    if (__atomic_load_n(&done, __ATOMIC_RELAXED) >> dev & 1) return true;
+    if (hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess) {
+        (void)hipGetLastError();
+        return false;
+    }
+    __atomic_fetch_or(&done, 1ull << dev, __ATOMIC_RELAXED);
+    return true;
+}
+
 struct TileGrid {
     int tilesM, tilesN, splits, steps_per;      // steps_per: K steps of one split
     float* part;                                // [splits][N][Mp] fp32 partial sums, Mp = M rounded up to 4; splits > 1
@@ -218,6 +231,10 @@ __device__ __forceinline__ void finish_rows(char* stage, const Epilogue& epi, co
 // checkpoint8.hip: x (N, D) in 8 bits; with `packed` also a copy of it in rows of ldp elements, zeros behind column D
 int save_codes(const char* what, const void* x, int dtype, int64_t ldx, int fmt, int keep_sign, uint8_t* codes, uint8_t* scales,
                int64_t ldq, void* packed, int64_t ldp, int64_t N, int64_t D, hipStream_t s);
+
+// linear_few.hip: the whole product for N <= 64, x and W contiguous in K (no codes of z)
+constexpr int FEW = 64;
+int launch_linear_few(const char* what, int dtype, const Operand& X, const Operand& W, const Epilogue& epi, int64_t K, hipStream_t s);
 
 // The LDS-DMA kernels (bf16): whether they take these operands, how they split K, their launch (the caller joins). KB: rows
 // of an OP_COLS B, which may be fewer than K (a multiple of 64 where A is OP_ROWS): B counts as zero from there on.

@@ -146,8 +146,8 @@ int launch_linear128(const char* what, int mode_a, int mode_b, const Operand& A,
                                        {linear128_kernel<OP_ROWS, OP_COLS, 2>, linear128_kernel<OP_ROWS, OP_COLS, 4>},
                                        {linear128_kernel<OP_COLS, OP_COLS, 2>, linear128_kernel<OP_COLS, OP_COLS, 4>}};
     const int lds = deep ? 4 * STAGE : FINISH;
-    SPHIP_REQUIRE(hipFuncSetAttribute((const void*)kerns[which][deep], hipFuncAttributeMaxDynamicSharedMemorySize, lds) == hipSuccess,
-                  SPHIP_ELAUNCH, "%s: cannot reserve %d bytes of LDS", what, lds);
+    static uint64_t done[3][2] = {};
+    SPHIP_REQUIRE(reserve_lds((const void*)kerns[which][deep], lds, done[which][deep]), SPHIP_ELAUNCH, "%s: cannot reserve %d bytes of LDS", what, lds);
     hipLaunchKernelGGL(kerns[which][deep], dim3((unsigned)blocks), dim3(256), lds, s, A, B, epi, K, KB, g);
     SPHIP_CHECK_LAUNCH(what);
     return SPHIP_OK;

@@ -197,8 +197,8 @@ int launch_linear256(const char* what, int mode_a, int mode_b, const Operand& A,
     const int which = mode_a == OP_ROWS ? (mode_b == OP_ROWS ? 0 : 1) : 2;
     static const kern_t kerns[3] = {linear256_kernel<OP_ROWS, OP_ROWS>, linear256_kernel<OP_ROWS, OP_COLS>,
                                     linear256_kernel<OP_COLS, OP_COLS>};
-    SPHIP_REQUIRE(hipFuncSetAttribute((const void*)kerns[which], hipFuncAttributeMaxDynamicSharedMemorySize, LDS256) == hipSuccess,
-                  SPHIP_ELAUNCH, "%s: cannot reserve %d bytes of LDS", what, LDS256);
+    static uint64_t done[3] = {};
+    SPHIP_REQUIRE(reserve_lds((const void*)kerns[which], LDS256, done[which]), SPHIP_ELAUNCH, "%s: cannot reserve %d bytes of LDS", what, LDS256);
     const int64_t blocks = (int64_t)g.tilesM * g.tilesN * g.splits;
     hipLaunchKernelGGL(kerns[which], dim3((unsigned)blocks), dim3(512), LDS256, s, A, B, epi, K, KB, g);
     SPHIP_CHECK_LAUNCH(what);

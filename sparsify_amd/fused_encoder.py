@@ -251,7 +251,7 @@ FUSE_MEAN_SEGMENT = int(os.environ.get("SPHIP_FUSE_MEAN", "64"))
 class FusedEncoder(torch.autograd.Function):
     @staticmethod
     def forward(ctx, input, weight, bias, k: int, activation: Literal["groupmax", "topk"], b_dec=None,
-                lazy_pre_acts: bool | None = None):
+                lazy_pre_acts: bool | None = None, kept=None):
         """
         input:  (N, D)      weight: (M, D)      bias: (M,)
         k:      number of latents to keep per row
@@ -259,6 +259,8 @@ class FusedEncoder(torch.autograd.Function):
                 (SparseCoder.encode, sparse_coder.py:191-192), fused here.
         lazy_pre_acts: None = the module default LAZY_PRE_ACTS; False = always store pre_acts
                 (a caller that will read them: AuxK, multi-top-k).
+        kept:   a Checkpoint8 of `input` (checkpoint8.py): the backward keeps it in place of the rows,
+                and the weight's gradient is the one at its values.
         """
         if activation not in ("topk", "groupmax"):
             raise ValueError(f"Unknown activation: {activation}")
@@ -280,7 +282,17 @@ class FusedEncoder(torch.autograd.Function):
             return values, indices, pre
 
         shift = None
-        if b_dec is not None and low and x2.dtype == torch.bfloat16:
+        ctx.kept = None
+        if kept is not None:
+            # the gradient reads the restored bf16 rows (exact for 8-bit values) and shifts them analytically
+            if kept.shape != input.shape or kept.device != input.device:
+                raise ValueError(f"the checkpoint holds {tuple(kept.shape)} on {kept.device}, input is {tuple(input.shape)} "
+                                 f"on {input.device}")
+            x_low = low_precision_input(x2, b_dec) if low else None
+            rows = None if low else ops.center_cast(x2, None if b_dec is None else b_dec.detach().contiguous(), True, False)[0]
+            shift = None if b_dec is None else b_dec.detach().clone()
+            ctx.kept = (kept.fmt, x2.shape)
+        elif b_dec is not None and low and x2.dtype == torch.bfloat16:
             # bf16 activations: the fp32 (x - b_dec) is never materialised; the backward reads
             # the bf16 rows (half the gather bytes) and applies the shift analytically
             x_low = ops.center_cast(x2, b_dec.detach().contiguous(), want_f32=False, want_bf16=True)[1]
@@ -336,7 +348,7 @@ class FusedEncoder(torch.autograd.Function):
             values, indices = ops.groupmax(pre, k)
         ops.forget_segments(indices)
 
-        ctx.save_for_backward(rows, weight, bias, indices, b_dec, shift)
+        ctx.save_for_backward(rows if kept is None else kept.data, weight, bias, indices, b_dec, shift)
         ctx.k = k
         ctx.lead = lead
         ctx.in_shape = input.shape
@@ -355,13 +367,16 @@ class FusedEncoder(torch.autograd.Function):
         rows, weight, bias, indices, b_dec, shift = ctx.saved_tensors
         grad_input = grad_weight = grad_bias = grad_bdec = None
         if grad_values is None:
-            return None, None, None, None, None, None, None
+            return None, None, None, None, None, None, None, None
         if ctx.empty:
             need = ctx.needs_input_grad
             return (torch.zeros(ctx.in_shape, dtype=torch.float32, device=weight.device) if need[0] else None,
                     torch.zeros_like(weight) if need[1] else None,
                     torch.zeros_like(bias) if bias is not None and need[2] else None, None, None,
-                    torch.zeros_like(b_dec) if b_dec is not None and need[5] else None, None)
+                    torch.zeros_like(b_dec) if b_dec is not None and need[5] else None, None, None)
+        if ctx.kept is not None and (ctx.needs_input_grad[1] or ctx.needs_input_grad[2] or ctx.needs_input_grad[5]):
+            fmt, (n_rows, n_cols) = ctx.kept
+            rows = ops.checkpoint8_restore(rows, fmt, n_rows, n_cols, torch.bfloat16)
         M = weight.shape[0]
         gv = grad_values.reshape(-1, ctx.k).contiguous()
         if weight.dtype != torch.float32:
@@ -410,11 +425,11 @@ class FusedEncoder(torch.autograd.Function):
             torch.autograd.graph.increment_version(weight)
             if shadow is not None:
                 register_bf16_shadow(weight, shadow)
-        return grad_input, grad_weight, grad_bias, None, None, grad_bdec, None
+        return grad_input, grad_weight, grad_bias, None, None, grad_bdec, None, None
 
 
 def fused_encoder(input, weight, bias, k: int, activation: Literal["groupmax", "topk"],
-                  lazy_pre_acts: bool | None = None) -> EncoderOutput:
+                  lazy_pre_acts: bool | None = None, kept=None) -> EncoderOutput:
     """nn.Linear + ReLU + `activation`, with the sparse backward (fused_encoder.py:90-103).
-    lazy_pre_acts (not in the reference): see FusedEncoder.forward."""
-    return EncoderOutput(*FusedEncoder.apply(input, weight, bias, k, activation, None, lazy_pre_acts))
+    lazy_pre_acts, kept (not in the reference): see FusedEncoder.forward."""
+    return EncoderOutput(*FusedEncoder.apply(input, weight, bias, k, activation, None, lazy_pre_acts, kept))

@@ -13,8 +13,10 @@ import torch
 from torch import Tensor, nn
 
 from . import dead_decode, ops, parallel
+from .checkpoint8 import Checkpoint8, checkpoint8
 from .config import SparseCoderConfig
 from .fused_encoder import EncoderOutput, FusedEncoder, bf16_shadow, block_maxima_of, low_precision_input
+from .fused_linear import fused_linear
 from .utils import SparseDecode, decoder_impl
 
 
@@ -134,6 +136,11 @@ class SparseCoder(nn.Module):
     """(not in the reference) True: forwards that do not read pre_acts do not store them
     (fused_encoder.LazyPreActs); None: the module default fused_encoder.LAZY_PRE_ACTS."""
 
+    checkpoint: str | None = None
+    """(not in the reference) "int8" / "e4m3": between forward and backward the input is kept once, in
+    8 bits (checkpoint8.py), for the encoder's and W_skip's gradients, which are those at its restored
+    values; the skip product then adds sae_out in its own epilogue (fused_linear), unrounded."""
+
     def __init__(
         self,
         d_in: int,
@@ -230,15 +237,23 @@ class SparseCoder(nn.Module):
         return self.encoder.weight.dtype
 
     # ------------------------------------------------------------------ hot path
-    def encode(self, x: Tensor, lazy_pre_acts: bool | None = None) -> EncoderOutput:
+    def encode(self, x: Tensor, lazy_pre_acts: bool | None = None, kept: Checkpoint8 | None = None) -> EncoderOutput:
         """Encode the input and select the top-k latents (sparse_coder.py:189-196).
-        The `x - b_dec` of the reference is fused into the encoder op. lazy_pre_acts (not in the
+        The `x - b_dec` of the reference is fused into the encoder op. lazy_pre_acts, kept (not in the
         reference): fused_encoder.FusedEncoder.forward."""
+        if kept is None:
+            kept = self._keep(x)
         b_dec = None if self.cfg.transcode else self.b_dec
         if lazy_pre_acts is None:
             lazy_pre_acts = self.lazy_pre_acts
         return EncoderOutput(*FusedEncoder.apply(
-            x, self.encoder.weight, self.encoder.bias, self.cfg.k, self.cfg.activation, b_dec, lazy_pre_acts))
+            x, self.encoder.weight, self.encoder.bias, self.cfg.k, self.cfg.activation, b_dec, lazy_pre_acts, kept))
+
+    def _keep(self, x: Tensor) -> Checkpoint8 | None:
+        """The 8-bit copy of x a backward pass will read, if this coder keeps one."""
+        if self.checkpoint is None or not torch.is_grad_enabled() or x.numel() == 0:
+            return None
+        return checkpoint8(x, self.checkpoint)
 
     def decode(self, top_acts: Tensor, top_indices: Tensor) -> Tensor:
         """sparse_coder.py:198-202; the bias add is fused into the gather kernel."""
@@ -261,13 +276,16 @@ class SparseCoder(nn.Module):
         otherwise it is read here, which makes the host wait for the device mid-forward."""
         # AuxK and multi-top-k read pre_acts (sparse_coder.py:240, 257): they get the stored matrix
         reads_pre = self.cfg.multi_topk or dead_mask is not None
-        top_acts, top_indices, pre_acts = self.encode(x, lazy_pre_acts=False if reads_pre else None)
+        kept = self._keep(x)
+        top_acts, top_indices, pre_acts = self.encode(x, lazy_pre_acts=False if reads_pre else None, kept=kept)
 
         if y is None:
             y = x
 
         sae_out = decoded = self.decode(top_acts, top_indices)
-        if self.W_skip is not None:
+        if self.W_skip is not None and self.checkpoint is not None:
+            sae_out = fused_linear(x, self.W_skip, residual=sae_out, checkpoint=kept)
+        elif self.W_skip is not None:
             from .fused_encoder import _autocast_bf16
             skip = SkipProduct.apply(x, self.W_skip, _autocast_bf16())
             sae_out = _AddSkip.apply(sae_out, skip)

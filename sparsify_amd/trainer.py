@@ -151,6 +151,9 @@ class Trainer:
         if cfg.lazy_pre_acts:
             for sae in self.saes.values():
                 sae.lazy_pre_acts = True
+        if cfg.checkpoint_8bit is not None:
+            for sae in self.saes.values():
+                sae.checkpoint = cfg.checkpoint_8bit
 
         # the source yields one micro-batch per item (the reference counts sequences:
         # len(dataset) // batch_size, trainer.py:90)

@@ -15,7 +15,7 @@ def lib():
 
 def linear(**kw):
     a = dict(x=P, ldx=64, W=P, ldw=64, dtype=BF16, bias=None, bias_dtype=0, act=0, res=None, res_dtype=0, ldr=0, out=P,
-             out_dtype=BF16, ldo=32, z=None, z_kind=0, z_scales=None, ldz=0, xc=None, xs=None, x_fmt=0, ldq=0, N=8, D=64, M=32,
+             out_dtype=BF16, ldo=32, z=None, z_kind=0, z_scales=None, ldz=0, xc=None, xs=None, x_fmt=0, ldq=0, N=80, D=64, M=32,
              ws=None, nws=0)
     assert set(kw) <= set(a)
     return lib().sphip_linear(*{**a, **kw}.values(), None)
@@ -67,8 +67,8 @@ def test_backward_entry(kw, status, word):
 def test_workspace_queries():
     L = lib()
     assert L.sphip_linear_workspace_bytes(BF16, 0, 0, 8, 8) == 0 and L.sphip_linear_workspace_bytes(9, 0, 8, 8, 8) == 0
-    assert L.sphip_linear_workspace_bytes(BF16, INT8, 8, 4096, 32) >= L.sphip_linear_workspace_bytes(BF16, F32, 8, 4096, 32) + 8 * 32 * 4
-    assert L.sphip_linear_workspace_bytes(BF16, INT8, 8, 64, 32) == 0
+    assert L.sphip_linear_workspace_bytes(BF16, INT8, 80, 4096, 32) >= L.sphip_linear_workspace_bytes(BF16, F32, 80, 4096, 32) + 80 * 32 * 4
+    assert L.sphip_linear_workspace_bytes(BF16, INT8, 80, 64, 32) == 0 and L.sphip_linear_workspace_bytes(BF16, F32, 8, 4096, 32) == 0
     assert L.sphip_linear_backward_workspace_bytes(BF16, INT8, 0, 0, 1, 64, 64, 32) == 2 * 32 * 4
     assert L.sphip_linear_backward_workspace_bytes(F32, F32, 1, 1, 1, 8, -1, 32) == 0
 
@@ -122,3 +122,13 @@ def test_python_surface_refuses_on_the_host():
         fused_linear(x, W, checkpoint=c)
     with pytest.raises(RuntimeError, match="no CPU fallback"):
         c.restore()
+
+
+def test_the_training_switch():
+    from sparsify_amd import SparseCoderConfig, TrainConfig
+    assert TrainConfig(sae=SparseCoderConfig()).checkpoint_8bit is None
+    assert TrainConfig(sae=SparseCoderConfig(), checkpoint_8bit="int8").checkpoint_8bit == "int8"
+    with pytest.raises(ValueError, match="checkpoint_8bit"):
+        TrainConfig(sae=SparseCoderConfig(), checkpoint_8bit="fp8")
+    with pytest.raises(ValueError, match="shard_latents"):
+        TrainConfig(sae=SparseCoderConfig(), checkpoint_8bit="int8", shard_latents=True)
