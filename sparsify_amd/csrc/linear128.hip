@@ -133,7 +133,7 @@ bool linear128_takes(int mode_a, int mode_b, const Operand& A, const Operand& B,
 int linear128_splits(int64_t N, int64_t M, int64_t K) {
     const int64_t tiles = cdiv(N, T128) * cdiv(M, T128), steps = cdiv(K, K64);
     int64_t s = 256 / tiles;
-    if (s > steps / 2) s = steps / 2;
+    if (s > steps / 8) s = steps / 8;
     return s < 1 ? 1 : (int)s;
 }
 
