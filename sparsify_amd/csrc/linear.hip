@@ -316,24 +316,24 @@ static void read_forced() {
     g_forced = e ? e[0] : 0;
 }
 
-// Which kernel a bf16 product of these sizes goes to if its operands are such that LDS-DMA can fetch them.
+// Which kernel a product of these sizes goes to if its operands are such that LDS-DMA can fetch them.
 enum { BY_TILES = 0, BY_128 = 1, BY_256 = 2 };
-static int kernel_for(int64_t N, int64_t M) {
-    if (g_forced) return g_forced == '2' ? BY_256 : g_forced == '1' ? BY_128 : BY_TILES;
+static int kernel_for(int dtype, int64_t N, int64_t M) {
+    if (g_forced) return g_forced == '2' && dtype == SPHIP_BF16 ? BY_256 : g_forced == '1' || g_forced == '2' ? BY_128 : BY_TILES;
+    if (dtype != SPHIP_BF16) return BY_128;
     // The 256 x 256 kernel where its tiles fill most of the 256 compute units once: 16384 x 1024 x 4096 takes 101 us against
     // 118 with 128 x 128 tiles, 8192 x 2048 x 2048 56 against 68. Below, splitting K for the large tile costs more than the
     // smaller tile does: 1000 x 4096 x 4096 (64 large tiles) 47 us against 41, 2048^3 37 against 25.
     return cdiv(N, 256) * cdiv(M, 256) >= 160 ? BY_256 : BY_128;
 }
-static int splits_of(int by, int64_t N, int64_t M, int64_t K) {
-    return by == BY_256 ? 1 : by == BY_128 ? linear128_splits(N, M, K) : split_count(N, M, cdiv(K, 64));
+static int splits_of(int dtype, int by, int64_t N, int64_t M, int64_t K) {
+    return by == BY_256 ? 1 : by == BY_128 ? linear128_splits(dtype, N, M, K) : split_count(N, M, cdiv(K, 128 / (int64_t)dtype_size(dtype)));
 }
 
 // the most a product needs for its partial tiles, whichever kernel takes it
 static size_t split_bytes(int dtype, int64_t N, int64_t M, int64_t K) {
-    if (dtype != SPHIP_BF16) return part_bytes(N, M, split_count(N, M, cdiv(K, 32)));
     const int64_t Kp = cdiv(K, 64) * 64;
-    const size_t a = part_bytes(N, M, split_count(N, M, cdiv(K, 64))), b = part_bytes(N, M, splits_of(kernel_for(N, M), N, M, Kp));
+    const size_t a = part_bytes(N, M, splits_of(dtype, BY_TILES, N, M, Kp)), b = part_bytes(N, M, splits_of(dtype, kernel_for(dtype, N, M), N, M, Kp));
     return a > b ? a : b;
 }
 
@@ -341,17 +341,18 @@ template <typename T, int MODE_A, int MODE_B>
 static int launch_product(const char* what, const Operand& A, const Operand& B, const Epilogue& epi, int64_t K, int64_t KB,
                           void* ws, size_t ws_bytes, hipStream_t s) {
     const int64_t N = A.rows, M = B.rows;
+    constexpr int dtype = sizeof(T) == 2 ? SPHIP_BF16 : SPHIP_F32;
     int by = BY_TILES;
-    if (sizeof(T) == 2 && MODE_B <= OP_COLS) {
-        by = kernel_for(N, M);
+    if (MODE_B <= OP_COLS) {
+        by = kernel_for(dtype, N, M);
         if (by == BY_256 && !linear256_takes(MODE_A, MODE_B, A, B, K)) by = BY_TILES;
-        if (by == BY_128 && !linear128_takes(MODE_A, MODE_B, A, B, K)) by = BY_TILES;
+        if (by == BY_128 && !linear128_takes(dtype, MODE_A, MODE_B, A, B, K)) by = BY_TILES;
     }
     const int tile = by == BY_256 ? 256 : 128;
     const int64_t steps = cdiv(K, LCH * Chunk<T>::E);
     TileGrid g;
     g.tilesM = (int)cdiv(M, tile), g.tilesN = (int)cdiv(N, tile);
-    const int want = by == BY_TILES ? split_count(N, M, steps) : splits_of(by, N, M, K);
+    const int want = splits_of(dtype, by, N, M, K);
     g.steps_per = (int)cdiv(steps, want);
     g.splits = (int)cdiv(steps, g.steps_per);
     g.part = (float*)ws;
@@ -365,7 +366,7 @@ static int launch_product(const char* what, const Operand& A, const Operand& B, 
                   "%s: grid too large", what);
     if (by != BY_TILES) {
         const int st = by == BY_256 ? launch_linear256(what, MODE_A, MODE_B, A, B, epi, K, KB, g, s)
-                                    : launch_linear128(what, MODE_A, MODE_B, A, B, epi, K, KB, g, s);
+                                    : launch_linear128(what, dtype, MODE_A, MODE_B, A, B, epi, K, KB, g, s);
         if (st != SPHIP_OK) return st;
     } else {
         hipLaunchKernelGGL((linear_tile_kernel<T, MODE_A, MODE_B>), dim3((unsigned)nblocks), dim3(256), 0, s, A, B, epi, K, KB, g);
@@ -381,31 +382,33 @@ static int launch_product(const char* what, const Operand& A, const Operand& B, 
     return SPHIP_OK;
 }
 
-// bf16 rows copied to a 16-byte aligned stride that is a multiple of 64, zeros behind them: what LDS-DMA asks of an operand.
-// Up to two matrices in one launch.
+// Rows copied to a stride that is a multiple of 64 elements, zeros behind them: what LDS-DMA asks of an operand. Up to two
+// matrices in one launch.
 struct PackArgs {
-    const bf16_t* src[2];
-    bf16_t* dst[2];
+    const void* src[2];
+    void* dst[2];
     int64_t ld[2], n[2];                   // n: 16-byte pieces of the copy
     int cols[2], pieces[2];                // pieces per row
 };
-__global__ __launch_bounds__(256) void linear_pack_kernel(PackArgs a) {
+template <typename T> __global__ __launch_bounds__(256) void linear_pack_kernel(PackArgs a) {
+    constexpr int E = Chunk<T>::E;
     int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     const int w = i >= a.n[0];
     if (w) i -= a.n[0];
     if (i >= a.n[w]) return;
     const int64_t row = i / a.pieces[w];
-    const int c = (int)(i - row * a.pieces[w]) * 8;
-    *reinterpret_cast<uint4*>(a.dst[w] + i * 8) = Chunk<bf16_t>::load(a.src[w] + row * a.ld[w] + c, a.cols[w] - c);
+    const int c = (int)(i - row * a.pieces[w]) * E;
+    *reinterpret_cast<uint4*>((T*)a.dst[w] + i * E) = Chunk<T>::load((const T*)a.src[w] + row * a.ld[w] + c, a.cols[w] - c);
 }
 static int64_t packed_ld(int64_t cols) { return cdiv(cols, 64) * 64; }
 struct Packing {
     PackArgs a = {};
-    int count = 0;
+    int count = 0, dtype;
+    explicit Packing(int dt) : dtype(dt) {}
     void add(Operand& o, int64_t rows, int64_t cols, void* dst) {
         const int64_t ld = packed_ld(cols);
-        a.src[count] = (const bf16_t*)o.p, a.dst[count] = (bf16_t*)dst, a.ld[count] = o.ld, a.cols[count] = (int)cols;
-        a.pieces[count] = (int)(ld / 8), a.n[count] = rows * (ld / 8);
+        a.src[count] = o.p, a.dst[count] = dst, a.ld[count] = o.ld, a.cols[count] = (int)cols;
+        a.pieces[count] = (int)(ld * (int64_t)dtype_size(dtype) / 16), a.n[count] = rows * a.pieces[count];
         ++count;
         o.p = dst, o.ld = ld;
     }
@@ -413,16 +416,19 @@ struct Packing {
         if (count == 0) return SPHIP_OK;
         const int64_t blocks = cdiv(a.n[0] + a.n[1], 256);
         SPHIP_REQUIRE(blocks < (1ll << 31), SPHIP_EUNSUPPORTED, "%s: grid too large", what);
-        hipLaunchKernelGGL(linear_pack_kernel, dim3((unsigned)blocks), dim3(256), 0, s, a);
+        if (dtype == SPHIP_BF16) hipLaunchKernelGGL(linear_pack_kernel<bf16_t>, dim3((unsigned)blocks), dim3(256), 0, s, a);
+        else hipLaunchKernelGGL(linear_pack_kernel<float>, dim3((unsigned)blocks), dim3(256), 0, s, a);
         SPHIP_CHECK_LAUNCH(what);
         return SPHIP_OK;
     }
 };
-// Whether a bf16 product is worth copying an operand whose rows LDS-DMA cannot fetch (they do not start at multiples of 16
-// bytes, or K is no multiple of 64)
-static bool worth_packing(int64_t N, int64_t M, int64_t K, int least = 29) {
+// Whether a product is worth copying an operand whose rows LDS-DMA cannot fetch (they do not start at multiples of 16 bytes,
+// or K is no whole number of steps)
+static bool worth_packing(int dtype, int64_t N, int64_t M, int64_t K, int least = 29) {
+    if (dtype != SPHIP_BF16) least -= 2;
     return g_forced ? g_forced != 't' : N * M * K >= (1ll << least);
 }
+static bool unaligned(int dtype, int64_t cols) { return cols * (int64_t)dtype_size(dtype) % 16 != 0; }
 
 // ---- dz = g act'(z) and its column sums. A workgroup takes 32 rows (the group one scale of an 8-bit z covers) of 32 x 16
 // bytes of columns: 32 lanes side by side, 8 rows at a time, every thread 4 rows whose loads are all in flight; the 8 row
@@ -574,7 +580,7 @@ static bool codes_ok(const void* codes, const void* scales, int64_t ld, int64_t 
 }
 static size_t up256(size_t b) { return (b + 255) / 256 * 256; }
 
-// workspace: partial tiles | z in fp32 on its way into 8 bits | x and W packed (D no multiple of 64)
+// workspace: partial tiles | z in fp32 on its way into 8 bits | x and W packed (rows that are no whole number of K steps)
 struct ForwardSpace {
     size_t part, z, pack, total;
 };
@@ -592,7 +598,8 @@ static ForwardSpace forward_space(int dtype, int z_kind, int64_t N, int64_t D, i
     const bool one = few(dtype, N, D, M);
     f.part = one ? 0 : up256(split_bytes(dtype, N, M, D));
     f.z = is_codes(z_kind) && (f.part || one) ? up256((size_t)N * (cdiv(M, 4) * 4) * 4) : 0;      // (no codes from a split K range or from few rows)
-    f.pack = dtype == SPHIP_BF16 && !one && D % 64 != 0 && worth_packing(N, M, D) ? (size_t)(N + M) * packed_ld(D) * 2 : 0;
+    f.pack = !one && D * (int64_t)dtype_size(dtype) % 128 != 0 && worth_packing(dtype, N, M, D)
+                 ? (size_t)(N + M) * packed_ld(D) * dtype_size(dtype) : 0;
     f.total = f.part + f.z + f.pack;
     return f;
 }
@@ -640,14 +647,14 @@ extern "C" int sphip_linear(const void* x, int64_t ldx, const void* W, int64_t l
     if (f.pack) {
         K = packed_ld(D);
         char* to = (char*)ws + f.part + f.z;
-        Packing p;
+        Packing p(dtype);
         if (x_codes) {                                          // x is read once for both
             st = save_codes("linear", x, dtype, ldx, x_fmt, 0, x_codes, x_scales, ldq, to, K, N, D, s);
             A.p = to, A.ld = K;
         } else {
             p.add(A, N, D, to);
         }
-        p.add(B, M, D, to + (size_t)N * K * 2);
+        p.add(B, M, D, to + (size_t)N * K * dtype_size(dtype));
         if (st == SPHIP_OK) st = p.launch("linear", s);
     } else if (x_codes) {
         st = save_codes("linear", x, dtype, ldx, x_fmt, 0, x_codes, x_scales, ldq, nullptr, 0, N, D, s);
@@ -666,14 +673,15 @@ extern "C" int sphip_linear(const void* x, int64_t ldx, const void* W, int64_t l
 struct BackwardSpace {
     size_t dz, sums, x, w, part, total;
 };
-static int64_t dz_stride(int dtype, int64_t M) { return dtype == SPHIP_BF16 ? packed_ld(M) : cdiv(M, 4) * 4; }
 static BackwardSpace backward_space(int dtype, int x_kind, int want_dx, int want_dw, int want_db, int64_t N, int64_t D, int64_t M) {
     BackwardSpace b;
-    const bool bf = dtype == SPHIP_BF16;
-    b.dz = want_dx || want_dw ? up256((size_t)N * dz_stride(dtype, M) * dtype_size(dtype)) : 0;
+    const size_t es = dtype_size(dtype);
+    const bool odd = unaligned(dtype, D);
+    b.dz = want_dx || want_dw ? up256((size_t)N * packed_ld(M) * es) : 0;
     b.sums = want_db ? up256((size_t)cdiv(N, 32) * M * 4) : 0;
-    b.x = want_dw && bf && (is_codes(x_kind) ? worth_packing(M, D, N, 31) : D % 8 != 0 && worth_packing(M, D, N)) ? up256((size_t)N * packed_ld(D) * 2) : 0;
-    b.w = want_dx && bf && worth_packing(N, D, M) && D % 8 != 0 ? up256((size_t)M * packed_ld(D) * 2) : 0;
+    b.x = want_dw && (is_codes(x_kind) ? worth_packing(dtype, M, D, N, 31) : odd && worth_packing(dtype, M, D, N))
+              ? up256((size_t)N * packed_ld(D) * es) : 0;
+    b.w = want_dx && odd && worth_packing(dtype, N, D, M) ? up256((size_t)M * packed_ld(D) * es) : 0;
     const size_t p1 = want_dx ? split_bytes(dtype, N, D, M) : 0, p2 = want_dw ? split_bytes(dtype, M, D, N) : 0;
     b.part = p1 > p2 ? p1 : p2;
     b.total = b.dz + b.sums + b.x + b.w + b.part;
@@ -710,10 +718,11 @@ static int backward_products(const Operand& dz, const void* W, int64_t ldw, cons
         int st;
         if (is_codes(x_kind)) {
             const int64_t ld = packed_ld(D);
-            st = sphip_checkpoint8_restore((const uint8_t*)x, x_scales, ldx, x_kind, xs, SPHIP_BF16, ld, N, D, s);
-            B.p = xs, B.ld = ld, x_kind = SPHIP_BF16;
+            constexpr int dtype = sizeof(T) == 2 ? SPHIP_BF16 : SPHIP_F32;
+            st = sphip_checkpoint8_restore((const uint8_t*)x, x_scales, ldx, x_kind, xs, dtype, ld, N, D, s);
+            B.p = xs, B.ld = ld, x_kind = dtype;
         } else {
-            Packing p;
+            Packing p(sizeof(T) == 2 ? SPHIP_BF16 : SPHIP_F32);
             p.add(B, N, D, xs);
             st = p.launch(what, s);
         }
@@ -759,17 +768,17 @@ extern "C" int sphip_linear_backward(const void* g, int g_dtype, int64_t ldg, co
     // where it does not have that dtype, or where LDS-DMA could not fetch it as it is.
     const bool products = dx || dW;
     bool direct = act == SPHIP_ACT_NONE && g_dtype == dtype;
-    if (direct && dtype == SPHIP_BF16 && (M % 64 != 0 || ldg % 8 != 0 || ((uintptr_t)g & 15) != 0))
-        direct = !((dx && worth_packing(N, D, M)) || (dW && worth_packing(M, D, N)));
+    if (direct && (M * (int64_t)dtype_size(dtype) % 128 != 0 || unaligned(dtype, ldg) || ((uintptr_t)g & 15) != 0))
+        direct = !((dx && worth_packing(dtype, N, D, M)) || (dW && worth_packing(dtype, M, D, N)));
     Operand dz = {g, nullptr, ldg, (int)N};
-    if (products && !direct) dz.p = w, dz.ld = dz_stride(dtype, M);
-    Packing pack;
+    if (products && !direct) dz.p = w, dz.ld = packed_ld(M);
+    Packing pack(dtype);
     if (sp.w) {
         Operand o = {W, nullptr, ldw, (int)M};
         pack.add(o, M, D, w + sp.dz + sp.sums + sp.x);
         W = o.p, ldw = o.ld;
     }
-    const bool copied = products && !direct && !db && act == SPHIP_ACT_NONE && g_dtype == dtype && dtype == SPHIP_BF16;
+    const bool copied = products && !direct && !db && act == SPHIP_ACT_NONE && g_dtype == dtype;
     if (copied) {                                               // g with padded rows is all there is to do
         Operand o = {g, nullptr, ldg, (int)N};
         pack.add(o, N, M, w);
@@ -792,6 +801,6 @@ extern "C" int sphip_linear_backward(const void* g, int g_dtype, int64_t ldg, co
     if (dtype == SPHIP_BF16)
         return backward_products<bf16_t>(dz, W, ldw, x, x_kind, x_scales, ldx, dx, dx_dtype, lddx, dW, dw_dtype, lddw, N, D, M,
                                          !direct, w, sp, s);
-    return backward_products<float>(dz, W, ldw, x, x_kind, x_scales, ldx, dx, dx_dtype, lddx, dW, dw_dtype, lddw, N, D, M, false,
+    return backward_products<float>(dz, W, ldw, x, x_kind, x_scales, ldx, dx, dx_dtype, lddx, dW, dw_dtype, lddw, N, D, M, !direct,
                                     w, sp, s);
 }

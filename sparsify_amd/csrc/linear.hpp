@@ -236,14 +236,14 @@ int save_codes(const char* what, const void* x, int dtype, int64_t ldx, int fmt,
 constexpr int FEW = 64;
 int launch_linear_few(const char* what, int dtype, const Operand& X, const Operand& W, const Epilogue& epi, int64_t K, hipStream_t s);
 
-// The LDS-DMA kernels (bf16): whether they take these operands, how they split K, their launch (the caller joins). KB: rows
-// of an OP_COLS B, which may be fewer than K (a multiple of 64 where A is OP_ROWS): B counts as zero from there on.
+// The LDS-DMA kernels (256: bf16 only): whether they take these operands, how they split K, their launch (the caller joins).
+// KB: rows of an OP_COLS B, which may be fewer than K (whole 128-byte steps where A is OP_ROWS): B counts as zero from there.
 bool linear256_takes(int mode_a, int mode_b, const Operand& A, const Operand& B, int64_t K);
 int launch_linear256(const char* what, int mode_a, int mode_b, const Operand& A, const Operand& B, const Epilogue& epi, int64_t K,
                      int64_t KB, const TileGrid& g, hipStream_t s);
-bool linear128_takes(int mode_a, int mode_b, const Operand& A, const Operand& B, int64_t K);
-int linear128_splits(int64_t N, int64_t M, int64_t K);
-int launch_linear128(const char* what, int mode_a, int mode_b, const Operand& A, const Operand& B, const Epilogue& epi, int64_t K,
-                     int64_t KB, const TileGrid& g, hipStream_t s);
+bool linear128_takes(int dtype, int mode_a, int mode_b, const Operand& A, const Operand& B, int64_t K);
+int linear128_splits(int dtype, int64_t N, int64_t M, int64_t K);
+int launch_linear128(const char* what, int dtype, int mode_a, int mode_b, const Operand& A, const Operand& B, const Epilogue& epi,
+                     int64_t K, int64_t KB, const TileGrid& g, hipStream_t s);
 
 }  // namespace sphip

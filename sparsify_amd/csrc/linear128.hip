@@ -1,5 +1,6 @@
-// The dense product's kernel for mid-size bf16 shapes: a 128 x 128 tile of C per workgroup of 4 waves (2 x 2 of 64 x 64
-// outputs), 64 of K per step, v_mfma_f32_16x16x32_bf16, operand tiles by LDS-DMA (images: linear_dma.hpp).
+// The dense product's kernel for mid-size bf16 shapes and for fp32: a 128 x 128 tile of C per workgroup of 4 waves (2 x 2 of
+// 64 x 64 outputs), 128 bytes of K per step (64 bf16, 32 fp32), v_mfma_f32_16x16x32_bf16 / v_mfma_f32_16x16x4_f32 (exact
+// products, fp32 sums), operand tiles by LDS-DMA (images: linear_dma.hpp).
 //
 // STAGES buffers of 32 KiB, one barrier per step: at step t a wave waits for its own DMA of step t, passes the barrier
 // (everybody's step t has landed, everybody has read step t - 1), sends off the DMA of step t + STAGES - 1 into the buffer
@@ -13,40 +14,46 @@ namespace sphip {
 constexpr int T128 = 128, IMG_A = 0, IMG_B = 16384, STAGE = 32768;
 constexpr int FINISH = 4 * 64 * OUT_ROW;            // the epilogue's staging: more than two stages, twice still within the LDS
 
-template <int MODE> struct Source128 {
+template <typename T, int MODE> struct Source128 {
+    static constexpr unsigned ES = sizeof(T), KS = 128 / ES;
     __amdgpu_buffer_rsrc_t rsrc;
-    unsigned voff, piece, step;            // bytes: lane offset, between the 4 pieces of a step, between K steps
+    unsigned voff[2], piece, step;         // bytes: lane offset of even and odd pieces, between the 4 pieces of a step, between K steps
     __device__ __forceinline__ void init(const Operand& o, int row0, int64_t k0, int64_t K, int tid) {
-        const bf16_t* p = (const bf16_t*)o.p;
-        const unsigned ld2 = (unsigned)o.ld * 2u;
+        const T* p = (const T*)o.p;
+        const unsigned ldb = (unsigned)o.ld * ES;
         if (MODE == OP_ROWS) {
             const int hr = tid >> 3, ch = (tid & 7) ^ ((hr >> 1) & 7);
             const int rows = min(T128, o.rows - row0);
             rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)(p + (int64_t)row0 * o.ld + k0), 0,
-                                                     (int)((unsigned)(rows - 1) * ld2 + (unsigned)(K - k0) * 2u), 0x00020000);
-            voff = (unsigned)hr * ld2 + (unsigned)ch * 16u;
-            piece = 32u * ld2;
-            step = K64 * 2;
+                                                     (int)((unsigned)(rows - 1) * ldb + (unsigned)(K - k0) * ES), 0x00020000);
+            voff[0] = voff[1] = (unsigned)hr * ldb + (unsigned)ch * 16u;
+            piece = 32u * ldb;
+            step = 128;
         } else {
-            const int kr = tid >> 4, f = (kr & 3) + 4 * ((kr >> 3) & 1);
-            const int c = (tid & 15) ^ (2 * f);
             // (the end rounded up to a piece, see linear256.hip)
             rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)(p + k0 * o.ld + row0), 0,
-                                                     (int)(K > k0 ? (unsigned)(K - 1 - k0) * ld2 + ((unsigned)(o.rows - row0) * 2u + 15u) / 16u * 16u : 0u),
+                                                     (int)(K > k0 ? (unsigned)(K - 1 - k0) * ldb + ((unsigned)(o.rows - row0) * ES + 15u) / 16u * 16u : 0u),
                                                      0x00020000);
-            voff = (unsigned)kr * ld2 + (unsigned)c * 16u;
-            piece = 16u * ld2;
-            step = K64 * ld2;
+            constexpr int LOG = ES == 2 ? 4 : 5;                // 16-byte chunks of 128 columns
+            const int kr = tid >> LOG, c = tid & ((1 << LOG) - 1);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int k = kr + (256 >> LOG) * i;
+                const int f = ES == 2 ? 2 * ((k & 3) + 4 * ((k >> 3) & 1)) : 4 * ((k >> 2) & 3);
+                voff[i] = (unsigned)kr * ldb + (unsigned)(c ^ f) * 16u;
+            }
+            piece = (256u >> LOG) * ldb;
+            step = KS * ldb;
         }
     }
     __device__ __forceinline__ void dma(char* lds, int t) const {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_t)(lds + 4096 * i), 16, voff + (unsigned)t * step + (unsigned)i * piece, 0, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_t)(lds + 4096 * i), 16, voff[i & 1] + (unsigned)t * step + (unsigned)i * piece, 0, 0, 0);
     }
 };
 
-template <int MA, int MB, int STAGES>
+template <typename T, int MA, int MB, int STAGES>
 __global__ __launch_bounds__(256, STAGES == 2 ? 2 : 1) void linear128_kernel(Operand A, Operand B, Epilogue epi, int64_t K, int64_t KB,
                                                                              TileGrid g) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -56,11 +63,12 @@ __global__ __launch_bounds__(256, STAGES == 2 ? 2 : 1) void linear128_kernel(Ope
     const int m0 = tm * T128, n0 = tn * T128;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave >> 1, wn = wave & 1;
-    const int64_t k0 = (int64_t)split * g.steps_per * K64;
-    const int steps = (int)min((int64_t)g.steps_per, (K - k0 + K64 - 1) / K64);
+    constexpr int KS = 128 / sizeof(T), PITCH = 128 * sizeof(T);
+    const int64_t k0 = (int64_t)split * g.steps_per * KS;
+    const int steps = (int)min((int64_t)g.steps_per, (K - k0 + KS - 1) / KS);
 
-    Source128<MA> sa;
-    Source128<MB> sb;
+    Source128<T, MA> sa;
+    Source128<T, MB> sb;
     sa.init(A, n0, k0, K, tid);
     sb.init(B, m0, k0, KB, tid);
     auto fetch = [&](int t, unsigned image) {      // 8 DMA instructions per wave
@@ -70,8 +78,10 @@ __global__ __launch_bounds__(256, STAGES == 2 ? 2 : 1) void linear128_kernel(Ope
         sb.dma(dst + IMG_B, t);
     };
     const unsigned lds0 = (unsigned)(size_t)(lds_t)smem;
-    Frag<MA, 256> fa;
-    Frag<MB, 256> fb;
+    typedef Frag<T, MA, PITCH> FA;
+    typedef Frag<T, MB, PITCH> FB;
+    FA fa;
+    FB fb;
     fa.init(lds0 + IMG_A, wn * 64, lane);
     fb.init(lds0 + IMG_B, wm * 64, lane);
     acc4_t acc[4][4];
@@ -100,14 +110,14 @@ __global__ __launch_bounds__(256, STAGES == 2 ? 2 : 1) void linear128_kernel(Ope
         fb.template read<0>(img);
         fa.template read<1>(img);
         fb.template read<1>(img);
-        constexpr int LATER = Frag<MA, 256>::READS + Frag<MB, 256>::READS;     // the counter holds 15 at most
+        constexpr int LATER = FA::READS + FB::READS;     // the counter holds 15 at most
         fa.template wait<0, (LATER > 15 ? 15 : LATER)>();
         fb.template wait<0, (LATER > 15 ? 15 : LATER)>();
 #pragma unroll
         for (int mt = 0; mt < 4; ++mt)
 #pragma unroll
             for (int nt = 0; nt < 4; ++nt)
-                acc[mt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb.get(mt, 0), fa.get(nt, 0), acc[mt][nt], 0, 0, 0);
+                acc[mt][nt] = mma16(fb.get(mt, 0), fa.get(nt, 0), acc[mt][nt], T{});
         __builtin_amdgcn_sched_barrier(0);         // these 16 MFMAs run while the other fragments arrive
         fa.template wait<1, 0>();
         fb.template wait<1, 0>();
@@ -115,7 +125,7 @@ __global__ __launch_bounds__(256, STAGES == 2 ? 2 : 1) void linear128_kernel(Ope
         for (int mt = 0; mt < 4; ++mt)
 #pragma unroll
             for (int nt = 0; nt < 4; ++nt)
-                acc[mt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb.get(mt, 1), fa.get(nt, 1), acc[mt][nt], 0, 0, 0);
+                acc[mt][nt] = mma16(fb.get(mt, 1), fa.get(nt, 1), acc[mt][nt], T{});
         freed = img;
         img = img + STAGE == STAGES * STAGE ? 0 : img + STAGE;
     }
@@ -124,31 +134,38 @@ __global__ __launch_bounds__(256, STAGES == 2 ? 2 : 1) void linear128_kernel(Ope
                    N, M, lane, res);
 }
 
-bool linear128_takes(int mode_a, int mode_b, const Operand& A, const Operand& B, int64_t K) {
-    return dma_ok(mode_a, A, K, T128) && dma_ok(mode_b, B, K, T128);
+bool linear128_takes(int dtype, int mode_a, int mode_b, const Operand& A, const Operand& B, int64_t K) {
+    const int es = (int)dtype_size(dtype);
+    return dma_ok(mode_a, A, K, T128, es) && dma_ok(mode_b, B, K, T128, es);
 }
 
-// Splits of the K range, towards one workgroup per compute unit, 2 steps each at least: a split costs a round trip of the
-// fp32 partial tiles, a step about what its first load takes.
-int linear128_splits(int64_t N, int64_t M, int64_t K) {
-    const int64_t tiles = cdiv(N, T128) * cdiv(M, T128), steps = cdiv(K, K64);
+// Splits of the K range, towards one workgroup per compute unit, several steps each: a split costs a round trip of the fp32
+// partial tiles and the joining launch. bf16: 8 steps (1024^3: 14.9 us, with 2 steps 17.1); a step of fp32 takes 8 times as
+// long: 2 steps.
+int linear128_splits(int dtype, int64_t N, int64_t M, int64_t K) {
+    const int64_t tiles = cdiv(N, T128) * cdiv(M, T128), steps = cdiv(K, 128 / (int64_t)dtype_size(dtype));
+    const int64_t least = dtype == SPHIP_BF16 ? 8 : 2;
     int64_t s = 256 / tiles;
-    if (s > steps / 8) s = steps / 8;
+    if (s > steps / least) s = steps / least;
     return s < 1 ? 1 : (int)s;
 }
 
-int launch_linear128(const char* what, int mode_a, int mode_b, const Operand& A, const Operand& B, const Epilogue& epi, int64_t K,
-                     int64_t KB, const TileGrid& g, hipStream_t s) {
+int launch_linear128(const char* what, int dtype, int mode_a, int mode_b, const Operand& A, const Operand& B, const Epilogue& epi,
+                     int64_t K, int64_t KB, const TileGrid& g, hipStream_t s) {
     typedef void (*kern_t)(Operand, Operand, Epilogue, int64_t, int64_t, TileGrid);
     const int64_t blocks = (int64_t)g.tilesM * g.tilesN * g.splits;
-    const int which = mode_a == OP_ROWS ? (mode_b == OP_ROWS ? 0 : 1) : 2, deep = blocks <= 256;
-    static const kern_t kerns[3][2] = {{linear128_kernel<OP_ROWS, OP_ROWS, 2>, linear128_kernel<OP_ROWS, OP_ROWS, 4>},
-                                       {linear128_kernel<OP_ROWS, OP_COLS, 2>, linear128_kernel<OP_ROWS, OP_COLS, 4>},
-                                       {linear128_kernel<OP_COLS, OP_COLS, 2>, linear128_kernel<OP_COLS, OP_COLS, 4>}};
+    const int which = mode_a == OP_ROWS ? (mode_b == OP_ROWS ? 0 : 1) : 2, deep = blocks <= 256, bf = dtype == SPHIP_BF16;
+#define LIN_KERNELS(T)                                                                                    \
+    {{linear128_kernel<T, OP_ROWS, OP_ROWS, 2>, linear128_kernel<T, OP_ROWS, OP_ROWS, 4>},                 \
+     {linear128_kernel<T, OP_ROWS, OP_COLS, 2>, linear128_kernel<T, OP_ROWS, OP_COLS, 4>},                 \
+     {linear128_kernel<T, OP_COLS, OP_COLS, 2>, linear128_kernel<T, OP_COLS, OP_COLS, 4>}}
+    static const kern_t kerns[2][3][2] = {LIN_KERNELS(float), LIN_KERNELS(bf16_t)};
+#undef LIN_KERNELS
     const int lds = deep ? 4 * STAGE : FINISH;
-    static uint64_t done[3][2] = {};
-    SPHIP_REQUIRE(reserve_lds((const void*)kerns[which][deep], lds, done[which][deep]), SPHIP_ELAUNCH, "%s: cannot reserve %d bytes of LDS", what, lds);
-    hipLaunchKernelGGL(kerns[which][deep], dim3((unsigned)blocks), dim3(256), lds, s, A, B, epi, K, KB, g);
+    static uint64_t done[2][3][2] = {};
+    const kern_t fn = kerns[bf][which][deep];
+    SPHIP_REQUIRE(reserve_lds((const void*)fn, lds, done[bf][which][deep]), SPHIP_ELAUNCH, "%s: cannot reserve %d bytes of LDS", what, lds);
+    hipLaunchKernelGGL(fn, dim3((unsigned)blocks), dim3(256), lds, s, A, B, epi, K, KB, g);
     SPHIP_CHECK_LAUNCH(what);
     return SPHIP_OK;
 }

@@ -86,8 +86,8 @@ __global__ __launch_bounds__(512, 2) void linear256_kernel(Operand A, Operand B,
     auto dma_b = [&](int hi, int t, int i) { sb.dma(dst + (t & 1) * IMG + (hi ? RG_BHI : RG_BLO) + 8192 * i, t, i, hi); };
 
     const unsigned lds0 = (unsigned)(size_t)(lds_t)smem;
-    Frag<MA, 512> fa;
-    Frag<MB, 256> fb;
+    Frag<bf16_t, MA, 512> fa;
+    Frag<bf16_t, MB, 256> fb;
     fa.init(lds0, wn * 64, lane);
     fb.init(lds0, wm * 64, lane);
     auto read_a = [&](unsigned bo) {
@@ -117,8 +117,7 @@ __global__ __launch_bounds__(512, 2) void linear256_kernel(Operand A, Operand B,
             for (int mt = 0; mt < 4; ++mt) {
 #pragma unroll
                 for (int nt = 0; nt < 4; ++nt)
-                    acc[mbase + mt][nt] =
-                        __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb.get(mt, ks), fa.get(nt, ks), acc[mbase + mt][nt], 0, 0, 0);
+                    acc[mbase + mt][nt] = mma16(fb.get(mt, ks), fa.get(nt, ks), acc[mbase + mt][nt], bf16_t{});
                 const int j = ks * 4 + mt;
                 if (j < ndma) {
                     __builtin_amdgcn_sched_barrier(0);
@@ -188,7 +187,7 @@ __global__ __launch_bounds__(512, 2) void linear256_kernel(Operand A, Operand B,
 }
 
 bool linear256_takes(int mode_a, int mode_b, const Operand& A, const Operand& B, int64_t K) {
-    return dma_ok(mode_a, A, K, T256) && dma_ok(mode_b, B, K, T256);
+    return dma_ok(mode_a, A, K, T256, 2) && dma_ok(mode_b, B, K, T256, 2);
 }
 
 int launch_linear256(const char* what, int mode_a, int mode_b, const Operand& A, const Operand& B, const Epilogue& epi, int64_t K,
