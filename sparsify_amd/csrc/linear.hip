@@ -309,7 +309,7 @@ static int split_count(int64_t N, int64_t M, int64_t steps) {
 static size_t part_bytes(int64_t N, int64_t M, int splits) {
     return splits > 1 ? (size_t)splits * N * ((M + 3) / 4 * 4) * 4 : 0;
 }
-// SPHIP_LINEAR=tile|128|256|few forces a kernel (tests, A/B runs); read once per entry point
+// SPHIP_LINEAR=tile|64|128|256|few forces a kernel (tests, A/B runs); read once per entry point
 static thread_local char g_forced = 0;
 static void read_forced() {
     const char* e = getenv("SPHIP_LINEAR");
@@ -317,23 +317,35 @@ static void read_forced() {
 }
 
 // Which kernel a product of these sizes goes to if its operands are such that LDS-DMA can fetch them.
-enum { BY_TILES = 0, BY_128 = 1, BY_256 = 2 };
-static int kernel_for(int dtype, int64_t N, int64_t M) {
-    if (g_forced) return g_forced == '2' && dtype == SPHIP_BF16 ? BY_256 : g_forced == '1' || g_forced == '2' ? BY_128 : BY_TILES;
-    if (dtype != SPHIP_BF16) return BY_128;
-    // The 256 x 256 kernel where its tiles fill most of the 256 compute units once: 16384 x 1024 x 4096 takes 101 us against
-    // 118 with 128 x 128 tiles, 8192 x 2048 x 2048 56 against 68. Below, splitting K for the large tile costs more than the
-    // smaller tile does: 1000 x 4096 x 4096 (64 large tiles) 47 us against 41, 2048^3 37 against 25.
-    return cdiv(N, 256) * cdiv(M, 256) >= 160 ? BY_256 : BY_128;
-}
+enum { BY_TILES = 0, BY_64 = 1, BY_128 = 2, BY_256 = 3 };
 static int splits_of(int dtype, int by, int64_t N, int64_t M, int64_t K) {
-    return by == BY_256 ? 1 : by == BY_128 ? linear128_splits(dtype, N, M, K) : split_count(N, M, cdiv(K, 128 / (int64_t)dtype_size(dtype)));
+    return by == BY_256 ? 1 : by == BY_128 ? linear128_splits(dtype, N, M, K) : by == BY_64 ? linear64_splits(dtype, N, M, K)
+         : split_count(N, M, cdiv(K, 128 / (int64_t)dtype_size(dtype)));
+}
+// Time of a product with 64 x 64 or 128 x 128 tiles in ns, without what both take: K steps one after the other, a step of one
+// workgroup `step` (measured: 64 x 64 200 bf16, 520 fp32; 128 x 128 570 and 2100 alone on its compute unit, 400 and 1950 where
+// two share one), and for a split K range the joining launch and a round trip of the partial tiles at 3 TB/s.
+static int64_t product_ns(int dtype, int by, int64_t N, int64_t M, int64_t K) {
+    const int64_t tile = by == BY_64 ? 64 : 128, splits = splits_of(dtype, by, N, M, K);
+    const int64_t groups = cdiv(N, tile) * cdiv(M, tile) * splits, steps = cdiv(cdiv(K, 128 / (int64_t)dtype_size(dtype)), splits);
+    const bool bf = dtype == SPHIP_BF16;
+    const int64_t step = by == BY_64 ? (bf ? 200 : 520) : groups <= 256 ? (bf ? 570 : 2100) : (bf ? 400 : 1950);
+    return steps * step * cdiv(groups, 256) + (splits > 1 ? 4000 + splits * N * M / 375 : 0);
+}
+static int kernel_for(int dtype, int64_t N, int64_t M, int64_t K) {
+    if (g_forced) return g_forced == '2' && dtype == SPHIP_BF16 ? BY_256 : g_forced == '1' || g_forced == '2' ? BY_128 : g_forced == '6' ? BY_64 : BY_TILES;
+    // The 256 x 256 kernel where its tiles fill most of the 256 compute units once: 16384 x 1024 x 4096 takes 101 us against
+    // 118 with 128 x 128 tiles, 8192 x 2048 x 2048 56 against 68; with fewer the smaller tiles win (2048^3 22 against 37).
+    if (dtype == SPHIP_BF16 && cdiv(N, 256) * cdiv(M, 256) >= 160) return BY_256;
+    // 64 against 128: 1024^3 7.1 us / 14.9, 2048 x 512 x 512 in fp32 13 / 24, but 2048^3 27 / 22 and 16384 tokens' gradient of
+    // a 768 x 768 weight 56 / 32
+    return product_ns(dtype, BY_64, N, M, K) <= product_ns(dtype, BY_128, N, M, K) ? BY_64 : BY_128;
 }
 
 // the most a product needs for its partial tiles, whichever kernel takes it
 static size_t split_bytes(int dtype, int64_t N, int64_t M, int64_t K) {
     const int64_t Kp = cdiv(K, 64) * 64;
-    const size_t a = part_bytes(N, M, splits_of(dtype, BY_TILES, N, M, Kp)), b = part_bytes(N, M, splits_of(dtype, kernel_for(dtype, N, M), N, M, Kp));
+    const size_t a = part_bytes(N, M, splits_of(dtype, BY_TILES, N, M, Kp)), b = part_bytes(N, M, splits_of(dtype, kernel_for(dtype, N, M, Kp), N, M, Kp));
     return a > b ? a : b;
 }
 
@@ -344,15 +356,16 @@ static int launch_product(const char* what, const Operand& A, const Operand& B, 
     constexpr int dtype = sizeof(T) == 2 ? SPHIP_BF16 : SPHIP_F32;
     int by = BY_TILES;
     if (MODE_B <= OP_COLS) {
-        by = kernel_for(dtype, N, M);
+        by = kernel_for(dtype, N, M, cdiv(K, 64) * 64);
         if (by == BY_256 && !linear256_takes(MODE_A, MODE_B, A, B, K)) by = BY_TILES;
         if (by == BY_128 && !linear128_takes(dtype, MODE_A, MODE_B, A, B, K)) by = BY_TILES;
+        if (by == BY_64 && !linear64_takes(dtype, MODE_A, MODE_B, A, B, K)) by = BY_TILES;
     }
-    const int tile = by == BY_256 ? 256 : 128;
+    const int tile = by == BY_256 ? 256 : by == BY_64 ? 64 : 128;
     const int64_t steps = cdiv(K, LCH * Chunk<T>::E);
     TileGrid g;
     g.tilesM = (int)cdiv(M, tile), g.tilesN = (int)cdiv(N, tile);
-    const int want = splits_of(dtype, by, N, M, K);
+    const int want = splits_of(dtype, by, N, M, cdiv(K, 64) * 64);
     g.steps_per = (int)cdiv(steps, want);
     g.splits = (int)cdiv(steps, g.steps_per);
     g.part = (float*)ws;
@@ -366,7 +379,8 @@ static int launch_product(const char* what, const Operand& A, const Operand& B, 
                   "%s: grid too large", what);
     if (by != BY_TILES) {
         const int st = by == BY_256 ? launch_linear256(what, MODE_A, MODE_B, A, B, epi, K, KB, g, s)
-                                    : launch_linear128(what, dtype, MODE_A, MODE_B, A, B, epi, K, KB, g, s);
+                     : by == BY_128 ? launch_linear128(what, dtype, MODE_A, MODE_B, A, B, epi, K, KB, g, s)
+                                    : launch_linear64(what, dtype, MODE_A, MODE_B, A, B, epi, K, KB, g, s);
         if (st != SPHIP_OK) return st;
     } else {
         hipLaunchKernelGGL((linear_tile_kernel<T, MODE_A, MODE_B>), dim3((unsigned)nblocks), dim3(256), 0, s, A, B, epi, K, KB, g);
@@ -422,12 +436,10 @@ struct Packing {
         return SPHIP_OK;
     }
 };
-// Whether a product is worth copying an operand whose rows LDS-DMA cannot fetch (they do not start at multiples of 16 bytes,
-// or K is no whole number of steps)
-static bool worth_packing(int dtype, int64_t N, int64_t M, int64_t K, int least = 29) {
-    if (dtype != SPHIP_BF16) least -= 2;
-    return g_forced ? g_forced != 't' : N * M * K >= (1ll << least);
-}
+// Whether a product is worth a launch that copies an operand whose rows LDS-DMA cannot fetch (they do not start at multiples
+// of 16 bytes, or K is no whole number of steps) or restores 8-bit codes, against the tile kernel that takes anything:
+// 300^3 8.1 us against 14.5, 5000 x 333 x 333 12.7 against 16.4.
+static bool worth_packing(int64_t N, int64_t M, int64_t K) { return g_forced ? g_forced != 't' : N * M * K >= (1ll << 24); }
 static bool unaligned(int dtype, int64_t cols) { return cols * (int64_t)dtype_size(dtype) % 16 != 0; }
 
 // ---- dz = g act'(z) and its column sums. A workgroup takes 32 rows (the group one scale of an 8-bit z covers) of 32 x 16
@@ -598,7 +610,7 @@ static ForwardSpace forward_space(int dtype, int z_kind, int64_t N, int64_t D, i
     const bool one = few(dtype, N, D, M);
     f.part = one ? 0 : up256(split_bytes(dtype, N, M, D));
     f.z = is_codes(z_kind) && (f.part || one) ? up256((size_t)N * (cdiv(M, 4) * 4) * 4) : 0;      // (no codes from a split K range or from few rows)
-    f.pack = !one && D * (int64_t)dtype_size(dtype) % 128 != 0 && worth_packing(dtype, N, M, D)
+    f.pack = !one && D * (int64_t)dtype_size(dtype) % 128 != 0 && worth_packing(N, M, D)
                  ? (size_t)(N + M) * packed_ld(D) * dtype_size(dtype) : 0;
     f.total = f.part + f.z + f.pack;
     return f;
@@ -679,9 +691,9 @@ static BackwardSpace backward_space(int dtype, int x_kind, int want_dx, int want
     const bool odd = unaligned(dtype, D);
     b.dz = want_dx || want_dw ? up256((size_t)N * packed_ld(M) * es) : 0;
     b.sums = want_db ? up256((size_t)cdiv(N, 32) * M * 4) : 0;
-    b.x = want_dw && (is_codes(x_kind) ? worth_packing(dtype, M, D, N, 31) : odd && worth_packing(dtype, M, D, N))
+    b.x = want_dw && (is_codes(x_kind) || odd) && worth_packing(M, D, N)
               ? up256((size_t)N * packed_ld(D) * es) : 0;
-    b.w = want_dx && odd && worth_packing(dtype, N, D, M) ? up256((size_t)M * packed_ld(D) * es) : 0;
+    b.w = want_dx && odd && worth_packing(N, D, M) ? up256((size_t)M * packed_ld(D) * es) : 0;
     const size_t p1 = want_dx ? split_bytes(dtype, N, D, M) : 0, p2 = want_dw ? split_bytes(dtype, M, D, N) : 0;
     b.part = p1 > p2 ? p1 : p2;
     b.total = b.dz + b.sums + b.x + b.w + b.part;
@@ -769,7 +781,7 @@ extern "C" int sphip_linear_backward(const void* g, int g_dtype, int64_t ldg, co
     const bool products = dx || dW;
     bool direct = act == SPHIP_ACT_NONE && g_dtype == dtype;
     if (direct && (M * (int64_t)dtype_size(dtype) % 128 != 0 || unaligned(dtype, ldg) || ((uintptr_t)g & 15) != 0))
-        direct = !((dx && worth_packing(dtype, N, D, M)) || (dW && worth_packing(dtype, M, D, N)));
+        direct = !((dx && worth_packing(N, D, M)) || (dW && worth_packing(M, D, N)));
     Operand dz = {g, nullptr, ldg, (int)N};
     if (products && !direct) dz.p = w, dz.ld = packed_ld(M);
     Packing pack(dtype);

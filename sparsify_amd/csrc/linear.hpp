@@ -241,6 +241,10 @@ int launch_linear_few(const char* what, int dtype, const Operand& X, const Opera
 bool linear256_takes(int mode_a, int mode_b, const Operand& A, const Operand& B, int64_t K);
 int launch_linear256(const char* what, int mode_a, int mode_b, const Operand& A, const Operand& B, const Epilogue& epi, int64_t K,
                      int64_t KB, const TileGrid& g, hipStream_t s);
+bool linear64_takes(int dtype, int mode_a, int mode_b, const Operand& A, const Operand& B, int64_t K);
+int linear64_splits(int dtype, int64_t N, int64_t M, int64_t K);
+int launch_linear64(const char* what, int dtype, int mode_a, int mode_b, const Operand& A, const Operand& B, const Epilogue& epi,
+                    int64_t K, int64_t KB, const TileGrid& g, hipStream_t s);
 bool linear128_takes(int dtype, int mode_a, int mode_b, const Operand& A, const Operand& B, int64_t K);
 int linear128_splits(int dtype, int64_t N, int64_t M, int64_t K);
 int launch_linear128(const char* what, int dtype, int mode_a, int mode_b, const Operand& A, const Operand& B, const Epilogue& epi,

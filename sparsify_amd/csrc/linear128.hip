@@ -14,45 +14,6 @@ namespace sphip {
 constexpr int T128 = 128, IMG_A = 0, IMG_B = 16384, STAGE = 32768;
 constexpr int FINISH = 4 * 64 * OUT_ROW;            // the epilogue's staging: more than two stages, twice still within the LDS
 
-template <typename T, int MODE> struct Source128 {
-    static constexpr unsigned ES = sizeof(T), KS = 128 / ES;
-    __amdgpu_buffer_rsrc_t rsrc;
-    unsigned voff[2], piece, step;         // bytes: lane offset of even and odd pieces, between the 4 pieces of a step, between K steps
-    __device__ __forceinline__ void init(const Operand& o, int row0, int64_t k0, int64_t K, int tid) {
-        const T* p = (const T*)o.p;
-        const unsigned ldb = (unsigned)o.ld * ES;
-        if (MODE == OP_ROWS) {
-            const int hr = tid >> 3, ch = (tid & 7) ^ ((hr >> 1) & 7);
-            const int rows = min(T128, o.rows - row0);
-            rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)(p + (int64_t)row0 * o.ld + k0), 0,
-                                                     (int)((unsigned)(rows - 1) * ldb + (unsigned)(K - k0) * ES), 0x00020000);
-            voff[0] = voff[1] = (unsigned)hr * ldb + (unsigned)ch * 16u;
-            piece = 32u * ldb;
-            step = 128;
-        } else {
-            // (the end rounded up to a piece, see linear256.hip)
-            rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)(p + k0 * o.ld + row0), 0,
-                                                     (int)(K > k0 ? (unsigned)(K - 1 - k0) * ldb + ((unsigned)(o.rows - row0) * ES + 15u) / 16u * 16u : 0u),
-                                                     0x00020000);
-            constexpr int LOG = ES == 2 ? 4 : 5;                // 16-byte chunks of 128 columns
-            const int kr = tid >> LOG, c = tid & ((1 << LOG) - 1);
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int k = kr + (256 >> LOG) * i;
-                const int f = ES == 2 ? 2 * ((k & 3) + 4 * ((k >> 3) & 1)) : 4 * ((k >> 2) & 3);
-                voff[i] = (unsigned)kr * ldb + (unsigned)(c ^ f) * 16u;
-            }
-            piece = (256u >> LOG) * ldb;
-            step = KS * ldb;
-        }
-    }
-    __device__ __forceinline__ void dma(char* lds, int t) const {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_t)(lds + 4096 * i), 16, voff[i & 1] + (unsigned)t * step + (unsigned)i * piece, 0, 0, 0);
-    }
-};
-
 template <typename T, int MA, int MB, int STAGES>
 __global__ __launch_bounds__(256, STAGES == 2 ? 2 : 1) void linear128_kernel(Operand A, Operand B, Epilogue epi, int64_t K, int64_t KB,
                                                                              TileGrid g) {
@@ -67,8 +28,8 @@ __global__ __launch_bounds__(256, STAGES == 2 ? 2 : 1) void linear128_kernel(Ope
     const int64_t k0 = (int64_t)split * g.steps_per * KS;
     const int steps = (int)min((int64_t)g.steps_per, (K - k0 + KS - 1) / KS);
 
-    Source128<T, MA> sa;
-    Source128<T, MB> sb;
+    Source<T, MA, T128> sa;
+    Source<T, MB, T128> sb;
     sa.init(A, n0, k0, K, tid);
     sb.init(B, m0, k0, KB, tid);
     auto fetch = [&](int t, unsigned image) {      // 8 DMA instructions per wave

@@ -26,7 +26,7 @@ __device__ __forceinline__ void segment_barrier() {
 
 // One operand of the kernel: descriptor, per-lane source offset, DMA pieces. Which = 0: A (one region of 256 rows, 4 pieces
 // per K step), 1: B (regions lo / hi of 128 rows, 2 pieces each: rows [0,64) and [64,128) of both 128-row wave groups).
-template <int MODE, int WHICH> struct Source {
+template <int MODE, int WHICH> struct Source256 {
     __amdgpu_buffer_rsrc_t rsrc;
     unsigned voff, piece, step;            // bytes: lane offset, between pieces, between K steps
     __device__ __forceinline__ void init(const Operand& o, int row0, int64_t k0, int64_t K, int tid) {
@@ -77,8 +77,8 @@ __global__ __launch_bounds__(512, 2) void linear256_kernel(Operand A, Operand B,
     const int64_t k0 = (int64_t)split * g.steps_per * K64;
     const int steps = (int)min((int64_t)g.steps_per, (K - k0 + K64 - 1) / K64);
 
-    Source<MA, 0> sa;
-    Source<MB, 1> sb;
+    Source256<MA, 0> sa;
+    Source256<MB, 1> sb;
     sa.init(A, n0, k0, K, tid);
     sb.init(B, m0, k0, KB, tid);
     char* const dst = smem + wave * 1024;              // wave-uniform base of a 1 KiB piece

@@ -4,7 +4,7 @@
 // contiguous in its rows (OP_COLS: the gradient products). The latter is not transposed in memory: its image is [k][chunks
 // of 8 rows] as it comes, and ds_read_b64_tr_b16 hands every lane 4 consecutive k of its row (of 16 lanes, lane i names
 // k = i / 4 and rows 4 (i % 4) .. + 3 and receives row i). Chunk XOR 2 ((k & 3) + 4 ((k >> 3) & 1)) spreads the 4 k of one
-// read, and the 8 apart ones of the neighbouring 16 lanes, over 8 different 32-byte slots: no bank conflicts.
+// read, and the 8 apart ones of the neighbouring 16 lanes, over 8 different 32-byte slots: no bank conflicts (cols_swizzle).
 // LDS-DMA writes linearly, so both swizzles are applied to the per-lane source address; rows and K past the end read as
 // zeros by the buffer descriptors' range check (K past the end of an OP_ROWS operand does not, hence K % 64 == 0 there).
 #pragma once
@@ -16,85 +16,98 @@ constexpr int K64 = 64;                            // bf16 K per step: 128 bytes
 
 #define LIN_VMCNT(n) asm volatile("s_waitcnt vmcnt(" #n ")" ::: "memory")
 
-// Four 16-row fragments of 64 k, the reads of one 32-k step at a time: read<0>(), read<1>(), wait<KS, COUNT>() once at most
-// COUNT later LDS operations are outstanding. Issued from inline asm (the compiler would drain the DMA queue before each
-// LDS read it sees); the wait names the step's destination registers, so that nothing reads them before.
-template <typename T, int MODE, int PITCH> struct Frag;
-template <typename T, int PITCH> struct Frag<T, OP_ROWS, PITCH> {
-    static constexpr int READS = 4;                    // LDS operations per 32-k step
-    w4_t v[4][2];
-    unsigned a[2];                                     // the lane's address per 32-k step; tiles are 16 rows = 2048 bytes apart
-    // the wave's 64 rows start at row0 of the image
-    __device__ __forceinline__ void init(unsigned lds0, int row0, int lane) {
+// Chunk swizzle of an OP_COLS image with PITCH bytes per k row, element size ES (see above; with 128-byte rows the low bit of
+// k already tells the two halves of the banks apart, and fp32 reads single dwords: there the four 16-lane groups, 4 k rows
+// apart, go to different 64-byte quarters).
+template <int ES, int PITCH> __device__ __forceinline__ int cols_swizzle(int k) {
+    if (ES == 4) return 4 * ((k >> 2) & 3);
+    if (PITCH == 128) return 2 * (((k >> 1) & 1) + 2 * ((k >> 3) & 1));
+    return 2 * ((k & 3) + 4 * ((k >> 3) & 1));
+}
+
+// TILES 16-row fragments of a 128-byte K step, the reads of one half (32 bf16 k, 16 fp32 k) at a time: read<0>(), read<1>(),
+// wait<H, COUNT>() once at most COUNT later LDS operations are outstanding. Issued from inline asm (the compiler would drain
+// the DMA queue before each LDS read it sees); wait() passes every destination register of the half through an asm statement
+// behind its s_waitcnt, so that nothing reads one before. init(): the wave's rows start at row0 of the image, half 0 is `h0`.
+template <typename T, int MODE, int PITCH, int TILES = 4> struct Frag;
+template <typename T, int PITCH, int TILES> struct Frag<T, OP_ROWS, PITCH, TILES> {
+    static constexpr int READS = TILES;                // LDS operations per half
+    w4_t v[TILES][2];
+    unsigned a[2];                                     // the lane's address per half; tiles are 16 rows = 2048 bytes apart
+    __device__ __forceinline__ void init(unsigned lds0, int row0, int lane, int h0 = 0) {
         const int r16 = lane & 15, q4 = lane >> 4;
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks) a[ks] = lds0 + (row0 + r16) * 128 + (((4 * ks + q4) ^ ((r16 >> 1) & 7)) << 4);
+        for (int h = 0; h < 2; ++h) a[h] = lds0 + (row0 + r16) * 128 + (((4 * (h ^ h0) + q4) ^ ((r16 >> 1) & 7)) << 4);
     }
-    template <int KS> __device__ __forceinline__ void read(unsigned image) {
-        const unsigned at = a[KS] + image;
-#define LIN_DSR(i) asm volatile("ds_read_b128 %0, %1 offset:%2" : "=v"(v[i][KS]) : "v"(at), "i"((i) * 2048))
+    template <int H> __device__ __forceinline__ void read(unsigned image) {
+        const unsigned at = a[H] + image;
+#define LIN_DSR(i) \
+    if constexpr (i < TILES) asm volatile("ds_read_b128 %0, %1 offset:%2" : "=v"(v[i][H]) : "v"(at), "i"((i) * 2048))
         LIN_DSR(0); LIN_DSR(1); LIN_DSR(2); LIN_DSR(3);
 #undef LIN_DSR
     }
-    template <int KS, int COUNT> __device__ __forceinline__ void wait() {
-        asm volatile("s_waitcnt lgkmcnt(%4)" : "+v"(v[0][KS]), "+v"(v[1][KS]), "+v"(v[2][KS]), "+v"(v[3][KS]) : "i"(COUNT));
-    }
-    __device__ __forceinline__ w4_t get(int i, int ks) const { return v[i][ks]; }
-};
-template <int PITCH> struct Frag<bf16_t, OP_COLS, PITCH> {      // PITCH bytes per k row of the image
-    static constexpr int READS = 8;
-    w2_t v[4][2][2];                                   // [tile][32-k step][4-k half]
-    unsigned a[4];                                     // the lane's address per tile
-    __device__ __forceinline__ void init(unsigned lds0, int row0, int lane) {
-        const int r16 = lane & 15, q4 = lane >> 4;
-        const int k = 8 * q4 + (r16 >> 2), f = (k & 3) + 4 * ((k >> 3) & 1);
+    template <int H, int COUNT> __device__ __forceinline__ void wait() {
+        asm volatile("s_waitcnt lgkmcnt(%0)" ::"i"(COUNT));
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            a[i] = lds0 + k * PITCH + (((row0 / 8 + 2 * i + ((r16 & 3) >> 1)) ^ (2 * f)) << 4) + (r16 & 1) * 8;
+        for (int i = 0; i < TILES; ++i) asm volatile("" : "+v"(v[i][H]));
     }
-    template <int KS> __device__ __forceinline__ void read(unsigned image) {
-#define LIN_DSR(i, h)                                                                                            \
-    asm volatile("ds_read_b64_tr_b16 %0, %1 offset:%2"                                                           \
-                 : "=v"(v[i][KS][h])                                                                             \
-                 : "v"(a[i] + image), "i"(KS * 32 * PITCH + (h) * 4 * PITCH))
+    __device__ __forceinline__ w4_t get(int i, int h) const { return v[i][h]; }
+};
+template <int PITCH, int TILES> struct Frag<bf16_t, OP_COLS, PITCH, TILES> {
+    static constexpr int READS = 2 * TILES;
+    w2_t v[TILES][2][2];                               // [tile][half][4-k quarter]
+    unsigned a[TILES];                                 // the lane's address per tile
+    __device__ __forceinline__ void init(unsigned lds0, int row0, int lane, int h0 = 0) {
+        const int r16 = lane & 15, q4 = lane >> 4, k = 8 * q4 + (r16 >> 2);
+#pragma unroll
+        for (int i = 0; i < TILES; ++i)
+            a[i] = lds0 + (k + 32 * h0) * PITCH + (((row0 / 8 + 2 * i + ((r16 & 3) >> 1)) ^ cols_swizzle<2, PITCH>(k)) << 4) + (r16 & 1) * 8;
+    }
+    template <int H> __device__ __forceinline__ void read(unsigned image) {
+#define LIN_DSR(i, q)                                                                                            \
+    if constexpr (i < TILES)                                                                                     \
+        asm volatile("ds_read_b64_tr_b16 %0, %1 offset:%2" : "=v"(v[i][H][q]) : "v"(a[i] + image), "i"(H * 32 * PITCH + (q) * 4 * PITCH))
         LIN_DSR(0, 0); LIN_DSR(0, 1); LIN_DSR(1, 0); LIN_DSR(1, 1);
         LIN_DSR(2, 0); LIN_DSR(2, 1); LIN_DSR(3, 0); LIN_DSR(3, 1);
 #undef LIN_DSR
     }
-    template <int KS, int COUNT> __device__ __forceinline__ void wait() {
-        asm volatile("s_waitcnt lgkmcnt(%8)"
-                     : "+v"(v[0][KS][0]), "+v"(v[0][KS][1]), "+v"(v[1][KS][0]), "+v"(v[1][KS][1]), "+v"(v[2][KS][0]),
-                       "+v"(v[2][KS][1]), "+v"(v[3][KS][0]), "+v"(v[3][KS][1])
-                     : "i"(COUNT));
+    template <int H, int COUNT> __device__ __forceinline__ void wait() {
+        asm volatile("s_waitcnt lgkmcnt(%0)" ::"i"(COUNT));
+#pragma unroll
+        for (int i = 0; i < TILES; ++i) {
+            asm volatile("" : "+v"(v[i][H][0]));
+            asm volatile("" : "+v"(v[i][H][1]));
+        }
     }
-    __device__ __forceinline__ w4_t get(int i, int ks) const { return __builtin_shufflevector(v[i][ks][0], v[i][ks][1], 0, 1, 2, 3); }
+    __device__ __forceinline__ w4_t get(int i, int h) const { return __builtin_shufflevector(v[i][h][0], v[i][h][1], 0, 1, 2, 3); }
 };
-// fp32 needs no transposing read: a lane's 4 k (4 (4 ks + q4) + j, as in the OP_ROWS image) are 4 dwords of its column.
-// Chunk XOR 4 ((k >> 2) & 3): the four 16-lane groups, 4 k rows apart, read different 64-byte quarters of the banks.
-template <int PITCH> struct Frag<float, OP_COLS, PITCH> {
-    static constexpr int READS = 16;
-    unsigned v[4][2][4];
-    unsigned a[4];
-    __device__ __forceinline__ void init(unsigned lds0, int row0, int lane) {
+// fp32 needs no transposing read: a lane's 4 k (4 (4 h + q4) + j, as in the OP_ROWS image) are 4 dwords of its column
+template <int PITCH, int TILES> struct Frag<float, OP_COLS, PITCH, TILES> {
+    static constexpr int READS = 4 * TILES;
+    unsigned v[TILES][2][4];
+    unsigned a[TILES];
+    __device__ __forceinline__ void init(unsigned lds0, int row0, int lane, int h0 = 0) {
         const int r16 = lane & 15, q4 = lane >> 4;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) a[i] = lds0 + 4 * q4 * PITCH + (((row0 / 4 + 4 * i + (r16 >> 2)) ^ (4 * q4)) << 4) + (r16 & 3) * 4;
+        for (int i = 0; i < TILES; ++i)
+            a[i] = lds0 + (4 * q4 + 16 * h0) * PITCH + (((row0 / 4 + 4 * i + (r16 >> 2)) ^ cols_swizzle<4, PITCH>(4 * q4)) << 4) + (r16 & 3) * 4;
     }
-    template <int KS> __device__ __forceinline__ void read(unsigned image) {
-#define LIN_DSR(i, j) \
-    asm volatile("ds_read_b32 %0, %1 offset:%2" : "=v"(v[i][KS][j]) : "v"(a[i] + image), "i"(KS * 16 * PITCH + (j) * PITCH))
+    template <int H> __device__ __forceinline__ void read(unsigned image) {
+#define LIN_DSR(i, j)        \
+    if constexpr (i < TILES) \
+        asm volatile("ds_read_b32 %0, %1 offset:%2" : "=v"(v[i][H][j]) : "v"(a[i] + image), "i"(H * 16 * PITCH + (j) * PITCH))
         LIN_DSR(0, 0); LIN_DSR(0, 1); LIN_DSR(0, 2); LIN_DSR(0, 3); LIN_DSR(1, 0); LIN_DSR(1, 1); LIN_DSR(1, 2); LIN_DSR(1, 3);
         LIN_DSR(2, 0); LIN_DSR(2, 1); LIN_DSR(2, 2); LIN_DSR(2, 3); LIN_DSR(3, 0); LIN_DSR(3, 1); LIN_DSR(3, 2); LIN_DSR(3, 3);
 #undef LIN_DSR
     }
-    template <int KS, int COUNT> __device__ __forceinline__ void wait() {
-        asm volatile("s_waitcnt lgkmcnt(%16)"
-                     : "+v"(v[0][KS][0]), "+v"(v[0][KS][1]), "+v"(v[0][KS][2]), "+v"(v[0][KS][3]), "+v"(v[1][KS][0]), "+v"(v[1][KS][1]),
-                       "+v"(v[1][KS][2]), "+v"(v[1][KS][3]), "+v"(v[2][KS][0]), "+v"(v[2][KS][1]), "+v"(v[2][KS][2]),
-                       "+v"(v[2][KS][3]), "+v"(v[3][KS][0]), "+v"(v[3][KS][1]), "+v"(v[3][KS][2]), "+v"(v[3][KS][3])
-                     : "i"(COUNT));
+    template <int H, int COUNT> __device__ __forceinline__ void wait() {
+        asm volatile("s_waitcnt lgkmcnt(%0)" ::"i"(COUNT));
+#pragma unroll
+        for (int i = 0; i < TILES; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) asm volatile("" : "+v"(v[i][H][j]));
     }
-    __device__ __forceinline__ w4_t get(int i, int ks) const { return (w4_t){v[i][ks][0], v[i][ks][1], v[i][ks][2], v[i][ks][3]}; }
+    __device__ __forceinline__ w4_t get(int i, int h) const { return (w4_t){v[i][h][0], v[i][h][1], v[i][h][2], v[i][h][3]}; }
 };
 
 // c += a b^T over 16 bytes of K per lane (32 bf16 k, or 16 fp32 k in four 4-wide MFMAs: element j of every lane each time)
@@ -119,6 +132,44 @@ __device__ __forceinline__ void finish_tile(Acc acc, char* stage, const Epilogue
             *reinterpret_cast<acc4_t*>(stage + (nt * 16 + r16) * OUT_ROW + (mt * 16 + q4 * 4) * 4) = acc(mt, nt);
     finish_rows<NT * 16>(stage, epi, g, split, n0, m0, N, M, lane, res);
 }
+
+// One operand of a kernel of 256 threads, TILE rows: descriptor, the lane's source offsets, the DMA of one 128-byte K step
+// (PIECES instructions of 4 KiB per workgroup).
+template <typename T, int MODE, int TILE> struct Source {
+    static constexpr unsigned ES = sizeof(T), KS = 128 / ES;
+    static constexpr int PIECES = TILE / 32, PITCH = TILE * ES;
+    __amdgpu_buffer_rsrc_t rsrc;
+    unsigned voff[2], piece, step;         // bytes: lane offset of even and odd pieces, between pieces, between K steps
+    __device__ __forceinline__ void init(const Operand& o, int row0, int64_t k0, int64_t K, int tid) {
+        const T* p = (const T*)o.p;
+        const unsigned ldb = (unsigned)o.ld * ES;
+        if (MODE == OP_ROWS) {
+            const int hr = tid >> 3, ch = (tid & 7) ^ ((hr >> 1) & 7);
+            const int rows = min(TILE, o.rows - row0);
+            rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)(p + (int64_t)row0 * o.ld + k0), 0,
+                                                     (int)((unsigned)(rows - 1) * ldb + (unsigned)(K - k0) * ES), 0x00020000);
+            voff[0] = voff[1] = (unsigned)hr * ldb + (unsigned)ch * 16u;
+            piece = 32u * ldb;
+            step = 128;
+        } else {
+            // (the end rounded up to a piece, see linear256.hip)
+            rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)(p + k0 * o.ld + row0), 0,
+                                                     (int)(K > k0 ? (unsigned)(K - 1 - k0) * ldb + ((unsigned)(o.rows - row0) * ES + 15u) / 16u * 16u : 0u),
+                                                     0x00020000);
+            constexpr int CH = PITCH / 16, KP = 256 / CH;       // 16-byte chunks of a k row, k rows of a piece
+            const int kr = tid / CH, c = tid % CH;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) voff[i] = (unsigned)kr * ldb + (unsigned)(c ^ cols_swizzle<ES, PITCH>(kr + KP * i)) * 16u;
+            piece = KP * ldb;
+            step = KS * ldb;
+        }
+    }
+    __device__ __forceinline__ void dma(char* lds, int t) const {
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_t)(lds + 4096 * i), 16, voff[i & 1] + (unsigned)t * step + (unsigned)i * piece, 0, 0, 0);
+    }
+};
 
 // whether LDS-DMA can fetch an operand of es-byte elements: 16-byte aligned rows, 32-bit byte offsets inside a tile's
 // descriptor, whole 128-byte steps of K where K is the contiguous index

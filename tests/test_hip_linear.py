@@ -376,8 +376,9 @@ def test_gradient_against_differences(device, act, fmt):
 
 @pytest.mark.parametrize("N,D,M", [(256, 64, 256), (300, 128, 520), (1000, 192, 704), (64, 1024, 136), (257, 256, 255), (1030, 320, 1000),
                                    (2048, 128, 257), (1, 64, 64), (129, 129, 129), (700, 77, 1001), (33, 1000, 3)])
-@pytest.mark.parametrize("kernel", ["tile", "128", "256", "few"])
-def test_every_product_kernel(device, monkeypatch, N, D, M, kernel):
+@pytest.mark.parametrize("kernel", ["tile", "64", "128", "256", "few"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_every_product_kernel(device, monkeypatch, N, D, M, kernel, dtype):
     """Each of the product's kernels on small and ragged shapes (SPHIP_LINEAR): forward, and both gradient products with
     their K-strided operands, packed or as they are, split over K and whole, against the definition."""
     from sparsify_amd import ops
@@ -387,21 +388,21 @@ def test_every_product_kernel(device, monkeypatch, N, D, M, kernel):
     ops._linear_bytes.cache_clear(), ops._linear_backward_bytes.cache_clear()
     try:
         for i, (act, fmt) in enumerate([("none", "int8"), ("gelu", None), ("relu", "e4m3"), ("silu", "int8")]):
-            res = [None, torch.float32, torch.bfloat16, None][i]
-            x, W, b, r = make(N, D, M, torch.bfloat16, N + i, bias=i != 1, res=res)
-            out_dtype = torch.bfloat16 if res is None else res
+            res = [None, torch.float32, dtype, None][i]
+            x, W, b, r = make(N, D, M, dtype, N + i, bias=i != 1, res=res)
+            out_dtype = dtype if res is None else torch.promote_types(dtype, res)
             xc, Wc, bc, rc = cuda(x, W, b, r)
             y, zk, _ = ops.linear(xc, Wc, bc, rc, act, keep_z=torch.float32)
             want, tol, z, ez = forward64(x, W, b, r, act, out_dtype)
             assert_within(y, want, tol, f"y {act}")
             assert_within(zk, z, ez + HALF[torch.float32] * z.abs() + TINY, f"z {act}")
-            _, zq, xq = ops.linear(xc, Wc, bc, rc, act, keep_z=fmt or torch.bfloat16, keep_x=fmt)
+            _, zq, xq = ops.linear(xc, Wc, bc, rc, act, keep_z=fmt or dtype, keep_x=fmt)
             zhat = ops.checkpoint8_restore(zq, fmt, N, M, torch.float32) if fmt else zq
             g = torch.randn(N, M, generator=torch.Generator().manual_seed(i)).to(out_dtype)
             dx, dW, db = ops.linear_backward(g.cuda(), Wc, zq, xq if fmt else xc, act, z_fmt=fmt, x_fmt=fmt,
-                                             dx_dtype=torch.bfloat16, dw_dtype=torch.bfloat16, db_dtype=torch.bfloat16)
-            ref = backward64(x, W, torch.zeros(M, dtype=torch.bfloat16), act, g, zhat.double().cpu(),
-                             codes64(x, fmt) if fmt else x, torch.bfloat16, torch.bfloat16, 0.0)
+                                             dx_dtype=dtype, dw_dtype=dtype, db_dtype=dtype)
+            ref = backward64(x, W, torch.zeros(M, dtype=dtype), act, g, zhat.double().cpu(),
+                             codes64(x, fmt) if fmt else x, dtype, dtype, 0.0)
             for n, got in (("x", dx), ("W", dW), ("b", db)):
                 assert_within(got, *ref[n], f"d{n} {act} {N}x{D}x{M}")
     finally:
