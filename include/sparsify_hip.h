@@ -519,9 +519,10 @@ int sphip_muon_apply(float* p, const void* o_bf16, int64_t n, float decay, float
  *
  * The skip connection of a transcoder (sparse_coder.py:219-222: sae_out += x @ W_skip.mT) and the dense layers a
  * transcoder stands in for. All tensors row-major with unit inner stride and a row stride ld* in elements (>= the
- * row); any sizes, strides and element-aligned addresses (16-byte aligned rows take wider accesses). dtype codes
- * SPHIP_F32 / SPHIP_BF16; sums are fp32, each output is rounded once when stored. Workspaces: the *_workspace_bytes
- * query of the same call, 16-byte aligned (0 bytes: may be NULL). */
+ * row), N below 2^31 - 256, D and M below 2^22 - 64; any strides and element-aligned addresses. dtype codes SPHIP_F32 /
+ * SPHIP_BF16; sums are fp32, each output is rounded once when stored. Workspaces: the *_workspace_bytes query of the same
+ * call, 16-byte aligned (0 bytes: may be NULL). `odd` in a query: 1 if the rows of x, plus 2 if those of W, do not all start
+ * at multiples of 16 bytes, or lie 2^22 elements or more apart; the call copies these. */
 enum { SPHIP_ACT_NONE = 0, SPHIP_ACT_RELU = 1, SPHIP_ACT_GELU = 2 /* z Phi(z) */, SPHIP_ACT_SILU = 3 /* z / (1 + e^-z) */ };
 
 /* what an operand of the gradients may be besides SPHIP_F32 / SPHIP_BF16: an 8-bit checkpoint (below) */
@@ -532,7 +533,7 @@ enum { SPHIP_INT8 = 16, SPHIP_E4M3 = 17 };
  * from the fp32 sums, as an 8-bit checkpoint with scales (z_kind SPHIP_INT8 / SPHIP_E4M3, keep_sign for a ReLU);
  * x_codes / x_scales: the 8-bit checkpoint of x (format x_fmt, row stride ldq).
  * out may be residual (same stride and type); no other output may overlap an input. */
-size_t sphip_linear_workspace_bytes(int dtype, int z_kind, int64_t N, int64_t D, int64_t M);
+size_t sphip_linear_workspace_bytes(int dtype, int z_kind, int64_t N, int64_t D, int64_t M, int odd);
 int sphip_linear(const void* x, int64_t ldx, const void* W, int64_t ldw, int dtype, const void* bias, int bias_dtype,
                  int act, const void* residual, int res_dtype, int64_t ldr, void* out, int out_dtype, int64_t ldo,
                  void* z, int z_kind, uint8_t* z_scales, int64_t ldz, uint8_t* x_codes, uint8_t* x_scales, int x_fmt,
@@ -543,7 +544,7 @@ int sphip_linear(const void* x, int64_t ldx, const void* W, int64_t ldw, int dty
  * dz is rounded once to `dtype`, the products' type (that of W). z and x: values (z_kind a dtype, x_kind = dtype) or
  * 8-bit checkpoints with scales. The residual's gradient is g. Sums have a fixed order. */
 size_t sphip_linear_backward_workspace_bytes(int dtype, int x_kind, int want_dx, int want_dw, int want_db, int64_t N,
-                                             int64_t D, int64_t M);
+                                             int64_t D, int64_t M, int odd);
 int sphip_linear_backward(const void* g, int g_dtype, int64_t ldg, const void* W, int64_t ldw, int dtype, int act,
                           const void* z, int z_kind, const uint8_t* z_scales, int64_t ldz, const void* x, int x_kind,
                           const uint8_t* x_scales, int64_t ldx, void* dx, int dx_dtype, int64_t lddx, void* dW, int dw_dtype,

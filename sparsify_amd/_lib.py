@@ -100,9 +100,9 @@ SIGNATURES: dict[str, tuple] = {
     "sphip_transpose": (_I, [_P, _P, _L, _L, _L, _I, _P]),
     "sphip_add": (_I, [_P, _P, _I, _P, _L, _P]),
     "sphip_muon_apply": (_I, [_P, _P, _L, _F, _F, _P, _P]),
-    "sphip_linear_workspace_bytes": (_Z, [_I, _I, _L, _L, _L]),
+    "sphip_linear_workspace_bytes": (_Z, [_I, _I, _L, _L, _L, _I]),
     "sphip_linear": (_I, [_P, _L, _P, _L, _I, _P, _I, _I, _P, _I, _L, _P, _I, _L, _P, _I, _P, _L, _P, _P, _I, _L, _L, _L, _L, _P, _Z, _P]),
-    "sphip_linear_backward_workspace_bytes": (_Z, [_I, _I, _I, _I, _I, _L, _L, _L]),
+    "sphip_linear_backward_workspace_bytes": (_Z, [_I, _I, _I, _I, _I, _L, _L, _L, _I]),
     "sphip_linear_backward": (_I, [_P, _I, _L, _P, _L, _I, _I, _P, _I, _P, _L, _P, _I, _P, _L, _P, _I, _L, _P, _I, _L, _P, _I, _L, _L,
                                    _L, _P, _Z, _P]),
     "sphip_checkpoint8_save": (_I, [_P, _I, _L, _I, _I, _P, _P, _L, _L, _L, _P]),

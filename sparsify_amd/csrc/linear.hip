@@ -4,28 +4,14 @@
 // x and z as they are or as 8-bit checkpoints (checkpoint8.hip).
 // The skip connection of a transcoder (sparsify/sparse_coder.py:219-222) is the first user.
 //
-// All three products are C[n, m] = sum_k A(n, k) B(m, k); what differs is which index of an operand is contiguous in
-// memory. The tile kernel here takes any of them, any size, stride and alignment: a 128 x 128 tile of C per workgroup of
-// four waves (2 x 2 of 64 x 64, 32x32 MFMA tiles), 128 bytes of K per step, staged through registers into a double-buffered
-// LDS image [row][8 chunks of 16 bytes of K], chunk index XOR (row >> 1) & 7 (16 lanes of a ds_read_b128 then touch 16
-// bank groups). An operand whose rows are contiguous in K goes in as 16-byte pieces; one whose K stride is the long one is
-// transposed on the way: a thread loads 4 rows x 8 (bf16) or 4 (fp32) consecutive K and interleaves them in registers
-// (v_perm: half an instruction per element), so one LDS image and one inner loop serve every combination.
-// Loads are unaligned-tolerant vectors; only the last chunk of a row or the last rows of a matrix take element loads.
-// Few tiles: the K range is split over workgroups, fp32 partial tiles are joined in a fixed order by a second kernel.
+// All three products are C[n, m] = sum_k A(n, k) B(m, k); what differs is which index of an operand is contiguous in memory.
+// linear64.hip, linear128.hip and linear256.hip are one tiling each, linear_few.hip is for few rows; this file chooses, copies
+// what LDS-DMA cannot fetch as it is (linear_pack_kernel), restores 8-bit codes, computes dz and db, and joins the fp32
+// partial tiles of a K range split over workgroups, in a fixed order.
 #include "linear.hpp"
 #include <stdlib.h>
 
 namespace sphip {
-
-typedef __bf16 lbf16x8 __attribute__((ext_vector_type(8)));
-typedef float lf32x4 __attribute__((ext_vector_type(4)));
-typedef float lf32x16 __attribute__((ext_vector_type(16)));
-
-constexpr int LT = 128;                 // tile rows of either operand
-constexpr int LCH = 8;                  // 16-byte chunks of K per row and step
-
-__device__ __forceinline__ unsigned pack2(bf16_t lo, bf16_t hi) { return (unsigned)lo | ((unsigned)hi << 16); }
 
 template <typename T> struct Chunk;
 template <> struct Chunk<bf16_t> {
@@ -60,213 +46,6 @@ template <> struct Chunk<float> {
     }
 };
 
-__device__ __forceinline__ int chunk_slot(int row, int ch) { return row * LCH + (ch ^ ((row >> 1) & 7)); }
-
-// One operand's 128 x 128-byte step, 4 chunks per thread (256 threads): fetch() into registers, put() into LDS.
-template <typename T, int MODE> struct Stage;
-
-template <typename T> struct Stage<T, OP_ROWS> {
-    static constexpr int E = Chunk<T>::E;
-    uint4 v[4];
-    __device__ __forceinline__ void fetch(const Operand& a, int row0, int64_t k0, int64_t K, int tid) {
-        const int ch = tid & 7, r = tid >> 3;
-        const int64_t k = k0 + ch * E;
-        const int n = (int)min((int64_t)E, K - k);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int row = row0 + r + 32 * i;
-            v[i] = Chunk<T>::load((const T*)a.p + (int64_t)row * a.ld + k, row < a.rows ? n : 0);
-        }
-    }
-    __device__ __forceinline__ void put(uint4* lds, int tid) const {
-        const int ch = tid & 7, r = tid >> 3;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) lds[chunk_slot(r + 32 * i, ch)] = v[i];
-    }
-};
-
-// thread: rows 4 rg .. 4 rg + 3, K chunk kc
-template <> struct Stage<bf16_t, OP_COLS> {
-    uint2 v[8];
-    __device__ __forceinline__ void fetch(const Operand& a, int row0, int64_t k0, int64_t K, int tid) {
-        const int row = row0 + 4 * (tid & 31), n = a.rows - row;
-        const int64_t k = k0 + (tid >> 5) * 8;
-        const bf16_t* p = (const bf16_t*)a.p + k * a.ld + row;
-#pragma unroll
-        for (int i = 0; i < 8; ++i, p += a.ld) {
-            v[i] = make_uint2(0, 0);
-            if (k + i >= K || n <= 0) continue;
-            if (n >= 4) __builtin_memcpy(&v[i], p, 8);
-            else v[i] = make_uint2((unsigned)p[0] | (n > 1 ? (unsigned)p[1] << 16 : 0u), n > 2 ? (unsigned)p[2] : 0u);
-        }
-    }
-    __device__ __forceinline__ void put(uint4* lds, int tid) const {
-        const int r = 4 * (tid & 31), kc = tid >> 5;
-        // dword of row j holding K (2 i, 2 i + 1): the low (j even) or high halves of two K rows' dwords
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            unsigned w[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const unsigned lo = j < 2 ? v[2 * i].x : v[2 * i].y, hi = j < 2 ? v[2 * i + 1].x : v[2 * i + 1].y;
-                w[i] = __builtin_amdgcn_perm(hi, lo, (j & 1) ? 0x07060302u : 0x05040100u);
-            }
-            lds[chunk_slot(r + j, kc)] = make_uint4(w[0], w[1], w[2], w[3]);
-        }
-    }
-};
-template <> struct Stage<float, OP_COLS> {
-    uint4 v[4];
-    __device__ __forceinline__ void fetch(const Operand& a, int row0, int64_t k0, int64_t K, int tid) {
-        const int row = row0 + 4 * (tid & 31);
-        const int64_t k = k0 + (tid >> 5) * 4;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            v[i] = Chunk<float>::load((const float*)a.p + (k + i) * a.ld + row, k + i < K ? a.rows - row : 0);
-    }
-    __device__ __forceinline__ void put(uint4* lds, int tid) const {
-        const int r = 4 * (tid & 31), kc = tid >> 5;
-        lds[chunk_slot(r + 0, kc)] = make_uint4(v[0].x, v[1].x, v[2].x, v[3].x);
-        lds[chunk_slot(r + 1, kc)] = make_uint4(v[0].y, v[1].y, v[2].y, v[3].y);
-        lds[chunk_slot(r + 2, kc)] = make_uint4(v[0].z, v[1].z, v[2].z, v[3].z);
-        lds[chunk_slot(r + 3, kc)] = make_uint4(v[0].w, v[1].w, v[2].w, v[3].w);
-    }
-};
-
-template <typename T, int FMT> struct StageCodes {
-    static constexpr int E = Chunk<T>::E;
-    unsigned v[E], s;
-    // ld is a multiple of 16, the code rows are padded to whole 32-token groups (zeros): whole dwords, no partial pieces
-    __device__ __forceinline__ void fetch(const Operand& a, int row0, int64_t k0, int64_t K, int tid) {
-        const int row = row0 + 4 * (tid & 31);
-        const int64_t k = k0 + (tid >> 5) * E;
-        const bool in = row < a.ld && k < K;
-        const uint8_t* p = (const uint8_t*)a.p + k * a.ld + row;
-        s = in ? *reinterpret_cast<const unsigned*>(a.scales + (k >> 5) * a.ld + row) : 0u;
-#pragma unroll
-        for (int i = 0; i < E; ++i, p += a.ld) v[i] = in ? *reinterpret_cast<const unsigned*>(p) : 0u;
-    }
-    __device__ __forceinline__ void put(uint4* lds, int tid) const {
-        const int r = 4 * (tid & 31), kc = tid >> 5;
-        // bytes transposed 4 x 4: w[h][j] holds K 4 h .. 4 h + 3 of row j
-        unsigned w[E / 4][4];
-#pragma unroll
-        for (int h = 0; h < E / 4; ++h) {
-            const unsigned a0 = __builtin_amdgcn_perm(v[4 * h + 1], v[4 * h], 0x05010400u);
-            const unsigned a1 = __builtin_amdgcn_perm(v[4 * h + 1], v[4 * h], 0x07030602u);
-            const unsigned b0 = __builtin_amdgcn_perm(v[4 * h + 3], v[4 * h + 2], 0x05010400u);
-            const unsigned b1 = __builtin_amdgcn_perm(v[4 * h + 3], v[4 * h + 2], 0x07030602u);
-            w[h][0] = __builtin_amdgcn_perm(b0, a0, 0x05040100u), w[h][1] = __builtin_amdgcn_perm(b0, a0, 0x07060302u);
-            w[h][2] = __builtin_amdgcn_perm(b1, a1, 0x05040100u), w[h][3] = __builtin_amdgcn_perm(b1, a1, 0x07060302u);
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float sj = scale_value((s >> (8 * j)) & 0xffu);
-            uint4 c;
-            float o[4];
-            code_values<FMT>(w[0][j], sj, o);
-            if constexpr (E == 8) {
-                float q[4];
-                code_values<FMT>(w[1][j], sj, q);
-                // (8-bit codes times a power of two are bf16 values: nothing is rounded)
-                c = make_uint4(pack2(f32_to_bf16(o[0]), f32_to_bf16(o[1])), pack2(f32_to_bf16(o[2]), f32_to_bf16(o[3])),
-                               pack2(f32_to_bf16(q[0]), f32_to_bf16(q[1])), pack2(f32_to_bf16(q[2]), f32_to_bf16(q[3])));
-            } else {
-                c = make_uint4(__float_as_uint(o[0]), __float_as_uint(o[1]), __float_as_uint(o[2]), __float_as_uint(o[3]));
-            }
-            lds[chunk_slot(r + j, kc)] = c;
-        }
-    }
-};
-template <typename T> struct Stage<T, OP_COLS_I8> : StageCodes<T, SPHIP_INT8> {};
-template <typename T> struct Stage<T, OP_COLS_E4M3> : StageCodes<T, SPHIP_E4M3> {};
-
-__device__ __forceinline__ void mma_step(const uint4& a, const uint4& b, lf32x16& c, bf16_t) {
-    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(lbf16x8, a), __builtin_bit_cast(lbf16x8, b), c, 0, 0, 0);
-}
-__device__ __forceinline__ void mma_step(const uint4& a, const uint4& b, lf32x16& c, float) {
-    // lane half h holds K 4 h + i of an 8-wide K group for MFMA i; both operands agree, the four together sum all 8
-    const lf32x4 fa = __builtin_bit_cast(lf32x4, a), fb = __builtin_bit_cast(lf32x4, b);
-    c = __builtin_amdgcn_mfma_f32_32x32x2f32(fa[0], fb[0], c, 0, 0, 0);
-    c = __builtin_amdgcn_mfma_f32_32x32x2f32(fa[1], fb[1], c, 0, 0, 0);
-    c = __builtin_amdgcn_mfma_f32_32x32x2f32(fa[2], fb[2], c, 0, 0, 0);
-    c = __builtin_amdgcn_mfma_f32_32x32x2f32(fa[3], fb[3], c, 0, 0, 0);
-}
-
-// B (rows m) is the MFMA's first operand: a lane then holds 4 consecutive m of one n per accumulator quad, i.e. vector
-// stores along a row of C.
-template <typename T, int MODE_A, int MODE_B>
-__global__ __launch_bounds__(256, 2) void linear_tile_kernel(Operand A, Operand B, Epilogue epi, int64_t K, int64_t KB, TileGrid g) {
-    constexpr int E = Chunk<T>::E, STEP = LCH * E;
-    __shared__ uint4 lds[2][2][LT * LCH];       // [buffer][B | A]
-
-    unsigned split;
-    int tm, tn;
-    tile_of(g, split, tm, tn);
-    const int m0 = tm * LT, n0 = tn * LT;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int wm = wave >> 1, wn = wave & 1, r = lane & 31, h = lane >> 5;
-    const int step0 = (int)split * g.steps_per;
-    const int steps = min(g.steps_per, (int)((K + STEP - 1) / STEP) - step0);
-
-    Stage<T, MODE_A> sa;
-    Stage<T, MODE_B> sb;
-    lf32x16 acc[2][2];
-#pragma unroll
-    for (int mi = 0; mi < 2; ++mi)
-#pragma unroll
-        for (int ni = 0; ni < 2; ++ni)
-#pragma unroll
-            for (int j = 0; j < 16; ++j) acc[mi][ni][j] = 0.f;
-
-    sb.fetch(B, m0, (int64_t)step0 * STEP, KB, tid);
-    sa.fetch(A, n0, (int64_t)step0 * STEP, K, tid);
-    sb.put(lds[0][0], tid);
-    sa.put(lds[0][1], tid);
-    __syncthreads();
-    for (int s = 0; s < steps; ++s) {
-        const int buf = s & 1;
-        if (s + 1 < steps) {
-            sb.fetch(B, m0, (int64_t)(step0 + s + 1) * STEP, KB, tid);
-            sa.fetch(A, n0, (int64_t)(step0 + s + 1) * STEP, K, tid);
-        }
-#pragma unroll
-        for (int ks = 0; ks < 4; ++ks) {
-            uint4 fb[2], fa[2];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                fb[i] = lds[buf][0][chunk_slot(wm * 64 + i * 32 + r, 2 * ks + h)];
-                fa[i] = lds[buf][1][chunk_slot(wn * 64 + i * 32 + r, 2 * ks + h)];
-            }
-#pragma unroll
-            for (int mi = 0; mi < 2; ++mi)
-#pragma unroll
-                for (int ni = 0; ni < 2; ++ni) mma_step(fb[mi], fa[ni], acc[mi][ni], T{});
-        }
-        if (s + 1 < steps) {
-            sb.put(lds[buf ^ 1][0], tid);
-            sa.put(lds[buf ^ 1][1], tid);
-        }
-        __syncthreads();
-    }
-
-    // 4 consecutive m of one n per accumulator quad: 32 n x 64 m per wave and pass through its part of the (dead) image
-    const int N = A.rows, M = B.rows;
-    char* const stage = reinterpret_cast<char*>(lds) + wave * 32 * OUT_ROW;
-#pragma unroll
-    for (int ni = 0; ni < 2; ++ni) {
-#pragma unroll
-        for (int mi = 0; mi < 2; ++mi)
-#pragma unroll
-            for (int qd = 0; qd < 4; ++qd)
-                *reinterpret_cast<float4*>(stage + r * OUT_ROW + (mi * 32 + 8 * qd + 4 * h) * 4) =
-                    make_float4(acc[mi][ni][4 * qd], acc[mi][ni][4 * qd + 1], acc[mi][ni][4 * qd + 2], acc[mi][ni][4 * qd + 3]);
-        Residual<32> res;
-        res.load(epi, g, n0 + wn * 64 + ni * 32, m0 + wm * 64, N, M, lane);
-        finish_rows<32>(stage, epi, g, split, n0 + wn * 64 + ni * 32, m0 + wm * 64, N, M, lane, res);
-    }
-}
-
 // Sum of the splits' partial tiles, then the epilogue. One thread per 4 outputs, the splits in order; with many splits of a
 // small product 8 threads share an output, each taking every eighth split (LANES = 8), their sums added in order.
 template <int LANES>
@@ -297,30 +76,20 @@ __global__ __launch_bounds__(256) void linear_join_kernel(const float* __restric
     if (i < total) epilogue4(epi, i / quads, (int)(i % quads) * 4, M, v);
 }
 
-// How many ways the K range of an (N, M) product of `steps` K steps is split: none when the tiles fill the 256 compute
-// units once, else towards two workgroups per unit, at least 4 steps each.
-static int split_count(int64_t N, int64_t M, int64_t steps) {
-    const int64_t tiles = cdiv(N, LT) * cdiv(M, LT);
-    if (tiles >= 256) return 1;
-    int64_t s = cdiv(512, tiles);
-    if (s > steps / 4) s = steps / 4;
-    return s < 1 ? 1 : (int)s;
-}
 static size_t part_bytes(int64_t N, int64_t M, int splits) {
     return splits > 1 ? (size_t)splits * N * ((M + 3) / 4 * 4) * 4 : 0;
 }
-// SPHIP_LINEAR=tile|64|128|256|few forces a kernel (tests, A/B runs); read once per entry point
+// SPHIP_LINEAR=64|128|256|few forces a kernel (tests, A/B runs); read once per entry point
 static thread_local char g_forced = 0;
 static void read_forced() {
     const char* e = getenv("SPHIP_LINEAR");
     g_forced = e ? e[0] : 0;
 }
 
-// Which kernel a product of these sizes goes to if its operands are such that LDS-DMA can fetch them.
-enum { BY_TILES = 0, BY_64 = 1, BY_128 = 2, BY_256 = 3 };
+// which kernel a product of these sizes goes to
+enum { BY_64 = 1, BY_128 = 2, BY_256 = 3 };
 static int splits_of(int dtype, int by, int64_t N, int64_t M, int64_t K) {
-    return by == BY_256 ? 1 : by == BY_128 ? linear128_splits(dtype, N, M, K) : by == BY_64 ? linear64_splits(dtype, N, M, K)
-         : split_count(N, M, cdiv(K, 128 / (int64_t)dtype_size(dtype)));
+    return by == BY_256 ? 1 : by == BY_128 ? linear128_splits(dtype, N, M, K) : linear64_splits(dtype, N, M, K);
 }
 // Time of a product with 64 x 64 or 128 x 128 tiles in ns, without what both take: K steps one after the other, a step of one
 // workgroup `step` (measured: 64 x 64 200 bf16, 520 fp32; 128 x 128 570 and 2100 alone on its compute unit, 400 and 1950 where
@@ -333,7 +102,8 @@ static int64_t product_ns(int dtype, int by, int64_t N, int64_t M, int64_t K) {
     return steps * step * cdiv(groups, 256) + (splits > 1 ? 4000 + splits * N * M / 375 : 0);
 }
 static int kernel_for(int dtype, int64_t N, int64_t M, int64_t K) {
-    if (g_forced) return g_forced == '2' && dtype == SPHIP_BF16 ? BY_256 : g_forced == '1' || g_forced == '2' ? BY_128 : g_forced == '6' ? BY_64 : BY_TILES;
+    if (g_forced == '6') return BY_64;
+    if (g_forced == '1' || g_forced == '2') return g_forced == '2' && dtype == SPHIP_BF16 ? BY_256 : BY_128;
     // The 256 x 256 kernel where its tiles fill most of the 256 compute units once: 16384 x 1024 x 4096 takes 101 us against
     // 118 with 128 x 128 tiles, 8192 x 2048 x 2048 56 against 68; with fewer the smaller tiles win (2048^3 22 against 37).
     if (dtype == SPHIP_BF16 && cdiv(N, 256) * cdiv(M, 256) >= 160) return BY_256;
@@ -342,11 +112,10 @@ static int kernel_for(int dtype, int64_t N, int64_t M, int64_t K) {
     return product_ns(dtype, BY_64, N, M, K) <= product_ns(dtype, BY_128, N, M, K) ? BY_64 : BY_128;
 }
 
-// the most a product needs for its partial tiles, whichever kernel takes it
+// what a product needs for its partial tiles
 static size_t split_bytes(int dtype, int64_t N, int64_t M, int64_t K) {
     const int64_t Kp = cdiv(K, 64) * 64;
-    const size_t a = part_bytes(N, M, splits_of(dtype, BY_TILES, N, M, Kp)), b = part_bytes(N, M, splits_of(dtype, kernel_for(dtype, N, M, Kp), N, M, Kp));
-    return a > b ? a : b;
+    return part_bytes(N, M, splits_of(dtype, kernel_for(dtype, N, M, Kp), N, M, Kp));
 }
 
 template <typename T, int MODE_A, int MODE_B>
@@ -354,15 +123,9 @@ static int launch_product(const char* what, const Operand& A, const Operand& B, 
                           void* ws, size_t ws_bytes, hipStream_t s) {
     const int64_t N = A.rows, M = B.rows;
     constexpr int dtype = sizeof(T) == 2 ? SPHIP_BF16 : SPHIP_F32;
-    int by = BY_TILES;
-    if (MODE_B <= OP_COLS) {
-        by = kernel_for(dtype, N, M, cdiv(K, 64) * 64);
-        if (by == BY_256 && !linear256_takes(MODE_A, MODE_B, A, B, K)) by = BY_TILES;
-        if (by == BY_128 && !linear128_takes(dtype, MODE_A, MODE_B, A, B, K)) by = BY_TILES;
-        if (by == BY_64 && !linear64_takes(dtype, MODE_A, MODE_B, A, B, K)) by = BY_TILES;
-    }
+    const int by = kernel_for(dtype, N, M, cdiv(K, 64) * 64);
     const int tile = by == BY_256 ? 256 : by == BY_64 ? 64 : 128;
-    const int64_t steps = cdiv(K, LCH * Chunk<T>::E);
+    const int64_t steps = cdiv(K, 128 / (int64_t)sizeof(T));
     TileGrid g;
     g.tilesM = (int)cdiv(M, tile), g.tilesN = (int)cdiv(N, tile);
     const int want = splits_of(dtype, by, N, M, cdiv(K, 64) * 64);
@@ -377,15 +140,10 @@ static int launch_product(const char* what, const Operand& A, const Operand& B, 
     const int64_t nblocks = (int64_t)g.tilesM * g.tilesN * g.splits, threads = N * ((M + 3) / 4);
     SPHIP_REQUIRE(nblocks < (1ll << 31) && (g.splits == 1 || cdiv(threads, 256) < (1ll << 31)), SPHIP_EUNSUPPORTED,
                   "%s: grid too large", what);
-    if (by != BY_TILES) {
-        const int st = by == BY_256 ? launch_linear256(what, MODE_A, MODE_B, A, B, epi, K, KB, g, s)
-                     : by == BY_128 ? launch_linear128(what, dtype, MODE_A, MODE_B, A, B, epi, K, KB, g, s)
-                                    : launch_linear64(what, dtype, MODE_A, MODE_B, A, B, epi, K, KB, g, s);
-        if (st != SPHIP_OK) return st;
-    } else {
-        hipLaunchKernelGGL((linear_tile_kernel<T, MODE_A, MODE_B>), dim3((unsigned)nblocks), dim3(256), 0, s, A, B, epi, K, KB, g);
-        SPHIP_CHECK_LAUNCH(what);
-    }
+    const int st = by == BY_256 ? launch_linear256(what, MODE_A, MODE_B, A, B, epi, K, KB, g, s)
+                 : by == BY_128 ? launch_linear128(what, dtype, MODE_A, MODE_B, A, B, epi, K, KB, g, s)
+                                : launch_linear64(what, dtype, MODE_A, MODE_B, A, B, epi, K, KB, g, s);
+    if (st != SPHIP_OK) return st;
     if (g.splits > 1) {
         if (g.splits > 8 && threads < (1 << 17))
             hipLaunchKernelGGL(linear_join_kernel<8>, dim3((unsigned)cdiv(threads, 32)), dim3(256), 0, s, g.part, epi, N, (int)M, g.splits);
@@ -396,25 +154,28 @@ static int launch_product(const char* what, const Operand& A, const Operand& B, 
     return SPHIP_OK;
 }
 
-// Rows copied to a stride that is a multiple of 64 elements, zeros behind them: what LDS-DMA asks of an operand. Up to two
-// matrices in one launch.
+// Rows copied to a stride that is a multiple of 64 elements, zeros behind them: for operands that LDS-DMA cannot fetch as they
+// are (fetchable(); products of K from D or M also need rows that are whole 16-byte pieces). Up to three matrices in one
+// launch.
 struct PackArgs {
-    const void* src[2];
-    void* dst[2];
-    int64_t ld[2], n[2];                   // n: 16-byte pieces of the copy
-    int cols[2], pieces[2];                // pieces per row
+    const void* src[3];
+    void* dst[3];
+    int64_t ld[3], n[3];                   // n: 16-byte pieces of the copy
+    int cols[3], pieces[3];                // pieces per row
 };
 template <typename T> __global__ __launch_bounds__(256) void linear_pack_kernel(PackArgs a) {
     constexpr int E = Chunk<T>::E;
     int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int w = i >= a.n[0];
-    if (w) i -= a.n[0];
+    int w = 0;
+    if (i >= a.n[0]) i -= a.n[0], w = 1;
+    if (w == 1 && i >= a.n[1]) i -= a.n[1], w = 2;
     if (i >= a.n[w]) return;
     const int64_t row = i / a.pieces[w];
     const int c = (int)(i - row * a.pieces[w]) * E;
     *reinterpret_cast<uint4*>((T*)a.dst[w] + i * E) = Chunk<T>::load((const T*)a.src[w] + row * a.ld[w] + c, a.cols[w] - c);
 }
 static int64_t packed_ld(int64_t cols) { return cdiv(cols, 64) * 64; }
+static int64_t whole_pieces(int dtype, int64_t cols) { const int64_t e = 16 / (int64_t)dtype_size(dtype); return cdiv(cols, e) * e; }
 struct Packing {
     PackArgs a = {};
     int count = 0, dtype;
@@ -428,7 +189,7 @@ struct Packing {
     }
     int launch(const char* what, hipStream_t s) {
         if (count == 0) return SPHIP_OK;
-        const int64_t blocks = cdiv(a.n[0] + a.n[1], 256);
+        const int64_t blocks = cdiv(a.n[0] + a.n[1] + a.n[2], 256);
         SPHIP_REQUIRE(blocks < (1ll << 31), SPHIP_EUNSUPPORTED, "%s: grid too large", what);
         if (dtype == SPHIP_BF16) hipLaunchKernelGGL(linear_pack_kernel<bf16_t>, dim3((unsigned)blocks), dim3(256), 0, s, a);
         else hipLaunchKernelGGL(linear_pack_kernel<float>, dim3((unsigned)blocks), dim3(256), 0, s, a);
@@ -436,10 +197,6 @@ struct Packing {
         return SPHIP_OK;
     }
 };
-// Whether a product is worth a launch that copies an operand whose rows LDS-DMA cannot fetch (they do not start at multiples
-// of 16 bytes, or K is no whole number of steps) or restores 8-bit codes, against the tile kernel that takes anything:
-// 300^3 8.1 us against 14.5, 5000 x 333 x 333 12.7 against 16.4.
-static bool worth_packing(int64_t N, int64_t M, int64_t K) { return g_forced ? g_forced != 't' : N * M * K >= (1ll << 24); }
 static bool unaligned(int dtype, int64_t cols) { return cols * (int64_t)dtype_size(dtype) % 16 != 0; }
 
 // ---- dz = g act'(z) and its column sums. A workgroup takes 32 rows (the group one scale of an 8-bit z covers) of 32 x 16
@@ -583,8 +340,9 @@ using namespace sphip;
 #define SPHIP_LINEAR_SIZES(what)                                                                                        \
     SPHIP_REQUIRE(N > 0 && D > 0 && M > 0, SPHIP_EINVAL, what ": empty shape N=%lld D=%lld M=%lld", (long long)N,        \
                   (long long)D, (long long)M);                                                                          \
-    SPHIP_REQUIRE(N < (1ll << 31) - 256 && D < (1ll << 31) - 256 && M < (1ll << 31) - 256, SPHIP_EUNSUPPORTED,           \
-                  what ": dimension exceeds int32")
+    SPHIP_REQUIRE(N < (1ll << 31) - 256 && D < MAX_LD - 64 && M < MAX_LD - 64, SPHIP_EUNSUPPORTED,                       \
+                  what ": N=%lld D=%lld M=%lld: a dimension exceeds int32 (N) or 2^22 features", (long long)N, (long long)D,     \
+                  (long long)M)
 
 static bool is_codes(int kind) { return kind == SPHIP_INT8 || kind == SPHIP_E4M3; }
 static bool codes_ok(const void* codes, const void* scales, int64_t ld, int64_t cols) {
@@ -592,33 +350,44 @@ static bool codes_ok(const void* codes, const void* scales, int64_t ld, int64_t 
 }
 static size_t up256(size_t b) { return (b + 255) / 256 * 256; }
 
-// workspace: partial tiles | z in fp32 on its way into 8 bits | x and W packed (rows that are no whole number of K steps)
+// workspace: partial tiles | z in fp32 on its way into 8 bits | x and W packed (rows that are no whole number of 16 bytes)
 struct ForwardSpace {
     size_t part, z, pack, total;
+    int copies;
+    bool one;
 };
-// Whether the forward product takes linear_few.hip. Its workgroups read x through the caches once each and share K among 8
-// waves only; the tile kernels stage x and split K further. bf16, us here / with 128 x 128 tiles: 1 x 4096 x 4096 7.2 / 10.4,
-// 16 x 4096 x 4096 9.7 / 11.1, 40 x 333 x 777 7.0 / 9.9, but 64 x 4096 x 4096 20 / 14 and 16 x 8192 x 256 16 / 7. fp32 (whose
-// tiles take 42 us at 1 x 4096 x 4096, here 12): but for a long K with few rows of W (16 x 8192 x 256 30 / 17).
-static bool few(int dtype, int64_t N, int64_t D, int64_t M) {
+// Whether the forward product takes linear_few.hip: one launch, no copies, but its workgroups read all of x each and share K
+// among 8 waves only. us here / with 64 x 64 tiles: bf16 1 x 4096 x 4096 6.9 / 8.8, 16 x 4096 x 4096 9.5 / 9.2,
+// 16 x 8192 x 256 16 / 7, 64 x 4096 x 4096 20 / 11; fp32 16 x 4096 x 4096 17 / 24, 64 x 2048 x 2048 21 / 12. With more rows
+// only where the tiles would need a copy of operands that are small: 40 x 333 x 777 7.0 / 8.3, in fp32 5.7 / 13.6.
+static bool few(int64_t N, int64_t D, int64_t M, int copies) {
     if (N > FEW || (g_forced && g_forced != 'f')) return false;
-    if (g_forced || dtype != SPHIP_BF16) return g_forced || D <= 4096 || M >= 2048;
-    return cdiv(N, 16) * 16 * D <= 65536 || (N <= 16 && M >= 4096);
+    if (g_forced) return true;
+    if (N <= 16) return D <= 4096 || M >= 4096;
+    return D <= 1024 && copies;
 }
-static ForwardSpace forward_space(int dtype, int z_kind, int64_t N, int64_t D, int64_t M) {
+// Which of the operands have to be copied, for a query and for a launch alike; `odd`: bits of those that are not fetchable().
+// Where the rows of x are no whole 16-byte pieces, what follows a row would be multiplied with what follows one of W: both.
+enum { COPY_X = 1, COPY_W = 2 };
+static int odd_rows(const void* x, int64_t ldx, const void* W, int64_t ldw, int dtype) {
+    return (x && !fetchable(x, ldx, (int)dtype_size(dtype)) ? COPY_X : 0) | (W && !fetchable(W, ldw, (int)dtype_size(dtype)) ? COPY_W : 0);
+}
+static ForwardSpace forward_space(int dtype, int z_kind, int64_t N, int64_t D, int64_t M, int odd) {
     ForwardSpace f;
-    const bool one = few(dtype, N, D, M);
+    f.copies = unaligned(dtype, D) ? COPY_X | COPY_W : odd & (COPY_X | COPY_W);
+    f.one = few(N, D, M, f.copies);
+    const bool one = f.one;
+    if (one) f.copies = 0;
     f.part = one ? 0 : up256(split_bytes(dtype, N, M, D));
     f.z = is_codes(z_kind) && (f.part || one) ? up256((size_t)N * (cdiv(M, 4) * 4) * 4) : 0;      // (no codes from a split K range or from few rows)
-    f.pack = !one && D * (int64_t)dtype_size(dtype) % 128 != 0 && worth_packing(N, M, D)
-                 ? (size_t)(N + M) * packed_ld(D) * dtype_size(dtype) : 0;
+    f.pack = (size_t)((f.copies & COPY_X ? N : 0) + (f.copies & COPY_W ? M : 0)) * packed_ld(D) * dtype_size(dtype);
     f.total = f.part + f.z + f.pack;
     return f;
 }
-extern "C" size_t sphip_linear_workspace_bytes(int dtype, int z_kind, int64_t N, int64_t D, int64_t M) {
+extern "C" size_t sphip_linear_workspace_bytes(int dtype, int z_kind, int64_t N, int64_t D, int64_t M, int odd) {
     if (N <= 0 || D <= 0 || M <= 0 || !valid_dtype(dtype)) return 0;
     read_forced();
-    return forward_space(dtype, z_kind, N, D, M).total;
+    return forward_space(dtype, z_kind, N, D, M, odd).total;
 }
 
 extern "C" int sphip_linear(const void* x, int64_t ldx, const void* W, int64_t ldw, int dtype, const void* bias,
@@ -642,7 +411,7 @@ extern "C" int sphip_linear(const void* x, int64_t ldx, const void* W, int64_t l
     SPHIP_REQUIRE((!zc || codes_ok(z, z_scales, ldz, M)) && (!x_codes || codes_ok(x_codes, x_scales, ldq, D)), SPHIP_EINVAL,
                   "linear: codes and scales need 16-byte aligned rows of at least their columns");
     read_forced();
-    const ForwardSpace f = forward_space(dtype, zc ? z_kind : SPHIP_F32, N, D, M);
+    const ForwardSpace f = forward_space(dtype, zc ? z_kind : SPHIP_F32, N, D, M, odd_rows(x, ldx, W, ldw, dtype));
     SPHIP_REQUIRE(f.total == 0 || (ws && ((uintptr_t)ws & 15) == 0 && ws_bytes >= f.total), SPHIP_EWORKSPACE,
                   "linear: workspace of %zu bytes, needs %zu, 16-byte aligned", ws_bytes, f.total);
     hipStream_t s = (hipStream_t)stream;
@@ -653,26 +422,22 @@ extern "C" int sphip_linear(const void* x, int64_t ldx, const void* W, int64_t l
     // which has no groups of rows (nor has the kernel for few rows), and z takes the way over fp32
     if (zc && f.z) e.z = (char*)ws + f.part, e.z_dt = SPHIP_F32, e.ldz = cdiv(M, 4) * 4;
     else e.z = z, e.z_dt = z_kind, e.ldz = ldz, e.z_scales = zc ? z_scales : nullptr;
-    Operand A = {x, nullptr, ldx, (int)N}, B = {W, nullptr, ldw, (int)M};
-    int64_t K = D;
+    Operand A = {x, ldx, (int)N}, B = {W, ldw, (int)M};
+    const int64_t K = f.copies ? whole_pieces(dtype, D) : D, ld = packed_ld(D);
+    char* to = (char*)ws + f.part + f.z;
     int st = SPHIP_OK;
-    if (f.pack) {
-        K = packed_ld(D);
-        char* to = (char*)ws + f.part + f.z;
-        Packing p(dtype);
-        if (x_codes) {                                          // x is read once for both
-            st = save_codes("linear", x, dtype, ldx, x_fmt, 0, x_codes, x_scales, ldq, to, K, N, D, s);
-            A.p = to, A.ld = K;
-        } else {
-            p.add(A, N, D, to);
-        }
-        p.add(B, M, D, to + (size_t)N * K * dtype_size(dtype));
-        if (st == SPHIP_OK) st = p.launch("linear", s);
-    } else if (x_codes) {
-        st = save_codes("linear", x, dtype, ldx, x_fmt, 0, x_codes, x_scales, ldq, nullptr, 0, N, D, s);
+    Packing p(dtype);
+    if (x_codes) {                                              // x is read once for its codes and its copy
+        const bool copy = f.copies & COPY_X;
+        st = save_codes("linear", x, dtype, ldx, x_fmt, 0, x_codes, x_scales, ldq, copy ? to : nullptr, copy ? ld : 0, N, D, s);
+        if (copy) A.p = to, A.ld = ld;
+    } else if (f.copies & COPY_X) {
+        p.add(A, N, D, to);
     }
+    if (f.copies & COPY_W) p.add(B, M, D, to + (f.copies & COPY_X ? (size_t)N * ld * dtype_size(dtype) : 0));
+    if (st == SPHIP_OK) st = p.launch("linear", s);
     if (st != SPHIP_OK) return st;
-    st = few(dtype, N, D, M) ? launch_linear_few("linear", dtype, A, B, e, K, s)
+    st = f.one ? launch_linear_few("linear", dtype, A, B, e, K, s)
          : dtype == SPHIP_BF16 ? launch_product<bf16_t, OP_ROWS, OP_ROWS>("linear", A, B, e, K, K, ws, f.part, s)
                                : launch_product<float, OP_ROWS, OP_ROWS>("linear", A, B, e, K, K, ws, f.part, s);
     if (st == SPHIP_OK && zc && f.z)
@@ -680,20 +445,19 @@ extern "C" int sphip_linear(const void* x, int64_t ldx, const void* W, int64_t l
     return st;
 }
 
-// workspace: dz | column sums of 32-row groups | x as aligned bf16 rows (restored from codes, or packed) | W packed | partial
-// tiles of a product
+// workspace: dz | column sums of 32-row groups | x as aligned rows (restored from codes, or packed) | W packed | partial tiles
+// of a product
 struct BackwardSpace {
     size_t dz, sums, x, w, part, total;
 };
-static BackwardSpace backward_space(int dtype, int x_kind, int want_dx, int want_dw, int want_db, int64_t N, int64_t D, int64_t M) {
+static BackwardSpace backward_space(int dtype, int x_kind, int want_dx, int want_dw, int want_db, int64_t N, int64_t D, int64_t M,
+                                    int odd) {
     BackwardSpace b;
     const size_t es = dtype_size(dtype);
-    const bool odd = unaligned(dtype, D);
     b.dz = want_dx || want_dw ? up256((size_t)N * packed_ld(M) * es) : 0;
     b.sums = want_db ? up256((size_t)cdiv(N, 32) * M * 4) : 0;
-    b.x = want_dw && (is_codes(x_kind) || odd) && worth_packing(M, D, N)
-              ? up256((size_t)N * packed_ld(D) * es) : 0;
-    b.w = want_dx && odd && worth_packing(N, D, M) ? up256((size_t)M * packed_ld(D) * es) : 0;
+    b.x = want_dw && (is_codes(x_kind) || (odd & COPY_X)) ? up256((size_t)N * packed_ld(D) * es) : 0;
+    b.w = want_dx && (odd & COPY_W) ? up256((size_t)M * packed_ld(D) * es) : 0;
     const size_t p1 = want_dx ? split_bytes(dtype, N, D, M) : 0, p2 = want_dw ? split_bytes(dtype, M, D, N) : 0;
     b.part = p1 > p2 ? p1 : p2;
     b.total = b.dz + b.sums + b.x + b.w + b.part;
@@ -701,48 +465,10 @@ static BackwardSpace backward_space(int dtype, int x_kind, int want_dx, int want
 }
 
 extern "C" size_t sphip_linear_backward_workspace_bytes(int dtype, int x_kind, int want_dx, int want_dw, int want_db, int64_t N,
-                                                        int64_t D, int64_t M) {
+                                                        int64_t D, int64_t M, int odd) {
     if (N <= 0 || D <= 0 || M <= 0 || !valid_dtype(dtype)) return 0;
     read_forced();
-    return backward_space(dtype, x_kind, want_dx, want_dw, want_db, N, D, M).total;
-}
-
-template <typename T>
-static int backward_products(const Operand& dz, const void* W, int64_t ldw, const void* x, int x_kind, const uint8_t* x_scales,
-                             int64_t ldx, void* dx, int dx_dtype, int64_t lddx, void* dW, int dw_dtype, int64_t lddw, int64_t N,
-                             int64_t D, int64_t M, bool padded, char* ws, const BackwardSpace& sp, hipStream_t s) {
-    char *xs = ws + sp.dz + sp.sums, *part = xs + sp.x + sp.w;
-    if (dx) {
-        const char* what = "linear_backward(dx)";
-        Epilogue e;
-        e.out = dx, e.out_dt = dx_dtype, e.ldo = lddx;
-            const Operand A = {dz.p, nullptr, dz.ld, (int)N}, B = {W, nullptr, ldw, (int)D};
-        const int st = launch_product<T, OP_ROWS, OP_COLS>(what, A, B, e, padded ? dz.ld : M, M, part, sp.part, s);
-        if (st != SPHIP_OK) return st;
-    }
-    if (!dW) return SPHIP_OK;
-    const char* what = "linear_backward(dW)";
-    Epilogue e;
-    e.out = dW, e.out_dt = dw_dtype, e.ldo = lddw;
-    const Operand A = {dz.p, nullptr, dz.ld, (int)M};
-    Operand B = {x, x_scales, ldx, (int)D};
-    if (sp.x) {
-        int st;
-        if (is_codes(x_kind)) {
-            const int64_t ld = packed_ld(D);
-            constexpr int dtype = sizeof(T) == 2 ? SPHIP_BF16 : SPHIP_F32;
-            st = sphip_checkpoint8_restore((const uint8_t*)x, x_scales, ldx, x_kind, xs, dtype, ld, N, D, s);
-            B.p = xs, B.ld = ld, x_kind = dtype;
-        } else {
-            Packing p(sizeof(T) == 2 ? SPHIP_BF16 : SPHIP_F32);
-            p.add(B, N, D, xs);
-            st = p.launch(what, s);
-        }
-        if (st != SPHIP_OK) return st;
-    }
-    if (x_kind == SPHIP_INT8) return launch_product<T, OP_COLS, OP_COLS_I8>(what, A, B, e, N, N, part, sp.part, s);
-    if (x_kind == SPHIP_E4M3) return launch_product<T, OP_COLS, OP_COLS_E4M3>(what, A, B, e, N, N, part, sp.part, s);
-    return launch_product<T, OP_COLS, OP_COLS>(what, A, B, e, N, N, part, sp.part, s);
+    return backward_space(dtype, x_kind, want_dx, want_dw, want_db, N, D, M, odd).total;
 }
 
 extern "C" int sphip_linear_backward(const void* g, int g_dtype, int64_t ldg, const void* W, int64_t ldw, int dtype, int act,
@@ -770,7 +496,8 @@ extern "C" int sphip_linear_backward(const void* g, int g_dtype, int64_t ldg, co
                       (act == SPHIP_ACT_NONE || zc || aligned_elem(z, z_kind)),
                   SPHIP_EINVAL, "linear_backward: a pointer is not aligned to its element");
     read_forced();
-    const BackwardSpace sp = backward_space(dtype, x_kind, dx != nullptr, dW != nullptr, db != nullptr, N, D, M);
+    const BackwardSpace sp = backward_space(dtype, x_kind, dx != nullptr, dW != nullptr, db != nullptr, N, D, M,
+                                            odd_rows(xc || !dW ? nullptr : x, ldx, dx ? W : nullptr, ldw, dtype));
     SPHIP_REQUIRE(sp.total == 0 || (ws && ((uintptr_t)ws & 15) == 0 && ws_bytes >= sp.total), SPHIP_EWORKSPACE,
                   "linear_backward: workspace of %zu bytes, needs %zu, 16-byte aligned", ws_bytes, sp.total);
     hipStream_t s = (hipStream_t)stream;
@@ -779,29 +506,22 @@ extern "C" int sphip_linear_backward(const void* g, int g_dtype, int64_t ldg, co
     // Without an activation the incoming gradient is dz. It is copied (into the product's dtype, rows padded to 64) only
     // where it does not have that dtype, or where LDS-DMA could not fetch it as it is.
     const bool products = dx || dW;
-    bool direct = act == SPHIP_ACT_NONE && g_dtype == dtype;
-    if (direct && (M * (int64_t)dtype_size(dtype) % 128 != 0 || unaligned(dtype, ldg) || ((uintptr_t)g & 15) != 0))
-        direct = !((dx && worth_packing(N, D, M)) || (dW && worth_packing(M, D, N)));
-    Operand dz = {g, nullptr, ldg, (int)N};
-    if (products && !direct) dz.p = w, dz.ld = packed_ld(M);
+    const bool direct = act == SPHIP_ACT_NONE && g_dtype == dtype && fetchable(g, ldg, (int)dtype_size(dtype)) && !(dx && unaligned(dtype, M));
+    Operand dz = {g, ldg, (int)N}, ow = {W, ldw, (int)D}, ox = {x, ldx, (int)D};
     Packing pack(dtype);
-    if (sp.w) {
-        Operand o = {W, nullptr, ldw, (int)M};
-        pack.add(o, M, D, w + sp.dz + sp.sums + sp.x);
-        W = o.p, ldw = o.ld;
-    }
     const bool copied = products && !direct && !db && act == SPHIP_ACT_NONE && g_dtype == dtype;
-    if (copied) {                                               // g with padded rows is all there is to do
-        Operand o = {g, nullptr, ldg, (int)N};
-        pack.add(o, N, M, w);
-    }
-    const int pst = pack.launch("linear_backward", s);
-    if (pst != SPHIP_OK) return pst;
+    if (copied) pack.add(dz, N, M, w);                          // g with padded rows is all there is to do
+    else if (products && !direct) dz.p = w, dz.ld = packed_ld(M);
+    char *const xs = w + sp.dz + sp.sums, *const part = xs + sp.x + sp.w;
+    if (sp.w) pack.add(ow, M, D, xs + sp.x);
+    if (sp.x && !xc) pack.add(ox, N, D, xs);
+    int st = pack.launch("linear_backward", s);
+    if (st != SPHIP_OK) return st;
     if (!copied && (db || (products && !direct))) {
         PreactArgs a;
         a.g = g, a.z = z, a.scales = z_scales, a.dz = products && !direct ? w : nullptr, a.part = db ? sums : nullptr;
         a.ldg = ldg, a.ldz = ldz, a.lddz = dz.ld, a.dz_dt = dtype, a.act = act;
-        const int st = g_dtype == SPHIP_BF16 ? launch_preact<bf16_t>(a, z_kind, N, M, s) : launch_preact<float>(a, z_kind, N, M, s);
+        st = g_dtype == SPHIP_BF16 ? launch_preact<bf16_t>(a, z_kind, N, M, s) : launch_preact<float>(a, z_kind, N, M, s);
         if (st != SPHIP_OK) return st;
         if (db) {
             hipLaunchKernelGGL(linear_bias_grad_kernel, dim3((unsigned)cdiv(M, 64)), dim3(1024), 0, s, (const float*)sums,
@@ -809,10 +529,24 @@ extern "C" int sphip_linear_backward(const void* g, int g_dtype, int64_t ldg, co
             SPHIP_CHECK_LAUNCH("linear_backward(db)");
         }
     }
-    if (!products) return SPHIP_OK;
-    if (dtype == SPHIP_BF16)
-        return backward_products<bf16_t>(dz, W, ldw, x, x_kind, x_scales, ldx, dx, dx_dtype, lddx, dW, dw_dtype, lddw, N, D, M,
-                                         !direct, w, sp, s);
-    return backward_products<float>(dz, W, ldw, x, x_kind, x_scales, ldx, dx, dx_dtype, lddx, dW, dw_dtype, lddw, N, D, M, !direct,
-                                    w, sp, s);
+    Epilogue e;
+    if (dx) {
+        e.out = dx, e.out_dt = dx_dtype, e.ldo = lddx;
+        const int64_t K = direct ? M : whole_pieces(dtype, M);  // (dz is padded with zeros)
+        st = dtype == SPHIP_BF16 ? launch_product<bf16_t, OP_ROWS, OP_COLS>("linear_backward(dx)", dz, ow, e, K, M, part, sp.part, s)
+                                 : launch_product<float, OP_ROWS, OP_COLS>("linear_backward(dx)", dz, ow, e, K, M, part, sp.part, s);
+        if (st != SPHIP_OK) return st;
+    }
+    if (dW) {
+        if (xc) {
+            ox.p = xs, ox.ld = packed_ld(D);
+            st = sphip_checkpoint8_restore((const uint8_t*)x, x_scales, ldx, x_kind, xs, dtype, ox.ld, N, D, s);
+            if (st != SPHIP_OK) return st;
+        }
+        e.out = dW, e.out_dt = dw_dtype, e.ldo = lddw;
+        dz.rows = (int)M;
+        st = dtype == SPHIP_BF16 ? launch_product<bf16_t, OP_COLS, OP_COLS>("linear_backward(dW)", dz, ox, e, N, N, part, sp.part, s)
+                                 : launch_product<float, OP_COLS, OP_COLS>("linear_backward(dW)", dz, ox, e, N, N, part, sp.part, s);
+    }
+    return st;
 }

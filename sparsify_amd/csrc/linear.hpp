@@ -7,16 +7,18 @@ namespace sphip {
 
 // how element (row, k) of an operand of C[n, m] = sum_k A(n, k) B(m, k) is found
 enum { OP_ROWS = 0,      // p[row * ld + k]
-       OP_COLS = 1,      // p[k * ld + row]
-       OP_COLS_I8 = 2,   // 8-bit codes at p[k * ld + row], scale byte at scales[(k / 32) * ld + row] (checkpoint8.hip)
-       OP_COLS_E4M3 = 3 };
+       OP_COLS = 1 };    // p[k * ld + row]
 
 struct Operand {
     const void* p;
-    const uint8_t* scales;
     int64_t ld;
     int rows;
 };
+
+// Whether LDS-DMA can fetch an operand's rows of es-byte elements where they are: from multiples of 16 bytes, with offsets that
+// fit a tile's buffer descriptor (2^31 bytes: 256 rows of bf16, 128 of fp32). Others are copied first.
+constexpr int64_t MAX_LD = 1ll << 22;
+static inline bool fetchable(const void* p, int64_t ld, int es) { return ((uintptr_t)p & 15) == 0 && ld * es % 16 == 0 && ld < MAX_LD; }
 
 // hipFuncAttributeMaxDynamicSharedMemorySize of a kernel, set once per device (`done`: a bit per device, one word a kernel)
 static inline bool reserve_lds(const void* kernel, int bytes, uint64_t& done) {
@@ -236,16 +238,14 @@ int save_codes(const char* what, const void* x, int dtype, int64_t ldx, int fmt,
 constexpr int FEW = 64;
 int launch_linear_few(const char* what, int dtype, const Operand& X, const Operand& W, const Epilogue& epi, int64_t K, hipStream_t s);
 
-// The LDS-DMA kernels (256: bf16 only): whether they take these operands, how they split K, their launch (the caller joins).
-// KB: rows of an OP_COLS B, which may be fewer than K (whole 128-byte steps where A is OP_ROWS): B counts as zero from there.
-bool linear256_takes(int mode_a, int mode_b, const Operand& A, const Operand& B, int64_t K);
+// The tiled kernels (256: bf16 only): how they split K, their launch (the caller joins). Operands: fetchable(), and K whole
+// 16-byte pieces where it is the contiguous index.
+// KB: rows of an OP_COLS B, which may be fewer than K (whole 16-byte pieces where A is OP_ROWS): B counts as zero from there.
 int launch_linear256(const char* what, int mode_a, int mode_b, const Operand& A, const Operand& B, const Epilogue& epi, int64_t K,
                      int64_t KB, const TileGrid& g, hipStream_t s);
-bool linear64_takes(int dtype, int mode_a, int mode_b, const Operand& A, const Operand& B, int64_t K);
 int linear64_splits(int dtype, int64_t N, int64_t M, int64_t K);
 int launch_linear64(const char* what, int dtype, int mode_a, int mode_b, const Operand& A, const Operand& B, const Epilogue& epi,
                     int64_t K, int64_t KB, const TileGrid& g, hipStream_t s);
-bool linear128_takes(int dtype, int mode_a, int mode_b, const Operand& A, const Operand& B, int64_t K);
 int linear128_splits(int dtype, int64_t N, int64_t M, int64_t K);
 int launch_linear128(const char* what, int dtype, int mode_a, int mode_b, const Operand& A, const Operand& B, const Epilogue& epi,
                      int64_t K, int64_t KB, const TileGrid& g, hipStream_t s);

@@ -34,6 +34,7 @@ __global__ __launch_bounds__(256, STAGES == 2 ? 2 : 1) void linear128_kernel(Ope
     sb.init(B, m0, k0, KB, tid);
     auto fetch = [&](int t, unsigned image) {      // 8 DMA instructions per wave
         if (t >= steps) return;
+        if (t == steps - 1) sa.last(t), sb.last(t);
         char* dst = smem + image + wave * 1024;
         sa.dma(dst + IMG_A, t);
         sb.dma(dst + IMG_B, t);
@@ -93,11 +94,6 @@ __global__ __launch_bounds__(256, STAGES == 2 ? 2 : 1) void linear128_kernel(Ope
     __syncthreads();                               // the last step has been read: the buffers become the staging area
     finish_tile<4>([&](int mt, int nt) { return acc[mt][nt]; }, smem + wave * 64 * OUT_ROW, epi, g, split, n0 + wn * 64, m0 + wm * 64,
                    N, M, lane, res);
-}
-
-bool linear128_takes(int dtype, int mode_a, int mode_b, const Operand& A, const Operand& B, int64_t K) {
-    const int es = (int)dtype_size(dtype);
-    return dma_ok(mode_a, A, K, T128, es) && dma_ok(mode_b, B, K, T128, es);
 }
 
 // Splits of the K range, towards one workgroup per compute unit, several steps each: a split costs a round trip of the fp32

@@ -27,39 +27,46 @@ __device__ __forceinline__ void segment_barrier() {
 // One operand of the kernel: descriptor, per-lane source offset, DMA pieces. Which = 0: A (one region of 256 rows, 4 pieces
 // per K step), 1: B (regions lo / hi of 128 rows, 2 pieces each: rows [0,64) and [64,128) of both 128-row wave groups).
 template <int MODE, int WHICH> struct Source256 {
-    __amdgpu_buffer_rsrc_t rsrc;
-    unsigned voff, piece, step;            // bytes: lane offset, between pieces, between K steps
+    const bf16_t* base;                    // of the tile and the split, uniform
+    unsigned ld2, edge;                    // bytes: row stride; OP_ROWS: of the descriptor, OP_COLS: of its last k row
+    unsigned voff, piece;                  // bytes: lane offset, between pieces
+    int left;                              // OP_ROWS: 16-byte pieces of K from the lane's on; OP_COLS: k rows
     __device__ __forceinline__ void init(const Operand& o, int row0, int64_t k0, int64_t K, int tid) {
-        const bf16_t* p = (const bf16_t*)o.p;
-        const unsigned ld2 = (unsigned)o.ld * 2u;
+        ld2 = (unsigned)o.ld * 2u;
         if (MODE == OP_ROWS) {
             const int hr = tid >> 3, ch = (tid & 7) ^ ((hr >> 1) & 7);
-            const int rows = min(T256, o.rows - row0);
-            rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)(p + (int64_t)row0 * o.ld + k0), 0,
-                                                     (int)((unsigned)(rows - 1) * ld2 + (unsigned)(K - k0) * 2u), 0x00020000);
+            base = (const bf16_t*)o.p + (int64_t)row0 * o.ld + k0;
+            edge = (unsigned)(min(T256, o.rows - row0) - 1) * ld2 + (unsigned)(K - k0) * 2u;
             voff = (unsigned)hr * ld2 + (unsigned)ch * 16u;
             piece = 64u * ld2;
-            step = K64 * 2;
+            left = (int)((K - k0) / 8) - ch;
         } else {
             constexpr int LOG = WHICH == 0 ? 5 : 4;    // chunks per k row: 32 (A), 16 (a half of B)
             const int kr = tid >> LOG, f = (kr & 3) + 4 * ((kr >> 3) & 1);
             const int c = (tid & ((1 << LOG) - 1)) ^ (2 * f);
             const int col = WHICH == 0 ? c * 8 : (c >> 3) * 128 + (c & 7) * 8;
-            // (the end rounded up to a piece: a dword that crosses the end reads as zero, with it the last of an odd number
-            // of rows; rows are 16-byte aligned, so the piece is the one that holds the last element)
-            rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)(p + k0 * o.ld + row0), 0,
-                                                     (int)(K > k0 ? (unsigned)(K - 1 - k0) * ld2 + ((unsigned)(o.rows - row0) * 2u + 15u) / 16u * 16u : 0u),
-                                                     0x00020000);
+            base = (const bf16_t*)o.p + k0 * o.ld + row0;
+            edge = ((unsigned)(o.rows - row0) * 2u + 15u) / 16u * 16u;         // (why a whole piece: linear_dma.hpp)
             voff = (unsigned)kr * ld2 + (unsigned)col * 2u;
             piece = (512u >> LOG) * ld2;
-            step = K64 * ld2;
+            left = (int)(K - k0);
         }
+    }
+    __device__ __forceinline__ __amdgpu_buffer_rsrc_t step(int t) const {      // (see linear_dma.hpp)
+        if (MODE == OP_ROWS) return __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (int)edge, 0x00020000);
+        const unsigned rows = (unsigned)min(K64, left - t * K64);
+        return __builtin_amdgcn_make_buffer_rsrc((void*)((const char*)base + (uint64_t)((unsigned)t * K64) * ld2), 0,
+                                                 (int)((rows - 1) * ld2 + edge), 0x00020000);
+    }
+    __device__ __forceinline__ void last(int t) {
+        if (MODE == OP_ROWS && 8 * t >= left) voff |= PAST_END;
     }
     // piece i of K step t; hi: the second half of B
     __device__ __forceinline__ void dma(char* lds, int t, int i, int hi) const {
-        unsigned so = (unsigned)t * step;
-        if (MODE == OP_ROWS) so += (unsigned)(WHICH == 0 ? i : 2 * i + hi) * piece;
-        else so += (unsigned)i * piece + (WHICH == 1 ? (unsigned)hi * 128u : 0u);
+        const __amdgpu_buffer_rsrc_t rsrc = step(t);
+        unsigned so;
+        if (MODE == OP_ROWS) so = (unsigned)t * 128u + (unsigned)(WHICH == 0 ? i : 2 * i + hi) * piece;
+        else so = (unsigned)i * piece + (WHICH == 1 ? (unsigned)hi * 128u : 0u);
         // the whole offset in the register the range check looks at
         __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_t)lds, 16, voff + so, 0, 0, 0);
     }
@@ -129,10 +136,15 @@ __global__ __launch_bounds__(512, 2) void linear256_kernel(Operand A, Operand B,
         __builtin_amdgcn_s_setprio(0);
     };
 
+    auto last = [&](int t) {
+        if (t == steps - 1) sa.last(t), sb.last(t);
+    };
+    last(0);
 #pragma unroll
     for (int i = 0; i < 4; ++i) dma_a(0, i);
     dma_b(0, 0, 0), dma_b(0, 0, 1), dma_b(1, 0, 0), dma_b(1, 0, 1);
     if (steps > 1) {
+        last(1);
 #pragma unroll
         for (int i = 0; i < 4; ++i) dma_a(1, i);
         dma_b(0, 1, 0), dma_b(0, 1, 1);
@@ -159,6 +171,7 @@ __global__ __launch_bounds__(512, 2) void linear256_kernel(Operand A, Operand B,
         WAIT_L1;                                                                                  \
         segment_barrier();                                                                        \
         wait_b();                                                                                 \
+        if (ISSUE_A) last(t + 2);                                                                 \
         multiply(4, (ISSUE_A) ? 6 : 0, [&](int j) {                                               \
             if (j < 4) dma_a(t + 2, j);                                                           \
             else dma_b(0, t + 2, j - 4);                                                          \
@@ -184,10 +197,6 @@ __global__ __launch_bounds__(512, 2) void linear256_kernel(Operand A, Operand B,
     Residual<64> res;
     res.load(epi, g, n0 + wn * 64, m0 + wm * 128 + 64, N, M, lane);
     finish_tile<4>([&](int mt, int nt) { return acc[4 + mt][nt]; }, stage, epi, g, split, n0 + wn * 64, m0 + wm * 128 + 64, N, M, lane, res);
-}
-
-bool linear256_takes(int mode_a, int mode_b, const Operand& A, const Operand& B, int64_t K) {
-    return dma_ok(mode_a, A, K, T256, 2) && dma_ok(mode_b, B, K, T256, 2);
 }
 
 int launch_linear256(const char* what, int mode_a, int mode_b, const Operand& A, const Operand& B, const Epilogue& epi, int64_t K,

@@ -6,13 +6,14 @@
 // k = i / 4 and rows 4 (i % 4) .. + 3 and receives row i). Chunk XOR 2 ((k & 3) + 4 ((k >> 3) & 1)) spreads the 4 k of one
 // read, and the 8 apart ones of the neighbouring 16 lanes, over 8 different 32-byte slots: no bank conflicts (cols_swizzle).
 // LDS-DMA writes linearly, so both swizzles are applied to the per-lane source address; rows and K past the end read as
-// zeros by the buffer descriptors' range check (K past the end of an OP_ROWS operand does not, hence K % 64 == 0 there).
+// zeros by the buffer descriptors' range check (K past the end of an OP_ROWS operand is the next row's memory: last()).
 #pragma once
 #include "linear.hpp"
 
 namespace sphip {
 
 constexpr int K64 = 64;                            // bf16 K per step: 128 bytes (32 fp32)
+constexpr unsigned PAST_END = 1u << 31;            // offset bit that lies behind every descriptor (MAX_LD)
 
 #define LIN_VMCNT(n) asm volatile("s_waitcnt vmcnt(" #n ")" ::: "memory")
 
@@ -138,45 +139,50 @@ __device__ __forceinline__ void finish_tile(Acc acc, char* stage, const Epilogue
 template <typename T, int MODE, int TILE> struct Source {
     static constexpr unsigned ES = sizeof(T), KS = 128 / ES;
     static constexpr int PIECES = TILE / 32, PITCH = TILE * ES;
-    __amdgpu_buffer_rsrc_t rsrc;
-    unsigned voff[2], piece, step;         // bytes: lane offset of even and odd pieces, between pieces, between K steps
+    const T* base;                         // of the tile and the split, uniform
+    unsigned ldb, edge;                    // bytes: row stride; OP_ROWS: of the descriptor, OP_COLS: of its last k row
+    unsigned voff[2], piece;               // bytes: lane offset of even and odd pieces, between pieces
+    int left;                              // OP_ROWS: 16-byte pieces of K from the lane's on; OP_COLS: k rows
     __device__ __forceinline__ void init(const Operand& o, int row0, int64_t k0, int64_t K, int tid) {
-        const T* p = (const T*)o.p;
-        const unsigned ldb = (unsigned)o.ld * ES;
+        ldb = (unsigned)o.ld * ES;
         if (MODE == OP_ROWS) {
             const int hr = tid >> 3, ch = (tid & 7) ^ ((hr >> 1) & 7);
-            const int rows = min(TILE, o.rows - row0);
-            rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)(p + (int64_t)row0 * o.ld + k0), 0,
-                                                     (int)((unsigned)(rows - 1) * ldb + (unsigned)(K - k0) * ES), 0x00020000);
+            base = (const T*)o.p + (int64_t)row0 * o.ld + k0;
+            edge = (unsigned)(min(TILE, o.rows - row0) - 1) * ldb + (unsigned)(K - k0) * ES;
             voff[0] = voff[1] = (unsigned)hr * ldb + (unsigned)ch * 16u;
             piece = 32u * ldb;
-            step = 128;
+            left = (int)((K - k0) * ES / 16) - ch;
         } else {
-            // (the end rounded up to a piece, see linear256.hip)
-            rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)(p + k0 * o.ld + row0), 0,
-                                                     (int)(K > k0 ? (unsigned)(K - 1 - k0) * ldb + ((unsigned)(o.rows - row0) * ES + 15u) / 16u * 16u : 0u),
-                                                     0x00020000);
             constexpr int CH = PITCH / 16, KP = 256 / CH;       // 16-byte chunks of a k row, k rows of a piece
             const int kr = tid / CH, c = tid % CH;
+            base = (const T*)o.p + k0 * o.ld + row0;
+            // rounded up to a piece: a dword that crosses the end reads as zero, with it the last of an odd number of rows
+            // (k rows are 16-byte aligned, so the piece is the one that holds the last element)
+            edge = ((unsigned)(o.rows - row0) * ES + 15u) / 16u * 16u;
 #pragma unroll
             for (int i = 0; i < 2; ++i) voff[i] = (unsigned)kr * ldb + (unsigned)(c ^ cols_swizzle<ES, PITCH>(kr + KP * i)) * 16u;
             piece = KP * ldb;
-            step = KS * ldb;
+            left = (int)(K - k0);
         }
     }
+    // The descriptor of K step t. OP_COLS: from the step's first k row, so that its offsets do not grow with K (many tokens).
+    __device__ __forceinline__ __amdgpu_buffer_rsrc_t step(int t) const {
+        if (MODE == OP_ROWS) return __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (int)edge, 0x00020000);
+        const unsigned rows = (unsigned)min((int)KS, left - t * (int)KS);
+        return __builtin_amdgcn_make_buffer_rsrc((void*)((const char*)base + (uint64_t)((unsigned)t * KS) * ldb), 0,
+                                                 (int)((rows - 1) * ldb + edge), 0x00020000);
+    }
+    // before the DMA of the last step: an OP_ROWS lane whose piece lies behind K names an offset behind the descriptor
+    __device__ __forceinline__ void last(int t) {
+        if (MODE == OP_ROWS && 8 * t >= left) voff[0] |= PAST_END, voff[1] |= PAST_END;
+    }
     __device__ __forceinline__ void dma(char* lds, int t) const {
+        const __amdgpu_buffer_rsrc_t rsrc = step(t);
+        const unsigned so = MODE == OP_ROWS ? (unsigned)t * 128u : 0u;
 #pragma unroll
-        for (int i = 0; i < PIECES; ++i)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_t)(lds + 4096 * i), 16, voff[i & 1] + (unsigned)t * step + (unsigned)i * piece, 0, 0, 0);
+        for (int i = 0; i < PIECES; ++i)      // (the whole offset in the register the range check looks at)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_t)(lds + 4096 * i), 16, voff[i & 1] + (unsigned)i * piece + so, 0, 0, 0);
     }
 };
-
-// whether LDS-DMA can fetch an operand of es-byte elements: 16-byte aligned rows, 32-bit byte offsets inside a tile's
-// descriptor, whole 128-byte steps of K where K is the contiguous index
-static inline bool dma_ok(int mode, const Operand& o, int64_t K, int tile, int es) {
-    if (((uintptr_t)o.p & 15) != 0 || o.ld * es % 16 != 0) return false;
-    if (mode == OP_ROWS) return K * es % 128 == 0 && (o.ld * tile + K) * es < (1ll << 31);
-    return mode == OP_COLS && (K + 128 / es) * o.ld * es < (1ll << 31);
-}
 
 }  // namespace sphip

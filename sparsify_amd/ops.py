@@ -1318,6 +1318,12 @@ def _linear_backward_bytes(*args) -> int:
     return _lib.load().sphip_linear_backward_workspace_bytes(*args)
 
 
+def _odd(t: Tensor) -> bool:
+    """Whether the rows of t have to be copied before a product: not all at multiples of 16 bytes, or 2^22 elements apart."""
+    ld = _ld(t)
+    return bool((t.data_ptr() | ld * t.element_size()) & 15) or ld >= 1 << 22
+
+
 def _act(activation: str) -> int:
     act = _lib.ACTIVATIONS.get(activation)
     if act is None:
@@ -1376,7 +1382,7 @@ def linear(x: Tensor, W: Tensor, bias: Tensor | None = None, residual: Tensor | 
     if N == 0:
         return out, z, codes
     dt = _dt(x)
-    nws = _linear_bytes(dt, z_kind, N, D, M)
+    nws = _linear_bytes(dt, z_kind, N, D, M, _odd(x) + 2 * _odd(W))
     ws = _scratch(x, nws)
     _call("sphip_linear", x, x.data_ptr(), _ld(x), W.data_ptr(), _ld(W), dt, _ptr(bias), 0 if bias is None else _dt(bias),
           act, _ptr(residual), 0 if residual is None else _dt(residual), 0 if residual is None else _ld(residual),
@@ -1427,7 +1433,8 @@ def linear_backward(g: Tensor, W: Tensor, z: Tensor | None, x: Tensor | None, ac
         return dx, None if dW is None else dW.zero_(), None if db is None else db.zero_()
     if dx is None and dW is None and db is None:
         return None, None, None
-    nws = _linear_backward_bytes(dt, xargs[1], dx is not None, dW is not None, db is not None, N, D, M)
+    odd = (x_fmt is None and dW is not None and _odd(x)) + 2 * (dx is not None and _odd(W))
+    nws = _linear_backward_bytes(dt, xargs[1], dx is not None, dW is not None, db is not None, N, D, M, odd)
     ws = _scratch(g, nws)
     _call("sphip_linear_backward", g, g.data_ptr(), _dt(g), _ld(g), W.data_ptr(), _ld(W), dt, act, *zargs, *xargs,
           _ptr(dx), 0 if dx is None else _dt(dx), D, _ptr(dW), 0 if dW is None else _dt(dW), D, _ptr(db),

@@ -145,7 +145,7 @@ def test_forward_writes_its_rows_only(device):
             out = torch.full((N + 2, M + 5), 7.0, dtype=dtype, device="cuda")
             z = torch.full((N + 2, M + 3), 7.0, device="cuda")
             dt = _lib.BF16 if dtype == torch.bfloat16 else _lib.F32
-            nws = lib.sphip_linear_workspace_bytes(dt, _lib.F32, N, D, M)
+            nws = lib.sphip_linear_workspace_bytes(dt, _lib.F32, N, D, M, 0)
             ws = torch.empty(max(nws, 16), dtype=torch.uint8, device="cuda")
             _lib.check(lib.sphip_linear(xc.data_ptr(), D, Wc.data_ptr(), D, dt, bc.data_ptr(), dt, 1, None, 0, 0,
                                         out[1:].data_ptr(), dt, M + 5, z[1:].data_ptr(), _lib.F32, None, M + 3, None, None,
@@ -376,7 +376,7 @@ def test_gradient_against_differences(device, act, fmt):
 
 @pytest.mark.parametrize("N,D,M", [(256, 64, 256), (300, 128, 520), (1000, 192, 704), (64, 1024, 136), (257, 256, 255), (1030, 320, 1000),
                                    (2048, 128, 257), (1, 64, 64), (129, 129, 129), (700, 77, 1001), (33, 1000, 3)])
-@pytest.mark.parametrize("kernel", ["tile", "64", "128", "256", "few"])
+@pytest.mark.parametrize("kernel", ["64", "128", "256", "few"])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_every_product_kernel(device, monkeypatch, N, D, M, kernel, dtype):
     """Each of the product's kernels on small and ragged shapes (SPHIP_LINEAR): forward, and both gradient products with
@@ -405,6 +405,42 @@ def test_every_product_kernel(device, monkeypatch, N, D, M, kernel, dtype):
                              codes64(x, fmt) if fmt else x, dtype, dtype, 0.0)
             for n, got in (("x", dx), ("W", dW), ("b", db)):
                 assert_within(got, *ref[n], f"d{n} {act} {N}x{D}x{M}")
+    finally:
+        monkeypatch.undo()
+        ops._linear_bytes.cache_clear(), ops._linear_backward_bytes.cache_clear()
+
+
+@pytest.mark.parametrize("N,D,M", [(300, 72, 88), (70, 1000, 328), (513, 200, 520)])
+@pytest.mark.parametrize("kernel", ["64", "128", "256", "few"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_nothing_behind_a_row_is_multiplied(device, monkeypatch, N, D, M, kernel, dtype):
+    """Rows that are whole 16-byte pieces but no whole number of K steps, inside larger tensors of NaN."""
+    from sparsify_amd import ops
+    if kernel == "few":
+        N = N % 64 + 1
+    monkeypatch.setenv("SPHIP_LINEAR", kernel)
+    ops._linear_bytes.cache_clear(), ops._linear_backward_bytes.cache_clear()
+
+    def framed(t, left):
+        big = torch.full((t.shape[0] + 2, t.shape[1] + left + 24), math.nan, dtype=t.dtype, device="cuda")
+        big[1:-1, left : left + t.shape[1]] = t.cuda()
+        return big[1:-1, left : left + t.shape[1]]
+
+    try:
+        x, W, _, _ = make(N, D, M, dtype, 5, bias=False)
+        g = torch.randn(N, M, generator=torch.Generator().manual_seed(6)).to(dtype)
+        for left in (16, 3):                              # on 16-byte boundaries, and off them
+            xc, Wc, gc = framed(x, left), framed(W, left), framed(g, left)
+            y, _, _ = ops.linear(xc, Wc)
+            want, tol, _, _ = forward64(x, W, None, None, "none", dtype)
+            assert_within(y, want, tol, f"y {left}")
+            dx, dW, db = ops.linear_backward(gc, Wc, None, xc, "none", dx_dtype=dtype, dw_dtype=dtype, db_dtype=dtype)
+            ref = backward64(x, W, torch.zeros(M, dtype=dtype), "none", g, torch.zeros(N, M).double(), x, dtype, dtype, 0.0)
+            for n, got in (("x", dx), ("W", dW), ("b", db)):
+                assert_within(got, *ref[n], f"d{n} {left}")
+            dx, dW, _ = ops.linear_backward(gc, Wc, None, xc, "none", dx_dtype=dtype, dw_dtype=dtype)
+            for n, got in (("x", dx), ("W", dW)):
+                assert_within(got, *ref[n], f"d{n} alone {left}")
     finally:
         monkeypatch.undo()
         ops._linear_bytes.cache_clear(), ops._linear_backward_bytes.cache_clear()

@@ -66,11 +66,27 @@ def test_backward_entry(kw, status, word):
 
 def test_workspace_queries():
     L = lib()
-    assert L.sphip_linear_workspace_bytes(BF16, 0, 0, 8, 8) == 0 and L.sphip_linear_workspace_bytes(9, 0, 8, 8, 8) == 0
-    assert L.sphip_linear_workspace_bytes(BF16, INT8, 80, 4096, 32) >= L.sphip_linear_workspace_bytes(BF16, F32, 80, 4096, 32) + 80 * 32 * 4
-    assert L.sphip_linear_workspace_bytes(BF16, INT8, 80, 64, 32) == 0 and L.sphip_linear_workspace_bytes(BF16, F32, 8, 4096, 32) == 0
-    assert L.sphip_linear_backward_workspace_bytes(BF16, INT8, 0, 0, 1, 64, 64, 32) == 2 * 32 * 4
-    assert L.sphip_linear_backward_workspace_bytes(F32, F32, 1, 1, 1, 8, -1, 32) == 0
+    assert L.sphip_linear_workspace_bytes(BF16, 0, 0, 8, 8, 0) == 0 and L.sphip_linear_workspace_bytes(9, 0, 8, 8, 8, 0) == 0
+    assert (L.sphip_linear_workspace_bytes(BF16, INT8, 80, 4096, 32, 0)
+            >= L.sphip_linear_workspace_bytes(BF16, F32, 80, 4096, 32, 0) + 80 * 32 * 4)
+    assert L.sphip_linear_workspace_bytes(BF16, INT8, 80, 64, 32, 0) == 0 and L.sphip_linear_workspace_bytes(BF16, F32, 8, 4096, 32, 0) == 0
+    assert L.sphip_linear_backward_workspace_bytes(BF16, INT8, 0, 0, 1, 64, 64, 32, 3) == 2 * 32 * 4
+    assert L.sphip_linear_backward_workspace_bytes(F32, F32, 1, 1, 1, 8, -1, 32, 0) == 0
+    # copies: of the operands that are named, of both where rows are no whole 16-byte pieces
+    for odd, rows in [(0, 0), (1, 80), (2, 40), (3, 120)]:
+        assert L.sphip_linear_workspace_bytes(BF16, F32, 80, 72, 40, odd) == rows * 128 * 2
+        assert L.sphip_linear_workspace_bytes(BF16, F32, 80, 71, 40, odd) == 120 * 128 * 2
+        want = L.sphip_linear_backward_workspace_bytes(F32, F32, 1, 1, 0, 64, 64, 64, 0)
+        assert L.sphip_linear_backward_workspace_bytes(F32, F32, 1, 1, 0, 64, 64, 64, odd) == want + 64 * 64 * 4 * bin(odd).count("1")
+
+
+def test_longest_rows():
+    most = (1 << 22) - 65
+    assert linear(D=most, ldx=most, ldw=most) == EWORKSPACE
+    for kw in (dict(D=most + 1, ldx=most + 1, ldw=most + 1), dict(M=most + 1, ldo=most + 1)):
+        assert linear(**kw) == EUNSUPPORTED and b"2^22" in lib().sphip_last_error()
+    for kw in (dict(D=most + 1, ldx=most + 1, ldw=most + 1, lddx=most + 1, lddw=most + 1), dict(M=most + 1, ldg=most + 1)):
+        assert backward(**kw) == EUNSUPPORTED and b"2^22" in lib().sphip_last_error()
 
 
 def test_checkpoint_entries():
