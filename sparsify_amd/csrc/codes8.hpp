@@ -9,15 +9,15 @@ __device__ __forceinline__ float scale_value(unsigned byte) {
     return __uint_as_float(byte == 255u ? 0x7fc00000u : byte << 23);
 }
 
-// The four codes of w, each under its own scale. int8: (u - 128) s with u the byte of w ^ 0x80808080, as one fused
-// u s - 128 s. Code times scale is exact in either format.
+// The four codes of w, each under its own scale. int8: (u - 128) s with u the byte of w ^ 0x80808080 (128 s may be past the
+// largest fp32: not u s - 128 s). Code times scale is exact in either format.
 template <int FMT> __device__ __forceinline__ void code_values(unsigned w, const float (&s)[4], float (&o)[4]) {
     if (FMT == SPHIP_INT8) {
         w ^= 0x80808080u;
-        o[0] = fmaf((float)(w & 0xffu), s[0], -128.f * s[0]);
-        o[1] = fmaf((float)((w >> 8) & 0xffu), s[1], -128.f * s[1]);
-        o[2] = fmaf((float)((w >> 16) & 0xffu), s[2], -128.f * s[2]);
-        o[3] = fmaf((float)(w >> 24), s[3], -128.f * s[3]);
+        o[0] = ((float)(w & 0xffu) - 128.f) * s[0];
+        o[1] = ((float)((w >> 8) & 0xffu) - 128.f) * s[1];
+        o[2] = ((float)((w >> 16) & 0xffu) - 128.f) * s[2];
+        o[3] = ((float)(w >> 24) - 128.f) * s[3];
     } else {
         typedef float f2 __attribute__((ext_vector_type(2)));
         const f2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);

@@ -410,6 +410,21 @@ def test_every_product_kernel(device, monkeypatch, N, D, M, kernel, dtype):
         ops._linear_bytes.cache_clear(), ops._linear_backward_bytes.cache_clear()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+def test_kept_z_near_the_largest_value(device, fmt, dtype):
+    """ReLU's slopes, 0 or 1, and the sums of up to 64 of them are whole numbers: exact."""
+    from sparsify_amd import ops
+    z = torch.tensor([3.0e38, -3.0e38, 1.8e38, -1.0, 0.0, 2.0**-100, 1.7e38, -1.7e38]).repeat(64, 8).to(dtype).cuda()
+    q = ops.checkpoint8_save(z, fmt, True)
+    g = torch.ones(64, 64, dtype=dtype, device="cuda")
+    W, x = torch.eye(64, dtype=dtype, device="cuda"), torch.ones(64, 64, dtype=dtype, device="cuda")
+    dx, dW, db = ops.linear_backward(g, W, q, x, "relu", z_fmt=fmt, dx_dtype=dtype, dw_dtype=dtype, db_dtype=dtype)
+    want = (z > 0).to(dtype)
+    assert torch.equal(dx, want)
+    assert torch.equal(db, want.sum(0)) and torch.equal(dW, want.T @ x)
+
+
 @pytest.mark.parametrize("N,D,M", [(300, 72, 88), (70, 1000, 328), (513, 200, 520)])
 @pytest.mark.parametrize("kernel", ["64", "128", "256", "few"])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
