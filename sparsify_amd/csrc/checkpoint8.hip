@@ -112,41 +112,8 @@ __global__ __launch_bounds__(256) void checkpoint8_save_kernel(SaveArgs a) {
     }
 }
 
-template <typename T, int V, int FMT>
-__global__ __launch_bounds__(256) void checkpoint8_restore_kernel(const uint8_t* __restrict__ codes,
-                                                                  const uint8_t* __restrict__ scales, int64_t ldq,
-                                                                  T* __restrict__ out, int64_t ldo, int64_t N, int D) {
-    constexpr int ROWS = 8;                                                  // rows of one group per thread
-    const int per_row = (int)(ldq / V);
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int64_t blk = i / per_row;
-    if (blk * ROWS >= N) return;
-    const int c0 = (int)(i % per_row) * V, n = D - c0;
-    if (n <= 0) return;
-    uint8_t sb[V], q[ROWS][V];
-    __builtin_memcpy(sb, scales + (blk * ROWS / 32) * ldq + c0, V);
-#pragma unroll
-    for (int t = 0; t < ROWS; ++t) __builtin_memcpy(q[t], codes + (blk * ROWS + t) * ldq + c0, V);
-    float s[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) s[j] = scale_value(sb[j]);
-#pragma unroll
-    for (int t = 0; t < ROWS; ++t) {
-        const int64_t row = blk * ROWS + t;
-        if (row >= N) break;
-        T o[V];
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const float f = FMT == SPHIP_INT8 ? (float)(int8_t)q[t][j] : __builtin_amdgcn_cvt_f32_fp8((int)q[t][j], 0);
-            Elem<T>::store(o, j, f * s[j]);                                  // exact
-        }
-        T* p = out + row * ldo + c0;
-        if (n >= V) __builtin_memcpy(p, o, sizeof(o));
-        else
-#pragma unroll
-            for (int j = 0; j < V; ++j)
-                if (j < n) p[j] = o[j];
-    }
+template <typename T, int FMT> __global__ __launch_bounds__(256) void checkpoint8_restore_kernel(RestoreArgs a) {
+    restore_block<T, FMT>(a, blockIdx.x);
 }
 
 static int check_codes(const char* what, const void* codes, const void* scales, int64_t ldq, int fmt, int dtype, int64_t N,
@@ -200,18 +167,16 @@ extern "C" int sphip_checkpoint8_restore(const uint8_t* codes, const uint8_t* sc
     SPHIP_REQUIRE(out && ((uintptr_t)out & (dtype_size(dtype) - 1)) == 0, SPHIP_EINVAL, "checkpoint8_restore: null or misaligned out");
     SPHIP_REQUIRE(ldo >= D, SPHIP_EINVAL, "checkpoint8_restore: ldo is shorter than a row");
     hipStream_t s = (hipStream_t)stream;
-    const int V = dtype == SPHIP_BF16 ? 8 : 4;
-    const int64_t blocks = cdiv(cdiv(N, 8) * (ldq / V), 256);
+    const RestoreArgs a = {codes, scales, out, ldq, ldo, N, (int)D};
+    const int64_t blocks = restore_blocks(a, dtype);
     SPHIP_REQUIRE(blocks < (1ll << 31), SPHIP_EUNSUPPORTED, "checkpoint8_restore: grid too large");
-#define SPHIP_RESTORE(T, V, F)                                                                                              \
-    hipLaunchKernelGGL((checkpoint8_restore_kernel<T, V, F>), dim3((unsigned)blocks), dim3(256), 0, s, codes, scales, ldq,   \
-                       (T*)out, ldo, N, (int)D)
+#define SPHIP_RESTORE(T, F) hipLaunchKernelGGL((checkpoint8_restore_kernel<T, F>), dim3((unsigned)blocks), dim3(256), 0, s, a)
     if (dtype == SPHIP_BF16) {
-        if (fmt == SPHIP_INT8) SPHIP_RESTORE(bf16_t, 8, SPHIP_INT8);
-        else SPHIP_RESTORE(bf16_t, 8, SPHIP_E4M3);
+        if (fmt == SPHIP_INT8) SPHIP_RESTORE(bf16_t, SPHIP_INT8);
+        else SPHIP_RESTORE(bf16_t, SPHIP_E4M3);
     } else {
-        if (fmt == SPHIP_INT8) SPHIP_RESTORE(float, 4, SPHIP_INT8);
-        else SPHIP_RESTORE(float, 4, SPHIP_E4M3);
+        if (fmt == SPHIP_INT8) SPHIP_RESTORE(float, SPHIP_INT8);
+        else SPHIP_RESTORE(float, SPHIP_E4M3);
     }
 #undef SPHIP_RESTORE
     SPHIP_CHECK_LAUNCH("checkpoint8_restore");

@@ -1,4 +1,4 @@
-// Values of the 8-bit checkpoint codes (checkpoint8.hip).
+// The 8-bit checkpoint's codes (checkpoint8.hip) and their values.
 #pragma once
 #include "common.hpp"
 
@@ -64,6 +64,48 @@ template <int FMT> __device__ __forceinline__ unsigned codes_of(const float (&a)
         }
     }
     return (w & ~bad) | (bad & 0x7f7f7f7fu);
+}
+
+// Codes to values: a thread takes 16 bytes of values of 8 consecutive rows of one group (their loads all in flight).
+struct RestoreArgs {
+    const uint8_t *codes, *scales;
+    void* out;
+    int64_t ldq, ldo, N;
+    int D;
+};
+static inline int64_t restore_blocks(const RestoreArgs& a, int dtype) { return cdiv(cdiv(a.N, 8) * (a.ldq / (16 / (int64_t)dtype_size(dtype))), 256); }
+template <typename T, int FMT> __device__ __forceinline__ void restore_block(const RestoreArgs& a, unsigned block) {
+    constexpr int ROWS = 8, V = 16 / sizeof(T);
+    const int per_row = (int)(a.ldq / V);
+    const int64_t i = (int64_t)block * 256 + threadIdx.x;
+    const int64_t blk = i / per_row;
+    if (blk * ROWS >= a.N) return;
+    const int c0 = (int)(i % per_row) * V, n = a.D - c0;
+    if (n <= 0) return;
+    uint8_t sb[V], q[ROWS][V];
+    __builtin_memcpy(sb, a.scales + (blk * ROWS / 32) * a.ldq + c0, V);
+#pragma unroll
+    for (int t = 0; t < ROWS; ++t) __builtin_memcpy(q[t], a.codes + (blk * ROWS + t) * a.ldq + c0, V);
+    float s[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) s[j] = scale_value(sb[j]);
+#pragma unroll
+    for (int t = 0; t < ROWS; ++t) {
+        const int64_t row = blk * ROWS + t;
+        if (row >= a.N) break;
+        T o[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const float f = FMT == SPHIP_INT8 ? (float)(int8_t)q[t][j] : __builtin_amdgcn_cvt_f32_fp8((int)q[t][j], 0);
+            Elem<T>::store(o, j, f * s[j]);                                  // exact
+        }
+        T* p = (T*)a.out + row * a.ldo + c0;
+        if (n >= V) __builtin_memcpy(p, o, sizeof(o));
+        else
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+                if (j < n) p[j] = o[j];
+    }
 }
 
 }  // namespace sphip

@@ -312,22 +312,50 @@ template <typename TG> static int launch_preact(PreactArgs& a, int z_kind, int64
     return SPHIP_OK;
 }
 
-// column sums of part (P, M) in row order by 16 interleaved chains: 64 columns per workgroup of 1024 threads
-__global__ __launch_bounds__(1024) void linear_bias_grad_kernel(const float* __restrict__ part, int64_t P, int M, void* db, int dt) {
-    __shared__ float red[16][64];
-    const int c = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int m = blockIdx.x * 64 + c;
+// What the products still need after dz, in one launch: the first a.restore workgroups restore x from its codes, the others sum
+// 16 columns each of part (P, M), 16 interleaved chains in row order. (Two launches took 3.6 and 3.3 us at 256 x 768 x 768.)
+struct FinishArgs {
+    RestoreArgs x;
+    const float* part;
+    void* db;
+    int64_t P;
+    unsigned restore;
+    int M, db_dt;
+};
+template <typename T, int FMT> __global__ __launch_bounds__(256) void linear_finish_kernel(FinishArgs a) {
+    if (blockIdx.x < a.restore) {
+        restore_block<T, FMT>(a.x, blockIdx.x);
+        return;
+    }
+    __shared__ float red[16][16];
+    const int c = threadIdx.x & 15, w = threadIdx.x >> 4;
+    const int m = (int)(blockIdx.x - a.restore) * 16 + c;
     float s = 0.f;
-    if (m < M)
-        for (int64_t p = w; p < P; p += 16) s += part[p * M + m];
+    if (m < a.M)
+        for (int64_t p = w; p < a.P; p += 16) s += a.part[p * a.M + m];
     red[w][c] = s;
     __syncthreads();
-    if (w == 0 && m < M) {
+    if (w == 0 && m < a.M) {
         float t = 0.f;
 #pragma unroll
         for (int j = 0; j < 16; ++j) t += red[j][c];
-        store_from_f32(db, dt, m, t);
+        store_from_f32(a.db, a.db_dt, m, t);
     }
+}
+static int launch_finish(FinishArgs& a, int dtype, int fmt, hipStream_t s) {
+    const int64_t restore = a.x.codes ? restore_blocks(a.x, dtype) : 0, blocks = restore + (a.db ? cdiv(a.M, 16) : 0);
+    SPHIP_REQUIRE(blocks < (1ll << 31), SPHIP_EUNSUPPORTED, "linear_backward: grid too large");
+    a.restore = (unsigned)restore;
+    const dim3 grid((unsigned)blocks), block(256);
+    if (dtype == SPHIP_BF16) {
+        if (fmt == SPHIP_E4M3) hipLaunchKernelGGL((linear_finish_kernel<bf16_t, SPHIP_E4M3>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((linear_finish_kernel<bf16_t, SPHIP_INT8>), grid, block, 0, s, a);
+    } else {
+        if (fmt == SPHIP_E4M3) hipLaunchKernelGGL((linear_finish_kernel<float, SPHIP_E4M3>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((linear_finish_kernel<float, SPHIP_INT8>), grid, block, 0, s, a);
+    }
+    SPHIP_CHECK_LAUNCH("linear_backward(db)");
+    return SPHIP_OK;
 }
 
 static bool valid_act(int act) { return act >= SPHIP_ACT_NONE && act <= SPHIP_ACT_SILU; }
@@ -523,11 +551,16 @@ extern "C" int sphip_linear_backward(const void* g, int g_dtype, int64_t ldg, co
         a.ldg = ldg, a.ldz = ldz, a.lddz = dz.ld, a.dz_dt = dtype, a.act = act;
         st = g_dtype == SPHIP_BF16 ? launch_preact<bf16_t>(a, z_kind, N, M, s) : launch_preact<float>(a, z_kind, N, M, s);
         if (st != SPHIP_OK) return st;
-        if (db) {
-            hipLaunchKernelGGL(linear_bias_grad_kernel, dim3((unsigned)cdiv(M, 64)), dim3(1024), 0, s, (const float*)sums,
-                               cdiv(N, 32), (int)M, db, db_dtype);
-            SPHIP_CHECK_LAUNCH("linear_backward(db)");
+    }
+    if (db || (dW && xc)) {
+        FinishArgs a = {};
+        if (dW && xc) {
+            a.x = {(const uint8_t*)x, x_scales, xs, ldx, packed_ld(D), N, (int)D};
+            ox.p = xs, ox.ld = a.x.ldo;
         }
+        a.part = sums, a.db = db, a.P = cdiv(N, 32), a.M = (int)M, a.db_dt = db_dtype;
+        st = launch_finish(a, dtype, x_kind, s);
+        if (st != SPHIP_OK) return st;
     }
     Epilogue e;
     if (dx) {
@@ -538,11 +571,6 @@ extern "C" int sphip_linear_backward(const void* g, int g_dtype, int64_t ldg, co
         if (st != SPHIP_OK) return st;
     }
     if (dW) {
-        if (xc) {
-            ox.p = xs, ox.ld = packed_ld(D);
-            st = sphip_checkpoint8_restore((const uint8_t*)x, x_scales, ldx, x_kind, xs, dtype, ox.ld, N, D, s);
-            if (st != SPHIP_OK) return st;
-        }
         e.out = dW, e.out_dt = dw_dtype, e.ldo = lddw;
         dz.rows = (int)M;
         st = dtype == SPHIP_BF16 ? launch_product<bf16_t, OP_COLS, OP_COLS>("linear_backward(dW)", dz, ox, e, N, N, part, sp.part, s)

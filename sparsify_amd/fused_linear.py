@@ -35,10 +35,6 @@ def _operands(input: Tensor, weight: Tensor):
     return x, as_rows(weight)
 
 
-def _shaped(t: Tensor, shape) -> Tensor:
-    return t if t.shape == shape else t.reshape(shape)
-
-
 class FusedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, input, weight, bias, residual, activation: str, checkpoint):
@@ -59,7 +55,7 @@ class FusedLinear(torch.autograd.Function):
         ctx.fmt, ctx.activation, ctx.compute = fmt, activation, x.dtype
         ctx.like = (input.shape, input.dtype, None if bias is None else bias.dtype, None if residual is None else residual.dtype)
         ctx.set_materialize_grads(False)
-        return _shaped(y, (*input.shape[:-1], weight.shape[0]))
+        return y if input.ndim == 2 else y.reshape(*input.shape[:-1], weight.shape[0])
 
     @staticmethod
     @once_differentiable
@@ -75,8 +71,8 @@ class FusedLinear(torch.autograd.Function):
             dx, dW, db = ops.linear_backward(as_rows(g), w, z, x, ctx.activation, z_fmt=ctx.fmt, x_fmt=ctx.fmt,
                                              dx_dtype=in_dtype if need_x else None, dw_dtype=weight.dtype if need_w else None,
                                              db_dtype=b_dtype if need_b else None)
-            if need_x:
-                dx = _shaped(dx, in_shape)
+            if need_x and len(in_shape) != 2:
+                dx = dx.reshape(in_shape)
         dr = None
         if need_r:
             dr = g if g.dtype == r_dtype else g.to(r_dtype)
@@ -115,4 +111,4 @@ def fused_linear(input: Tensor, weight: Tensor, bias: Tensor | None = None, *, r
     x, w = _operands(input, weight)
     y = ops.linear(x, w, None if bias is None else bias.detach().contiguous(), None if residual is None else as_rows(residual),
                    activation)[0]
-    return _shaped(y, (*input.shape[:-1], M))
+    return y if input.ndim == 2 else y.reshape(*input.shape[:-1], M)

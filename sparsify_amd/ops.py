@@ -1269,29 +1269,27 @@ def is_rows(t: Tensor) -> bool:
     return (s1 == 1 or d <= 1) and (s0 >= d or n <= 1)
 
 
-def _rows(t: Tensor, name: str, shape: tuple | None = None, like: Tensor | None = None) -> Tensor:
-    """A (rows, columns) tensor these ops take: on the GPU, fp32 or bf16, columns next to each other, any row stride."""
+def _rows(t: Tensor, name: str, shape: tuple | None = None, like: Tensor | None = None) -> tuple[int, int, int]:
+    """(address, row stride, dtype) of a (rows, columns) tensor these ops take: on the GPU, fp32 or bf16, columns next to each
+    other, any row stride."""
     if not t.is_cuda:
         raise RuntimeError(f"{name} is on {t.device}: sparsify_amd runs on the MI355X HIP path only (no CPU fallback)")
-    _dt(t)
-    if t.ndim != 2 or (shape is not None and t.shape != shape):
-        raise ValueError(f"{name}: expected {'2 dims' if shape is None else shape}, got shape {tuple(t.shape)}")
+    dt, size = _dt(t), t.shape
+    if len(size) != 2 or (shape is not None and size != shape):
+        raise ValueError(f"{name}: expected {'2 dims' if shape is None else shape}, got shape {tuple(size)}")
     if like is not None and t.device != like.device:
         raise ValueError(f"{name} is on {t.device}, the others on {like.device}")
-    if not is_rows(t):
+    (n, d), (ld, inner) = size, t.stride()
+    if (inner != 1 and d > 1) or (ld < d and n > 1):
         raise ValueError(f"{name} must have its columns next to each other and rows that do not overlap "
-                         f"(strides {t.stride()} for shape {tuple(t.shape)})")
-    return t
-
-
-def _ld(t: Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+                         f"(strides {t.stride()} for shape {tuple(size)})")
+    return t.data_ptr(), ld if n > 1 else d, dt
 
 
 def _call(what: str, t: Tensor, *args) -> None:
     """One entry point on t's device and its current stream (the last argument)."""
     fn = getattr(_lib.load(), what)
-    ev = timer.start(what, t)
+    ev = timer.start(what, t) if timer.enabled else None
     if t.device.index == torch.cuda.current_device():
         st = fn(*args, _stream(t))
     else:
@@ -1299,7 +1297,8 @@ def _call(what: str, t: Tensor, *args) -> None:
             st = fn(*args, _stream(t))
     if st:
         check(st, what)
-    timer.stop(ev, t)
+    if ev is not None:
+        timer.stop(ev, t)
 
 
 def _scratch(t: Tensor, nbytes: int) -> Tensor | None:
@@ -1318,10 +1317,9 @@ def _linear_backward_bytes(*args) -> int:
     return _lib.load().sphip_linear_backward_workspace_bytes(*args)
 
 
-def _odd(t: Tensor) -> bool:
-    """Whether the rows of t have to be copied before a product: not all at multiples of 16 bytes, or 2^22 elements apart."""
-    ld = _ld(t)
-    return bool((t.data_ptr() | ld * t.element_size()) & 15) or ld >= 1 << 22
+def _odd(address: int, ld: int, dt: int) -> bool:
+    """Whether rows have to be copied before a product: not all at multiples of 16 bytes, or 2^22 elements apart."""
+    return (address | ld * (2 if dt == BF16 else 4)) & 15 != 0 or ld >= 1 << 22
 
 
 def _act(activation: str) -> int:
@@ -1353,20 +1351,22 @@ def linear(x: Tensor, W: Tensor, bias: Tensor | None = None, residual: Tensor | 
     keep_z: a dtype, or an 8-bit format, in which z = x @ W.T + bias is kept for linear_backward; keep_x: an 8-bit format
     for x. Kept 8-bit data is a checkpoint buffer (checkpoint8_save). (sparse_coder.py:219-222: sae_out += x @ W_skip.mT)"""
     act = _act(activation)
-    _rows(x, "x")
-    N, D = x.shape
-    _rows(W, "weight", like=x)
-    M = W.shape[0]
-    if W.shape[1] != D or W.dtype != x.dtype:
+    xp, ldx, dt = _rows(x, "x")
+    Wp, ldw, w_dt = _rows(W, "weight", like=x)
+    (N, D), (M, K) = x.shape, W.shape
+    if K != D or w_dt != dt:
         raise ValueError(f"linear: x {tuple(x.shape)} {x.dtype} does not go with weight {tuple(W.shape)} {W.dtype}")
+    bp = rp = None
+    b_dt = r_dt = ldr = 0
     if bias is not None:
         _req(bias, "bias", ndim=1)
         if bias.shape[0] != M or bias.device != x.device:
             raise ValueError(f"bias: expected ({M},) on {x.device}, got {tuple(bias.shape)} on {bias.device}")
+        bp, b_dt = bias.data_ptr(), _dt(bias)
     if residual is not None:
-        _rows(residual, "residual", (N, M), like=x)
+        rp, ldr, r_dt = _rows(residual, "residual", (N, M), like=x)
         if out_dtype is None:
-            out_dtype = torch.promote_types(x.dtype, residual.dtype)
+            out_dtype = x.dtype if r_dt == dt else torch.float32
     out = x.new_empty((N, M), dtype=out_dtype)
     z = codes = z_scales = x_scales = None
     z_kind = x_fmt = z_ld = x_ld = 0
@@ -1381,20 +1381,18 @@ def linear(x: Tensor, W: Tensor, bias: Tensor | None = None, residual: Tensor | 
         codes, x_scales, x_ld = _new_codes(x, N, D)
     if N == 0:
         return out, z, codes
-    dt = _dt(x)
-    nws = _linear_bytes(dt, z_kind, N, D, M, _odd(x) + 2 * _odd(W))
+    nws = _linear_bytes(dt, z_kind, N, D, M, _odd(xp, ldx, dt) + 2 * _odd(Wp, ldw, dt))
     ws = _scratch(x, nws)
-    _call("sphip_linear", x, x.data_ptr(), _ld(x), W.data_ptr(), _ld(W), dt, _ptr(bias), 0 if bias is None else _dt(bias),
-          act, _ptr(residual), 0 if residual is None else _dt(residual), 0 if residual is None else _ld(residual),
-          out.data_ptr(), _dt(out), M, _ptr(z), z_kind, z_scales, z_ld, _ptr(codes), x_scales, x_fmt, x_ld, N, D, M, _ptr(ws), nws)
+    _call("sphip_linear", x, xp, ldx, Wp, ldw, dt, bp, b_dt, act, rp, r_dt, ldr, out.data_ptr(), _dt(out), M, _ptr(z), z_kind,
+          z_scales, z_ld, _ptr(codes), x_scales, x_fmt, x_ld, N, D, M, _ptr(ws), nws)
     return out, z, codes
 
 
 def _kept(t: Tensor, fmt: str | None, name: str, N: int, D: int, like: Tensor):
     """(address, kind, address of the scales, row stride) of something linear kept."""
     if fmt is None:
-        _rows(t, name, (N, D), like=like)
-        return t.data_ptr(), _dt(t), None, _ld(t)
+        address, ld, dt = _rows(t, name, (N, D), like=like)
+        return address, dt, None, ld
     groups, ldq = -(-N // CODE_GROUP), -(-D // 16) * 16
     _req(t, name, torch.uint8, 2)
     if t.shape != (33 * groups, ldq) or t.device != like.device:
@@ -1410,12 +1408,10 @@ def linear_backward(g: Tensor, W: Tensor, z: Tensor | None, x: Tensor | None, ac
     of None leaves that one out. z and x: tensors, or checkpoint buffers (z_fmt / x_fmt) that are read as they are. The
     products run in W's dtype (dz rounded to it once), db sums dz unrounded; every sum has a fixed order."""
     act = _act(activation)
-    _rows(g, "grad")
-    N, M = g.shape
-    _rows(W, "weight", like=g)
-    D = W.shape[1]
-    dt = _dt(W)
-    if W.shape[0] != M:
+    gp, ldg, g_dt = _rows(g, "grad")
+    Wp, ldw, dt = _rows(W, "weight", like=g)
+    (N, M), (K, D) = g.shape, W.shape
+    if K != M:
         raise ValueError(f"linear_backward: grad {tuple(g.shape)} does not go with weight {tuple(W.shape)}")
     zargs = xargs = (None, 0, None, 0)
     if act:
@@ -1433,10 +1429,10 @@ def linear_backward(g: Tensor, W: Tensor, z: Tensor | None, x: Tensor | None, ac
         return dx, None if dW is None else dW.zero_(), None if db is None else db.zero_()
     if dx is None and dW is None and db is None:
         return None, None, None
-    odd = (x_fmt is None and dW is not None and _odd(x)) + 2 * (dx is not None and _odd(W))
+    odd = (x_fmt is None and dW is not None and _odd(xargs[0], xargs[3], dt)) + 2 * (dx is not None and _odd(Wp, ldw, dt))
     nws = _linear_backward_bytes(dt, xargs[1], dx is not None, dW is not None, db is not None, N, D, M, odd)
     ws = _scratch(g, nws)
-    _call("sphip_linear_backward", g, g.data_ptr(), _dt(g), _ld(g), W.data_ptr(), _ld(W), dt, act, *zargs, *xargs,
+    _call("sphip_linear_backward", g, gp, g_dt, ldg, Wp, ldw, dt, act, *zargs, *xargs,
           _ptr(dx), 0 if dx is None else _dt(dx), D, _ptr(dW), 0 if dW is None else _dt(dW), D, _ptr(db),
           0 if db is None else _dt(db), N, D, M, _ptr(ws), nws)
     return dx, dW, db
@@ -1446,11 +1442,11 @@ def linear_backward(g: Tensor, W: Tensor, z: Tensor | None, x: Tensor | None, ac
 def checkpoint8_save(x: Tensor, fmt: str, keep_sign: bool = False) -> Tensor:
     """x (N, D) in 8 bits: uint8 (33 G, ldq), G = ceil(N / 32), ldq = D rounded up to 16; 32 G rows of codes, G of scales."""
     code = _code(fmt)
-    _rows(x, "x")
+    xp, ldx, dt = _rows(x, "x")
     N, D = x.shape
     data, scales, ldq = _new_codes(x, N, D)
     if N and D:
-        _call("sphip_checkpoint8_save", x, x.data_ptr(), _dt(x), _ld(x), code, int(keep_sign), data.data_ptr(), scales, ldq, N, D)
+        _call("sphip_checkpoint8_save", x, xp, dt, ldx, code, int(keep_sign), data.data_ptr(), scales, ldq, N, D)
     return data
 
 
