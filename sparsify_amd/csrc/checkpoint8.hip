@@ -36,6 +36,7 @@ __global__ __launch_bounds__(256) void checkpoint8_save_kernel(SaveArgs a) {
     const int cl = threadIdx.x & 31, rl = threadIdx.x >> 5, wave = threadIdx.x >> 6;
     const int64_t grp = blockIdx.x / (unsigned)a.strips, r0 = grp * 32 + rl;
     const int c0 = ((int)(blockIdx.x % (unsigned)a.strips) * 32 + cl) * V, n = a.D - c0;
+    const int miss = max(V - n, 0);                              // (see drop_front)
     unsigned w[W][4];                                            // 4 rows of 16 bytes, raw
 #pragma unroll
     for (int t = 0; t < W; ++t) {
@@ -44,18 +45,12 @@ __global__ __launch_bounds__(256) void checkpoint8_save_kernel(SaveArgs a) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) w[t][j] = 0;
         if (row >= a.N || n <= 0) continue;
-        if (n >= V) {
-            __builtin_memcpy(w[t], p, 16);
-        } else if (sizeof(T) == 2) {
-#pragma unroll
-            for (int j = 0; j < V; ++j)
-                if (j < n) w[t][j / 2] |= (unsigned)((const bf16_t*)p)[j] << ((j & 1) * 16);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (j < n) w[t][j] = ((const unsigned*)p)[j];
-        }
+        if (a.D >= V) __builtin_memcpy(w[t], p - miss, 16);
+        else load_short(p, n, w[t]);
     }
+    if (miss > 0 && a.D >= V)
+#pragma unroll
+        for (int t = 0; t < W; ++t) drop_front(w[t], miss < V ? miss * (int)sizeof(T) : 0);
     // element j of a row as fp32 bits
     auto bits = [&](int t, int j) {
         if (sizeof(T) == 4) return w[t][j % 4];

@@ -4,6 +4,29 @@
 
 namespace sphip {
 
+// The last piece of a row may hold fewer elements than 16 bytes do. Its load is moved back to end where the row ends (rows of
+// at least 16 bytes; a load per element, each waited for, took as long as the rest: saving 5001 x 1111 in 8 bits 10.1 us
+// against 8.2), and the `bytes` in front that belong to the piece before are dropped, zeros behind.
+__device__ __forceinline__ void drop_front(unsigned (&w)[4], int bytes) {
+    uint64_t lo = ((uint64_t)w[1] << 32) | w[0], hi = ((uint64_t)w[3] << 32) | w[2];
+    const int s = 8 * bytes;
+    if (s >= 64) lo = hi >> (s - 64), hi = 0;
+    else if (s > 0) lo = (lo >> s) | (hi << (64 - s)), hi >>= s;
+    w[0] = (unsigned)lo, w[1] = (unsigned)(lo >> 32), w[2] = (unsigned)hi, w[3] = (unsigned)(hi >> 32);
+}
+// n >= 1 elements from p of a row that has fewer than 16 bytes
+template <typename T> __device__ __forceinline__ void load_short(const T* p, int n, unsigned (&w)[4]) {
+    constexpr int E = 16 / sizeof(T);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] = 0;
+#pragma unroll
+    for (int j = 0; j < E - 1; ++j) {
+        if (j >= n) continue;
+        if constexpr (sizeof(T) == 2) w[j / 2] |= (unsigned)p[j] << ((j & 1) * 16);
+        else w[j] = __float_as_uint(p[j]);
+    }
+}
+
 // 2^(byte - 127); byte 255 marks a group that held an infinity or a NaN: every value of it is NaN
 __device__ __forceinline__ float scale_value(unsigned byte) {
     return __uint_as_float(byte == 255u ? 0x7fc00000u : byte << 23);

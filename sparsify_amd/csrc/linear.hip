@@ -13,39 +13,6 @@
 
 namespace sphip {
 
-template <typename T> struct Chunk;
-template <> struct Chunk<bf16_t> {
-    static constexpr int E = 8;
-    // n valid elements from p, zeros after
-    static __device__ __forceinline__ uint4 load(const bf16_t* p, int n) {
-        uint4 r = make_uint4(0, 0, 0, 0);
-        if (n >= 8) {
-            __builtin_memcpy(&r, p, 16);
-        } else if (n > 0) {
-            unsigned w[4] = {0, 0, 0, 0};
-#pragma unroll
-            for (int j = 0; j < 7; ++j)
-                if (j < n) w[j >> 1] |= (unsigned)p[j] << ((j & 1) * 16);
-            r = make_uint4(w[0], w[1], w[2], w[3]);
-        }
-        return r;
-    }
-};
-template <> struct Chunk<float> {
-    static constexpr int E = 4;
-    static __device__ __forceinline__ uint4 load(const float* p, int n) {
-        uint4 r = make_uint4(0, 0, 0, 0);
-        if (n >= 4) {
-            __builtin_memcpy(&r, p, 16);
-        } else if (n > 0) {
-            r.x = __float_as_uint(p[0]);
-            if (n > 1) r.y = __float_as_uint(p[1]);
-            if (n > 2) r.z = __float_as_uint(p[2]);
-        }
-        return r;
-    }
-};
-
 // Sum of the splits' partial tiles, then the epilogue. One thread per 4 outputs, the splits in order; with many splits of a
 // small product 8 threads share an output, each taking every eighth split (LANES = 8), their sums added in order.
 template <int LANES>
@@ -160,19 +127,32 @@ static int launch_product(const char* what, const Operand& A, const Operand& B, 
 struct PackArgs {
     const void* src[3];
     void* dst[3];
-    int64_t ld[3], n[3];                   // n: 16-byte pieces of the copy
-    int cols[3], pieces[3];                // pieces per row
+    int64_t ld[3], rows[3];
+    int cols[3], pieces[3], log[3];        // 16-byte pieces per row; a row is taken by 2^log threads of a workgroup
+    unsigned first[3];                     // the first workgroup of each (of none: behind the last)
 };
 template <typename T> __global__ __launch_bounds__(256) void linear_pack_kernel(PackArgs a) {
-    constexpr int E = Chunk<T>::E;
-    int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    int w = 0;
-    if (i >= a.n[0]) i -= a.n[0], w = 1;
-    if (w == 1 && i >= a.n[1]) i -= a.n[1], w = 2;
-    if (i >= a.n[w]) return;
-    const int64_t row = i / a.pieces[w];
-    const int c = (int)(i - row * a.pieces[w]) * E;
-    *reinterpret_cast<uint4*>((T*)a.dst[w] + i * E) = Chunk<T>::load((const T*)a.src[w] + row * a.ld[w] + c, a.cols[w] - c);
+    constexpr int E = 16 / sizeof(T);
+    const int w = (int)(blockIdx.x >= a.first[1]) + (int)(blockIdx.x >= a.first[2]);
+    const int64_t row = ((int64_t)(blockIdx.x - a.first[w]) << (8 - a.log[w])) + (threadIdx.x >> a.log[w]);
+    if (row >= a.rows[w]) return;
+    const int cols = a.cols[w], pieces = a.pieces[w];
+    const T* src = (const T*)a.src[w] + row * a.ld[w];
+    uint4* dst = (uint4*)a.dst[w] + row * pieces;
+#pragma unroll 2
+    for (int i = (int)threadIdx.x & ((1 << a.log[w]) - 1); i < pieces; i += 1 << a.log[w]) {
+        const int c = i * E, miss = max(c + E - cols, 0);
+        unsigned v[4] = {0, 0, 0, 0};
+        if (c < cols) {
+            if (cols >= E) {
+                __builtin_memcpy(v, src + c - miss, 16);
+                if (miss > 0) drop_front(v, miss * (int)sizeof(T));
+            } else {
+                load_short(src, cols, v);
+            }
+        }
+        dst[i] = make_uint4(v[0], v[1], v[2], v[3]);
+    }
 }
 static int64_t packed_ld(int64_t cols) { return cdiv(cols, 64) * 64; }
 static int64_t whole_pieces(int dtype, int64_t cols) { const int64_t e = 16 / (int64_t)dtype_size(dtype); return cdiv(cols, e) * e; }
@@ -182,15 +162,20 @@ struct Packing {
     explicit Packing(int dt) : dtype(dt) {}
     void add(Operand& o, int64_t rows, int64_t cols, void* dst) {
         const int64_t ld = packed_ld(cols);
-        a.src[count] = o.p, a.dst[count] = dst, a.ld[count] = o.ld, a.cols[count] = (int)cols;
-        a.pieces[count] = (int)(ld * (int64_t)dtype_size(dtype) / 16), a.n[count] = rows * a.pieces[count];
+        a.src[count] = o.p, a.dst[count] = dst, a.ld[count] = o.ld, a.rows[count] = rows, a.cols[count] = (int)cols;
+        a.pieces[count] = (int)(ld * (int64_t)dtype_size(dtype) / 16);
+        while (a.log[count] < 8 && (1 << a.log[count]) < a.pieces[count]) ++a.log[count];
         ++count;
         o.p = dst, o.ld = ld;
     }
     int launch(const char* what, hipStream_t s) {
         if (count == 0) return SPHIP_OK;
-        const int64_t blocks = cdiv(a.n[0] + a.n[1] + a.n[2], 256);
-        SPHIP_REQUIRE(blocks < (1ll << 31), SPHIP_EUNSUPPORTED, "%s: grid too large", what);
+        int64_t blocks = 0;
+        for (int i = 0; i < 3; ++i) {
+            a.first[i] = (unsigned)blocks;
+            if (i < count) blocks += cdiv(a.rows[i], 256 >> a.log[i]);
+            SPHIP_REQUIRE(blocks < (1ll << 31), SPHIP_EUNSUPPORTED, "%s: grid too large", what);
+        }
         if (dtype == SPHIP_BF16) hipLaunchKernelGGL(linear_pack_kernel<bf16_t>, dim3((unsigned)blocks), dim3(256), 0, s, a);
         else hipLaunchKernelGGL(linear_pack_kernel<float>, dim3((unsigned)blocks), dim3(256), 0, s, a);
         SPHIP_CHECK_LAUNCH(what);
@@ -209,27 +194,35 @@ struct PreactArgs {
     void* dz;                      // row stride lddz (zeros in [M, lddz)), or null
     float* part;                   // [ceil(N / 32)][M], or null
     int64_t ldg, ldz, lddz;
-    int dz_dt, act, strips;        // strips: workgroups side by side along a row
+    int dz_dt, strips;             // strips: workgroups side by side along a row
 };
 
-template <int V> __device__ __forceinline__ void load_row(const bf16_t* p, int n, float (&v)[V]) {
+// V elements from p
+template <int V> __device__ __forceinline__ void load_row(const bf16_t* p, float (&v)[V]) {
     unsigned w[V / 2];
-    if (n >= V) __builtin_memcpy(w, p, V * 2);
-    else
-#pragma unroll
-        for (int j = 0; j < V; ++j) w[j >> 1] = (j & 1 ? w[j >> 1] : 0u) | (j < n ? (unsigned)p[j] << ((j & 1) * 16) : 0u);
+    __builtin_memcpy(w, p, V * 2);
 #pragma unroll
     for (int j = 0; j < V; ++j) v[j] = __uint_as_float(j & 1 ? w[j >> 1] & 0xffff0000u : w[j >> 1] << 16);
 }
-template <int V> __device__ __forceinline__ void load_row(const float* p, int n, float (&v)[V]) {
-    if (n >= V) __builtin_memcpy(v, p, V * 4);
-    else
+template <int V> __device__ __forceinline__ void load_row(const float* p, float (&v)[V]) { __builtin_memcpy(v, p, V * 4); }
+// `miss` of V values dropped in front, zeros behind (see drop_front)
+template <int V> __device__ __forceinline__ void drop_values(float (&v)[V], int miss) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) v[j] = j < n ? p[j] : 0.f;
+    for (int s = 1; s < V; s *= 2)
+        if (miss & s)
+#pragma unroll
+            for (int j = 0; j < V; ++j) v[j] = j + s < V ? v[j + s] : 0.f;
+}
+// n of V elements of a row shorter than V, zeros behind
+template <int V, typename T> __device__ __forceinline__ void load_few(const T* p, int n, float (&v)[V]) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] = j < n ? Elem<T>::load(p, j) : 0.f;
 }
 
-// ZK: SPHIP_F32, SPHIP_BF16, SPHIP_INT8, SPHIP_E4M3, or -1: no activation, z is not read
-template <typename TG, int ZK>
+// ZK: SPHIP_F32, SPHIP_BF16, SPHIP_INT8, SPHIP_E4M3, or -1: no activation, z is not read. (The activation as an argument, its
+// choice at each of a thread's 32 values, made a kernel four times as long: 256 x 768 9.6 us against 8.4, 4099 x 1500 13.0
+// against 11.7.)
+template <typename TG, int ZK, int ACT>
 __global__ __launch_bounds__(256) void linear_preact_kernel(PreactArgs a, int64_t N, int M) {
     constexpr int V = 16 / sizeof(TG), B = 4;
     constexpr bool CODES = ZK == SPHIP_INT8 || ZK == SPHIP_E4M3;
@@ -237,6 +230,7 @@ __global__ __launch_bounds__(256) void linear_preact_kernel(PreactArgs a, int64_
     const int cl = threadIdx.x & 31, rl = threadIdx.x >> 5;
     const int64_t grp = blockIdx.x / (unsigned)a.strips, r0 = grp * 32 + rl;
     const int m = ((int)(blockIdx.x % (unsigned)a.strips) * 32 + cl) * V, cols = min(V, M - m);    // <= 0: padding of dz
+    const int miss = V - cols;
     float sum[V], v[B][V], z[B][V];
     unsigned q[B][V / 4];
     uint8_t s8[V];
@@ -247,15 +241,29 @@ __global__ __launch_bounds__(256) void linear_preact_kernel(PreactArgs a, int64_
     for (int t = 0; t < B; ++t) {
         const int64_t row = r0 + 8 * t;
         const int n = row < N ? cols : 0;
-        load_row<V>((const TG*)a.g + row * a.ldg + m, n, v[t]);
-        if (ZK == SPHIP_F32) load_row<V>((const float*)a.z + row * a.ldz + m, n, z[t]);
-        if (ZK == SPHIP_BF16) load_row<V>((const bf16_t*)a.z + row * a.ldz + m, n, z[t]);
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[t][j] = z[t][j] = 0.f;
+        if (n > 0 && M >= V) {
+            load_row<V>((const TG*)a.g + row * a.ldg + m - miss, v[t]);
+            if (ZK == SPHIP_F32) load_row<V>((const float*)a.z + row * a.ldz + m - miss, z[t]);
+            if (ZK == SPHIP_BF16) load_row<V>((const bf16_t*)a.z + row * a.ldz + m - miss, z[t]);
+        } else if (n > 0) {
+            load_few<V>((const TG*)a.g + row * a.ldg, n, v[t]);
+            if (ZK == SPHIP_F32) load_few<V>((const float*)a.z + row * a.ldz, n, z[t]);
+            if (ZK == SPHIP_BF16) load_few<V>((const bf16_t*)a.z + row * a.ldz, n, z[t]);
+        }
         if (CODES) {
 #pragma unroll
             for (int j = 0; j < V / 4; ++j) q[t][j] = 0;
             if (n > 0) __builtin_memcpy(q[t], (const uint8_t*)a.z + row * a.ldz + m, V);
         }
     }
+    if (cols > 0 && miss > 0 && M >= V)
+#pragma unroll
+        for (int t = 0; t < B; ++t) {
+            drop_values<V>(v[t], miss);
+            if (ZK == SPHIP_F32 || ZK == SPHIP_BF16) drop_values<V>(z[t], miss);
+        }
 #pragma unroll
     for (int t = 0; t < B; ++t) {
         const int64_t row = r0 + 8 * t;
@@ -272,7 +280,7 @@ __global__ __launch_bounds__(256) void linear_preact_kernel(PreactArgs a, int64_
         if (row >= N) continue;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            if (ZK >= 0) v[t][j] = j < cols ? v[t][j] * act_slope(z[t][j], a.act) : 0.f;
+            if (ZK >= 0) v[t][j] = j < cols ? v[t][j] * act_slope(z[t][j], ACT) : 0.f;
             sum[j] += v[t][j];
         }
         if (a.dz != nullptr) {
@@ -297,17 +305,19 @@ __global__ __launch_bounds__(256) void linear_preact_kernel(PreactArgs a, int64_
     }
 }
 
-template <typename TG> static int launch_preact(PreactArgs& a, int z_kind, int64_t N, int64_t M, hipStream_t s) {
+template <typename TG> static int launch_preact(PreactArgs& a, int act, int z_kind, int64_t N, int64_t M, hipStream_t s) {
     constexpr int V = 16 / sizeof(TG);
     const int64_t strips = cdiv(a.dz != nullptr ? a.lddz : M, 32 * V), blocks = cdiv(N, 32) * strips;
     SPHIP_REQUIRE(blocks < (1ll << 31), SPHIP_EUNSUPPORTED, "linear_backward: grid too large");
     a.strips = (int)strips;
     const dim3 grid((unsigned)blocks), block(256);
-    if (a.act == SPHIP_ACT_NONE) hipLaunchKernelGGL((linear_preact_kernel<TG, -1>), grid, block, 0, s, a, N, (int)M);
-    else if (z_kind == SPHIP_F32) hipLaunchKernelGGL((linear_preact_kernel<TG, SPHIP_F32>), grid, block, 0, s, a, N, (int)M);
-    else if (z_kind == SPHIP_BF16) hipLaunchKernelGGL((linear_preact_kernel<TG, SPHIP_BF16>), grid, block, 0, s, a, N, (int)M);
-    else if (z_kind == SPHIP_INT8) hipLaunchKernelGGL((linear_preact_kernel<TG, SPHIP_INT8>), grid, block, 0, s, a, N, (int)M);
-    else hipLaunchKernelGGL((linear_preact_kernel<TG, SPHIP_E4M3>), grid, block, 0, s, a, N, (int)M);
+    typedef void (*kern_t)(PreactArgs, int64_t, int);
+#define LIN_PREACT(ZK) {linear_preact_kernel<TG, ZK, SPHIP_ACT_RELU>, linear_preact_kernel<TG, ZK, SPHIP_ACT_GELU>, linear_preact_kernel<TG, ZK, SPHIP_ACT_SILU>}
+    static const kern_t kerns[4][3] = {LIN_PREACT(SPHIP_F32), LIN_PREACT(SPHIP_BF16), LIN_PREACT(SPHIP_INT8), LIN_PREACT(SPHIP_E4M3)};
+#undef LIN_PREACT
+    const int zk = z_kind == SPHIP_F32 ? 0 : z_kind == SPHIP_BF16 ? 1 : z_kind == SPHIP_INT8 ? 2 : 3;
+    const kern_t fn = act == SPHIP_ACT_NONE ? linear_preact_kernel<TG, -1, SPHIP_ACT_NONE> : kerns[zk][act - SPHIP_ACT_RELU];
+    hipLaunchKernelGGL(fn, grid, block, 0, s, a, N, (int)M);
     SPHIP_CHECK_LAUNCH("linear_backward(dz)");
     return SPHIP_OK;
 }
@@ -548,8 +558,8 @@ extern "C" int sphip_linear_backward(const void* g, int g_dtype, int64_t ldg, co
     if (!copied && (db || (products && !direct))) {
         PreactArgs a;
         a.g = g, a.z = z, a.scales = z_scales, a.dz = products && !direct ? w : nullptr, a.part = db ? sums : nullptr;
-        a.ldg = ldg, a.ldz = ldz, a.lddz = dz.ld, a.dz_dt = dtype, a.act = act;
-        st = g_dtype == SPHIP_BF16 ? launch_preact<bf16_t>(a, z_kind, N, M, s) : launch_preact<float>(a, z_kind, N, M, s);
+        a.ldg = ldg, a.ldz = ldz, a.lddz = dz.ld, a.dz_dt = dtype;
+        st = g_dtype == SPHIP_BF16 ? launch_preact<bf16_t>(a, act, z_kind, N, M, s) : launch_preact<float>(a, act, z_kind, N, M, s);
         if (st != SPHIP_OK) return st;
     }
     if (db || (dW && xc)) {
