@@ -71,10 +71,10 @@ static int64_t product_ns(int dtype, int by, int64_t N, int64_t M, int64_t K) {
 static int kernel_for(int dtype, int64_t N, int64_t M, int64_t K) {
     if (g_forced == '6') return BY_64;
     if (g_forced == '1' || g_forced == '2') return g_forced == '2' && dtype == SPHIP_BF16 ? BY_256 : BY_128;
-    // The 256 x 256 kernel where its tiles fill most of the 256 compute units once: 16384 x 1024 x 4096 takes 101 us against
-    // 118 with 128 x 128 tiles, 8192 x 2048 x 2048 56 against 68; with fewer the smaller tiles win (2048^3 22 against 37).
+    // The 256 x 256 kernel where its tiles fill most of the 256 compute units once: 16384 x 1024 x 4096 takes 117 us against
+    // 136 with 128 x 128 tiles, 8192 x 2048 x 2048 53 against 62; with fewer the smaller tiles win (2048^3 24 against 37).
     if (dtype == SPHIP_BF16 && cdiv(N, 256) * cdiv(M, 256) >= 160) return BY_256;
-    // 64 against 128: 1024^3 7.1 us / 14.9, 2048 x 512 x 512 in fp32 13 / 24, but 2048^3 27 / 22 and 16384 tokens' gradient of
+    // 64 against 128: 1024^3 7.1 us / 14.9, 2048 x 512 x 512 in fp32 13 / 24, but 2048^3 27 / 24 and 16384 tokens' gradient of
     // a 768 x 768 weight 56 / 32
     return product_ns(dtype, BY_64, N, M, K) <= product_ns(dtype, BY_128, N, M, K) ? BY_64 : BY_128;
 }
