@@ -123,7 +123,9 @@ template <typename T, int FMT> __device__ __forceinline__ void restore_block(con
             Elem<T>::store(o, j, f * s[j]);                                  // exact
         }
         T* p = (T*)a.out + row * a.ldo + c0;
-        if (n >= V) __builtin_memcpy(p, o, sizeof(o));
+        // past the caches (65536 x 4096 bf16 190 -> 125 us, 4096 x 4096 13.3 -> 7.3)
+        typedef unsigned u4_out __attribute__((ext_vector_type(4), aligned(2)));
+        if (n >= V) __builtin_nontemporal_store(__builtin_bit_cast(u4_out, o), (u4_out*)p);
         else
 #pragma unroll
             for (int j = 0; j < V; ++j)

@@ -102,6 +102,15 @@ __device__ __forceinline__ void store4_from_f32(void* p, int dt, int64_t i, cons
                                               (unsigned)f32_to_bf16(v[2]) | ((unsigned)f32_to_bf16(v[3]) << 16)};
     else *(u4_any*)((float*)p + i) = (u4_any){__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
 }
+// the same past the caches: what no kernel reads soon
+__device__ __forceinline__ void store4_stream(void* p, int dt, int64_t i, const float (&v)[4]) {
+    if (dt == SPHIP_BF16)
+        __builtin_nontemporal_store((u2_any){(unsigned)f32_to_bf16(v[0]) | ((unsigned)f32_to_bf16(v[1]) << 16),
+                                             (unsigned)f32_to_bf16(v[2]) | ((unsigned)f32_to_bf16(v[3]) << 16)}, (u2_any*)((bf16_t*)p + i));
+    else
+        __builtin_nontemporal_store((u4_any){__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])},
+                                    (u4_any*)((float*)p + i));
+}
 __device__ __forceinline__ void store_from_f32(void* p, int dt, int64_t i, float v) {
     if (dt == SPHIP_BF16) ((bf16_t*)p)[i] = f32_to_bf16(v);
     else ((float*)p)[i] = v;

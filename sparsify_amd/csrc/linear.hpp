@@ -187,7 +187,7 @@ __device__ __forceinline__ void finish_rows(char* stage, const Epilogue& epi, co
                 const float4 c = *at;
                 float v[4] = {c.x + bias[0], c.y + bias[1], c.z + bias[2], c.w + bias[3]};
                 if (values && n < N) {
-                    if (cols >= 4) store4_from_f32(epi.z, epi.z_dt, n * epi.ldz + m, v);
+                    if (cols >= 4) store4_stream(epi.z, epi.z_dt, n * epi.ldz + m, v);
                     else
 #pragma unroll
                         for (int j = 0; j < 3; ++j)
@@ -210,14 +210,7 @@ __device__ __forceinline__ void finish_rows(char* stage, const Epilogue& epi, co
                 for (int j = 0; j < 4; ++j) v[j] += r[j];
             }
             if (cols >= 4) {
-                if (epi.out_dt == SPHIP_F32) {
-                    const u4_any o = {__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
-                    __builtin_nontemporal_store(o, (u4_any*)((float*)epi.out + n * epi.ldo + m));
-                } else {
-                    const u2_any o = {(unsigned)f32_to_bf16(v[0]) | ((unsigned)f32_to_bf16(v[1]) << 16),
-                                      (unsigned)f32_to_bf16(v[2]) | ((unsigned)f32_to_bf16(v[3]) << 16)};
-                    __builtin_nontemporal_store(o, (u2_any*)((bf16_t*)epi.out + n * epi.ldo + m));
-                }
+                store4_stream(epi.out, epi.out_dt, n * epi.ldo + m, v);
             } else {
 #pragma unroll
                 for (int j = 0; j < 3; ++j)
