@@ -130,7 +130,7 @@ int save_codes(const char* what, const void* x, int dtype, int64_t ldx, int fmt,
                int64_t ldq, void* packed, int64_t ldp, int64_t N, int64_t D, hipStream_t s) {
     const int V = dtype == SPHIP_BF16 ? 8 : 4;
     const int64_t strips = cdiv(packed && ldp > ldq ? ldp : ldq, 32 * V), blocks = cdiv(N, 32) * strips;
-    SPHIP_REQUIRE(blocks < (1ll << 31), SPHIP_EUNSUPPORTED, "%s: grid too large", what);
+    SPHIP_REQUIRE(blocks < MAX_GROUPS, SPHIP_EUNSUPPORTED, "%s: grid too large", what);
     const SaveArgs a = {x, codes, scales, packed, ldx, ldq, ldp, N, (int)D, (int)strips, keep_sign};
     const dim3 grid((unsigned)blocks), block(256);
     if (dtype == SPHIP_BF16) {
@@ -166,7 +166,7 @@ extern "C" int sphip_checkpoint8_restore(const uint8_t* codes, const uint8_t* sc
     hipStream_t s = (hipStream_t)stream;
     const RestoreArgs a = {codes, scales, out, ldq, ldo, N, (int)D};
     const int64_t blocks = restore_blocks(a, dtype);
-    SPHIP_REQUIRE(blocks < (1ll << 31), SPHIP_EUNSUPPORTED, "checkpoint8_restore: grid too large");
+    SPHIP_REQUIRE(blocks < MAX_GROUPS, SPHIP_EUNSUPPORTED, "checkpoint8_restore: grid too large");
 #define SPHIP_RESTORE(T, F) hipLaunchKernelGGL((checkpoint8_restore_kernel<T, F>), dim3((unsigned)blocks), dim3(256), 0, s, a)
     if (dtype == SPHIP_BF16) {
         if (fmt == SPHIP_INT8) SPHIP_RESTORE(bf16_t, SPHIP_INT8);

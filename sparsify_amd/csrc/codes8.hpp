@@ -4,6 +4,8 @@
 
 namespace sphip {
 
+constexpr int64_t MAX_GROUPS = 1ll << 23;          // workgroups in a launch of up to 512 threads each: fewer than 2^32 work-items
+
 // The last piece of a row may hold fewer elements than 16 bytes do. Its load is moved back to end where the row ends (rows of
 // at least 16 bytes; a load per element, each waited for, took as long as the rest: saving 5001 x 1111 in 8 bits 10.1 us
 // against 8.2), and the `bytes` in front that belong to the piece before are dropped, zeros behind.

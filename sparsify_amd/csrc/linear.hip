@@ -105,7 +105,7 @@ static int launch_product(const char* what, const Operand& A, const Operand& B, 
                       "%s: workspace of %zu bytes, needs %zu, 16-byte aligned", what, ws_bytes, need);
     }
     const int64_t nblocks = (int64_t)g.tilesM * g.tilesN * g.splits, threads = N * ((M + 3) / 4);
-    SPHIP_REQUIRE(nblocks < (1ll << 31) && (g.splits == 1 || cdiv(threads, 256) < (1ll << 31)), SPHIP_EUNSUPPORTED,
+    SPHIP_REQUIRE(nblocks < MAX_GROUPS && (g.splits == 1 || cdiv(threads, 256) < MAX_GROUPS), SPHIP_EUNSUPPORTED,
                   "%s: grid too large", what);
     const int st = by == BY_256 ? launch_linear256(what, MODE_A, MODE_B, A, B, epi, K, KB, g, s)
                  : by == BY_128 ? launch_linear128(what, dtype, MODE_A, MODE_B, A, B, epi, K, KB, g, s)
@@ -174,7 +174,7 @@ struct Packing {
         for (int i = 0; i < 3; ++i) {
             a.first[i] = (unsigned)blocks;
             if (i < count) blocks += cdiv(a.rows[i], 256 >> a.log[i]);
-            SPHIP_REQUIRE(blocks < (1ll << 31), SPHIP_EUNSUPPORTED, "%s: grid too large", what);
+            SPHIP_REQUIRE(blocks < MAX_GROUPS, SPHIP_EUNSUPPORTED, "%s: grid too large", what);
         }
         if (dtype == SPHIP_BF16) hipLaunchKernelGGL(linear_pack_kernel<bf16_t>, dim3((unsigned)blocks), dim3(256), 0, s, a);
         else hipLaunchKernelGGL(linear_pack_kernel<float>, dim3((unsigned)blocks), dim3(256), 0, s, a);
@@ -308,7 +308,7 @@ __global__ __launch_bounds__(256) void linear_preact_kernel(PreactArgs a, int64_
 template <typename TG> static int launch_preact(PreactArgs& a, int act, int z_kind, int64_t N, int64_t M, hipStream_t s) {
     constexpr int V = 16 / sizeof(TG);
     const int64_t strips = cdiv(a.dz != nullptr ? a.lddz : M, 32 * V), blocks = cdiv(N, 32) * strips;
-    SPHIP_REQUIRE(blocks < (1ll << 31), SPHIP_EUNSUPPORTED, "linear_backward: grid too large");
+    SPHIP_REQUIRE(blocks < MAX_GROUPS, SPHIP_EUNSUPPORTED, "linear_backward: grid too large");
     a.strips = (int)strips;
     const dim3 grid((unsigned)blocks), block(256);
     typedef void (*kern_t)(PreactArgs, int64_t, int);
@@ -354,7 +354,7 @@ template <typename T, int FMT> __global__ __launch_bounds__(256) void linear_fin
 }
 static int launch_finish(FinishArgs& a, int dtype, int fmt, hipStream_t s) {
     const int64_t restore = a.x.codes ? restore_blocks(a.x, dtype) : 0, blocks = restore + (a.db ? cdiv(a.M, 16) : 0);
-    SPHIP_REQUIRE(blocks < (1ll << 31), SPHIP_EUNSUPPORTED, "linear_backward: grid too large");
+    SPHIP_REQUIRE(blocks < MAX_GROUPS, SPHIP_EUNSUPPORTED, "linear_backward: grid too large");
     a.restore = (unsigned)restore;
     const dim3 grid((unsigned)blocks), block(256);
     if (dtype == SPHIP_BF16) {

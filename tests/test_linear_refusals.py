@@ -89,6 +89,16 @@ def test_longest_rows():
         assert backward(**kw) == EUNSUPPORTED and b"2^22" in lib().sphip_last_error()
 
 
+def test_more_work_than_a_launch_holds():
+    N = (1 << 31) - 300
+    assert linear(N=N, M=4096, ldo=4096) == EUNSUPPORTED and b"grid" in lib().sphip_last_error()
+    L = lib()
+    assert L.sphip_checkpoint8_save(P, BF16, 64, INT8, 0, P, P, 64, N, 64, None) == EUNSUPPORTED and b"grid" in L.sphip_last_error()
+    assert L.sphip_checkpoint8_restore(P, P, 256, INT8, P, BF16, 256, N, 256, None) == EUNSUPPORTED and b"grid" in L.sphip_last_error()
+    nws = L.sphip_linear_backward_workspace_bytes(BF16, BF16, 0, 0, 1, N, 64, 32, 0)
+    assert backward(N=N, dx=None, dW=None, db=P, db_dtype=F32, ws=P, nws=nws) == EUNSUPPORTED and b"grid" in L.sphip_last_error()
+
+
 def test_checkpoint_entries():
     L = lib()
 
