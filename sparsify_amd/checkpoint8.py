@@ -54,8 +54,8 @@ def checkpoint8(x: Tensor, fmt: str = "int8", *, keep_sign: bool = False) -> Che
 
 
 def as_rows(t: Tensor) -> Tensor:
-    """(..., D) as (tokens, D) with columns next to each other: a view where the strides allow one. Detached."""
-    t = t.detach()
+    """(..., D) as (tokens, D) with columns next to each other: t itself or a view where the strides allow one. For kernels,
+    which read addresses: no autograd history is wanted of it."""
     if t.ndim != 2:
-        t = t.reshape(t.shape[:-1].numel(), t.shape[-1])
-    return t if ops.is_rows(t) else t.contiguous()
+        t = t.detach().reshape(t.shape[:-1].numel(), t.shape[-1])
+    return t if ops.is_rows(t) else t.detach().contiguous()

@@ -1,4 +1,4 @@
-// Shared by the kernels of the dense product (linear.hip, linear256.hip).
+// Shared by the kernels of the dense product (linear.hip, linear_few.hip, linear64.hip, linear128.hip, linear256.hip).
 #pragma once
 #include "codes8.hpp"
 #include "epilogue.hpp"

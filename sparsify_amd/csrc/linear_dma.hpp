@@ -1,4 +1,5 @@
-// LDS-DMA staging and fragment reads shared by the dense product's kernels (linear256.hip: bf16, linear128.hip: bf16, fp32).
+// LDS-DMA staging and fragment reads shared by the dense product's kernels (linear64.hip, linear128.hip: bf16, fp32;
+// linear256.hip: bf16).
 //
 // An operand is either contiguous in K (OP_ROWS: image [row][8 chunks of 8 k], chunk XOR (row >> 1) & 7, ds_read_b128) or
 // contiguous in its rows (OP_COLS: the gradient products). The latter is not transposed in memory: its image is [k][chunks

@@ -45,7 +45,7 @@ class FusedLinear(torch.autograd.Function):
         keep_z = None
         if activation != "none" and (need_x or need_w or need_b):
             keep_z = x.dtype if fmt is None else fmt
-        y, z, codes = ops.linear(x, w, None if bias is None else bias.detach().contiguous(),
+        y, z, codes = ops.linear(x, w, None if bias is None else bias.contiguous(),
                                  None if residual is None else as_rows(residual), activation, keep_z=keep_z,
                                  keep_x=fmt if need_w and made is None else None)
         kept_x = None
@@ -92,13 +92,15 @@ def fused_linear(input: Tensor, weight: Tensor, bias: Tensor | None = None, *, r
     gradients are those at the restored values. A Checkpoint8 of this very input (already made for another layer that
     reads it) is kept instead of a second one."""
     ops._act(activation)
-    if weight.ndim != 2 or input.ndim < 1 or input.shape[-1] != weight.shape[1] or 0 in weight.shape:
-        raise ValueError(f"fused_linear: input {tuple(input.shape)} does not go with weight {tuple(weight.shape)}")
-    M = weight.shape[0]
+    in_shape, w_shape = input.shape, weight.shape
+    if len(w_shape) != 2 or not in_shape or in_shape[-1] != w_shape[1] or 0 in w_shape:
+        raise ValueError(f"fused_linear: input {tuple(in_shape)} does not go with weight {tuple(w_shape)}")
+    M = w_shape[0]
+    out_shape = (*in_shape[:-1], M)
     if bias is not None and bias.shape != (M,):
         raise ValueError(f"fused_linear: bias must be ({M},), got {tuple(bias.shape)}")
-    if residual is not None and residual.shape != (*input.shape[:-1], M):
-        raise ValueError(f"fused_linear: residual must be {(*input.shape[:-1], M)}, got {tuple(residual.shape)}")
+    if residual is not None and residual.shape != out_shape:
+        raise ValueError(f"fused_linear: residual must be {out_shape}, got {tuple(residual.shape)}")
     if isinstance(checkpoint, Checkpoint8):
         if checkpoint.shape != input.shape or checkpoint.device != input.device:
             raise ValueError(f"fused_linear: the checkpoint holds {tuple(checkpoint.shape)} on {checkpoint.device}, "
@@ -109,6 +111,6 @@ def fused_linear(input: Tensor, weight: Tensor, bias: Tensor | None = None, *, r
                                     or (residual is not None and residual.requires_grad)):
         return FusedLinear.apply(input, weight, bias, residual, activation, checkpoint)
     x, w = _operands(input, weight)
-    y = ops.linear(x, w, None if bias is None else bias.detach().contiguous(), None if residual is None else as_rows(residual),
+    y = ops.linear(x, w, None if bias is None else bias.contiguous(), None if residual is None else as_rows(residual),
                    activation)[0]
-    return y if input.ndim == 2 else y.reshape(*input.shape[:-1], M)
+    return y if len(out_shape) == 2 else y.reshape(out_shape)
