@@ -60,13 +60,14 @@ static int splits_of(int dtype, int by, int64_t N, int64_t M, int64_t K) {
 }
 // Time of a product with 64 x 64 or 128 x 128 tiles in ns, without what both take: K steps one after the other, a step of one
 // workgroup `step` (measured: 64 x 64 200 bf16, 520 fp32; 128 x 128 570 and 2100 alone on its compute unit, 400 and 1950 where
-// two share one), and for a split K range the joining launch and a round trip of the partial tiles at 3 TB/s.
+// two share one), 1.2 us more of filling and finishing for the larger tile, and for a split K range the joining launch and a
+// round trip of the partial tiles at 3 TB/s.
 static int64_t product_ns(int dtype, int by, int64_t N, int64_t M, int64_t K) {
     const int64_t tile = by == BY_64 ? 64 : 128, splits = splits_of(dtype, by, N, M, K);
     const int64_t groups = cdiv(N, tile) * cdiv(M, tile) * splits, steps = cdiv(cdiv(K, 128 / (int64_t)dtype_size(dtype)), splits);
     const bool bf = dtype == SPHIP_BF16;
     const int64_t step = by == BY_64 ? (bf ? 200 : 520) : groups <= 256 ? (bf ? 570 : 2100) : (bf ? 400 : 1950);
-    return steps * step * cdiv(groups, 256) + (splits > 1 ? 4000 + splits * N * M / 375 : 0);
+    return steps * step * cdiv(groups, 256) + (by == BY_64 ? 0 : 1200) + (splits > 1 ? 4000 + splits * N * M / 375 : 0);
 }
 static int kernel_for(int dtype, int64_t N, int64_t M, int64_t K) {
     if (g_forced == '6') return BY_64;
@@ -74,8 +75,8 @@ static int kernel_for(int dtype, int64_t N, int64_t M, int64_t K) {
     // The 256 x 256 kernel where its tiles fill most of the 256 compute units once: 16384 x 1024 x 4096 takes 117 us against
     // 136 with 128 x 128 tiles, 8192 x 2048 x 2048 53 against 62; with fewer the smaller tiles win (2048^3 24 against 37).
     if (dtype == SPHIP_BF16 && cdiv(N, 256) * cdiv(M, 256) >= 160) return BY_256;
-    // 64 against 128: 1024^3 7.1 us / 14.9, 2048 x 512 x 512 in fp32 13 / 24, but 2048^3 27 / 24 and 16384 tokens' gradient of
-    // a 768 x 768 weight 56 / 32
+    // 64 against 128: 1024^3 7.1 us / 14.9, 2048 x 512 x 512 in fp32 13 / 24, 1003 x 769 x 2050 with bias, SiLU and residual
+    // 22.5 / 25.1, but 2048^3 27 / 24 and 16384 tokens' gradient of a 768 x 768 weight 56 / 32
     return product_ns(dtype, BY_64, N, M, K) <= product_ns(dtype, BY_128, N, M, K) ? BY_64 : BY_128;
 }
 
@@ -395,14 +396,24 @@ struct ForwardSpace {
     bool one;
 };
 // Whether the forward product takes linear_few.hip: one launch, no copies, but its workgroups read all of x each and share K
-// among 8 waves only. us here / with 64 x 64 tiles: bf16 1 x 4096 x 4096 6.9 / 8.8, 16 x 4096 x 4096 9.5 / 9.2,
-// 16 x 8192 x 256 16 / 7, 64 x 4096 x 4096 20 / 11; fp32 16 x 4096 x 4096 17 / 24, 64 x 2048 x 2048 21 / 12. With more rows
-// only where the tiles would need a copy of operands that are small: 40 x 333 x 777 7.0 / 8.3, in fp32 5.7 / 13.6.
-static bool few(int64_t N, int64_t D, int64_t M, int copies) {
+// among 8 waves only. us here / with 64 x 64 tiles:
+//   bf16, up to 16 tokens: one token 4096 x 4096 7.3 / 9.3, 4096 x 8192 12.8 / 14.8, 8192 x 8192 21.2 / 23.4; 16 tokens 2048 x
+//   8192 8.1 / 10.4, 4096 x 4096 9.8 / 9.8, but 8192 x 256 16 / 7, 8192 x 8192 30 / 24, and beyond one round of workgroups the
+//   tiles stream W faster: 4096 x 14336 23.5 / 18.9. 24 tokens: 768 x 768 4.5 / 6.1, 2048 x 8192 9.4 / 10.6, 4096 x 4096 12.2 / 10.
+//   fp32: one token 4096 x 4096 13 / 25, 16 tokens 8192 x 28672 228 / 263, but 8192 x 256 29 / 10; 24 tokens 4096 x 4096 23.2 /
+//   25.5, 4096 x 14336 71 / 77, but 4096 x 28672 140 / 135, 2048 x 2048 12.7 / 11.2.
+// Where the tiles would have to copy W or x first: in fp32 any, in bf16 as long as x is short (24 x 2049 x 8192 and 40 x 333 x
+// 777 7.0 / 8.3, but 48 x 1537 x 3333 22 / 17, 16 x 4097 x 4096 27 / 24).
+static bool few(int dtype, int64_t N, int64_t D, int64_t M, int copies) {
     if (N > FEW || (g_forced && g_forced != 'f')) return false;
     if (g_forced) return true;
-    if (N <= 16) return D <= 4096 || M >= 4096;
-    return D <= 1024 && copies;
+    const bool bf = dtype == SPHIP_BF16;
+    if (copies) return !bf || N * D <= 65536;
+    if (N > 32) return false;
+    if (!bf) return N <= 16 ? D <= 4096 || M >= 2048 : D <= 1024 || (M >= 4096 && (M <= 16384 || D <= 2048));
+    if (M > 8192) return false;
+    if (N <= 16) return D <= 4096 || (N == 1 && M >= 4096);
+    return D <= (cdiv(M, 32) >= 256 ? 2048 : 1024);
 }
 // Which of the operands have to be copied, for a query and for a launch alike; `odd`: bits of those that are not fetchable().
 // Where the rows of x are no whole 16-byte pieces, what follows a row would be multiplied with what follows one of W: both.
@@ -413,7 +424,7 @@ static int odd_rows(const void* x, int64_t ldx, const void* W, int64_t ldw, int 
 static ForwardSpace forward_space(int dtype, int z_kind, int64_t N, int64_t D, int64_t M, int odd) {
     ForwardSpace f;
     f.copies = unaligned(dtype, D) ? COPY_X | COPY_W : odd & (COPY_X | COPY_W);
-    f.one = few(N, D, M, f.copies);
+    f.one = few(dtype, N, D, M, f.copies);
     const bool one = f.one;
     if (one) f.copies = 0;
     f.part = one ? 0 : up256(split_bytes(dtype, N, M, D));

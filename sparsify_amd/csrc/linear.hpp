@@ -58,42 +58,57 @@ typedef unsigned w4_t __attribute__((ext_vector_type(4)));
 typedef unsigned w2_t __attribute__((ext_vector_type(2)));
 typedef void __attribute__((address_space(3)))* lds_t;
 
-// The tail the product's kernels share: ROWS x 64 values of C that a wave has put into its own LDS area [row][OUT_ROW bytes],
-// row r being n = n0 + r, leave so that 16 lanes store 64 consecutive m of a row. A lane keeps its m: one bias load.
+// The tail the product's kernels share: ROWS x COLS values of C that a wave has put into its own LDS area [row][out_row(COLS)
+// bytes], row r being n = n0 + r, leave so that COLS / 4 lanes store COLS consecutive m of a row. A lane keeps its m: one bias
+// load.
 // The activation and the 8-bit codes of z are rolled loops over LDS, not unrolled with the rest: inlined per output quad
 // they made kernels of 60 to 90 KB, more than the instruction cache holds. Residual and result bypass L2, which holds the
 // operands.
-constexpr int OUT_ROW = 272;                       // 64 fp32 + 16 bytes
+constexpr int out_row(int cols) { return cols * 4 + 16; }
+constexpr int OUT_ROW = out_row(64);
 
-// The lane's residual pieces, raw, all in flight before the first is used: little else hides their latency. No branch and no
-// arithmetic between the loads (either would wait for them one by one): rows past the end load the last row again.
-template <int ROWS> struct Residual {
-    w4_t v[ROWS / 4];
+// The lane's residual pieces and its 4 of the bias, raw, all in flight before the first is used: little else hides their
+// latency. No branch and no arithmetic between the loads (either would wait for them one by one): rows past the end load the
+// last row again, columns past the end the last column.
+template <int ROWS, int COLS = 64> struct Residual {
+    static constexpr int LANES = COLS / 4, STEP = 64 / LANES, P = ROWS / STEP;     // lanes of a row, rows of a piece, pieces
+    w4_t v[P], b;
     __device__ __forceinline__ void load(const Epilogue& epi, const TileGrid& g, int n0, int m0, int N, int M, int lane) {
-        const int m = m0 + (lane & 15) * 4, nb = n0 + (lane >> 4), cols = M - m;
-        if (epi.res == nullptr || g.splits > 1 || cols <= 0) return;
+        const int m = m0 + lane % LANES * 4, nb = n0 + lane / LANES, cols = M - m;
+        if (g.splits > 1 || cols <= 0) return;
+        if (epi.bias != nullptr) {
+            const int c1 = min(1, cols - 1), c2 = min(2, cols - 1), c3 = min(3, cols - 1);
+            if (epi.bias_dt == SPHIP_F32) {
+                const unsigned* p = (const unsigned*)epi.bias + m;
+                b = (w4_t){p[0], p[c1], p[c2], p[c3]};
+            } else {
+                const bf16_t* p = (const bf16_t*)epi.bias + m;
+                b = (w4_t){p[0], p[c1], p[c2], p[c3]};
+            }
+        }
+        if (epi.res == nullptr) return;
         if (cols >= 4) {
             if (epi.res_dt == SPHIP_F32) {
 #pragma unroll
-                for (int i = 0; i < ROWS / 4; ++i)
-                    v[i] = __builtin_nontemporal_load((const u4_any*)((const float*)epi.res + (int64_t)min(nb + 4 * i, N - 1) * epi.ldr + m));
+                for (int i = 0; i < P; ++i)
+                    v[i] = __builtin_nontemporal_load((const u4_any*)((const float*)epi.res + (int64_t)min(nb + STEP * i, N - 1) * epi.ldr + m));
             } else {
 #pragma unroll
-                for (int i = 0; i < ROWS / 4; ++i) {
-                    const u2_any r = __builtin_nontemporal_load((const u2_any*)((const bf16_t*)epi.res + (int64_t)min(nb + 4 * i, N - 1) * epi.ldr + m));
+                for (int i = 0; i < P; ++i) {
+                    const u2_any r = __builtin_nontemporal_load((const u2_any*)((const bf16_t*)epi.res + (int64_t)min(nb + STEP * i, N - 1) * epi.ldr + m));
                     v[i].x = r.x, v[i].y = r.y;
                 }
             }
         } else if (epi.res_dt == SPHIP_F32) {      // the row's last, partial piece: missing columns load the last one again
 #pragma unroll
-            for (int i = 0; i < ROWS / 4; ++i) {
-                const unsigned* p = (const unsigned*)epi.res + (int64_t)min(nb + 4 * i, N - 1) * epi.ldr + m;
+            for (int i = 0; i < P; ++i) {
+                const unsigned* p = (const unsigned*)epi.res + (int64_t)min(nb + STEP * i, N - 1) * epi.ldr + m;
                 v[i].x = p[0], v[i].y = p[min(1, cols - 1)], v[i].z = p[cols - 1];
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < ROWS / 4; ++i) {
-                const bf16_t* p = (const bf16_t*)epi.res + (int64_t)min(nb + 4 * i, N - 1) * epi.ldr + m;
+            for (int i = 0; i < P; ++i) {
+                const bf16_t* p = (const bf16_t*)epi.res + (int64_t)min(nb + STEP * i, N - 1) * epi.ldr + m;
                 v[i].x = p[0], v[i].y = p[min(1, cols - 1)], v[i].z = p[cols - 1];
             }
         }
@@ -112,15 +127,16 @@ template <int ROWS> struct Residual {
     }
 };
 
-// z + bias of 32 staged rows (a group of the checkpoint) into 8-bit codes: the maxima of a lane's 4 columns over its 8 rows,
-// then over the 4 lanes that share them; padding rows and columns get zero codes
-template <int FMT>
+// z + bias of 32 staged rows (a group of the checkpoint) into 8-bit codes: the maxima of a lane's 4 columns over its rows,
+// then over the lanes that share them; padding rows and columns get zero codes
+template <int FMT, int COLS>
 __device__ __forceinline__ void store_codes(const char* mine, const Epilogue& epi, int nb, int m, int N, int M, const float (&bias)[4], int lane) {
-    float v[8][4];
+    constexpr int LANES = COLS / 4, STEP = 64 / LANES, P = 32 / STEP;
+    float v[P][4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float4 c = *reinterpret_cast<const float4*>(mine + i * 4 * OUT_ROW);
-        const bool in = nb + 4 * i < N;
+    for (int i = 0; i < P; ++i) {
+        const float4 c = *reinterpret_cast<const float4*>(mine + i * STEP * out_row(COLS));
+        const bool in = nb + STEP * i < N;
         v[i][0] = in && m < M ? c.x + bias[0] : 0.f, v[i][1] = in && m + 1 < M ? c.y + bias[1] : 0.f;
         v[i][2] = in && m + 2 < M ? c.z + bias[2] : 0.f, v[i][3] = in && m + 3 < M ? c.w + bias[3] : 0.f;
     }
@@ -130,60 +146,56 @@ __device__ __forceinline__ void store_codes(const char* mine, const Epilogue& ep
     for (int j = 0; j < 4; ++j) {
         unsigned top = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i][j]) & 0x7fffffffu);
-        top = max(top, (unsigned)__shfl_xor((int)top, 16, 64));
-        top = max(top, (unsigned)__shfl_xor((int)top, 32, 64));
+        for (int i = 0; i < P; ++i) top = max(top, __float_as_uint(v[i][j]) & 0x7fffffffu);
+#pragma unroll
+        for (int o = LANES; o < 64; o *= 2) top = max(top, (unsigned)__shfl_xor((int)top, o, 64));
         const unsigned b = scale_byte<FMT>(top);
         scales |= b << (8 * j);
         bad |= b == 255u ? 0xffu << (8 * j) : 0u;
         inv[j] = inverse_scale(b);
     }
-    if (m >= epi.ldz || nb - (lane >> 4) >= N) return;
-    if (lane < 16) *reinterpret_cast<unsigned*>(epi.z_scales + (int64_t)(nb >> 5) * epi.ldz + m) = scales;
+    if (m >= epi.ldz || nb - lane / LANES >= N) return;
+    if (lane < LANES) *reinterpret_cast<unsigned*>(epi.z_scales + (int64_t)(nb >> 5) * epi.ldz + m) = scales;
     const bool keep = epi.act == SPHIP_ACT_RELU;
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-        *reinterpret_cast<unsigned*>((uint8_t*)epi.z + (int64_t)(nb + 4 * i) * epi.ldz + m) = codes_of<FMT>(v[i], inv, keep, bad);
+    for (int i = 0; i < P; ++i)
+        *reinterpret_cast<unsigned*>((uint8_t*)epi.z + (int64_t)(nb + STEP * i) * epi.ldz + m) = codes_of<FMT>(v[i], inv, keep, bad);
 }
 
-template <int ROWS>
+template <int ROWS, int COLS>
 __device__ __forceinline__ void finish_rows(char* stage, const Epilogue& epi, const TileGrid& g, unsigned split, int n0, int m0,
-                                            int N, int M, int lane, const Residual<ROWS>& res) {
-    constexpr int P = ROWS / 4;                    // pieces of 4 outputs per lane
-    const int r16 = lane & 15, q4 = lane >> 4, Mp = (M + 3) & ~3;
-    const int m = m0 + r16 * 4, nb = n0 + q4, cols = M - m;
-    char* const mine = stage + q4 * OUT_ROW + r16 * 16;        // piece i is 4 OUT_ROW i further on
+                                            int N, int M, int lane, const Residual<ROWS, COLS>& res) {
+    constexpr int LANES = COLS / 4, STEP = 64 / LANES, P = ROWS / STEP, PITCH = out_row(COLS);
+    const int Mp = (M + 3) & ~3;
+    const int m = m0 + lane % LANES * 4, nb = n0 + lane / LANES, cols = M - m;
+    char* const mine = stage + lane / LANES * PITCH + lane % LANES * 16;           // piece i is STEP rows of PITCH further on
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     if (g.splits > 1) {
 #pragma unroll 4
         for (int i = 0; i < P; ++i)
-            if (nb + 4 * i < N && cols > 0)
-                *reinterpret_cast<float4*>(g.part + ((int64_t)split * N + nb + 4 * i) * Mp + m) =
-                    *reinterpret_cast<const float4*>(mine + i * 4 * OUT_ROW);
+            if (nb + STEP * i < N && cols > 0)
+                *reinterpret_cast<float4*>(g.part + ((int64_t)split * N + nb + STEP * i) * Mp + m) =
+                    *reinterpret_cast<const float4*>(mine + i * STEP * PITCH);
     } else {
         float bias[4] = {0.f, 0.f, 0.f, 0.f};
-        if (epi.bias != nullptr) {
-            if (cols >= 4) load4_as_f32(epi.bias, epi.bias_dt, m, bias);
-            else
+        if (epi.bias != nullptr && cols > 0)
 #pragma unroll
-                for (int j = 0; j < 3; ++j)
-                    if (j < cols) bias[j] = load_as_f32(epi.bias, epi.bias_dt, m + j);
-        }
+            for (int j = 0; j < 4; ++j) bias[j] = __uint_as_float(epi.bias_dt == SPHIP_F32 ? res.b[j] : res.b[j] << 16);
         if (epi.z_scales != nullptr) {                          // (the whole wave: lanes exchange maxima)
 #pragma unroll 1
             for (int h = 0; h < ROWS; h += 32) {
-                if (epi.z_dt == SPHIP_INT8) store_codes<SPHIP_INT8>(mine + h * OUT_ROW, epi, nb + h, m, N, M, bias, lane);
-                else store_codes<SPHIP_E4M3>(mine + h * OUT_ROW, epi, nb + h, m, N, M, bias, lane);
+                if (epi.z_dt == SPHIP_INT8) store_codes<SPHIP_INT8, COLS>(mine + h * PITCH, epi, nb + h, m, N, M, bias, lane);
+                else store_codes<SPHIP_E4M3, COLS>(mine + h * PITCH, epi, nb + h, m, N, M, bias, lane);
             }
         }
         if (epi.bias != nullptr || epi.act != SPHIP_ACT_NONE || epi.z != nullptr) {
             const bool values = epi.z != nullptr && epi.z_scales == nullptr;
 #pragma unroll 2
             for (int i = 0; i < P; ++i) {
-                const int n = nb + 4 * i;
-                float4* at = reinterpret_cast<float4*>(mine + i * 4 * OUT_ROW);
+                const int n = nb + STEP * i;
+                float4* at = reinterpret_cast<float4*>(mine + i * STEP * PITCH);
                 const float4 c = *at;
                 float v[4] = {c.x + bias[0], c.y + bias[1], c.z + bias[2], c.w + bias[3]};
                 if (values && n < N) {
@@ -199,9 +211,9 @@ __device__ __forceinline__ void finish_rows(char* stage, const Epilogue& epi, co
         }
 #pragma unroll
         for (int i = 0; i < P; ++i) {
-            const int n = nb + 4 * i;
+            const int n = nb + STEP * i;
             if (n >= N) continue;
-            const float4 c = *reinterpret_cast<const float4*>(mine + i * 4 * OUT_ROW);
+            const float4 c = *reinterpret_cast<const float4*>(mine + i * STEP * PITCH);
             float v[4] = {c.x, c.y, c.z, c.w};
             if (epi.res != nullptr) {
                 float r[4];

@@ -3,8 +3,9 @@
 //
 // Four times the workgroups of the 128 x 128 kernel, so that a product too small to give every compute unit one of its tiles
 // need not split K over workgroups (which costs a round trip of fp32 partial tiles and a second launch). Inside a workgroup
-// the waves split K: two halves of the rows of A times two halves of each step's K, 32 x 64 outputs per wave; the halves of a
-// sum meet in LDS at the end. 4 buffers of 16 KiB, one barrier per step, three steps on their way at any time; two
+// the waves split K: two halves of the rows of A times two halves of each step's K, 32 x 64 outputs per wave; at the end the
+// two waves of a half of the rows exchange 32 of their 64 columns through LDS and each finishes the others (one of them doing
+// all 64 took longer: 48 x 768 x 768 with a GELU 8.4 us against 7.2). 4 buffers of 16 KiB, one barrier per step, three steps on their way at any time; two
 // workgroups share a compute unit.
 #include "linear_dma.hpp"
 
@@ -46,8 +47,8 @@ __global__ __launch_bounds__(256, 2) void linear64_kernel(Operand A, Operand B, 
     for (int i = 0; i < 4; ++i) acc[i][0] = acc[i][1] = (acc4_t){0.f, 0.f, 0.f, 0.f};
 
     const int N = A.rows, M = B.rows;
-    Residual<32> res;                              // waits in registers until the product is done
-    if (kh == 0) res.load(epi, g, n0 + wn * 32, m0, N, M, lane);
+    Residual<32, 32> res;                          // waits in registers until the product is done
+    res.load(epi, g, n0 + wn * 32, m0 + kh * 32, N, M, lane);
 #pragma unroll
     for (int t = 0; t < STAGES - 1; ++t) fetch(t, t * STAGE);
     unsigned img = 0, freed = (STAGES - 1) * STAGE;            // buffers of step t and of step t - 1
@@ -73,16 +74,19 @@ __global__ __launch_bounds__(256, 2) void linear64_kernel(Operand A, Operand B, 
         img = img + STAGE == STAGES * STAGE ? 0 : img + STAGE;
     }
     __syncthreads();                               // the last step has been read: the buffers are free
-    acc4_t* other = reinterpret_cast<acc4_t*>(smem) + wn * 512 + lane;
-    if (kh == 1)
+    acc4_t* const give = reinterpret_cast<acc4_t*>(smem) + wave * 256 + lane;
+    const acc4_t* const take = reinterpret_cast<const acc4_t*>(smem) + (wave ^ 2) * 256 + lane;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) other[i * 64] = acc[i >> 1][i & 1];
+    for (int i = 0; i < 4; ++i) give[i * 64] = kh ? acc[i >> 1][i & 1] : acc[2 + (i >> 1)][i & 1];
     __syncthreads();
-    if (kh == 1) return;
+    char* const stage = smem + 16384 + wave * 32 * out_row(32);
+    const int r16 = lane & 15, q4 = lane >> 4;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) acc[i >> 1][i & 1] += other[i * 64];
-    finish_tile<2>([&](int mt, int nt) { return acc[mt][nt]; }, smem + 16384 + wn * 32 * OUT_ROW, epi, g, split, n0 + wn * 32, m0, N, M,
-                   lane, res);
+    for (int i = 0; i < 4; ++i) {
+        const acc4_t own = kh ? acc[2 + (i >> 1)][i & 1] : acc[i >> 1][i & 1];
+        *reinterpret_cast<acc4_t*>(stage + ((i & 1) * 16 + r16) * out_row(32) + ((i >> 1) * 16 + q4 * 4) * 4) = own + take[i * 64];
+    }
+    finish_rows<32, 32>(stage, epi, g, split, n0 + wn * 32, m0 + kh * 32, N, M, lane, res);
 }
 
 // Splits of the K range: the power of two (or as many as fill the compute units once) with the least time by the step's

@@ -132,7 +132,7 @@ __device__ __forceinline__ void finish_tile(Acc acc, char* stage, const Epilogue
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
             *reinterpret_cast<acc4_t*>(stage + (nt * 16 + r16) * OUT_ROW + (mt * 16 + q4 * 4) * 4) = acc(mt, nt);
-    finish_rows<NT * 16>(stage, epi, g, split, n0, m0, N, M, lane, res);
+    finish_rows<NT * 16, 64>(stage, epi, g, split, n0, m0, N, M, lane, res);
 }
 
 // One operand of a kernel of 256 threads, TILE rows: descriptor, the lane's source offsets, the DMA of one 128-byte K step

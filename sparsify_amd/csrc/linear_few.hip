@@ -1,7 +1,7 @@
 // The dense product for a few tokens (N <= 64): y = act(x W^T + b) + r, one launch.
 //
 // Bound: reading W once (M D elements; 4096 x 4096 bf16: 32 MiB, 6.5 us at the 5.15 TB/s a large copy reaches; one token
-// takes 6.9). So W goes from memory straight into MFMA operands, nothing staged: a workgroup owns 16 rows of W, its 8 waves
+// takes 6.9). So W goes from memory straight into MFMA operands, nothing staged: a workgroup owns 16 or 32 rows of W, its 8 waves
 // take turns at pieces of K (consecutive waves read consecutive pieces of a row), each lane 16 bytes of one row per
 // instruction, the next pieces requested before the present ones are multiplied. x is read through the caches by every
 // workgroup, as the MFMA's other operand (rows past N repeat the last one; their results are dropped). The 8 partial sums
@@ -43,29 +43,34 @@ template <> struct Piece<float> {
     }
 };
 
-constexpr int FEW_WAVES = 8, FEW_UNROLL = 4;
+constexpr int FEW_WAVES = 8;
 
-template <typename T, int NT>
+// NT x MT tiles of 16 tokens x 16 rows of W; U pieces of K per wave and round
+template <typename T, int NT, int MT, int U>
 __global__ __launch_bounds__(512) void linear_few_kernel(Operand X, Operand W, Epilogue epi, int64_t K) {
-    constexpr int E = Piece<T>::E, KG = Piece<T>::K, U = FEW_UNROLL;
-    __shared__ acc4_t red[FEW_WAVES][NT][64];
+    constexpr int E = Piece<T>::E, KG = Piece<T>::K;
+    __shared__ acc4_t red[FEW_WAVES][NT * MT][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r16 = lane & 15, q4 = lane >> 4;
-    const int N = X.rows, M = W.rows, m0 = blockIdx.x * 16;
-    const T* w = (const T*)W.p + (int64_t)min(m0 + r16, M - 1) * W.ld + q4 * E;
-    const T* x[NT];
+    const int N = X.rows, M = W.rows, m0 = blockIdx.x * (16 * MT);
+    const T *w[MT], *x[NT];
+#pragma unroll
+    for (int j = 0; j < MT; ++j) w[j] = (const T*)W.p + (int64_t)min(m0 + j * 16 + r16, M - 1) * W.ld + q4 * E;
 #pragma unroll
     for (int i = 0; i < NT; ++i) x[i] = (const T*)X.p + (int64_t)min(i * 16 + r16, N - 1) * X.ld + q4 * E;
 
-    acc4_t acc[NT];
+    acc4_t acc[MT][NT];
 #pragma unroll
-    for (int i = 0; i < NT; ++i) acc[i] = (acc4_t){0.f, 0.f, 0.f, 0.f};
-    w4_t wa[2][U], xa[2][NT][U];
+    for (int j = 0; j < MT; ++j)
+#pragma unroll
+        for (int i = 0; i < NT; ++i) acc[j][i] = (acc4_t){0.f, 0.f, 0.f, 0.f};
+    w4_t wa[2][MT][U], xa[2][NT][U];
     // whole rounds: U groups of KG per wave
     const int64_t round = (int64_t)FEW_WAVES * U * KG, rounds = K / round;
     auto load = [&](int b, int64_t k) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            __builtin_memcpy(&wa[b][u], w + k + u * KG, 16);
+#pragma unroll
+            for (int j = 0; j < MT; ++j) __builtin_memcpy(&wa[b][j][u], w[j] + k + u * KG, 16);
 #pragma unroll
             for (int i = 0; i < NT; ++i) __builtin_memcpy(&xa[b][i][u], x[i] + k + u * KG, 16);
         }
@@ -74,7 +79,9 @@ __global__ __launch_bounds__(512) void linear_few_kernel(Operand X, Operand W, E
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
-            for (int i = 0; i < NT; ++i) acc[i] = Piece<T>::mma(wa[b][u], xa[b][i][u], acc[i]);
+            for (int j = 0; j < MT; ++j)
+#pragma unroll
+                for (int i = 0; i < NT; ++i) acc[j][i] = Piece<T>::mma(wa[b][j][u], xa[b][i][u], acc[j][i]);
     };
     const int64_t k0 = (int64_t)wave * U * KG;
     if (rounds > 0) load(0, k0);
@@ -89,9 +96,13 @@ __global__ __launch_bounds__(512) void linear_few_kernel(Operand X, Operand W, E
     // the rest, group by group
     for (int64_t k = rounds * round + wave * KG; k < K; k += FEW_WAVES * KG) {
         const int n = (int)min((int64_t)E, K - k - q4 * E);
-        w4_t a = {0, 0, 0, 0}, b[NT];
-        if (n >= E) __builtin_memcpy(&a, w + k, 16);
-        else if (n > 0) a = Piece<T>::tail(w + k, n);
+        w4_t a[MT], b[NT];
+#pragma unroll
+        for (int j = 0; j < MT; ++j) {
+            a[j] = (w4_t){0, 0, 0, 0};
+            if (n >= E) __builtin_memcpy(&a[j], w[j] + k, 16);
+            else if (n > 0) a[j] = Piece<T>::tail(w[j] + k, n);
+        }
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
             b[i] = (w4_t){0, 0, 0, 0};
@@ -99,32 +110,44 @@ __global__ __launch_bounds__(512) void linear_few_kernel(Operand X, Operand W, E
             else if (n > 0) b[i] = Piece<T>::tail(x[i] + k, n);
         }
 #pragma unroll
-        for (int i = 0; i < NT; ++i) acc[i] = Piece<T>::mma(a, b[i], acc[i]);
+        for (int j = 0; j < MT; ++j)
+#pragma unroll
+            for (int i = 0; i < NT; ++i) acc[j][i] = Piece<T>::mma(a[j], b[i], acc[j][i]);
     }
 #pragma unroll
-    for (int i = 0; i < NT; ++i) red[wave][i][lane] = acc[i];
+    for (int j = 0; j < MT; ++j)
+#pragma unroll
+        for (int i = 0; i < NT; ++i) red[wave][j * NT + i][lane] = acc[j][i];
     __syncthreads();
     // a lane of the accumulator layout holds 4 consecutive m of one n
-    if (threadIdx.x >= 64 * NT) return;
-    const int i = threadIdx.x >> 6, n = i * 16 + r16, m = m0 + q4 * 4;
+    const int tile = threadIdx.x >> 6;
+    if (tile >= NT * MT) return;
+    const int n = tile % NT * 16 + r16, m = m0 + tile / NT * 16 + q4 * 4;
     float v[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int s = 0; s < FEW_WAVES; ++s)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] += red[s][i][lane][j];
+        for (int j = 0; j < 4; ++j) v[j] += red[s][tile][lane][j];
     if (n < N && m < M) epilogue4(epi, n, m, M, v);
 }
 
-template <typename T> static void launch(const Operand& X, const Operand& W, const Epilogue& epi, int64_t K, hipStream_t s) {
-    const dim3 grid((unsigned)cdiv(W.rows, 16)), block(512);
-    if (X.rows <= 16) hipLaunchKernelGGL((linear_few_kernel<T, 1>), grid, block, 0, s, X, W, epi, K);
-    else if (X.rows <= 32) hipLaunchKernelGGL((linear_few_kernel<T, 2>), grid, block, 0, s, X, W, epi, K);
-    else hipLaunchKernelGGL((linear_few_kernel<T, 4>), grid, block, 0, s, X, W, epi, K);
+template <typename T, int MT> static void launch(const Operand& X, const Operand& W, const Epilogue& epi, int64_t K, hipStream_t s) {
+    const dim3 grid((unsigned)cdiv(W.rows, 16 * MT)), block(512);
+    if (X.rows <= 16) hipLaunchKernelGGL((linear_few_kernel<T, 1, MT, 4>), grid, block, 0, s, X, W, epi, K);
+    else if (X.rows <= 32) hipLaunchKernelGGL((linear_few_kernel<T, 2, MT, 4>), grid, block, 0, s, X, W, epi, K);
+    else hipLaunchKernelGGL((linear_few_kernel<T, 4, MT, MT == 1 ? 4 : 2>), grid, block, 0, s, X, W, epi, K);
 }
 
+// 32 rows of W per workgroup (half the reads of x) where that still gives every compute unit one: 24 x 2048 x 8192 9.4 us
+// against 12.5, one token 4096 x 8192 12.8 against 14.4 (fp32 16 x 2048 x 8192 14.7 against 16.9); where it does not, 16 x 4096 x
+// 4096 takes 13.2 against 9.8. Long K needs the second workgroup of a unit: 8192 x 8192 29.6 against 21.2, fp32 4096 x 8192 31.9
+// against 21.8 (24 tokens 39.5 against 44.2).
 int launch_linear_few(const char* what, int dtype, const Operand& X, const Operand& W, const Epilogue& epi, int64_t K, hipStream_t s) {
-    if (dtype == SPHIP_BF16) launch<bf16_t>(X, W, epi, K, s);
-    else launch<float>(X, W, epi, K, s);
+    const bool bf = dtype == SPHIP_BF16, wide = cdiv(W.rows, 32) >= 256 && (K <= 2048 || (bf ? K <= 4096 : X.rows > 16));
+    if (bf && wide) launch<bf16_t, 2>(X, W, epi, K, s);
+    else if (bf) launch<bf16_t, 1>(X, W, epi, K, s);
+    else if (wide) launch<float, 2>(X, W, epi, K, s);
+    else launch<float, 1>(X, W, epi, K, s);
     SPHIP_CHECK_LAUNCH(what);
     return SPHIP_OK;
 }
