@@ -69,14 +69,15 @@ constexpr int OUT_ROW = out_row(64);
 
 // The lane's residual pieces and its 4 of the bias, raw, all in flight before the first is used: little else hides their
 // latency. No branch and no arithmetic between the loads (either would wait for them one by one): rows past the end load the
-// last row again, columns past the end the last column.
-template <int ROWS, int COLS = 64> struct Residual {
+// last row again, columns past the end the last column. BIAS false: the bias stays where it is until the end (256 x 256 tiles,
+// which load all of this after the product: 16384 x 768 x 3584 91 us against 96).
+template <int ROWS, int COLS = 64, bool BIAS = true> struct Residual {
     static constexpr int LANES = COLS / 4, STEP = 64 / LANES, P = ROWS / STEP;     // lanes of a row, rows of a piece, pieces
     w4_t v[P], b;
     __device__ __forceinline__ void load(const Epilogue& epi, const TileGrid& g, int n0, int m0, int N, int M, int lane) {
         const int m = m0 + lane % LANES * 4, nb = n0 + lane / LANES, cols = M - m;
         if (g.splits > 1 || cols <= 0) return;
-        if (epi.bias != nullptr) {
+        if (BIAS && epi.bias != nullptr) {
             const int c1 = min(1, cols - 1), c2 = min(2, cols - 1), c3 = min(3, cols - 1);
             if (epi.bias_dt == SPHIP_F32) {
                 const unsigned* p = (const unsigned*)epi.bias + m;
@@ -162,9 +163,9 @@ __device__ __forceinline__ void store_codes(const char* mine, const Epilogue& ep
         *reinterpret_cast<unsigned*>((uint8_t*)epi.z + (int64_t)(nb + STEP * i) * epi.ldz + m) = codes_of<FMT>(v[i], inv, keep, bad);
 }
 
-template <int ROWS, int COLS>
+template <int ROWS, int COLS, bool BIAS>
 __device__ __forceinline__ void finish_rows(char* stage, const Epilogue& epi, const TileGrid& g, unsigned split, int n0, int m0,
-                                            int N, int M, int lane, const Residual<ROWS, COLS>& res) {
+                                            int N, int M, int lane, const Residual<ROWS, COLS, BIAS>& res) {
     constexpr int LANES = COLS / 4, STEP = 64 / LANES, P = ROWS / STEP, PITCH = out_row(COLS);
     const int Mp = (M + 3) & ~3;
     const int m = m0 + lane % LANES * 4, nb = n0 + lane / LANES, cols = M - m;
@@ -180,7 +181,14 @@ __device__ __forceinline__ void finish_rows(char* stage, const Epilogue& epi, co
                     *reinterpret_cast<const float4*>(mine + i * STEP * PITCH);
     } else {
         float bias[4] = {0.f, 0.f, 0.f, 0.f};
-        if (epi.bias != nullptr && cols > 0)
+        if (!BIAS && epi.bias != nullptr) {
+            if (cols >= 4) load4_as_f32(epi.bias, epi.bias_dt, m, bias);
+            else
+#pragma unroll
+                for (int j = 0; j < 3; ++j)
+                    if (j < cols) bias[j] = load_as_f32(epi.bias, epi.bias_dt, m + j);
+        }
+        if (BIAS && epi.bias != nullptr && cols > 0)
 #pragma unroll
             for (int j = 0; j < 4; ++j) bias[j] = __uint_as_float(epi.bias_dt == SPHIP_F32 ? res.b[j] : res.b[j] << 16);
         if (epi.z_scales != nullptr) {                          // (the whole wave: lanes exchange maxima)

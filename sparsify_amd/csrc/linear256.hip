@@ -190,11 +190,11 @@ __global__ __launch_bounds__(512, 2) void linear256_kernel(Operand A, Operand B,
     const int N = A.rows, M = B.rows;
     char* const stage = smem + wave * OUT_WAVE;
     {
-        Residual<64> res;
+        Residual<64, 64, false> res;
         res.load(epi, g, n0 + wn * 64, m0 + wm * 128, N, M, lane);
         finish_tile<4>([&](int mt, int nt) { return acc[mt][nt]; }, stage, epi, g, split, n0 + wn * 64, m0 + wm * 128, N, M, lane, res);
     }
-    Residual<64> res;
+    Residual<64, 64, false> res;
     res.load(epi, g, n0 + wn * 64, m0 + wm * 128 + 64, N, M, lane);
     finish_tile<4>([&](int mt, int nt) { return acc[4 + mt][nt]; }, stage, epi, g, split, n0 + wn * 64, m0 + wm * 128 + 64, N, M, lane, res);
 }

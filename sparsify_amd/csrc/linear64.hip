@@ -86,7 +86,7 @@ __global__ __launch_bounds__(256, 2) void linear64_kernel(Operand A, Operand B, 
         const acc4_t own = kh ? acc[2 + (i >> 1)][i & 1] : acc[i >> 1][i & 1];
         *reinterpret_cast<acc4_t*>(stage + ((i & 1) * 16 + r16) * out_row(32) + ((i >> 1) * 16 + q4 * 4) * 4) = own + take[i * 64];
     }
-    finish_rows<32, 32>(stage, epi, g, split, n0 + wn * 32, m0 + kh * 32, N, M, lane, res);
+    finish_rows(stage, epi, g, split, n0 + wn * 32, m0 + kh * 32, N, M, lane, res);
 }
 
 // Splits of the K range: the power of two (or as many as fill the compute units once) with the least time by the step's

@@ -123,16 +123,16 @@ __device__ __forceinline__ acc4_t mma16(const w4_t& a, const w4_t& b, acc4_t c, 
 }
 
 // The 16x16 accumulators acc(mt, nt) of a wave (4 consecutive m of one n per lane), 16 NT rows of n, through its LDS area.
-template <int NT, typename Acc>
+template <int NT, typename Acc, bool BIAS>
 __device__ __forceinline__ void finish_tile(Acc acc, char* stage, const Epilogue& epi, const TileGrid& g, unsigned split, int n0,
-                                            int m0, int N, int M, int lane, const Residual<NT * 16>& res) {
+                                            int m0, int N, int M, int lane, const Residual<NT * 16, 64, BIAS>& res) {
     const int r16 = lane & 15, q4 = lane >> 4;
 #pragma unroll
     for (int mt = 0; mt < 4; ++mt)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
             *reinterpret_cast<acc4_t*>(stage + (nt * 16 + r16) * OUT_ROW + (mt * 16 + q4 * 4) * 4) = acc(mt, nt);
-    finish_rows<NT * 16, 64>(stage, epi, g, split, n0, m0, N, M, lane, res);
+    finish_rows(stage, epi, g, split, n0, m0, N, M, lane, res);
 }
 
 // One operand of a kernel of 256 threads, TILE rows: descriptor, the lane's source offsets, the DMA of one 128-byte K step
