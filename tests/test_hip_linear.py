@@ -461,6 +461,33 @@ def test_nothing_behind_a_row_is_multiplied(device, monkeypatch, N, D, M, kernel
         ops._linear_bytes.cache_clear(), ops._linear_backward_bytes.cache_clear()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("D", [40, 770, 2048, 3001])
+@pytest.mark.parametrize("N", [1, 9, 16, 17, 32, 33, 64])
+def test_few_rows_of_a_wide_layer(device, monkeypatch, N, D, dtype):
+    """The kernel for few rows with 32 rows of W per workgroup (M from 8161 on), forced and as it is chosen."""
+    from sparsify_amd import ops
+    M = 8197
+    x, W, b, r = make(N, D, M, dtype, D + N, res=torch.float32)
+    want, tol, z, ez = forward64(x, W, b, r, "gelu", torch.float32)
+    xc, Wc, bc, rc = cuda(x, W, b, r)
+    try:
+        for kernel in ("few", None):
+            if kernel:
+                monkeypatch.setenv("SPHIP_LINEAR", kernel)
+            else:
+                monkeypatch.undo()
+            ops._linear_bytes.cache_clear()
+            y, zk, _ = ops.linear(xc, Wc, bc, rc, "gelu", keep_z=torch.float32)
+            assert_within(y, want, tol, f"y {kernel}")
+            assert_within(zk, z, ez + HALF[torch.float32] * z.abs() + TINY, f"z {kernel}")
+            _, zq, _ = ops.linear(xc, Wc, bc, rc, "gelu", keep_z="int8")
+            assert torch.equal(ops.checkpoint8_restore(zq, "int8", N, M, torch.float32).double().cpu(), codes64(zk.cpu(), "int8"))
+    finally:
+        monkeypatch.undo()
+        ops._linear_bytes.cache_clear()
+
+
 def test_only_the_asked_gradients_and_reuse(device):
     from sparsify_amd import checkpoint8, fused_linear
     x, W, b, r = cuda(*make(200, 96, 64, torch.bfloat16, 4, res=torch.float32))
