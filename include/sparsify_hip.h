@@ -521,8 +521,8 @@ int sphip_muon_apply(float* p, const void* o_bf16, int64_t n, float decay, float
  * transcoder stands in for. All tensors row-major with unit inner stride and a row stride ld* in elements (>= the
  * row), N below 2^31 - 256, D and M below 2^22 - 64; any strides and element-aligned addresses. dtype codes SPHIP_F32 /
  * SPHIP_BF16; sums are fp32, each output is rounded once when stored. Workspaces: the *_workspace_bytes query of the same
- * call, 16-byte aligned (0 bytes: may be NULL). `odd` in a query: 1 if the rows of x, plus 2 if those of W, do not all start
- * at multiples of 16 bytes, or lie 2^22 elements or more apart; the call copies these. */
+ * call, 16-byte aligned (0 bytes: may be NULL). `odd` in a query: 1 if the rows of x, plus 2 if those of W, lie 2^22
+ * elements or more apart or, in bf16, do not all start at multiples of 16 bytes; the call copies these. */
 enum { SPHIP_ACT_NONE = 0, SPHIP_ACT_RELU = 1, SPHIP_ACT_GELU = 2 /* z Phi(z) */, SPHIP_ACT_SILU = 3 /* z / (1 + e^-z) */ };
 
 /* what an operand of the gradients may be besides SPHIP_F32 / SPHIP_BF16: an 8-bit checkpoint (below) */

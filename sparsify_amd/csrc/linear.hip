@@ -108,9 +108,10 @@ static int launch_product(const char* what, const Operand& A, const Operand& B, 
     const int64_t nblocks = (int64_t)g.tilesM * g.tilesN * g.splits, threads = N * ((M + 3) / 4);
     SPHIP_REQUIRE(nblocks < MAX_GROUPS && (g.splits == 1 || cdiv(threads, 256) < MAX_GROUPS), SPHIP_EUNSUPPORTED,
                   "%s: grid too large", what);
+    const int bytes = aligned16(A.p, A.ld, sizeof(T)) && aligned16(B.p, B.ld, sizeof(T)) && (MODE_A == OP_COLS || K * (int64_t)sizeof(T) % 16 == 0) ? 16 : 4;
     const int st = by == BY_256 ? launch_linear256(what, MODE_A, MODE_B, A, B, epi, K, KB, g, s)
-                 : by == BY_128 ? launch_linear128(what, dtype, MODE_A, MODE_B, A, B, epi, K, KB, g, s)
-                                : launch_linear64(what, dtype, MODE_A, MODE_B, A, B, epi, K, KB, g, s);
+                 : by == BY_128 ? launch_linear128(what, dtype, bytes, MODE_A, MODE_B, A, B, epi, K, KB, g, s)
+                                : launch_linear64(what, dtype, bytes, MODE_A, MODE_B, A, B, epi, K, KB, g, s);
     if (st != SPHIP_OK) return st;
     if (g.splits > 1) {
         if (g.splits > 8 && threads < (1 << 17))
@@ -156,7 +157,7 @@ template <typename T> __global__ __launch_bounds__(256) void linear_pack_kernel(
     }
 }
 static int64_t packed_ld(int64_t cols) { return cdiv(cols, 64) * 64; }
-static int64_t whole_pieces(int dtype, int64_t cols) { const int64_t e = 16 / (int64_t)dtype_size(dtype); return cdiv(cols, e) * e; }
+static int64_t whole_pieces(int64_t cols) { return cdiv(cols, 8) * 8; }
 struct Packing {
     PackArgs a = {};
     int count = 0, dtype;
@@ -183,7 +184,8 @@ struct Packing {
         return SPHIP_OK;
     }
 };
-static bool unaligned(int dtype, int64_t cols) { return cols * (int64_t)dtype_size(dtype) % 16 != 0; }
+// whether rows of so many elements end inside a 16-byte piece that LDS-DMA would fetch whole
+static bool unaligned(int dtype, int64_t cols) { return dtype == SPHIP_BF16 && cols % 8 != 0; }
 
 // ---- dz = g act'(z) and its column sums. A workgroup takes 32 rows (the group one scale of an 8-bit z covers) of 32 x 16
 // bytes of columns: 32 lanes side by side, 8 rows at a time, every thread 4 rows whose loads are all in flight; the 8 row
@@ -400,20 +402,22 @@ struct ForwardSpace {
 //   bf16, up to 16 tokens: one token 4096 x 4096 7.3 / 9.3, 4096 x 8192 12.8 / 14.8, 8192 x 8192 21.2 / 23.4; 16 tokens 2048 x
 //   8192 8.1 / 10.4, 4096 x 4096 9.8 / 9.8, but 8192 x 256 16 / 7, 8192 x 8192 30 / 24, and beyond one round of workgroups the
 //   tiles stream W faster: 4096 x 14336 23.5 / 18.9. 24 tokens: 768 x 768 4.5 / 6.1, 2048 x 8192 9.4 / 10.6, 4096 x 4096 12.2 / 10.
+//   up to 64 tokens: 48 x 768 x 768 5.7 / 6.0, but 48 x 1537 x 3333 22 / 11.
 //   fp32: one token 4096 x 4096 13 / 25, 16 tokens 8192 x 28672 228 / 263, but 8192 x 256 29 / 10; 24 tokens 4096 x 4096 23.2 /
-//   25.5, 4096 x 14336 71 / 77, but 4096 x 28672 140 / 135, 2048 x 2048 12.7 / 11.2.
-// Where the tiles would have to copy W or x first: in fp32 any, in bf16 as long as x is short (24 x 2049 x 8192 and 40 x 333 x
-// 777 7.0 / 8.3, but 48 x 1537 x 3333 22 / 17, 16 x 4097 x 4096 27 / 24).
+//   25.5, 4096 x 14336 71 / 77, 8192 x 8192 64 / 81, but 6500 x 4800 60 / 46, 4096 x 28672 140 / 135, 2048 x 2048 12.7 / 11.2;
+//   40 x 333 x 777 6.1 / 11.2, but 48 x 768 x 768 9.4 / 8.6.
+// Where the tiles would have to copy W or x first (bf16), as long as x is short: 24 x 2049 x 8192 24.9 / 25.8, 40 x 333 x 777
+// 7.0 / 8.3, but 48 x 1537 x 3333 22 / 17, 16 x 4097 x 4096 27 / 24.
 static bool few(int dtype, int64_t N, int64_t D, int64_t M, int copies) {
     if (N > FEW || (g_forced && g_forced != 'f')) return false;
     if (g_forced) return true;
-    const bool bf = dtype == SPHIP_BF16;
-    if (copies) return !bf || N * D <= 65536;
-    if (N > 32) return false;
-    if (!bf) return N <= 16 ? D <= 4096 || M >= 2048 : D <= 1024 || (M >= 4096 && (M <= 16384 || D <= 2048));
+    const bool bf = dtype == SPHIP_BF16, wide = cdiv(M, 32) >= 256;
+    if (copies) return N * D <= 65536;
+    if (N > 32) return D <= (bf ? 768 : 512) && M <= 2048;
+    if (!bf) return N <= 16 ? D <= 4096 || M >= 2048 : D <= 1024 || wide ? M <= 16384 || D <= 2048 : M >= 2560 && D <= 5120;
     if (M > 8192) return false;
     if (N <= 16) return D <= 4096 || (N == 1 && M >= 4096);
-    return D <= (cdiv(M, 32) >= 256 ? 2048 : 1024);
+    return D <= (wide ? 2048 : 1024);
 }
 // Which of the operands have to be copied, for a query and for a launch alike; `odd`: bits of those that are not fetchable().
 // Where the rows of x are no whole 16-byte pieces, what follows a row would be multiplied with what follows one of W: both.
@@ -472,7 +476,7 @@ extern "C" int sphip_linear(const void* x, int64_t ldx, const void* W, int64_t l
     if (zc && f.z) e.z = (char*)ws + f.part, e.z_dt = SPHIP_F32, e.ldz = cdiv(M, 4) * 4;
     else e.z = z, e.z_dt = z_kind, e.ldz = ldz, e.z_scales = zc ? z_scales : nullptr;
     Operand A = {x, ldx, (int)N}, B = {W, ldw, (int)M};
-    const int64_t K = f.copies ? whole_pieces(dtype, D) : D, ld = packed_ld(D);
+    const int64_t K = f.copies ? whole_pieces(D) : D, ld = packed_ld(D);
     char* to = (char*)ws + f.part + f.z;
     int st = SPHIP_OK;
     Packing p(dtype);
@@ -586,7 +590,7 @@ extern "C" int sphip_linear_backward(const void* g, int g_dtype, int64_t ldg, co
     Epilogue e;
     if (dx) {
         e.out = dx, e.out_dt = dx_dtype, e.ldo = lddx;
-        const int64_t K = direct ? M : whole_pieces(dtype, M);  // (dz is padded with zeros)
+        const int64_t K = direct ? M : whole_pieces(M);         // (dz is padded with zeros)
         st = dtype == SPHIP_BF16 ? launch_product<bf16_t, OP_ROWS, OP_COLS>("linear_backward(dx)", dz, ow, e, K, M, part, sp.part, s)
                                  : launch_product<float, OP_ROWS, OP_COLS>("linear_backward(dx)", dz, ow, e, K, M, part, sp.part, s);
         if (st != SPHIP_OK) return st;

@@ -15,10 +15,12 @@ struct Operand {
     int rows;
 };
 
-// Whether LDS-DMA can fetch an operand's rows of es-byte elements where they are: from multiples of 16 bytes, with offsets that
-// fit a tile's buffer descriptor (2^31 bytes: 256 rows of bf16, 128 of fp32). Others are copied first.
+// Whether LDS-DMA can fetch an operand's rows where they are: offsets that fit a tile's buffer descriptor (2^31 bytes: 256 rows
+// of bf16, 128 of fp32), bf16 from multiples of 16 bytes. Others are copied first. fp32 elements may lie anywhere: where rows
+// are not aligned16 they go 4 bytes at a time.
 constexpr int64_t MAX_LD = 1ll << 22;
-static inline bool fetchable(const void* p, int64_t ld, int es) { return ((uintptr_t)p & 15) == 0 && ld * es % 16 == 0 && ld < MAX_LD; }
+static inline bool aligned16(const void* p, int64_t ld, int es) { return ((uintptr_t)p & 15) == 0 && ld * es % 16 == 0; }
+static inline bool fetchable(const void* p, int64_t ld, int es) { return ld < MAX_LD && (es == 4 || aligned16(p, ld, es)); }
 
 // hipFuncAttributeMaxDynamicSharedMemorySize of a kernel, set once per device (`done`: a bit per device, one word a kernel)
 static inline bool reserve_lds(const void* kernel, int bytes, uint64_t& done) {
@@ -251,16 +253,16 @@ int save_codes(const char* what, const void* x, int dtype, int64_t ldx, int fmt,
 constexpr int FEW = 64;
 int launch_linear_few(const char* what, int dtype, const Operand& X, const Operand& W, const Epilogue& epi, int64_t K, hipStream_t s);
 
-// The tiled kernels (256: bf16 only): how they split K, their launch (the caller joins). Operands: fetchable(), and K whole
-// 16-byte pieces where it is the contiguous index.
+// The tiled kernels (256: bf16 only): how they split K, their launch (the caller joins). Operands: fetchable(), in bf16 and
+// with 16 of `bytes` K whole 16-byte pieces where it is the contiguous index.
 // KB: rows of an OP_COLS B, which may be fewer than K (whole 16-byte pieces where A is OP_ROWS): B counts as zero from there.
 int launch_linear256(const char* what, int mode_a, int mode_b, const Operand& A, const Operand& B, const Epilogue& epi, int64_t K,
                      int64_t KB, const TileGrid& g, hipStream_t s);
 int linear64_splits(int dtype, int64_t N, int64_t M, int64_t K);
-int launch_linear64(const char* what, int dtype, int mode_a, int mode_b, const Operand& A, const Operand& B, const Epilogue& epi,
-                    int64_t K, int64_t KB, const TileGrid& g, hipStream_t s);
+int launch_linear64(const char* what, int dtype, int bytes, int mode_a, int mode_b, const Operand& A, const Operand& B,
+                    const Epilogue& epi, int64_t K, int64_t KB, const TileGrid& g, hipStream_t s);
 int linear128_splits(int dtype, int64_t N, int64_t M, int64_t K);
-int launch_linear128(const char* what, int dtype, int mode_a, int mode_b, const Operand& A, const Operand& B, const Epilogue& epi,
-                     int64_t K, int64_t KB, const TileGrid& g, hipStream_t s);
+int launch_linear128(const char* what, int dtype, int bytes, int mode_a, int mode_b, const Operand& A, const Operand& B,
+                     const Epilogue& epi, int64_t K, int64_t KB, const TileGrid& g, hipStream_t s);
 
 }  // namespace sphip

@@ -14,7 +14,7 @@ namespace sphip {
 constexpr int T128 = 128, IMG_A = 0, IMG_B = 16384, STAGE = 32768;
 constexpr int FINISH = 4 * 64 * OUT_ROW;            // the epilogue's staging: more than two stages, twice still within the LDS
 
-template <typename T, int MA, int MB, int STAGES>
+template <typename T, int MA, int MB, int STAGES, int BYTES>
 __global__ __launch_bounds__(256, STAGES == 2 ? 2 : 1) void linear128_kernel(Operand A, Operand B, Epilogue epi, int64_t K, int64_t KB,
                                                                              TileGrid g) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -28,11 +28,14 @@ __global__ __launch_bounds__(256, STAGES == 2 ? 2 : 1) void linear128_kernel(Ope
     const int64_t k0 = (int64_t)split * g.steps_per * KS;
     const int steps = (int)min((int64_t)g.steps_per, (K - k0 + KS - 1) / KS);
 
-    Source<T, MA, T128> sa;
-    Source<T, MB, T128> sb;
+    typedef Source<T, MA, T128, BYTES> SA;
+    typedef Source<T, MB, T128, BYTES> SB;
+    constexpr int LOADS = SA::LOADS + SB::LOADS;   // DMA instructions per wave and step
+    SA sa;
+    SB sb;
     sa.init(A, n0, k0, K, tid);
     sb.init(B, m0, k0, KB, tid);
-    auto fetch = [&](int t, unsigned image) {      // 8 DMA instructions per wave
+    auto fetch = [&](int t, unsigned image) {
         if (t >= steps) return;
         if (t == steps - 1) sa.last(t), sb.last(t);
         char* dst = smem + image + wave * 1024;
@@ -61,8 +64,8 @@ __global__ __launch_bounds__(256, STAGES == 2 ? 2 : 1) void linear128_kernel(Ope
     for (int t = 0; t < steps; ++t) {
         // step t has landed; the (at most STAGES - 2) steps after it that are on their way may still be out
         const int later = min(STAGES - 2, steps - 1 - t);
-        if (later == 2) LIN_VMCNT(16);
-        else if (later == 1) LIN_VMCNT(8);
+        if (later == 2) LIN_VMCNT(2 * LOADS);
+        else if (later == 1) LIN_VMCNT(LOADS);
         else LIN_VMCNT(0);
         __builtin_amdgcn_sched_barrier(0);
         __builtin_amdgcn_s_barrier();
@@ -107,21 +110,22 @@ int linear128_splits(int dtype, int64_t N, int64_t M, int64_t K) {
     return s < 1 ? 1 : (int)s;
 }
 
-int launch_linear128(const char* what, int dtype, int mode_a, int mode_b, const Operand& A, const Operand& B, const Epilogue& epi,
-                     int64_t K, int64_t KB, const TileGrid& g, hipStream_t s) {
+int launch_linear128(const char* what, int dtype, int bytes, int mode_a, int mode_b, const Operand& A, const Operand& B,
+                     const Epilogue& epi, int64_t K, int64_t KB, const TileGrid& g, hipStream_t s) {
     typedef void (*kern_t)(Operand, Operand, Epilogue, int64_t, int64_t, TileGrid);
     const int64_t blocks = (int64_t)g.tilesM * g.tilesN * g.splits;
-    const int which = mode_a == OP_ROWS ? (mode_b == OP_ROWS ? 0 : 1) : 2, deep = blocks <= 256, bf = dtype == SPHIP_BF16;
-#define LIN_KERNELS(T)                                                                                    \
-    {{linear128_kernel<T, OP_ROWS, OP_ROWS, 2>, linear128_kernel<T, OP_ROWS, OP_ROWS, 4>},                 \
-     {linear128_kernel<T, OP_ROWS, OP_COLS, 2>, linear128_kernel<T, OP_ROWS, OP_COLS, 4>},                 \
-     {linear128_kernel<T, OP_COLS, OP_COLS, 2>, linear128_kernel<T, OP_COLS, OP_COLS, 4>}}
-    static const kern_t kerns[2][3][2] = {LIN_KERNELS(float), LIN_KERNELS(bf16_t)};
+    const int which = mode_a == OP_ROWS ? (mode_b == OP_ROWS ? 0 : 1) : 2, deep = blocks <= 256;
+    const int type = dtype == SPHIP_BF16 ? 0 : bytes == 16 ? 1 : 2;
+#define LIN_KERNELS(T, B)                                                                                       \
+    {{linear128_kernel<T, OP_ROWS, OP_ROWS, 2, B>, linear128_kernel<T, OP_ROWS, OP_ROWS, 4, B>},                 \
+     {linear128_kernel<T, OP_ROWS, OP_COLS, 2, B>, linear128_kernel<T, OP_ROWS, OP_COLS, 4, B>},                 \
+     {linear128_kernel<T, OP_COLS, OP_COLS, 2, B>, linear128_kernel<T, OP_COLS, OP_COLS, 4, B>}}
+    static const kern_t kerns[3][3][2] = {LIN_KERNELS(bf16_t, 16), LIN_KERNELS(float, 16), LIN_KERNELS(float, 4)};
 #undef LIN_KERNELS
     const int lds = deep ? 4 * STAGE : FINISH;
-    static uint64_t done[2][3][2] = {};
-    const kern_t fn = kerns[bf][which][deep];
-    SPHIP_REQUIRE(reserve_lds((const void*)fn, lds, done[bf][which][deep]), SPHIP_ELAUNCH, "%s: cannot reserve %d bytes of LDS", what, lds);
+    static uint64_t done[3][3][2] = {};
+    const kern_t fn = kerns[type][which][deep];
+    SPHIP_REQUIRE(reserve_lds((const void*)fn, lds, done[type][which][deep]), SPHIP_ELAUNCH, "%s: cannot reserve %d bytes of LDS", what, lds);
     hipLaunchKernelGGL(fn, dim3((unsigned)blocks), dim3(256), lds, s, A, B, epi, K, KB, g);
     SPHIP_CHECK_LAUNCH(what);
     return SPHIP_OK;

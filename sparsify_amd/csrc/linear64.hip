@@ -13,7 +13,7 @@ namespace sphip {
 
 constexpr int T64 = 64, STAGES = 4, STAGE = 16384, IMG_B = 8192;
 
-template <typename T, int MA, int MB>
+template <typename T, int MA, int MB, int BYTES>
 __global__ __launch_bounds__(256, 2) void linear64_kernel(Operand A, Operand B, Epilogue epi, int64_t K, int64_t KB, TileGrid g) {
     __shared__ __attribute__((aligned(16))) char smem[STAGES * STAGE];
     unsigned split;
@@ -26,11 +26,14 @@ __global__ __launch_bounds__(256, 2) void linear64_kernel(Operand A, Operand B, 
     const int64_t k0 = (int64_t)split * g.steps_per * KS;
     const int steps = (int)min((int64_t)g.steps_per, (K - k0 + KS - 1) / KS);
 
-    Source<T, MA, T64> sa;
-    Source<T, MB, T64> sb;
+    typedef Source<T, MA, T64, BYTES> SA;
+    typedef Source<T, MB, T64, BYTES> SB;
+    constexpr int LOADS = SA::LOADS + SB::LOADS;   // DMA instructions per wave and step
+    SA sa;
+    SB sb;
     sa.init(A, n0, k0, K, tid);
     sb.init(B, m0, k0, KB, tid);
-    auto fetch = [&](int t, unsigned image) {      // 4 DMA instructions per wave
+    auto fetch = [&](int t, unsigned image) {
         if (t >= steps) return;
         if (t == steps - 1) sa.last(t), sb.last(t);
         char* dst = smem + image + wave * 1024;
@@ -55,8 +58,8 @@ __global__ __launch_bounds__(256, 2) void linear64_kernel(Operand A, Operand B, 
     for (int t = 0; t < steps; ++t) {
         // step t has landed; the at most 2 steps after it that are on their way may still be out
         const int later = steps - 1 - t;
-        if (later >= 2) LIN_VMCNT(8);
-        else if (later == 1) LIN_VMCNT(4);
+        if (later >= 2) LIN_VMCNT(2 * LOADS);
+        else if (later == 1) LIN_VMCNT(LOADS);
         else LIN_VMCNT(0);
         __builtin_amdgcn_sched_barrier(0);
         __builtin_amdgcn_s_barrier();
@@ -91,27 +94,31 @@ __global__ __launch_bounds__(256, 2) void linear64_kernel(Operand A, Operand B, 
 
 // Splits of the K range: the power of two (or as many as fill the compute units once) with the least time by the step's
 // measured 200 ns (bf16; 520 fp32) and, for a split, 4 us of joining launch and a round trip of the partial tiles at 3 TB/s.
+// (Also where the tiles fill the units, but leave most of them idle in their last round: fp32 1136 x 3467 x 1218 128 us whole,
+// 112 in two.)
 int linear64_splits(int dtype, int64_t N, int64_t M, int64_t K) {
     const int64_t tiles = cdiv(N, T64) * cdiv(M, T64), steps = cdiv(K, 128 / (int64_t)dtype_size(dtype));
-    const int64_t step = dtype == SPHIP_BF16 ? 200 : 520, most = 256 / tiles < steps / 4 ? 256 / tiles : steps / 4;
+    const int64_t step = dtype == SPHIP_BF16 ? 200 : 520, fill = 256 / tiles < steps / 4 ? 256 / tiles : steps / 4;
     int64_t best = 1, least = steps * step * cdiv(tiles, 256);
-    for (int64_t s = 2; most > 1; s = s * 2 < most ? s * 2 : most) {
+    auto consider = [&](int64_t s) {
         const int64_t t = cdiv(steps, s) * step * cdiv(tiles * s, 256) + 4000 + s * N * M / 375;
         if (t < least) best = s, least = t;
-        if (s >= most) break;
-    }
+    };
+    for (int64_t s = 2; s <= steps / 4 && tiles * s <= 1024; s *= 2) consider(s);
+    if (fill > 1) consider(fill);
     return (int)best;
 }
 
-int launch_linear64(const char* what, int dtype, int mode_a, int mode_b, const Operand& A, const Operand& B, const Epilogue& epi,
-                    int64_t K, int64_t KB, const TileGrid& g, hipStream_t s) {
+int launch_linear64(const char* what, int dtype, int bytes, int mode_a, int mode_b, const Operand& A, const Operand& B,
+                    const Epilogue& epi, int64_t K, int64_t KB, const TileGrid& g, hipStream_t s) {
     typedef void (*kern_t)(Operand, Operand, Epilogue, int64_t, int64_t, TileGrid);
     const int64_t blocks = (int64_t)g.tilesM * g.tilesN * g.splits;
     const int which = mode_a == OP_ROWS ? (mode_b == OP_ROWS ? 0 : 1) : 2;
-    static const kern_t kerns[2][3] = {
-        {linear64_kernel<float, OP_ROWS, OP_ROWS>, linear64_kernel<float, OP_ROWS, OP_COLS>, linear64_kernel<float, OP_COLS, OP_COLS>},
-        {linear64_kernel<bf16_t, OP_ROWS, OP_ROWS>, linear64_kernel<bf16_t, OP_ROWS, OP_COLS>, linear64_kernel<bf16_t, OP_COLS, OP_COLS>}};
-    hipLaunchKernelGGL(kerns[dtype == SPHIP_BF16][which], dim3((unsigned)blocks), dim3(256), 0, s, A, B, epi, K, KB, g);
+#define LIN_KERNELS(T, BYTES) \
+    {linear64_kernel<T, OP_ROWS, OP_ROWS, BYTES>, linear64_kernel<T, OP_ROWS, OP_COLS, BYTES>, linear64_kernel<T, OP_COLS, OP_COLS, BYTES>}
+    static const kern_t kerns[3][3] = {LIN_KERNELS(bf16_t, 16), LIN_KERNELS(float, 16), LIN_KERNELS(float, 4)};
+#undef LIN_KERNELS
+    hipLaunchKernelGGL(kerns[dtype == SPHIP_BF16 ? 0 : bytes == 16 ? 1 : 2][which], dim3((unsigned)blocks), dim3(256), 0, s, A, B, epi, K, KB, g);
     SPHIP_CHECK_LAUNCH(what);
     return SPHIP_OK;
 }

@@ -16,7 +16,7 @@ namespace sphip {
 constexpr int K64 = 64;                            // bf16 K per step: 128 bytes (32 fp32)
 constexpr unsigned PAST_END = 1u << 31;            // offset bit that lies behind every descriptor (MAX_LD)
 
-#define LIN_VMCNT(n) asm volatile("s_waitcnt vmcnt(" #n ")" ::: "memory")
+#define LIN_VMCNT(n) asm volatile("s_waitcnt vmcnt(%0)" ::"i"((n) < 63 ? (n) : 63) : "memory")     // (6 bits)
 
 // Chunk swizzle of an OP_COLS image with PITCH bytes per k row, element size ES (see above; with 128-byte rows the low bit of
 // k already tells the two halves of the banks apart, and fp32 reads single dwords: there the four 16-lane groups, 4 k rows
@@ -136,53 +136,73 @@ __device__ __forceinline__ void finish_tile(Acc acc, char* stage, const Epilogue
 }
 
 // One operand of a kernel of 256 threads, TILE rows: descriptor, the lane's source offsets, the DMA of one 128-byte K step
-// (PIECES instructions of 4 KiB per workgroup).
-template <typename T, int MODE, int TILE> struct Source {
+// (PIECES times 4 KiB per workgroup, an instruction BYTES per lane). BYTES 16: rows from multiples of 16 bytes, K whole such
+// pieces where it is contiguous; BYTES 4: fp32 at any address (four times the instructions: 2048 x 1025 x 1024 44 us; copied
+// first, then by 16 bytes, 50; 98 x 5502 x 7155 118 against 173).
+template <typename T, int MODE, int TILE, int BYTES> struct Source {
     static constexpr unsigned ES = sizeof(T), KS = 128 / ES;
-    static constexpr int PIECES = TILE / 32, PITCH = TILE * ES;
+    static constexpr int PIECES = TILE / 32, PITCH = TILE * ES, J = 16 / BYTES, ALT = MODE == OP_ROWS ? 1 : 2;
+    static constexpr int LOADS = PIECES * J;                    // instructions per wave and step
     const T* base;                         // of the tile and the split, uniform
     unsigned ldb, edge;                    // bytes: row stride; OP_ROWS: of the descriptor, OP_COLS: of its last k row
-    unsigned voff[2], piece;               // bytes: lane offset of even and odd pieces, between pieces
-    int left;                              // OP_ROWS: 16-byte pieces of K from the lane's on; OP_COLS: k rows
+    unsigned voff[ALT][J], piece;          // bytes: lane offset of even and odd pieces, between pieces
+    int left[J];                           // OP_ROWS: K from the lane's on in units of BYTES; OP_COLS: k rows
     __device__ __forceinline__ void init(const Operand& o, int row0, int64_t k0, int64_t K, int tid) {
         ldb = (unsigned)o.ld * ES;
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            // the 16-byte slot of the image the lane writes (a part of) with load j of a piece
+            const int u = J == 1 ? tid : (tid & ~63) + j * 16 + ((tid & 63) >> 2), sub = J == 1 ? 0 : (tid & 3) * 4;
+            if (MODE == OP_ROWS) {
+                const int hr = u >> 3, ch = (u & 7) ^ ((hr >> 1) & 7);
+                voff[0][j] = (unsigned)hr * ldb + (unsigned)(ch * 16 + sub);
+                left[j] = (int)((K - k0) * ES / BYTES) - (ch * 16 + sub) / BYTES;
+            } else {
+                constexpr int CH = PITCH / 16, KP = 256 / CH;   // 16-byte chunks of a k row, k rows of a piece
+                const int kr = u / CH, c = u % CH;
+#pragma unroll
+                for (int i = 0; i < ALT; ++i) voff[i][j] = (unsigned)kr * ldb + (unsigned)((c ^ cols_swizzle<ES, PITCH>(kr + KP * i)) * 16 + sub);
+                piece = KP * ldb;
+                left[j] = (int)(K - k0);
+            }
+        }
         if (MODE == OP_ROWS) {
-            const int hr = tid >> 3, ch = (tid & 7) ^ ((hr >> 1) & 7);
             base = (const T*)o.p + (int64_t)row0 * o.ld + k0;
             edge = (unsigned)(min(TILE, o.rows - row0) - 1) * ldb + (unsigned)(K - k0) * ES;
-            voff[0] = voff[1] = (unsigned)hr * ldb + (unsigned)ch * 16u;
             piece = 32u * ldb;
-            left = (int)((K - k0) * ES / 16) - ch;
         } else {
-            constexpr int CH = PITCH / 16, KP = 256 / CH;       // 16-byte chunks of a k row, k rows of a piece
-            const int kr = tid / CH, c = tid % CH;
             base = (const T*)o.p + k0 * o.ld + row0;
-            // rounded up to a piece: a dword that crosses the end reads as zero, with it the last of an odd number of rows
-            // (k rows are 16-byte aligned, so the piece is the one that holds the last element)
-            edge = ((unsigned)(o.rows - row0) * ES + 15u) / 16u * 16u;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) voff[i] = (unsigned)kr * ldb + (unsigned)(c ^ cols_swizzle<ES, PITCH>(kr + KP * i)) * 16u;
-            piece = KP * ldb;
-            left = (int)(K - k0);
+            // rounded up to what a lane loads: a dword that crosses the end reads as zero, with it the last of an odd number of
+            // rows (k rows are 16-byte aligned then, so the piece is the one that holds the last element)
+            edge = ((unsigned)(o.rows - row0) * ES + (BYTES - 1u)) / BYTES * BYTES;
         }
     }
     // The descriptor of K step t. OP_COLS: from the step's first k row, so that its offsets do not grow with K (many tokens).
     __device__ __forceinline__ __amdgpu_buffer_rsrc_t step(int t) const {
         if (MODE == OP_ROWS) return __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (int)edge, 0x00020000);
-        const unsigned rows = (unsigned)min((int)KS, left - t * (int)KS);
+        const unsigned rows = (unsigned)min((int)KS, left[0] - t * (int)KS);
         return __builtin_amdgcn_make_buffer_rsrc((void*)((const char*)base + (uint64_t)((unsigned)t * KS) * ldb), 0,
                                                  (int)((rows - 1) * ldb + edge), 0x00020000);
     }
     // before the DMA of the last step: an OP_ROWS lane whose piece lies behind K names an offset behind the descriptor
     __device__ __forceinline__ void last(int t) {
-        if (MODE == OP_ROWS && 8 * t >= left) voff[0] |= PAST_END, voff[1] |= PAST_END;
+        if (MODE == OP_ROWS)
+#pragma unroll
+            for (int j = 0; j < J; ++j)
+                if (128 / BYTES * t >= left[j]) voff[0][j] |= PAST_END;
     }
     __device__ __forceinline__ void dma(char* lds, int t) const {
         const __amdgpu_buffer_rsrc_t rsrc = step(t);
         const unsigned so = MODE == OP_ROWS ? (unsigned)t * 128u : 0u;
 #pragma unroll
-        for (int i = 0; i < PIECES; ++i)      // (the whole offset in the register the range check looks at)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_t)(lds + 4096 * i), 16, voff[i & 1] + (unsigned)i * piece + so, 0, 0, 0);
+        for (int i = 0; i < PIECES; ++i)
+#pragma unroll
+            for (int j = 0; j < J; ++j) {     // (the whole offset in the register the range check looks at)
+                const lds_t to = (lds_t)(lds + 4096 * i + 1024 / J * j);
+                const unsigned from = voff[i & (ALT - 1)][j] + (unsigned)i * piece + so;
+                if constexpr (BYTES == 16) __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, to, 16, from, 0, 0, 0);
+                else __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, to, 4, from, 0, 0, 0);
+            }
     }
 };
 

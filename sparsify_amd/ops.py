@@ -1318,8 +1318,8 @@ def _linear_backward_bytes(*args) -> int:
 
 
 def _odd(address: int, ld: int, dt: int) -> bool:
-    """Whether rows have to be copied before a product: not all at multiples of 16 bytes, or 2^22 elements apart."""
-    return (address | ld * (2 if dt == BF16 else 4)) & 15 != 0 or ld >= 1 << 22
+    """Whether rows have to be copied before a product: 2^22 elements apart, or bf16 not all at multiples of 16 bytes."""
+    return ld >= 1 << 22 or (dt == BF16 and (address | 2 * ld) & 15 != 0)
 
 
 def _act(activation: str) -> int:
