@@ -1266,7 +1266,7 @@ def is_rows(t: Tensor) -> bool:
     """Whether a 2-D tensor has its columns next to each other and rows that do not overlap (any row stride)."""
     n, d = t.shape
     s0, s1 = t.stride()
-    return (s1 == 1 or d <= 1) and (s0 >= d or n <= 1)
+    return (s1 == 1 or d <= 1 or n == 0) and (s0 >= d or n <= 1)
 
 
 def _rows(t: Tensor, name: str, shape: tuple | None = None, like: Tensor | None = None) -> tuple[int, int, int]:
@@ -1280,7 +1280,7 @@ def _rows(t: Tensor, name: str, shape: tuple | None = None, like: Tensor | None 
     if like is not None and t.device != like.device:
         raise ValueError(f"{name} is on {t.device}, the others on {like.device}")
     (n, d), (ld, inner) = size, t.stride()
-    if (inner != 1 and d > 1) or (ld < d and n > 1):
+    if (inner != 1 and d > 1 and n > 0) or (ld < d and n > 1):
         raise ValueError(f"{name} must have its columns next to each other and rows that do not overlap "
                          f"(strides {t.stride()} for shape {tuple(size)})")
     return t.data_ptr(), ld if n > 1 else d, dt

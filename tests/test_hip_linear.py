@@ -549,6 +549,19 @@ def test_empty_batch(device):
         assert dx.shape == x.shape and not dW.any() and not db.any()
 
 
+def test_empty_batch_with_an_expanded_gradient(device):
+    """The gradient of a sum is one value, expanded: strides of zero, also where there are no rows."""
+    from sparsify_amd import fused_linear
+    for lead in ((0,), (3,), (2, 0), (2, 5)):
+        ts = [t.requires_grad_() for t in cuda(torch.randn(*lead, 40), torch.randn(24, 40), torch.randn(24))]
+        for fmt in (None, "int8"):
+            y = fused_linear(*ts, activation="silu", checkpoint=fmt)
+            got = torch.autograd.grad(y.sum(), ts)
+            want = torch.autograd.grad(fused_linear(*ts, activation="silu", checkpoint=fmt), ts, torch.ones_like(y))
+            for a, c, t in zip(got, want, ts):
+                assert a.shape == t.shape and torch.equal(a, c)
+
+
 def test_masked_rows_of_a_padded_batch(device):
     """Rows behind the last sequence (zero gradient) add nothing to dW and db and get a zero dx, whatever finite values
     they hold; whole groups of 32 of them may hold anything that "none" or "relu" passes on."""
