@@ -488,6 +488,51 @@ def test_few_rows_of_a_wide_layer(device, monkeypatch, N, D, dtype):
         ops._linear_bytes.cache_clear()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("fmt", [None, "e4m3"])
+def test_rows_far_apart(device, dtype, fmt):
+    """Rows 2^22 elements apart lie behind a tile's descriptor: copied first, the same bits as from dense rows."""
+    from sparsify_amd import fused_linear
+    x, W, b, _ = make(130, 200, 72, dtype, 3)
+    ld = (1 << 22) + 8
+
+    def far(t):
+        big = torch.empty(t.shape[0], ld, dtype=dtype, device="cuda")
+        big[:, :8], big[:, 8 + t.shape[1] : 64 + t.shape[1]] = math.nan, math.nan
+        big[:, 8 : 8 + t.shape[1]] = t.cuda()
+        return big[:, 8 : 8 + t.shape[1]]
+
+    g = torch.randn(130, 72, device="cuda").to(dtype)
+    outs = []
+    for xi, wi in ((x.cuda(), W.cuda()), (far(x), W.cuda()), (x.cuda(), far(W)), (far(x), far(W))):
+        ts = [t.detach().requires_grad_() for t in (xi, wi, b.cuda())]
+        y = fused_linear(*ts, activation="gelu", checkpoint=fmt)
+        outs.append((y.detach(), *torch.autograd.grad(y, ts, g)))
+    for o in outs[1:]:
+        for a, c in zip(o, outs[0]):
+            assert torch.equal(a, c)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("N", [3, 20, 70])
+def test_longest_rows(device, dtype, N):
+    """2^22 - 65 features, the most that is taken, on either side; sums of -1, 0 and 1 are whole numbers below 2^24: exact."""
+    from sparsify_amd import ops
+    most, few = (1 << 22) - 65, 5
+    gen = torch.Generator("cuda").manual_seed(N)
+    a, b = (torch.randint(-1, 2, (n, most), device="cuda", generator=gen).to(dtype) for n in (N, few))
+    want = torch.stack([(a.float() * r.float()).sum(1, dtype=torch.float64) for r in b], 1)
+    y, _, _ = ops.linear(a, b, out_dtype=torch.float32)                            # K = most
+    assert torch.equal(y.double(), want)
+    W = b.t().contiguous()                                                         # (most, few)
+    dx, _, _ = ops.linear_backward(a, W, None, None, dx_dtype=torch.float32)       # K = most, W's columns
+    assert torch.equal(dx.double(), want)
+    x = torch.randint(-1, 2, (N, few), device="cuda", generator=gen).to(dtype)
+    _, dW, db = ops.linear_backward(a, W, None, x, dw_dtype=torch.float32, db_dtype=torch.float32)
+    assert torch.equal(db.double(), a.sum(0, dtype=torch.float64))
+    assert torch.equal(dW.double(), torch.stack([(a.float() * c[:, None].float()).sum(0, dtype=torch.float64) for c in x.t()], 1))
+
+
 def test_only_the_asked_gradients_and_reuse(device):
     from sparsify_amd import checkpoint8, fused_linear
     x, W, b, r = cuda(*make(200, 96, 64, torch.bfloat16, 4, res=torch.float32))
