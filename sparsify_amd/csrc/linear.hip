@@ -124,7 +124,7 @@ static int launch_product(const char* what, const Operand& A, const Operand& B, 
 }
 
 // Rows copied to a stride that is a multiple of 64 elements, zeros behind them: for operands that LDS-DMA cannot fetch as they
-// are (fetchable(); products of K from D or M also need rows that are whole 16-byte pieces). Up to three matrices in one
+// are (fetchable(); bf16 products of K from D or M also need rows that are whole 16-byte pieces). Up to three matrices in one
 // launch.
 struct PackArgs {
     const void* src[3];
@@ -402,7 +402,7 @@ struct ForwardSpace {
 //   bf16, up to 16 tokens: one token 4096 x 4096 7.3 / 9.3, 4096 x 8192 12.8 / 14.8, 8192 x 8192 21.2 / 23.4; 16 tokens 2048 x
 //   8192 8.1 / 10.4, 4096 x 4096 9.8 / 9.8, but 8192 x 256 16 / 7, 8192 x 8192 30 / 24, and beyond one round of workgroups the
 //   tiles stream W faster: 4096 x 14336 23.5 / 18.9. 24 tokens: 768 x 768 4.5 / 6.1, 2048 x 8192 9.4 / 10.6, 4096 x 4096 12.2 / 10.
-//   up to 64 tokens: 48 x 768 x 768 5.7 / 6.0, but 48 x 1537 x 3333 22 / 11.
+//   up to 64 tokens: 48 x 768 x 768 5.7 / 6.0, but 64 x 2048 x 2048 11 / 7.7.
 //   fp32: one token 4096 x 4096 13 / 25, 16 tokens 8192 x 28672 228 / 263, but 8192 x 256 29 / 10; 24 tokens 4096 x 4096 23.2 /
 //   25.5, 4096 x 14336 71 / 77, 8192 x 8192 64 / 81, but 6500 x 4800 60 / 46, 4096 x 28672 140 / 135, 2048 x 2048 12.7 / 11.2;
 //   40 x 333 x 777 6.1 / 11.2, but 48 x 768 x 768 9.4 / 8.6.
