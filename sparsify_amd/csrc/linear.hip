@@ -60,14 +60,14 @@ static int splits_of(int dtype, int by, int64_t N, int64_t M, int64_t K) {
 }
 // Time of a product with 64 x 64 or 128 x 128 tiles in ns, without what both take: K steps one after the other, a step of one
 // workgroup `step` (measured: 64 x 64 200 bf16, 520 fp32; 128 x 128 570 and 2100 alone on its compute unit, 400 and 1950 where
-// two share one), 1.2 us more of filling and finishing for the larger tile, and for a split K range the joining launch and a
-// round trip of the partial tiles at 3 TB/s.
+// two share one), 1.2 us more of filling and finishing for the larger tile, and for a split K range 3 us of joining launch
+// and a round trip of the partial tiles at 8 TB/s (they stay in the Infinity Cache: 100 x 7152 x 5504 31 us whole, 25 split).
 static int64_t product_ns(int dtype, int by, int64_t N, int64_t M, int64_t K) {
     const int64_t tile = by == BY_64 ? 64 : 128, splits = splits_of(dtype, by, N, M, K);
     const int64_t groups = cdiv(N, tile) * cdiv(M, tile) * splits, steps = cdiv(cdiv(K, 128 / (int64_t)dtype_size(dtype)), splits);
     const bool bf = dtype == SPHIP_BF16;
     const int64_t step = by == BY_64 ? (bf ? 200 : 520) : groups <= 256 ? (bf ? 570 : 2100) : (bf ? 400 : 1950);
-    return steps * step * cdiv(groups, 256) + (by == BY_64 ? 0 : 1200) + (splits > 1 ? 4000 + splits * N * M / 375 : 0);
+    return steps * step * cdiv(groups, 256) + (by == BY_64 ? 0 : 1200) + (splits > 1 ? 3000 + splits * N * M / 1000 : 0);
 }
 static int kernel_for(int dtype, int64_t N, int64_t M, int64_t K) {
     if (g_forced == '6') return BY_64;

@@ -93,15 +93,15 @@ __global__ __launch_bounds__(256, 2) void linear64_kernel(Operand A, Operand B, 
 }
 
 // Splits of the K range: the power of two (or as many as fill the compute units once) with the least time by the step's
-// measured 200 ns (bf16; 520 fp32) and, for a split, 4 us of joining launch and a round trip of the partial tiles at 3 TB/s.
-// (Also where the tiles fill the units, but leave most of them idle in their last round: fp32 1136 x 3467 x 1218 128 us whole,
-// 112 in two.)
+// measured 200 ns (bf16; 520 fp32) and, for a split, the joining launch and the partial tiles' round trip (as in linear.hip).
+// (Also into more workgroups than there are units, where that leaves them idle for less of the time: fp32 300 x 2048 x 2048 40 us
+// whole, 38 in two.)
 int linear64_splits(int dtype, int64_t N, int64_t M, int64_t K) {
     const int64_t tiles = cdiv(N, T64) * cdiv(M, T64), steps = cdiv(K, 128 / (int64_t)dtype_size(dtype));
     const int64_t step = dtype == SPHIP_BF16 ? 200 : 520, fill = 256 / tiles < steps / 4 ? 256 / tiles : steps / 4;
     int64_t best = 1, least = steps * step * cdiv(tiles, 256);
     auto consider = [&](int64_t s) {
-        const int64_t t = cdiv(steps, s) * step * cdiv(tiles * s, 256) + 4000 + s * N * M / 375;
+        const int64_t t = cdiv(steps, s) * step * cdiv(tiles * s, 256) + 3000 + s * N * M / 1000;
         if (t < least) best = s, least = t;
     };
     for (int64_t s = 2; s <= steps / 4 && tiles * s <= 1024; s *= 2) consider(s);
