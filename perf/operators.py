@@ -156,8 +156,7 @@ def _round_trip(x, fmt, keep_sign=False):
         e = expo - 7 + (mant > 127 / 128).to(expo.dtype)
     else:
         e = expo - 9 + (mant > 0.875).to(expo.dtype)
-    least = -126 if fmt == "int8" else -117          # the smallest code is a normal number
-    e = torch.where(top > 0, e, torch.full_like(e, least)).clamp(min=least)
+    e = torch.where(top > 0, e, torch.full_like(e, -126)).clamp(min=-126)
     q = torch.ldexp(groups, -e)
     code = torch.round(q) if fmt == "int8" else q.to(torch.float8_e4m3fn).float()
     if keep_sign:
@@ -225,7 +224,7 @@ def _code_values(v, fmt, keep_sign):
         need = top.clamp(min=2.0 ** -200) / most
         e = torch.ceil(torch.log2(need))
         e = torch.where(torch.exp2(e - 1) >= need, e - 1, e)          # log2 may round either way
-        e = torch.where(torch.exp2(e) < need, e + 1, e).clamp(min=-126.0 if fmt == "int8" else -117.0)
+        e = torch.where(torch.exp2(e) < need, e + 1, e).clamp(min=-126.0)
         q = rows / torch.exp2(e)
         if fmt == "int8":
             step = torch.ones_like(q)
