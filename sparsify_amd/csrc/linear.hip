@@ -476,7 +476,9 @@ extern "C" int sphip_linear(const void* x, int64_t ldx, const void* W, int64_t l
     if (zc && f.z) e.z = (char*)ws + f.part, e.z_dt = SPHIP_F32, e.ldz = cdiv(M, 4) * 4;
     else e.z = z, e.z_dt = z_kind, e.ldz = ldz, e.z_scales = zc ? z_scales : nullptr;
     Operand A = {x, ldx, (int)N}, B = {W, ldw, (int)M};
-    const int64_t K = f.copies ? whole_pieces(D) : D, ld = packed_ld(D);
+    // K up to whole pieces only where zeros follow the rows of both operands: behind the rows of one that is not copied lies
+    // the next row, or the end of its memory (fp32 copies one alone, whatever D is; bf16 with such a D copies both)
+    const int64_t K = f.copies == (COPY_X | COPY_W) ? whole_pieces(D) : D, ld = packed_ld(D);
     char* to = (char*)ws + f.part + f.z;
     int st = SPHIP_OK;
     Packing p(dtype);
