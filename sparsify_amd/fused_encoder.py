@@ -102,12 +102,21 @@ class LazyPreActs:
         return func(*unwrap(args), **{k_: unwrap(v) for k_, v in (kwargs or {}).items()})
 
 
-# address -> (weak reference to the owning tensor, (version, shape), bf16 buffer). The weak
+# address -> (weak reference to the owning tensor, (version, shape, strides), bf16 buffer). The weak
 # reference pins an entry to the tensor it was made for: the caching allocator hands a freed
 # block to the next same-sized request, so a later parameter can live at the same address with
 # the same shape and version counter (every coder loaded from disk sits at version 2). An entry
-# whose owner has died is dropped, together with its (M, D) bf16 buffer.
+# whose owner has died is dropped, together with its (M, D) bf16 buffer. Views share their base's
+# address and version: strides tell W from W.t() and B[:n] from B[::2], and a view makes no entry.
 _shadows: dict[int, tuple] = {}
+
+
+def _state(t: Tensor) -> tuple:
+    return t._version, tuple(t.shape), t.stride()
+
+
+def _same_layout(a: Tensor, b: Tensor) -> bool:
+    return a.data_ptr() == b.data_ptr() and a.shape == b.shape and a.stride() == b.stride()
 
 
 def _shadow_entry(t: Tensor):
@@ -115,9 +124,9 @@ def _shadow_entry(t: Tensor):
     if hit is None:
         return None
     owner = hit[0]()
-    if owner is None or owner.data_ptr() != t.data_ptr() or owner.shape != t.shape or owner._version != t._version:
-        # the owner is gone, or `t` is another tensor at a recycled address (an alias of the owner
-        # -- a view, .detach() -- shares its version counter and passes)
+    if owner is None or not _same_layout(owner, t) or owner._version != t._version:
+        # the owner is gone, or `t` is another tensor at a recycled address or another view of that
+        # memory (an alias of the owner -- .detach() -- shares its version counter and passes)
         if owner is None:
             _shadows.pop(t.data_ptr(), None)
         return None
@@ -132,7 +141,7 @@ def _store_shadow(t: Tensor, shadow: Tensor) -> None:
         if hit is not None and hit[0] is ref:
             del _shadows[key]
 
-    _shadows[key] = (weakref.ref(t, _drop), (t._version, tuple(t.shape)), shadow)
+    _shadows[key] = (weakref.ref(t, _drop), _state(t), shadow)
 
 
 def bf16_shadow(t: Tensor) -> Tensor:
@@ -145,11 +154,12 @@ def bf16_shadow(t: Tensor) -> Tensor:
     if t.dtype == torch.bfloat16:
         return t
     hit = _shadow_entry(t)
-    if hit is not None and hit[1] == (t._version, tuple(t.shape)):
+    if hit is not None and hit[1] == _state(t):
         return hit[2]
     buf = hit[2] if hit is not None and hit[2].shape == t.shape else None
     sh = ops.cast_bf16(t.detach().contiguous(), buf)
-    _store_shadow(t, sh)
+    if not t._is_view():
+        _store_shadow(t, sh)
     return sh
 
 
@@ -164,14 +174,14 @@ def peek_bf16_shadow(t: Tensor) -> Tensor | None:
     if hit is None:
         return None
     owner = hit[0]()
-    if owner is None or owner.data_ptr() != t.data_ptr() or owner.shape != t.shape:
+    if owner is None or not _same_layout(owner, t):
         return None
     return hit[2]
 
 
 def shadow_is_current(t: Tensor) -> bool:
     hit = _shadow_entry(t)
-    return hit is not None and hit[1] == (t._version, tuple(t.shape))
+    return hit is not None and hit[1] == _state(t)
 
 
 # Optimizer-in-backward for the encoder matrix (sign_sgd.SignSGD.fuse_encoder_update,

@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-from test_hip_linear import assert_within, forward64, make
+from test_hip_linear import TINY, assert_within, backward64, forward64, make
 
 pytestmark = pytest.mark.gpu
 
@@ -54,3 +54,36 @@ def test_one_operand_with_rows_far_apart(device, dtype, N, D, M, far):
     got = fused_linear(far_rows(x) if far == "x" else framed(x), Wc, b.cuda(), activation="silu")
     keep = torch.arange(N, device="cuda") != 7
     assert torch.isnan(got[7]).all() and torch.equal(got[keep], outs[0][0][keep])
+
+
+# ------------------------------------------------------------------ fp32 weights under bf16 autocast
+def autocast_linear(*args, **kw):
+    from sparsify_amd import fused_linear
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        return fused_linear(*args, **kw)
+
+
+def assert_autocast_step(x, W, g):
+    """One step of fp32 x and W under autocast: the product of their bf16 values, gradients from bf16 operands with g (bf16)
+    as it is, fp32 results. W: the tensor or view itself, gradients taken at it."""
+    xi = x.detach().requires_grad_()
+    y = autocast_linear(xi, W)
+    xb, Wb = x.detach().cpu().bfloat16(), W.detach().cpu().bfloat16()
+    want, tol, _, _ = forward64(xb, Wb, None, None, "none", torch.bfloat16)
+    assert_within(y.detach(), want, tol, "y")
+    dx, dW = torch.autograd.grad(y, [xi, W], g)
+    ref = backward64(xb, Wb, None, "none", g.cpu(), want, xb, torch.float32, torch.bfloat16, 0.0)
+    assert_within(dx, *ref["x"], "dx")
+    want, mag = g.cpu().double().T @ xb.double(), g.cpu().double().abs().T @ xb.double().abs()
+    assert_within(dW, want, (x.shape[0] + 4) * 2.0**-23 * mag + 2.0**-24 * want.abs() + TINY, "dW")
+
+
+def test_weights_at_one_address(device):
+    """A weight, its transpose, and two views of one size: each by its own values, forward and gradients, in any order."""
+    gen = torch.Generator().manual_seed(1)
+    W = (torch.randn(96, 96, generator=gen) / 10).cuda().requires_grad_()
+    x = torch.randn(130, 96, generator=gen).cuda()
+    g = {m: torch.randn(130, m, generator=gen).bfloat16().cuda() for m in (96, 48)}
+    views = [W, W.t(), W[:48], W[::2], W.t()[:48], W]
+    for v in views + views[::-1]:
+        assert_autocast_step(x, v, g[v.shape[0]])
