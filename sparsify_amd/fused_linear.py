@@ -10,7 +10,7 @@ from torch.autograd.function import once_differentiable
 
 from . import ops, parallel
 from .checkpoint8 import Checkpoint8, as_rows
-from .fused_encoder import _autocast_bf16, bf16_shadow
+from .fused_encoder import _autocast_bf16
 
 
 def _operands(input: Tensor, weight: Tensor):
@@ -26,7 +26,9 @@ def _operands(input: Tensor, weight: Tensor):
     if _autocast_bf16():
         if x.dtype != torch.bfloat16:
             x = ops.center_cast(x.contiguous(), None, False, True)[1] if x.numel() else x.bfloat16()
-        return x, as_rows(bf16_shadow(weight))
+        # cast by every call, on its stream and inside its graph (4096 x 4096: 64 MiB read): a copy kept between calls would
+        # be the old weight in the replays of a graph
+        return x, as_rows(weight) if weight.dtype == torch.bfloat16 else ops.cast_bf16(weight.detach().contiguous())
     if weight.dtype != torch.float32:
         raise TypeError(f"fused_linear: weight is {weight.dtype} and input {input.dtype}; bf16 products need both in bf16 "
                         "or bf16 autocast")
@@ -51,8 +53,9 @@ class FusedLinear(torch.autograd.Function):
         kept_x = None
         if need_w:
             kept_x = x if fmt is None else codes if made is None else made.data
-        ctx.save_for_backward(weight, kept_x, z)
-        ctx.fmt, ctx.activation, ctx.compute = fmt, activation, x.dtype
+        # dx reads the weight the product ran with; dW and db only its shape
+        ctx.save_for_backward(w if need_x and w.dtype != weight.dtype else weight, kept_x, z)
+        ctx.fmt, ctx.activation, ctx.compute, ctx.w_dtype = fmt, activation, x.dtype, weight.dtype
         ctx.like = (input.shape, input.dtype, None if bias is None else bias.dtype, None if residual is None else residual.dtype)
         ctx.set_materialize_grads(False)
         return y if input.ndim == 2 else y.reshape(*input.shape[:-1], weight.shape[0])
@@ -67,10 +70,9 @@ class FusedLinear(torch.autograd.Function):
         in_shape, in_dtype, b_dtype, r_dtype = ctx.like
         dx = dW = db = None
         if need_x or need_w or need_b:
-            w = as_rows(bf16_shadow(weight) if ctx.compute == torch.bfloat16 else weight)
-            dx, dW, db = ops.linear_backward(as_rows(g), w, z, x, ctx.activation, z_fmt=ctx.fmt, x_fmt=ctx.fmt,
-                                             dx_dtype=in_dtype if need_x else None, dw_dtype=weight.dtype if need_w else None,
-                                             db_dtype=b_dtype if need_b else None)
+            dx, dW, db = ops.linear_backward(as_rows(g), as_rows(weight), z, x, ctx.activation, z_fmt=ctx.fmt, x_fmt=ctx.fmt,
+                                             dx_dtype=in_dtype if need_x else None, dw_dtype=ctx.w_dtype if need_w else None,
+                                             db_dtype=b_dtype if need_b else None, dtype=ctx.compute)
             if need_x and len(in_shape) != 2:
                 dx = dx.reshape(in_shape)
         dr = None

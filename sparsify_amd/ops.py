@@ -1403,13 +1403,20 @@ def _kept(t: Tensor, fmt: str | None, name: str, N: int, D: int, like: Tensor):
 
 def linear_backward(g: Tensor, W: Tensor, z: Tensor | None, x: Tensor | None, activation: str = "none", *,
                     z_fmt: str | None = None, x_fmt: str | None = None, dx_dtype: torch.dtype | None = None,
-                    dw_dtype: torch.dtype | None = None, db_dtype: torch.dtype | None = None):
+                    dw_dtype: torch.dtype | None = None, db_dtype: torch.dtype | None = None, dtype: torch.dtype | None = None):
     """(dx, dW, db) of linear from g = dL/dout (N, M): dz = g act'(z), dx = dz @ W, dW = dz.T @ x, db = dz.sum(0); a dtype
     of None leaves that one out. z and x: tensors, or checkpoint buffers (z_fmt / x_fmt) that are read as they are. The
-    products run in W's dtype (dz rounded to it once), db sums dz unrounded; every sum has a fixed order."""
+    products run in `dtype`, W's by default (dz rounded to it once), db sums dz unrounded; every sum has a fixed order. Only
+    dx reads W, which then has to have that dtype; of another one only its shape counts."""
     act = _act(activation)
     gp, ldg, g_dt = _rows(g, "grad")
     Wp, ldw, dt = _rows(W, "weight", like=g)
+    if dtype is None:
+        dtype = W.dtype
+    elif dtype != W.dtype:
+        if dx_dtype is not None:
+            raise ValueError(f"linear_backward: products in {dtype} with a weight of {W.dtype}")
+        dt = BF16 if dtype == torch.bfloat16 else F32
     (N, M), (K, D) = g.shape, W.shape
     if K != M:
         raise ValueError(f"linear_backward: grad {tuple(g.shape)} does not go with weight {tuple(W.shape)}")
@@ -1419,7 +1426,7 @@ def linear_backward(g: Tensor, W: Tensor, z: Tensor | None, x: Tensor | None, ac
             raise ValueError(f"linear_backward: activation {activation!r} needs z")
         zargs = _kept(z, z_fmt, "z", N, M, g)
     if dw_dtype is not None:
-        if x is None or (x_fmt is None and x.dtype != W.dtype):
+        if x is None or (x_fmt is None and x.dtype != dtype):
             raise ValueError("linear_backward: the weight's gradient needs x, in the weight's dtype or 8 bits")
         xargs = _kept(x, x_fmt, "x", N, D, g)
     dx = None if dx_dtype is None else g.new_empty((N, D), dtype=dx_dtype)

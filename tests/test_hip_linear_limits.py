@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-from test_hip_linear import TINY, assert_within, backward64, forward64, make
+from test_hip_linear import TINY, assert_within, backward64, cuda, forward64, make
 
 pytestmark = pytest.mark.gpu
 
@@ -87,3 +87,123 @@ def test_weights_at_one_address(device):
     views = [W, W.t(), W[:48], W[::2], W.t()[:48], W]
     for v in views + views[::-1]:
         assert_autocast_step(x, v, g[v.shape[0]])
+
+
+def autocast_inputs(seed, N=130, D=260, M=70):
+    x, W, b, r = make(N, D, M, torch.float32, seed, res=torch.float32)
+    g = torch.randn(N, M, generator=torch.Generator().manual_seed(seed)).cuda()
+    return [t.requires_grad_() for t in cuda(x, W, b, r)], g
+
+
+def autocast_step(ts, g):
+    y = autocast_linear(*ts[:3], residual=ts[3], activation="gelu", checkpoint="e4m3")
+    return (y.detach(), *torch.autograd.grad(y, ts, g))
+
+
+def test_captured_autocast_steps_read_the_weight_of_each_replay(device):
+    """fp32 parameters under autocast in two captured graphs, the parameters changed between replays; an eager call between
+    capture and first replay, and between replays, sees its own weights too."""
+    want = {s: autocast_step(*autocast_inputs(s)) for s in range(5)}
+    graphs = []
+    for seed in range(2):
+        ts, g = autocast_inputs(seed)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            autocast_step(ts, g)                    # (the eager call before leaves nothing that the capture takes up)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = autocast_step(ts, g)
+        for a, c in zip(autocast_step(ts, g), want[seed]):
+            assert torch.equal(a, c)
+        graphs.append((graph, ts, g, outs))
+    for seed in (2, 3, 4):
+        new, ng = autocast_inputs(seed)
+        for graph, ts, g, outs in graphs:
+            with torch.no_grad():
+                for t, n in zip(ts, new):
+                    t.copy_(n)
+                g.copy_(ng)
+            graph.replay()
+        torch.cuda.synchronize()
+        for _, ts, g, outs in graphs:
+            for a, c in zip(outs, want[seed]):
+                assert torch.equal(a, c)
+            for a, c in zip(autocast_step(ts, g), want[seed]):
+                assert torch.equal(a, c)
+
+
+def test_a_graph_that_changes_its_weight(device):
+    """Training inside a graph: every replay moves W, whose version the host never sees. An eager call reads the new W."""
+    ts, g = autocast_inputs(3)
+
+    def train():
+        y = autocast_linear(*ts[:3], residual=ts[3])
+        (dW,) = torch.autograd.grad(y, ts[1:2], g)
+        with torch.no_grad():
+            ts[1].sub_(dW)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        train()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        train()
+    for _ in range(3):
+        autocast_step(ts, g)
+        before = ts[1].detach().clone()
+        graph.replay()
+        fresh = [t.detach().clone().requires_grad_() for t in ts]
+        assert not torch.equal(fresh[1], before)
+        for a, c in zip(autocast_step(ts, g), autocast_step(fresh, g)):
+            assert torch.equal(a, c)
+
+
+def test_autocast_steps_on_two_streams(device):
+    """Two streams that share a weight, changed in place between rounds: neither reads what the other has not written yet."""
+    (x, W, b, r), g = autocast_inputs(4, 300, 700, 90)
+    other, _ = autocast_inputs(5, 300, 700, 90)
+    values = [W.detach().clone(), other[1].detach().clone()]
+    want = []
+    for v in values:
+        want.append(autocast_step([x, v.clone().requires_grad_(), b, r], g))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for i in range(6):
+        for st in streams:
+            torch.cuda.current_stream().wait_stream(st)
+        with torch.no_grad():
+            W.copy_(values[i % 2])
+        for j, st in enumerate(streams if i % 4 < 2 else streams[::-1]):
+            st.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(st):
+                if j == 0:
+                    torch.cuda._sleep(10_000_000)   # the first stream is behind the second by some milliseconds
+                got.append((i % 2, autocast_step([x, W, b, r], g)))
+    torch.cuda.synchronize()
+    for i, outs in got:
+        for a, c in zip(outs, want[i]):
+            assert torch.equal(a, c)
+
+
+def test_a_weight_changed_behind_its_version(device):
+    ts, g = autocast_inputs(6)
+    autocast_step(ts, g)
+    ts[1].data.mul_(0.5)                            # (.data has a version counter of its own)
+    fresh = [t.detach().clone().requires_grad_() for t in ts]
+    for a, c in zip(autocast_step(ts, g), autocast_step(fresh, g)):
+        assert torch.equal(a, c)
+
+
+def test_a_weight_that_changes_between_forward_and_backward(device):
+    """dx reads the bf16 copy of the forward, dW no weight: the gradients are those at the forward's weight."""
+    ts, g = autocast_inputs(7)
+    want = autocast_step(ts, g)
+    y = autocast_linear(*ts[:3], residual=ts[3], activation="gelu", checkpoint="e4m3")
+    with torch.no_grad():
+        ts[1].zero_()
+    for a, c in zip(torch.autograd.grad(y, ts, g), want[1:]):
+        assert torch.equal(a, c)

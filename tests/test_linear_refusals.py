@@ -158,3 +158,11 @@ def test_the_training_switch():
         TrainConfig(sae=SparseCoderConfig(), checkpoint_8bit="fp8")
     with pytest.raises(ValueError, match="shard_latents"):
         TrainConfig(sae=SparseCoderConfig(), checkpoint_8bit="int8", shard_latents=True)
+
+
+def test_a_gradient_of_x_needs_the_weight_in_the_products_type(monkeypatch):
+    from sparsify_amd import ops
+    monkeypatch.setattr(ops, "_rows", lambda t, name, shape=None, like=None: (P, t.shape[1], ops._dt(t)))
+    g, W = torch.zeros(4, 5), torch.zeros(5, 8)
+    with pytest.raises(ValueError, match="products in torch.bfloat16 with a weight of torch.float32"):
+        ops.linear_backward(g, W, None, None, dx_dtype=torch.float32, dtype=torch.bfloat16)
