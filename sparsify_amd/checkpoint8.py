@@ -40,7 +40,9 @@ class Checkpoint8:
         return self.data.numel()
 
     def restore(self, dtype: torch.dtype | None = None) -> Tensor:
-        """The values the codes stand for, in the dtype of what was saved or another one (exact in fp32 and bf16)."""
+        """The values the codes stand for, in the dtype of what was saved or another one (exact in fp32 and bf16). New
+        values: no gradient leads from them to what was saved."""
+        _not_in_a_trace()
         out = ops.checkpoint8_restore(self.data, self.fmt, self.rows, self.columns, self.dtype if dtype is None else dtype)
         return out if len(self.shape) == 2 else out.reshape(self.shape)
 
@@ -48,9 +50,16 @@ class Checkpoint8:
 def checkpoint8(x: Tensor, fmt: str = "int8", *, keep_sign: bool = False) -> Checkpoint8:
     """x (..., D), fp32 or bf16, in 8 bits; the leading dims are the tokens, groups of 32 in their order.
     fmt: "int8" or "e4m3". keep_sign: a value other than zero never becomes zero (a ReLU's mask survives)."""
+    _not_in_a_trace()
     if x.ndim < 1:
         raise ValueError("checkpoint8: expected (..., D), got a scalar")
     return Checkpoint8(ops.checkpoint8_save(as_rows(x), fmt, keep_sign), fmt, x.shape, x.dtype)
+
+
+def _not_in_a_trace() -> None:
+    if torch.jit.is_tracing():
+        raise RuntimeError("8-bit checkpoints cannot be traced: the trace would hold the codes of this input, or memory that "
+                           "nothing fills")
 
 
 def as_rows(t: Tensor) -> Tensor:

@@ -6,6 +6,7 @@ from __future__ import annotations
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import ops, parallel
@@ -111,6 +112,10 @@ def fused_linear(input: Tensor, weight: Tensor, bias: Tensor | None = None, *, r
         ops._code(checkpoint)
     if torch.is_grad_enabled() and (input.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
                                     or (residual is not None and residual.requires_grad)):
+        return FusedLinear.apply(input, weight, bias, residual, activation, checkpoint)
+    if forward_ad._current_level >= 0 or torch.jit.is_tracing():
+        # the Function refuses an input with a tangent (there is no forward-mode derivative) and is what a trace records: the
+        # kernels' launches are in neither's sight
         return FusedLinear.apply(input, weight, bias, residual, activation, checkpoint)
     x, w = _operands(input, weight)
     y = ops.linear(x, w, None if bias is None else bias.contiguous(), None if residual is None else as_rows(residual),

@@ -207,3 +207,16 @@ def test_a_weight_that_changes_between_forward_and_backward(device):
         ts[1].zero_()
     for a, c in zip(torch.autograd.grad(y, ts, g), want[1:]):
         assert torch.equal(a, c)
+
+
+def test_a_traced_call_launches_the_kernels(device):
+    from sparsify_amd import fused_linear
+    x, W, b, r = cuda(*make(40, 72, 56, torch.bfloat16, 2, res=torch.float32))
+
+    def f(x, W, b, r):
+        return fused_linear(x, W, b, residual=r, activation="silu")
+
+    traced = torch.jit.trace(f, (x, W, b, r), check_trace=False)
+    for seed in (3, 4):
+        args = cuda(*make(40, 72, 56, torch.bfloat16, seed, res=torch.float32))
+        assert torch.equal(traced(*args), f(*args))
