@@ -1307,13 +1307,14 @@ def _scratch(t: Tensor, nbytes: int) -> Tensor | None:
     return t.new_empty((nbytes,), dtype=torch.uint8) if nbytes else None
 
 
+# `forced`: SPHIP_LINEAR, which the library reads again in every call
 @functools.lru_cache(maxsize=1024)
-def _linear_bytes(*args) -> int:
+def _linear_bytes(forced: str | None, *args) -> int:
     return _lib.load().sphip_linear_workspace_bytes(*args)
 
 
 @functools.lru_cache(maxsize=1024)
-def _linear_backward_bytes(*args) -> int:
+def _linear_backward_bytes(forced: str | None, *args) -> int:
     return _lib.load().sphip_linear_backward_workspace_bytes(*args)
 
 
@@ -1381,7 +1382,7 @@ def linear(x: Tensor, W: Tensor, bias: Tensor | None = None, residual: Tensor | 
         codes, x_scales, x_ld = _new_codes(x, N, D)
     if N == 0:
         return out, z, codes
-    nws = _linear_bytes(dt, z_kind, N, D, M, _odd(xp, ldx, dt) + 2 * _odd(Wp, ldw, dt))
+    nws = _linear_bytes(os.environ.get("SPHIP_LINEAR"), dt, z_kind, N, D, M, _odd(xp, ldx, dt) + 2 * _odd(Wp, ldw, dt))
     ws = _scratch(x, nws)
     _call("sphip_linear", x, xp, ldx, Wp, ldw, dt, bp, b_dt, act, rp, r_dt, ldr, out.data_ptr(), _dt(out), M, _ptr(z), z_kind,
           z_scales, z_ld, _ptr(codes), x_scales, x_fmt, x_ld, N, D, M, _ptr(ws), nws)
@@ -1437,7 +1438,8 @@ def linear_backward(g: Tensor, W: Tensor, z: Tensor | None, x: Tensor | None, ac
     if dx is None and dW is None and db is None:
         return None, None, None
     odd = (x_fmt is None and dW is not None and _odd(xargs[0], xargs[3], dt)) + 2 * (dx is not None and _odd(Wp, ldw, dt))
-    nws = _linear_backward_bytes(dt, xargs[1], dx is not None, dW is not None, db is not None, N, D, M, odd)
+    nws = _linear_backward_bytes(os.environ.get("SPHIP_LINEAR"), dt, xargs[1], dx is not None, dW is not None, db is not None, N, D,
+                                 M, odd)
     ws = _scratch(g, nws)
     _call("sphip_linear_backward", g, gp, g_dt, ldg, Wp, ldw, dt, act, *zargs, *xargs,
           _ptr(dx), 0 if dx is None else _dt(dx), D, _ptr(dW), 0 if dW is None else _dt(dW), D, _ptr(db),

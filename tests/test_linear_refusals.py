@@ -166,3 +166,24 @@ def test_a_gradient_of_x_needs_the_weight_in_the_products_type(monkeypatch):
     g, W = torch.zeros(4, 5), torch.zeros(5, 8)
     with pytest.raises(ValueError, match="products in torch.bfloat16 with a weight of torch.float32"):
         ops.linear_backward(g, W, None, None, dx_dtype=torch.float32, dtype=torch.bfloat16)
+
+
+def test_the_workspace_follows_the_forced_kernel(monkeypatch):
+    """SPHIP_LINEAR set to something else between two calls of one shape: each passes what the library asks for now."""
+    from sparsify_amd import ops
+    sizes = []
+    monkeypatch.setattr(ops, "_rows", lambda t, name, shape=None, like=None: (P, t.shape[1], ops._dt(t)))
+    monkeypatch.setattr(ops, "_scratch", lambda t, nbytes: sizes.append(nbytes))
+    monkeypatch.setattr(ops, "_call", lambda *args: None)
+    N, D, M = 64, 4096, 136
+    x, W, g = (torch.zeros(s, dtype=torch.bfloat16) for s in ((N, D), (M, D), (N, M)))
+    seen = set()
+    for kernel in ("64", "128", "few", "256", "64"):
+        monkeypatch.setenv("SPHIP_LINEAR", kernel)
+        ops.linear(x, W)
+        ops.linear_backward(g, W, None, x, dx_dtype=torch.bfloat16, dw_dtype=torch.bfloat16)
+        want = (lib().sphip_linear_workspace_bytes(BF16, 0, N, D, M, 0),
+                lib().sphip_linear_backward_workspace_bytes(BF16, BF16, 1, 1, 0, N, D, M, 0))
+        assert tuple(sizes[-2:]) == want, kernel
+        seen.add(want)
+    assert len(seen) >= 3
