@@ -557,7 +557,8 @@ int sphip_linear_backward(const void* g, int g_dtype, int64_t ldg, const void* W
  * tokens of one feature share the scale 2^(byte - 127), the smallest that keeps them within 127 (SPHIP_INT8: signed
  * integers) or 448 (SPHIP_E4M3: 8-bit floats, 4 exponent and 3 mantissa bits), at least
  * 2^-126 or 2^-117 (the smallest code is a normal number); values are rounded to the nearest code,
- * ties to even. keep_sign: a non-zero value never becomes zero (smallest code of its sign). A group holding an infinity
+ * ties to even; what would restore past the largest fp32 (from 63.5 2^122 or 248 2^120 on) takes the code below.
+ * keep_sign: a non-zero value never becomes zero (smallest code of its sign). A group holding an infinity
  * or a NaN restores as NaN. Padding rows and columns are written as zero codes.
  * restore: the values, exact in either dtype. */
 int sphip_checkpoint8_save(const void* x, int dtype, int64_t ldx, int fmt, int keep_sign, uint8_t* codes, uint8_t* scales,

@@ -9,6 +9,7 @@
 //   int8  q = x / 2^e rounded to nearest even, |q| <= 127: off by at most 2^(e-1), i.e. 1/128 of the group's maximum
 //   e4m3  x / 2^e rounded to the nearest 8-bit float of 4 exponent and 3 mantissa bits (OCP, no infinities): off by at
 //         most 2^-4 of the value (2^(e-10) below 2^(e-6))
+// Values from 63.5 2^122 (248 2^120) on, whose nearest code would stand for 2^128, take the code below: finite (codes_of).
 // A power of two makes the division exact (one rounding per value) and code times scale a bf16 number exactly.
 // keep_sign: a value other than zero keeps its sign, the smallest code in place of zero (a ReLU's mask).
 // A group with an infinity or a NaN in it has scale byte 255 and restores as NaN throughout.

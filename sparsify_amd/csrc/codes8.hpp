@@ -67,8 +67,14 @@ template <int FMT> __device__ __forceinline__ unsigned scale_byte(unsigned top) 
 __device__ __forceinline__ float inverse_scale(unsigned byte) { return __uint_as_float((byte == 255u ? 127u : 254u - byte) << 23); }
 // Codes of four values, given the inverse scales: powers of two, so that a * inv is exact and there is one rounding, to
 // nearest even. bad: 0xff in the bytes whose group is to read as NaN (their codes are not looked at; kept finite).
-template <int FMT> __device__ __forceinline__ unsigned codes_of(const float (&a)[4], const float (&inv)[4], bool keep_sign, unsigned bad) {
+// Under the largest scale the next code up, 64 2^122 (256 2^120), is past the largest fp32: what would round to it, from
+// 63.5 2^122 (248 2^120) on, is taken as the number just below, so that a finite value restores as one.
+template <int FMT> __device__ __forceinline__ unsigned codes_of(const float (&v)[4], const float (&inv)[4], bool keep_sign, unsigned bad) {
+    const float most = __uint_as_float(FMT == SPHIP_INT8 ? 0x7f7dffffu : 0x7f77ffffu);
     unsigned w;
+    float a[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) a[j] = __builtin_amdgcn_fmed3f(v[j], -most, most);
     if (FMT == SPHIP_INT8) {
         // + 1.5 2^23: the low byte is the two's complement code
         unsigned c[4];

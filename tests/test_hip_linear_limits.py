@@ -220,3 +220,50 @@ def test_a_traced_call_launches_the_kernels(device):
     for seed in (3, 4):
         args = cuda(*make(40, 72, 56, torch.bfloat16, seed, res=torch.float32))
         assert torch.equal(traced(*args), f(*args))
+
+
+# ------------------------------------------------------------------ values near the largest
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+def test_finite_values_restore_as_finite_ones(device, fmt, dtype):
+    """Groups whose largest value is 2^127 and up. Codes under the scale that keeps it; where the nearest one stands for 2^128,
+    the one below it: off by at most a step, 2^122, instead of half of one (int8), or by 2^-4 of the value (e4m3)."""
+    from sparsify_amd import checkpoint8
+    from test_hip_linear import codes64
+    most = torch.finfo(dtype).max
+    edges = [1.0, 1.5, 1.75, 1.765625, 1.875, 1.9296875, 1.9375, 1.9765625, 1.984375, 1.9921875]
+    tops = torch.tensor([e * 2.0**127 for e in edges] + [most], dtype=torch.float64).to(dtype)
+    assert torch.isfinite(tops).all()
+    x = torch.randn(64, tops.numel(), generator=torch.Generator().manual_seed(0)).double()
+    x = (x / x.abs().amax(0) * 2.0**126).to(dtype)
+    x[5], x[40] = tops, -tops
+    x[6] = torch.nextafter(tops.float(), torch.zeros(())).to(dtype)
+    x[6] = torch.where(torch.isfinite(x[6]), x[6], tops)
+    want = codes64(x, fmt)
+    last = 63 * 2.0**122 if fmt == "int8" else 240 * 2.0**120
+    want = torch.where(want.abs() >= 2.0**128, torch.sign(want) * last, want)
+    for keep_sign in (False, True):
+        c = checkpoint8(x.cuda(), fmt, keep_sign=keep_sign)
+        for kept in (torch.float32, torch.bfloat16):
+            got = c.restore(kept)
+            assert torch.isfinite(got).all()
+            pick = torch.ones_like(want, dtype=torch.bool) if not keep_sign else want != 0
+            assert torch.equal(got.double().cpu()[pick], want[pick])
+    off = (want - x.double()).abs()
+    bound = 2.0**-4 * x.double().abs() + 2.0**-13 * 2.0**127 if fmt == "e4m3" else torch.full_like(off, 2.0**122)
+    assert (off <= bound).all()
+
+
+def test_kept_pre_activation_near_the_largest(device):
+    """The product's own codes of z: an identity's values as they come."""
+    from sparsify_amd import ops
+    top = torch.finfo(torch.float32).max
+    x = torch.tensor([top, -top, 2.0**127, 1.9375 * 2.0**127, 1.0, 0.0, -3e38, 3.3e38]).repeat(64, 8).cuda()
+    W = torch.eye(64, device="cuda")
+    for fmt in ("int8", "e4m3"):
+        for kernel_rows in (64, 130):               # the few-rows kernel's way over fp32, and codes in the epilogue
+            xi = x.repeat(3, 1)[:kernel_rows]
+            _, z, _ = ops.linear(xi, W, activation="silu", keep_z=fmt)
+            got = ops.checkpoint8_restore(z, fmt, kernel_rows, 64, torch.float32)
+            want = ops.checkpoint8_restore(ops.checkpoint8_save(xi, fmt), fmt, kernel_rows, 64, torch.float32)
+            assert torch.isfinite(got).all() and torch.equal(got, want)
