@@ -398,26 +398,36 @@ struct ForwardSpace {
     bool one;
 };
 // Whether the forward product takes linear_few.hip: one launch, no copies, but its workgroups read all of x each and share K
-// among 8 waves only. us here / with 64 x 64 tiles:
-//   bf16, up to 16 tokens: one token 4096 x 4096 7.3 / 9.3, 4096 x 8192 12.8 / 14.8, 8192 x 8192 21.2 / 23.4; 16 tokens 2048 x
-//   8192 8.1 / 10.4, 4096 x 4096 9.8 / 9.8, but 8192 x 256 16 / 7, 8192 x 8192 30 / 24, and beyond one round of workgroups the
-//   tiles stream W faster: 4096 x 14336 23.5 / 18.9. 24 tokens: 768 x 768 4.5 / 6.1, 2048 x 8192 9.4 / 10.6, 4096 x 4096 12.2 / 10.
-//   up to 64 tokens: 48 x 768 x 768 5.7 / 6.0, but 64 x 2048 x 2048 11 / 7.7.
-//   fp32: one token 4096 x 4096 13 / 25, 16 tokens 8192 x 28672 228 / 263, but 8192 x 256 29 / 10; 24 tokens 4096 x 4096 23.2 /
-//   25.5, 4096 x 14336 71 / 77, 8192 x 8192 64 / 81, but 6500 x 4800 60 / 46, 4096 x 28672 140 / 135, 2048 x 2048 12.7 / 11.2;
-//   40 x 333 x 777 6.1 / 11.2, but 48 x 768 x 768 9.4 / 8.6.
+// among 8 waves only. Its time follows K and the rounds of its workgroups, one per compute unit up to 4096 (or 8192) rows of W;
+// the tiles', which also split K, follows W's size. us here / with 64 x 64 tiles, W from HBM (widths around the borders and
+// 1700 shapes in all: these rules come within 2 % of the better side on average, 26 % at worst):
+//   bf16, up to 8 tokens: 1 x 4096 x 768 6.8 / 7.0, 4096 x 4096 8.6 / 10.8, 8192 x 4096 14.7 / 20.1, 8192 x 768 11.4 / 8.7; 8 x 2048 x
+//   8000 9.1 / 11.4, 2048 x 8256 11.7 / 12.6, 4096 x 14336 26.9 / 27.5, but 1024 x 14336 9.5 / 8.6.
+//   up to 16: 16 x 3000 x 1000 6.6 / 7.6, 4096 x 4096 10.2 / 11.3, 4096 x 8192 15.5 / 20.6, 4096 x 2048 9.9 / 9.4, 2048 x 8256 13.6 / 12.8.
+//   up to 32: 24 x 1536 x 1000 6.1 / 7.5, 2048 x 2048 7.3 / 7.8, 2048 x 6000 9.8 / 12.8, 2048 x 8000 10.1 / 13.0, 2048 x 8192 10.2 / 13.0,
+//   4096 x 8000 18.5 / 20.5, but 2048 x 768 7.2 / 7.1, 4096 x 4096 12.6 / 11.5, 2048 x 8256 17.2 / 13.0.
+//   fp32, up to 16: 16 x 2048 x 2048 10.2 / 12.0, 4096 x 2048 17.2 / 16.7, 8192 x 4096 36.6 / 46.1, 8192 x 2048 31.6 / 26.5.
+//   up to 32: 24 x 1024 x 768 7.4 / 8.6, 2048 x 4096 14.2 / 16.5, 2048 x 2048 13.8 / 12.3; between 4096 and 8192 rows, a round of 32
+//   each however few they are: 4096 x 4800 35.8 / 32.7, 4096 x 6000 36.5 / 41.1, 4096 x 8000 40 / 44; 4096 x 9000 68 / 63, 4096 x
+//   20000 105 / 135.
+//   up to 64: bf16 48 x 512 x 6000 5.5 / 5.8, fp32 48 x 512 x 8000 10.5 / 13.1, but 64 x 1024 x 768 7.1 / 6.8, fp32 11.8 / 8.9.
 // Where the tiles would have to copy W or x first (bf16), as long as x is short: 24 x 2049 x 8192 24.9 / 25.8, 40 x 333 x 777
 // 7.0 / 8.3, but 48 x 1537 x 3333 22 / 17, 16 x 4097 x 4096 27 / 24.
 static bool few(int dtype, int64_t N, int64_t D, int64_t M, int copies) {
     if (N > FEW || (g_forced && g_forced != 'f')) return false;
     if (g_forced) return true;
-    const bool bf = dtype == SPHIP_BF16, wide = cdiv(M, 32) >= 256;
+    const bool bf = dtype == SPHIP_BF16;
     if (copies) return N * D <= 65536;
-    if (N > 32) return D <= (bf ? 768 : 512) && M <= 2048;
-    if (!bf) return N <= 16 ? D <= 4096 || M >= 2048 : D <= 1024 || wide ? M <= 16384 || D <= 2048 : M >= 2560 && D <= 5120;
-    if (M > 8192) return false;
-    if (N <= 16) return D <= 4096 || (N == 1 && M >= 4096);
-    return D <= (wide ? 2048 : 1024);
+    if (N > 32) return D <= (bf ? 768 : 512) && M <= 8192;
+    if (bf) {
+        if (N <= 8) return M > 8192 ? D >= 2048 : D <= 4096 || 2 * M >= D;
+        if (M > 8192) return false;
+        if (N <= 16) return D <= 3000 || (D <= 4096 && M >= 3000);
+        return D <= 1536 || M >= 2 * (D - 1024);
+    }
+    if (N <= 16) return D <= 2048 || 5 * M >= 2 * D;
+    if (D <= 1024) return true;
+    return M <= 4096 ? M >= 2 * (D - 1024) : M <= 8192 ? 3 * M >= 2 * 8192 : M > 16384;
 }
 // Which of the operands have to be copied, for a query and for a launch alike; `odd`: bits of those that are not fetchable().
 // Where the rows of x are no whole 16-byte pieces, what follows a row would be multiplied with what follows one of W: both.

@@ -138,12 +138,12 @@ template <typename T, int MT> static void launch(const Operand& X, const Operand
     else hipLaunchKernelGGL((linear_few_kernel<T, 4, MT, MT == 1 ? 4 : 2>), grid, block, 0, s, X, W, epi, K);
 }
 
-// 32 rows of W per workgroup (half the reads of x) where that still gives every compute unit one: 24 x 2048 x 8192 9.4 us
-// against 12.5, one token 4096 x 8192 12.8 against 14.4 (fp32 16 x 2048 x 8192 14.7 against 16.9); where it does not, 16 x 4096 x
-// 4096 takes 13.2 against 9.8. Long K needs the second workgroup of a unit: 8192 x 8192 29.6 against 21.2, fp32 4096 x 8192 31.9
-// against 21.8 (24 tokens 39.5 against 44.2).
+// 32 rows of W per workgroup (half the reads of x) where 16 would give a compute unit more than one of them: 24 x 2048 x 6000
+// 9.8 us against 13.1, 2048 x 8000 10.1 against 13.5 (fp32 20.7 against 26.2); where they would not, 24 x 2048 x 4096 takes 9.5
+// against 7.8. Up to 16 tokens only while 32 rows still are one round, 16 x 2048 x 8000 9.1 against 10.3, 2048 x 8256 14.6 against
+// 13.6; up to 8 not at all: one token 4096 x 8000 16.0 against 13.5 (8 tokens: 2048 x 6000 8.0 against 9.2, 4096 x 8000 16.3 / 15.3).
 int launch_linear_few(const char* what, int dtype, const Operand& X, const Operand& W, const Epilogue& epi, int64_t K, hipStream_t s) {
-    const bool bf = dtype == SPHIP_BF16, wide = cdiv(W.rows, 32) >= 256 && (K <= 2048 || (bf ? K <= 4096 : X.rows > 16));
+    const bool bf = dtype == SPHIP_BF16, wide = W.rows > 4096 && (X.rows > 16 || (X.rows > 8 && W.rows <= 8192));
     if (bf && wide) launch<bf16_t, 2>(X, W, epi, K, s);
     else if (bf) launch<bf16_t, 1>(X, W, epi, K, s);
     else if (wide) launch<float, 2>(X, W, epi, K, s);

@@ -267,3 +267,19 @@ def test_kept_pre_activation_near_the_largest(device):
             got = ops.checkpoint8_restore(z, fmt, kernel_rows, 64, torch.float32)
             want = ops.checkpoint8_restore(ops.checkpoint8_save(xi, fmt), fmt, kernel_rows, 64, torch.float32)
             assert torch.isfinite(got).all() and torch.equal(got, want)
+
+
+# ------------------------------------------------------------------ few rows, on both sides of the rules' borders
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("D,M", [(1024, 4095), (2048, 4097), (2050, 6000), (520, 8192), (1536, 8200), (4096, 2047), (48, 9001)])
+def test_few_rows_of_any_width(device, monkeypatch, D, M, dtype):
+    from sparsify_amd import ops
+    for N in (1, 4, 8, 9, 16, 17, 24, 32, 33, 64):
+        x, W, b, r = make(N, D, M, dtype, D + N, res=dtype)
+        want, tol, z, ez = forward64(x, W, b, r, "silu", dtype)
+        xc, Wc, bc, rc = cuda(x, W, b, r)
+        for kernel in ("few", None):
+            monkeypatch.setenv("SPHIP_LINEAR", kernel) if kernel else monkeypatch.delenv("SPHIP_LINEAR")
+            y, zk, _ = ops.linear(xc, Wc, bc, rc, "silu", keep_z=torch.float32)
+            assert_within(y, want, tol, f"y {N} {kernel}")
+            assert_within(zk, z, ez + 2.0**-24 * z.abs() + TINY, f"z {N} {kernel}")
