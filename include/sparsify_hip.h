@@ -542,7 +542,8 @@ int sphip_linear(const void* x, int64_t ldx, const void* W, int64_t ldw, int dty
 /* Its gradients from g = dL/dout (N,M): dz = g act'(z), dx = dz W (N,D), dW = dz^T x (M,D), db = column sums of the
  * unrounded dz (M); any of dx, dW, db may be NULL, and W (for dx), x (for dW), z (SPHIP_ACT_NONE) then are not read.
  * dz is rounded once to `dtype`, the products' type (that of W). z and x: values (z_kind a dtype, x_kind = dtype) or
- * 8-bit checkpoints with scales. The residual's gradient is g. Sums have a fixed order. */
+ * 8-bit checkpoints with scales: z's codes are read as they are, x's restored into the workspace first (N rows of D
+ * elements, D rounded up to 64). The residual's gradient is g. Sums have a fixed order. */
 size_t sphip_linear_backward_workspace_bytes(int dtype, int x_kind, int want_dx, int want_dw, int want_db, int64_t N,
                                              int64_t D, int64_t M, int odd);
 int sphip_linear_backward(const void* g, int g_dtype, int64_t ldg, const void* W, int64_t ldw, int dtype, int act,

@@ -2,8 +2,9 @@
 
 32 consecutive tokens of one feature share a power-of-two scale: the large values of a residual stream sit in a few
 features at nearly all tokens, so a group holds values of one size. ``"int8"`` rounds to 255 even steps (at most 1/127 of
-the group's largest value off), ``"e4m3"`` to 8-bit floats with 4 exponent bits (at most 2^-4 of each value off). Values
-times scales are exact in bf16 and fp32. A group that holds an infinity or a NaN restores as NaN."""
+the group's largest value off), ``"e4m3"`` to 8-bit floats with 4 exponent bits (at most 2^-4 of each value off, or half the
+smallest code's step). Both hold above the smallest scale, 2^-126 or 2^-117; the last step below 2^128 rounds down (1/64 off in
+int8). Values times scales are exact in bf16 and fp32. A group that holds an infinity or a NaN restores as NaN."""
 from __future__ import annotations
 
 import torch
@@ -13,8 +14,8 @@ from . import ops
 
 
 class Checkpoint8:
-    """An activation held in 8 bits: ``checkpoint8(x, fmt)``, read back by ``restore()`` or, without being restored, by
-    the gradients of ``fused_linear(..., checkpoint=...)``.
+    """An activation held in 8 bits: ``checkpoint8(x, fmt)``, read back by ``restore()`` or by the gradients of
+    ``fused_linear(..., checkpoint=...)`` and ``fused_encoder(..., kept=...)``, which restore it for as long as they run.
 
     data: the buffer ops.checkpoint8_save writes; fmt: "int8" / "e4m3"; shape, dtype: of what was saved."""
 

@@ -96,7 +96,8 @@ class TrainConfig(_Serializable):
     checkpoint_8bit: Literal["int8", "e4m3"] | None = None
     """(not in the reference) keep every coder's input between forward and backward in 8 bits, once for the encoder and the
     skip connection (SparseCoder.checkpoint): half the bytes of a bf16 batch, a quarter of an fp32 one. What it saves adds
-    up where many coders wait for one backward pass, the end-to-end losses ("ce", "kl"). Gradients of encoder.weight and
+    up where many coders wait for one backward pass, the end-to-end losses ("ce", "kl"); a coder's own backward restores its
+    input while it runs. Gradients of encoder.weight and
     W_skip are then those at the 8-bit values. Not with `shard_latents`."""
     save_every: int = 1000
     save_best: bool = False

@@ -6,7 +6,8 @@
 // dW = dz^T x contracts over: every 32 terms of its sum share a scale.
 //   e     the smallest with max|x| / 2^e <= 127 (int8) or 448 (e4m3), at least -126 or -117: the smallest code
 //         is then a normal number, 2^-126, in bf16 as in fp32
-//   int8  q = x / 2^e rounded to nearest even, |q| <= 127: off by at most 2^(e-1), i.e. 1/128 of the group's maximum
+//   int8  q = x / 2^e rounded to nearest even, |q| <= 127: off by at most 2^(e-1), above the smallest scale at most 1/127 of
+//         the group's maximum (which is more than 63.5 steps)
 //   e4m3  x / 2^e rounded to the nearest 8-bit float of 4 exponent and 3 mantissa bits (OCP, no infinities): off by at
 //         most 2^-4 of the value (2^(e-10) below 2^(e-6))
 // Values from 63.5 2^122 (248 2^120) on, whose nearest code would stand for 2^128, take the code below: finite (codes_of).

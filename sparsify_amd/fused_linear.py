@@ -1,7 +1,8 @@
 """A dense layer in one pass, ``act(x W^T + b) + residual``, with a backward that can run from 8-bit checkpoints.
 
 The dense counterpart of ``fused_encoder``: the skip connection of a transcoder (sparse_coder.py:219-222,
-``sae_out += x @ W_skip.mT``) is ``fused_linear(x, W_skip, residual=sae_out)``."""
+``sae_out += x @ W_skip.mT``) is ``fused_linear(x, W_skip, residual=sae_out)``, which a SparseCoder with ``checkpoint``
+calls (without it, its SkipProduct)."""
 from __future__ import annotations
 
 import torch
@@ -88,12 +89,18 @@ def fused_linear(input: Tensor, weight: Tensor, bias: Tensor | None = None, *, r
 
     input (..., D), weight (M, D), bias (M), residual (..., M); fp32 or bf16. The product runs in bf16 (fp32 sums) under
     bf16 autocast or when input and weight are bf16, else in exact fp32; the result has the wider dtype of the product
-    and the residual. activation: "none", "relu", "gelu" (exact) or "silu".
+    and the residual. activation: "none", "relu", "gelu" (exact) or "silu". Under autocast an fp32 weight is cast in every
+    call (4096 x 4096: 13 us); hold it in bf16 where it does not change.
+
+    Gradients: dz = grad act'(z) in fp32, rounded once to the product's dtype (a bf16 product: to bf16, also where the
+    result and its gradient are fp32); from it the input's and the weight's with fp32 sums, while the bias's sums dz
+    unrounded. The residual's is grad itself.
 
     checkpoint: what the backward keeps of the input and of the activation's argument. None: as they are in the
-    product's dtype. "int8" / "e4m3": 8-bit checkpoints (checkpoint8.py); the weight's gradient then reads the codes, and
-    gradients are those at the restored values. A Checkpoint8 of this very input (already made for another layer that
-    reads it) is kept instead of a second one."""
+    product's dtype. "int8" / "e4m3": 8-bit checkpoints (checkpoint8.py); gradients are those at the restored values. The
+    backward reads z's codes as they are and, for the weight's gradient, restores the input's into scratch of the input's
+    size in the product's dtype. A Checkpoint8 of this very input (already made for another layer that reads it) is kept
+    instead of a second one."""
     ops._act(activation)
     in_shape, w_shape = input.shape, weight.shape
     if len(w_shape) != 2 or not in_shape or in_shape[-1] != w_shape[1] or 0 in w_shape:

@@ -1410,8 +1410,8 @@ def linear_backward(g: Tensor, W: Tensor, z: Tensor | None, x: Tensor | None, ac
                     z_fmt: str | None = None, x_fmt: str | None = None, dx_dtype: torch.dtype | None = None,
                     dw_dtype: torch.dtype | None = None, db_dtype: torch.dtype | None = None, dtype: torch.dtype | None = None):
     """(dx, dW, db) of linear from g = dL/dout (N, M): dz = g act'(z), dx = dz @ W, dW = dz.T @ x, db = dz.sum(0); a dtype
-    of None leaves that one out. z and x: tensors, or checkpoint buffers (z_fmt / x_fmt) that are read as they are. The
-    products run in `dtype`, W's by default (dz rounded to it once), db sums dz unrounded; every sum has a fixed order. Only
+    of None leaves that one out. z and x: tensors, or checkpoint buffers (z_fmt / x_fmt): z's codes are read as they are, x's
+    are restored into scratch of N x D elements (D rounded up to 64) before the product that reads them. The products run in `dtype`, W's by default (dz rounded to it once), db sums dz unrounded; every sum has a fixed order. Only
     dx reads W, which then has to have that dtype; of another one only its shape counts."""
     act = _act(activation)
     gp, ldg, g_dt = _rows(g, "grad")

@@ -139,7 +139,9 @@ class SparseCoder(nn.Module):
     checkpoint: str | None = None
     """(not in the reference) "int8" / "e4m3": between forward and backward the input is kept once, in
     8 bits (checkpoint8.py), for the encoder's and W_skip's gradients, which are those at its restored
-    values; the skip product then adds sae_out in its own epilogue (fused_linear), unrounded."""
+    values; the skip product then adds sae_out in its own epilogue (fused_linear), unrounded. Each of the two
+    gradients restores the input in bf16 while it runs: what is saved is held between the passes, not
+    at the backward's peak."""
 
     def __init__(
         self,
