@@ -1,7 +1,7 @@
 // The dense product for a few tokens (N <= 64): y = act(x W^T + b) + r, one launch.
 //
 // Bound: reading W once (M D elements; 4096 x 4096 bf16: 32 MiB, 6.5 us at the 5.15 TB/s a large copy reaches; one token
-// takes 6.9). So W goes from memory straight into MFMA operands, nothing staged: a workgroup owns 16 or 32 rows of W, its 8 waves
+// takes 7.6). So W goes from memory straight into MFMA operands, nothing staged: a workgroup owns 16 or 32 rows of W, its 8 waves
 // take turns at pieces of K (consecutive waves read consecutive pieces of a row), each lane 16 bytes of one row per
 // instruction, the next pieces requested before the present ones are multiplied. x is read through the caches by every
 // workgroup, as the MFMA's other operand (rows past N repeat the last one; their results are dropped). The 8 partial sums
